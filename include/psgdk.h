@@ -28,9 +28,9 @@ extern "C" {
 typedef struct ihipStream_t* psgdk_stream_t; /* hipStream_t */
 typedef struct ihipEvent_t* psgdk_event_t;   /* hipEvent_t */
 
-/* 5: option 8 chooses how fp32 products are summed (in 4: whether a k-contiguous fp32 kernel is taken), option 13, kernel
+/* 6: level 3 (the training step's operators). 5: option 8 chooses how fp32 products are summed (in 4: whether a k-contiguous fp32 kernel is taken), option 13, kernel
  * ids 6000 and 8000 (in 4: other engines' ids below 5000 and at 6000), smaller workspaces of psgdk_trmm_ws. */
-#define PSGDK_VERSION 5
+#define PSGDK_VERSION 6
 #define PSGDK_MAXB 16 /* problems per grouped call */
 #define PSGDK_MAX_GROUPS 64 /* groups per psgdk_kron2d_update_groups call */
 #define PSGDK_NLB_K 32 /* rows of the random start of the norm lower bounds */
@@ -303,6 +303,85 @@ int psgdk_momentum_multi(int nb, const int64_t* numel, float beta, const int32_t
  * psgd_pro_fast.py:200-206 and 482-483 draw with torch.randn on the device). out: 16-byte aligned (fp32) or 8-byte
  * (bf16). */
 int psgdk_fill_normal(void* out, int64_t n, int dtype, uint64_t seed, uint64_t stream_id, psgdk_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Level 3: operators of the training step in front of the optimizer. Rows are stored with the last dimension
+ * contiguous; ld* are row strides in elements. Storage dtypes are PSGDK_F32 or PSGDK_BF16; statistics, sums and
+ * accumulators are fp32 and every output is rounded once. No counterparts in the reference.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* y = dropout(x) over rows x d. Element (i, c) is kept where the 16-bit number c % 8 (low half of a word first) of
+ * block i * ceil(d / 8) + c / 8 of Philox4x32-10 (key seed; upper counter words stream_id, as psgdk_fill_normal) is
+ * at least t = round(65536 p), and is then scaled by 65536 / (65536 - t); a dropped element is 0 whatever x holds.
+ * The mask is never stored: the gradient of x is the same call on the gradient of y. 0 <= p <= 1. y may be x. */
+int psgdk_dropout(int64_t rows, int64_t d, int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, float p,
+                  uint64_t seed, uint64_t stream_id, psgdk_stream_t stream);
+
+enum { PSGDK_NORM_NONE = 0, PSGDK_NORM_RMS = 1, PSGDK_NORM_LAYER = 2 };
+
+/* The residual sum between two blocks of a transformer with the norm after the one and before the other:
+ *   u = Npost(f);  b = dropout(u);  y = x + scale * gate * b;  h = Npre(y)
+ * RMS: N(v) = v / sqrt(mean(v^2) + eps) * w; LAYER: N(v) = (v - mean(v)) / sqrt(var(v) + eps) * w + bias (w, bias
+ * NULL: 1, 0); NONE as post: u = f, as pre: no h. f NULL: y = x. The gate has gate_rows rows (0: no gate), row i of x
+ * taking gate row i / (rows / gate_rows); gate_rows divides rows. */
+typedef struct psgdk_residual_norm {
+  int64_t rows, d;          /* d up to 2^20 */
+  int32_t dtype;            /* x, f, y, h, and the gradients dy, dh, dx, df */
+  int32_t pre, post;        /* PSGDK_NORM_* */
+  int32_t w_dtype;          /* the norms' weights and biases, and their gradients */
+  int32_t gate_dtype;       /* the gate and its gradient */
+  float eps, scale;
+  float p;                  /* dropout of the branch as psgdk_dropout(u, p, seed, stream_id) */
+  uint64_t seed, stream_id;
+  int64_t gate_rows;
+  const void* x;
+  int64_t ldx;
+  const void* f;
+  int64_t ldf;
+  const void* gate;
+  int64_t ldgate;
+  const void *pre_w, *pre_b, *post_w, *post_b;
+  void* y;                  /* outputs of the forward call (y NULL: not stored); the backward call reads neither */
+  int64_t ldy;
+  void* h;
+  int64_t ldh;
+  float* stats;             /* 4 floats a row, 16-byte aligned: output of the forward call (NULL: not stored), input of
+                               the backward call */
+} psgdk_residual_norm_t;
+int psgdk_residual_norm(const psgdk_residual_norm_t* a, psgdk_stream_t stream);
+
+/* Gradients of x, f, the gate, the weights and the biases from those of y and h (dy, dh; NULL: zero). Outputs that are
+ * NULL are not computed. Sums over rows are added in a fixed order. */
+typedef struct psgdk_residual_norm_grads {
+  const void* dy;
+  int64_t lddy;
+  const void* dh;
+  int64_t lddh;
+  void* dx;
+  int64_t lddx;
+  void* df;
+  int64_t lddf;
+  void* dgate;
+  int64_t lddgate;
+  void *dpre_w, *dpre_b, *dpost_w, *dpost_b;
+} psgdk_residual_norm_grads_t;
+int psgdk_residual_norm_backward(const psgdk_residual_norm_t* a, const psgdk_residual_norm_grads_t* g, void* ws,
+                                 size_t* ws_bytes, psgdk_stream_t stream);
+
+/* Softmax cross entropy of logits x W^T (x rows x d, w vocab x d, one dtype) without the logits:
+ *   loss[i] = log sum_v exp(x_i . w_v) - x_i . w_t,  t = target[i];  0 where target[i] == ignore
+ * and, where dx or dw is non-NULL, that gradient of sum_i row_weight[i] loss[i], in the dtype of x and w; row_weight NULL: 1 for every row (mean 0) or 1 / (number of rows not ignored) (mean 1). A target outside
+ * 0 .. vocab - 1 that is not `ignore` gives a NaN loss (and NaN gradients of its row). mean_loss (optional, one float)
+ * receives sum_i row_weight[i] loss[i] under the same rule. An ignored row's x is read but reaches no result. */
+int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype, const void* x, int64_t ldx,
+                               const void* w, int64_t ldw, const int64_t* target, int64_t ignore,
+                               const float* row_weight, int mean, float* loss, float* mean_loss, void* dx,
+                               int64_t lddx, void* dw, int64_t lddw, void* ws, size_t* ws_bytes,
+                               psgdk_stream_t stream);
+
+/* x[b][i] *= *scale (device memory, one float) for the n[b] elements of nb (1 .. 4) tensors of one dtype; nothing but
+ * the scale is read, and nothing written, where it is 1. n and x are host arrays. */
+int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const float* scale, psgdk_stream_t stream);
 
 /* Launch profiling (diagnostic, per host thread): after psgdk_profile_start every MFMA-engine launch the thread makes is
  * bracketed by a pair of HIP events on its stream. psgdk_profile_stop ends the recording and, with out non-NULL,

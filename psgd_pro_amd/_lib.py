@@ -21,6 +21,7 @@ F32, BF16 = 0, 1
 PREC_F32, PREC_BF16 = 0, 1
 OUT_UPPER, OUT_MIRROR, OUT_PACKED = 0, 1, 2
 FACTOR_NONE, FACTOR_DIAG, FACTOR_DENSE = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 
 _vp = C.c_void_p
 _vpa = C.POINTER(C.c_void_p)  # host array of device pointers
@@ -51,6 +52,25 @@ class Draws(C.Structure):
     """psgdk_draws_t: a group's noise generated inside the update (normals offset[b] .. of the
     psgdk_fill_normal(seed, stream_id) sequence)."""
     _fields_ = [("seed", C.c_uint64), ("stream_id", C.c_uint64), ("offset", C.c_int64 * MAXB)]
+
+
+class ResidualNorm(C.Structure):
+    """psgdk_residual_norm_t"""
+    _fields_ = [("rows", C.c_int64), ("d", C.c_int64), ("dtype", C.c_int32), ("pre", C.c_int32), ("post", C.c_int32),
+                ("w_dtype", C.c_int32), ("gate_dtype", C.c_int32), ("eps", C.c_float), ("scale", C.c_float),
+                ("p", C.c_float), ("seed", C.c_uint64), ("stream_id", C.c_uint64), ("gate_rows", C.c_int64),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("f", C.c_void_p), ("ldf", C.c_int64), ("gate", C.c_void_p),
+                ("ldgate", C.c_int64), ("pre_w", C.c_void_p), ("pre_b", C.c_void_p), ("post_w", C.c_void_p),
+                ("post_b", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_int64), ("h", C.c_void_p), ("ldh", C.c_int64),
+                ("stats", C.c_void_p)]
+
+
+class ResidualNormGrads(C.Structure):
+    """psgdk_residual_norm_grads_t"""
+    _fields_ = [("dy", C.c_void_p), ("lddy", C.c_int64), ("dh", C.c_void_p), ("lddh", C.c_int64), ("dx", C.c_void_p),
+                ("lddx", C.c_int64), ("df", C.c_void_p), ("lddf", C.c_int64), ("dgate", C.c_void_p),
+                ("lddgate", C.c_int64), ("dpre_w", C.c_void_p), ("dpre_b", C.c_void_p), ("dpost_w", C.c_void_p),
+                ("dpost_b", C.c_void_p)]
 
 
 class ProfRecord(C.Structure):
@@ -102,6 +122,12 @@ _SIGS = {
     "psgdk_kron2d_balance": (_i32, [C.POINTER(Kron2d), C.POINTER(C.c_int32), _i32, _vp, _szp, _vp]),
     "psgdk_momentum": (_i32, [_i64, _f, _i32, _i32, _vpa, _vpa, _vp]),
     "psgdk_momentum_multi": (_i32, [_i32, C.POINTER(C.c_int64), _f, C.POINTER(C.c_int32), _vpa, _vpa, _vp]),
+    "psgdk_dropout": (_i32, [_i64, _i64, _i32, _vp, _i64, _vp, _i64, _f, C.c_uint64, C.c_uint64, _vp]),
+    "psgdk_residual_norm": (_i32, [C.POINTER(ResidualNorm), _vp]),
+    "psgdk_residual_norm_backward": (_i32, [C.POINTER(ResidualNorm), C.POINTER(ResidualNormGrads), _vp, _szp, _vp]),
+    "psgdk_linear_cross_entropy": (_i32, [_i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _vp,
+                                          _vp, _i64, _vp, _i64, _vp, _szp, _vp]),
+    "psgdk_scale_by": (_i32, [_i32, C.POINTER(C.c_int64), _i32, _vpa, _vp, _vp]),
     "psgdk_set_option": (_i32, [_i32, _i32]),
     "psgdk_get_option": (_i32, [_i32, C.POINTER(C.c_int)]),
     "psgdk_profile_start": (_i32, []),
@@ -110,7 +136,7 @@ _SIGS = {
 }
 
 EXPORTED = tuple(_SIGS)
-ABI_VERSION = 5  # PSGDK_VERSION of include/psgdk.h that these signatures and structures follow
+ABI_VERSION = 6  # PSGDK_VERSION of include/psgdk.h that these signatures and structures follow
 
 _lib = None
 

@@ -6,7 +6,7 @@ Objects go to psgd_pro_amd/_build/; sources are compiled in parallel and the lib
 
     python -m psgd_pro_amd.build --asan
 
-also builds psgd_pro_amd/_build/libpsgdk_asan.so: the same library with its host code (capi.cpp, the C ABI's
+also builds psgd_pro_amd/_build/libpsgdk_asan.so: the same library with its host code (HOST_SOURCES, the C ABI's
 argument checks, workspace planning and launch set-up) built with AddressSanitizer, for the CPU tests that drive the
 C ABI without a GPU (tests/test_asan_cpu.py loads it with the sanitizer runtime preloaded). Device code is built as
 usual; the sanitizer applies to host code only.
@@ -21,8 +21,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpsgdk.so")
-SOURCES = ["gemm_cv.hip", "gemm_bf16.hip", "gemm_small.hip", "nlb.hip", "elem.hip", "capi.cpp", "noalloc.hip",
-           "measure.hip"]
+SOURCES = ["gemm_cv.hip", "gemm_bf16.hip", "gemm_small.hip", "nlb.hip", "elem.hip", "block.hip", "xent.hip", "capi.cpp",
+           "train_capi.cpp", "noalloc.hip", "measure.hip"]
+HOST_SOURCES = ["capi.cpp", "train_capi.cpp"]  # the C ABI's host code, which the sanitizer build instruments
 ARCH = os.environ.get("PSGDK_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -58,16 +59,20 @@ def asan_runtime():
 
 
 def build_asan(objects):
-    """capi.cpp with the host sanitizer, linked with the other (regular) objects into ASAN_LIB."""
-    obj = os.path.join(BUILD, "capi_asan.o")
-    cmd = [HIPCC, "-O1", "-g", *[f for f in COMMON if f != "-O3"], *DEVICE_FLAGS, *ASAN_HOST, "-c",
-           os.path.join(CSRC, "capi.cpp"), "-o", obj]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stderr}")
-    others = [o for o in objects if os.path.basename(o) != "capi.o"]
+    """HOST_SOURCES with the host sanitizer, linked with the other (regular) objects into ASAN_LIB."""
+    objs = []
+    for src in HOST_SOURCES:
+        stem = os.path.splitext(src)[0]
+        objs.append(os.path.join(BUILD, stem + "_asan.o"))
+        cmd = [HIPCC, "-O1", "-g", *[f for f in COMMON if f != "-O3"], *DEVICE_FLAGS, *ASAN_HOST, "-c",
+               os.path.join(CSRC, src), "-o", objs[-1]]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stderr}")
+    host = {os.path.splitext(s)[0] + ".o" for s in HOST_SOURCES}
+    others = [o for o in objects if os.path.basename(o) not in host]
     cmd = [HIPCC, "-shared", f"--offload-arch={ARCH}", "-Xarch_host", "-fsanitize=address", "-shared-libasan",
-           "-o", ASAN_LIB, obj, *others]
+           "-o", ASAN_LIB, *objs, *others]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stderr}")

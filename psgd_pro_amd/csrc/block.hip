@@ -1,0 +1,845 @@
+// Dropout, and the residual sum between two blocks of a transformer with its norms, gate, scale and dropout. Both are
+// bound by memory: every tensor passes once, a row stays in registers between its statistics and its use, sums are fp32.
+#include "block.h"
+#include "philox.h"
+
+namespace psgdk {
+
+namespace {
+
+constexpr int VE = 8;  // elements a thread holds together: one 16-byte bf16 access, one Philox block of dropout
+
+// VE consecutive elements as floats. The pointers are only element-aligned (rows of odd length): the copies become
+// 16-byte accesses, which this GPU serves at any alignment.
+__device__ __forceinline__ void ld8(const bf16_t* p, float (&v)[VE]) {
+  bf16_t h[VE];
+  __builtin_memcpy(h, p, sizeof h);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) v[e] = bf16_to_f32(h[e]);
+}
+__device__ __forceinline__ void ld8(const float* p, float (&v)[VE]) { __builtin_memcpy(v, p, sizeof v); }
+__device__ __forceinline__ void st8(bf16_t* p, const float (&v)[VE]) {
+  bf16_t h[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) h[e] = f32_to_bf16(v[e]);
+  __builtin_memcpy(p, h, sizeof h);
+}
+__device__ __forceinline__ void st8(float* p, const float (&v)[VE]) { __builtin_memcpy(p, v, sizeof v); }
+
+// Elements c .. c + 7 of a row of d (zeros past its end).
+template <typename T>
+__device__ __forceinline__ void ld_row(const T* row, int c, int d, float (&v)[VE]) {
+  if (c + VE <= d) {
+    ld8(row + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = c + e < d ? to_f32<T>(row[c + e]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void st_row(T* row, int c, int d, const float (&v)[VE]) {
+  if (c + VE <= d) {
+    st8(row + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (c + e < d) row[c + e] = from_f32<T>(v[e]);
+  }
+}
+// The same of a vector with a dtype of its own; `none` where it is absent.
+__device__ __forceinline__ void ld_vec(const Vec& w, long long off, int c, int d, float none, float (&v)[VE]) {
+  if (!w.p) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = none;
+  } else if (w.dt == 1) {
+    ld_row(reinterpret_cast<const bf16_t*>(w.p) + off, c, d, v);
+  } else {
+    ld_row(reinterpret_cast<const float*>(w.p) + off, c, d, v);
+  }
+}
+
+// One thread's 8 elements c .. c + 7 of rows of d >= 8 elements. Where the row ends inside them the load starts 8
+// elements before its end and the values move down (zeros behind the end): every lane loads one whole vector. RAGGED:
+// d is no multiple of 8 (else there is nothing to move and to mask).
+template <bool RAGGED>
+struct Span {
+  int c, d, at, move;
+  bool in;  // the thread has elements of the row
+  __device__ __forceinline__ Span(int c_, int d_) : c(c_), d(d_) {
+    in = c < d;
+    at = RAGGED ? min(c, d - VE) : c;
+    move = c - at;
+  }
+  __device__ __forceinline__ void zero(float (&v)[VE]) const {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = 0.f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, float (&v)[VE]) const {
+    if (!in) {
+      zero(v);
+      return;
+    }
+    ld8(row + at, v);
+    if constexpr (RAGGED) {
+#pragma unroll
+      for (int s = 4; s > 0; s >>= 1) {
+        const bool m = move & s;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[e] = m ? (e + s < VE ? v[e + s] : 0.f) : v[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const Vec& w, long long off, float none, float (&v)[VE]) const {
+    if (!w.p) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = none;
+    } else if (w.dt == 1) {
+      load(reinterpret_cast<const bf16_t*>(w.p) + off, v);
+    } else {
+      load(reinterpret_cast<const float*>(w.p) + off, v);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, const float (&v)[VE]) const {
+    if (!in) return;
+    if constexpr (RAGGED) st_row(row, c, d, v);
+    else st8(row + c, v);
+  }
+  // whether element e is the row's (in a centred sum, the zeros behind its end are not)
+  __device__ __forceinline__ bool has(int e) const { return RAGGED ? c + e < d : in; }
+};
+
+// Dropout's factors of elements c .. c + 7 (c a multiple of 8) of a row.
+__device__ __forceinline__ void drop8(const Drop& dr, long long row, int c, int d, float (&m)[VE]) {
+  const unsigned long long blk = (unsigned long long)row * (unsigned)((d + VE - 1) / VE) + (unsigned)(c / VE);
+  uint32_t w[4] = {(uint32_t)blk, (uint32_t)(blk >> 32), dr.s0, dr.s1};
+  philox4x32_10(w, dr.k0, dr.k1);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    const uint32_t u = (e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
+    m[e] = u >= dr.thr ? dr.scale : 0.f;
+  }
+}
+
+// A dropped element is 0 whatever it holds (an infinity too).
+__device__ __forceinline__ float dropped(float v, float m) { return m == 0.f ? 0.f : v * m; }
+
+}  // namespace
+
+// ---------------------------------------------------------------------------------------------------------------
+// y = dropout(x): one Philox block of 128 bits serves 8 elements, 16 bits each (drop probabilities in steps of 2^-16).
+template <typename T>
+__global__ void __launch_bounds__(256) dropout_kernel(const DropArgs a) {
+  const long long per = (a.d + VE - 1) / VE, total = a.rows * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / per;
+    const int c = (int)(i - row * per) * VE;
+    float v[VE], m[VE];
+    ld_row(reinterpret_cast<const T*>(a.x) + row * a.ldx, c, a.d, v);
+    drop8(a.drop, row, c, a.d, m);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = dropped(v[e], m[e]);
+    st_row(reinterpret_cast<T*>(a.y) + row * a.ldy, c, a.d, v);
+  }
+}
+
+hipError_t dropout_launch(const DropArgs& a, hipStream_t st) {
+  const long long want = (a.rows * ((a.d + VE - 1) / VE) + 255) / 256;
+  const int blocks = (int)(want > 4096 ? 4096 : want);
+  if (a.dt == 1) hipLaunchKernelGGL(dropout_kernel<bf16_t>, dim3(blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(dropout_kernel<float>, dim3(blocks), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// y = x + scale gate dropout(Npost(f)), h = Npre(y). TPR threads hold a row, 8 elements each; a workgroup of at least
+// 256 threads holds 256 / TPR rows. The waves' sums meet in LDS where a row has more than one. The
+// variance of a layer norm is the mean of the squared centred values, summed from the registers (no difference of large
+// sums). h is made from y before y's rounding.
+namespace {
+
+constexpr int res_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// Sums over the TPR threads of a row, every thread of the workgroup taking part. red holds one value for each wave; its
+// next use has to come after a barrier.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = wave_sum(v);
+  if constexpr (TPR > 64) {
+    const int w = threadIdx.x >> 6, w0 = w / (TPR / 64) * (TPR / 64);
+    if ((threadIdx.x & 63) == 0) red[w] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) v += red[w0 + i];
+  }
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ float2 row_sum2(float2 v, float2* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    v.x += __shfl_xor(v.x, o, 64);
+    v.y += __shfl_xor(v.y, o, 64);
+  }
+  if constexpr (TPR > 64) {
+    const int w = threadIdx.x >> 6, w0 = w / (TPR / 64) * (TPR / 64);
+    if ((threadIdx.x & 63) == 0) red[w] = v;
+    __syncthreads();
+    v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) {
+      v.x += red[w0 + i].x;
+      v.y += red[w0 + i].y;
+    }
+  }
+  return v;
+}
+
+// mean and 1 / std of a row held in u; u is centred in place for a layer norm (red: 2 x 16 floats)
+template <int TPR, bool RAGGED>
+__device__ __forceinline__ float2 row_stats(float (&u)[VE], const Span<RAGGED>& sp, int kind, float eps, float* red) {
+  const float inv_d = 1.f / (float)sp.d;
+  float mean = 0.f, s = 0.f;
+  if (kind == NORM_LAYER) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) s += u[e];
+    mean = row_sum<TPR>(s, red) * inv_d;
+    s = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) u[e] = sp.has(e) ? u[e] - mean : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) s += u[e] * u[e];
+  return make_float2(mean, 1.f / sqrtf(row_sum<TPR>(s, red + 16) * inv_d + eps));
+}
+
+template <typename T, int TPR, bool RAGGED>
+__global__ void __launch_bounds__(res_threads(TPR)) residual_norm_kernel(const ResArgs a) {
+  __shared__ float red[2][32];
+  const long long want =
+      (long long)blockIdx.x * (res_threads(TPR) / TPR) + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+  const bool live = want < a.rows;
+  const long long row = live ? want : a.rows - 1;  // a row behind the last one takes part in the barriers only
+  const int t = threadIdx.x % TPR;
+  const Span<RAGGED> sp(t * VE, a.d);
+  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+  float x[VE];
+  sp.load(reinterpret_cast<const T*>(a.x) + row * a.ldx, x);
+  if (a.f) {
+    float u[VE], g[VE];
+    sp.load(reinterpret_cast<const T*>(a.f) + row * a.ldf, u);
+    sp.load(a.gate, row / a.gate_every * a.ldg, 1.f, g);
+    if (a.post != NORM_NONE) {
+      float w[VE], b[VE];
+      sp.load(a.post_w, 0, 1.f, w);
+      sp.load(a.post_b, 0, 0.f, b);
+      const float2 s = row_stats<TPR, RAGGED>(u, sp, a.post, a.eps, red[0]);
+      st.z = s.x;
+      st.w = s.y;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) u[e] = u[e] * s.y * w[e] + b[e];
+    }
+    if (a.drop.thr) {
+      float m[VE];
+      drop8(a.drop, row, sp.c, a.d, m);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) u[e] = dropped(u[e], m[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x[e] += sp.has(e) ? a.scale * g[e] * u[e] : 0.f;
+  }
+  if (a.y && live) sp.store(reinterpret_cast<T*>(a.y) + row * a.ldy, x);
+  if (a.pre != NORM_NONE) {
+    float w[VE], b[VE];
+    sp.load(a.pre_w, 0, 1.f, w);
+    sp.load(a.pre_b, 0, 0.f, b);
+    const float2 s = row_stats<TPR, RAGGED>(x, sp, a.pre, a.eps, red[1]);
+    st.x = s.x;
+    st.y = s.y;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) w[e] = x[e] * s.y * w[e] + b[e];
+    if (live) sp.store(reinterpret_cast<T*>(a.h) + row * a.ldh, w);
+  }
+  if (a.stats && t == 0 && live) a.stats[row] = st;
+}
+
+// Rows too long for the registers, or too short for a vector: every pass reads the row again (from the caches), with
+// the same sums.
+template <typename T>
+__global__ void __launch_bounds__(1024) residual_norm_wide_kernel(const ResArgs a) {
+  __shared__ float red[16];
+  const long long row = blockIdx.x;
+  const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+  const T* fr = reinterpret_cast<const T*>(a.f) + (a.f ? row * a.ldf : 0);
+  const long long goff = row / a.gate_every * a.ldg;
+  const float inv_d = 1.f / (float)a.d;
+  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto each = [&](auto fn) {
+    for (int c = threadIdx.x * VE; c < a.d; c += 1024 * VE) fn(c);
+  };
+  // y's elements c .. c + 7
+  auto y_of = [&](int c, float (&y)[VE]) {
+    ld_row(xr, c, a.d, y);
+    if (!a.f) return;
+    float b[VE], g[VE];
+    ld_row(fr, c, a.d, b);
+    if (a.post != NORM_NONE) {
+      float w[VE], bs[VE];
+      ld_vec(a.post_w, 0, c, a.d, 1.f, w);
+      ld_vec(a.post_b, 0, c, a.d, 0.f, bs);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) b[e] = (b[e] - st.z) * st.w * w[e] + bs[e];
+    }
+    ld_vec(a.gate, goff, c, a.d, 1.f, g);
+    if (a.drop.thr) {
+      float m[VE];
+      drop8(a.drop, row, c, a.d, m);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) b[e] = dropped(b[e], m[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) y[e] += a.scale * g[e] * b[e];
+  };
+  auto stats = [&](int kind, auto at) {
+    float mean = 0.f, s = 0.f;
+    if (kind == NORM_LAYER) {
+      each([&](int c) {
+        float v[VE];
+        at(c, v);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) s += c + e < a.d ? v[e] : 0.f;
+      });
+      mean = block_sum(s, red) * inv_d;
+      s = 0.f;
+    }
+    each([&](int c) {
+      float v[VE];
+      at(c, v);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s += c + e < a.d ? (v[e] - mean) * (v[e] - mean) : 0.f;
+    });
+    return make_float2(mean, 1.f / sqrtf(block_sum(s, red) * inv_d + a.eps));
+  };
+  if (a.f && a.post != NORM_NONE) {
+    const float2 s = stats(a.post, [&](int c, float (&v)[VE]) { ld_row(fr, c, a.d, v); });
+    st.z = s.x;
+    st.w = s.y;
+  }
+  if (a.pre != NORM_NONE) {
+    const float2 s = stats(a.pre, y_of);
+    st.x = s.x;
+    st.y = s.y;
+  }
+  each([&](int c) {
+    float y[VE];
+    y_of(c, y);
+    if (a.y) st_row(reinterpret_cast<T*>(a.y) + row * a.ldy, c, a.d, y);
+    if (a.pre != NORM_NONE) {
+      float w[VE], b[VE];
+      ld_vec(a.pre_w, 0, c, a.d, 1.f, w);
+      ld_vec(a.pre_b, 0, c, a.d, 0.f, b);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) w[e] = (y[e] - st.x) * st.y * w[e] + b[e];
+      st_row(reinterpret_cast<T*>(a.h) + row * a.ldh, c, a.d, w);
+    }
+  });
+  if (a.stats && threadIdx.x == 0) a.stats[row] = st;
+}
+
+}  // namespace
+
+template <typename T, int TPR>
+static void residual_norm_sized(const ResArgs& a, hipStream_t st) {
+  constexpr int RW = res_threads(TPR) / TPR;
+  const dim3 grid((unsigned)((a.rows + RW - 1) / RW)), block(res_threads(TPR));
+  if (a.d % VE) hipLaunchKernelGGL((residual_norm_kernel<T, TPR, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((residual_norm_kernel<T, TPR, false>), grid, block, 0, st, a);
+}
+template <typename T>
+static hipError_t residual_norm_t(const ResArgs& a, hipStream_t st) {
+  if (res_wide(a.d)) hipLaunchKernelGGL(residual_norm_wide_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+  else if (a.d <= 512) residual_norm_sized<T, 64>(a, st);
+  else if (a.d <= 1024) residual_norm_sized<T, 128>(a, st);
+  else if (a.d <= 2048) residual_norm_sized<T, 256>(a, st);
+  else if (a.d <= 4096) residual_norm_sized<T, 512>(a, st);
+  else hipLaunchKernelGGL((residual_norm_kernel<T, 1024, false>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+  return hipGetLastError();
+}
+hipError_t residual_norm_launch(const ResArgs& a, hipStream_t st) {
+  return a.dt == 1 ? residual_norm_t<bf16_t>(a, st) : residual_norm_t<float>(a, st);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Backward. y is made again from x and f, as many bytes as the stored y and f and without y's rounding. With
+// hat = (y - mean) / std, c = dh w:
+//   dyt = dy + (c - [layer] mean(c) - hat mean(c hat)) / std;  dx = dyt
+//   dgate = sum over its rows of scale dyt b;  du = scale gate dropout'(dyt);  df from du and f as dyt from dh and y
+//   weights: column sums of dh hat and du fhat, biases: of dh and du
+// A workgroup takes `chunk` consecutive rows and keeps its column sums in registers; they go to one row of `part` each
+// and a second kernel adds those in a fixed order. A gate row whose rows all lie in one workgroup is written at once.
+namespace {
+
+// Stores a workgroup's column sum as a row of the partial sums and starts it again from zero.
+template <int TPR, bool RAGGED>
+__device__ __forceinline__ void put_sum(float (&s)[VE], float* dst, const Span<RAGGED>& sp, float* lds) {
+  if constexpr (TPR < 256) {  // the sums of the workgroup's rows meet in LDS, in order
+    const int k = threadIdx.x / TPR, t = threadIdx.x % TPR;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) lds[(k * VE + e) * TPR + t] = s[e];
+    __syncthreads();
+    if (k == 0) {
+#pragma unroll
+      for (int q = 1; q < 256 / TPR; ++q)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) s[e] += lds[(q * VE + e) * TPR + t];
+      sp.store(dst, s);
+    }
+    __syncthreads();
+  } else {
+    sp.store(dst, s);
+  }
+  sp.zero(s);
+}
+
+// SUMS: column sums in registers (bit 0: of the norm before, bit 1: of the norm after, bit 2: of the gate)
+template <typename T, int TPR, int SUMS, bool RAGGED>
+__global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kernel(const ResArgs a) {
+  constexpr int RW = res_threads(TPR) / TPR;  // rows the workgroup has in hand at once
+  __shared__ float2 red[2][16];
+  __shared__ float lds[TPR < 256 && SUMS ? VE * 256 : 1];
+  // a row's waves are whole: its number is a scalar, and so are the addresses of its start
+  const int t = threadIdx.x % TPR, w = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+  const Span<RAGGED> sp(t * VE, a.d);
+  // rows r0 .. r1 - 1: `chunk` rows (whole gates), or a part of one gate's
+  long long r0, r1;
+  if (a.per_gate > 1) {
+    const long long gate = (long long)blockIdx.x / a.per_gate;
+    r0 = gate * a.gate_every + (long long)blockIdx.x % a.per_gate * a.chunk;
+    r1 = min(r0 + a.chunk, (gate + 1) * a.gate_every);
+  } else {
+    r0 = (long long)blockIdx.x * a.chunk;
+    r1 = min(r0 + a.chunk, a.rows);
+  }
+  float s_pw[VE] = {}, s_pb[VE] = {}, s_qw[VE] = {}, s_qb[VE] = {}, s_g[VE] = {};
+  const float inv_d = 1.f / (float)a.d;
+
+  // The weights of a row, read again for each row where a thread has no registers left to keep them (1024 threads have
+  // 128 each): an empty asm statement hides from the compiler that the addresses stay the same.
+  auto vec = [&](const Vec& v) {
+    Vec q = v;
+    if constexpr (TPR == 1024) asm volatile("" : "+s"(q.p));
+    return q;
+  };
+  auto one_row = [&](long long want, bool live) {
+    const long long row = live ? want : r0;  // a row behind the last one takes part in the barriers only
+    const float4 st = a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    float v[VE], fh[VE], b[VE], g[VE], wt[VE];  // v: dyt, then du
+    unsigned kept = 0;
+    if (a.dy) sp.load(reinterpret_cast<const T*>(a.dy) + row * a.lddy, v);
+    else sp.zero(v);
+    if (a.f) {  // the branch again: fh = f's normalised values, b = dropout(Npost(f))
+      sp.load(reinterpret_cast<const T*>(a.f) + row * a.ldf, fh);
+      sp.load(vec(a.gate), row / a.gate_every * a.ldg, 1.f, g);
+      if (a.post != NORM_NONE) {
+        sp.load(vec(a.post_w), 0, 1.f, wt);
+        sp.load(vec(a.post_b), 0, 0.f, b);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          fh[e] = (fh[e] - st.z) * st.w;
+          b[e] += fh[e] * wt[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) b[e] = fh[e];
+      }
+      if (a.drop.thr) {
+        float m[VE];
+        drop8(a.drop, row, sp.c, a.d, m);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          b[e] = dropped(b[e], m[e]);
+          kept |= m[e] != 0.f ? 1u << e : 0u;
+        }
+      }
+    }
+    if (a.dh) {
+      float hat[VE], c[VE], w[VE];
+      float2 m = make_float2(0.f, 0.f);
+      sp.load(reinterpret_cast<const T*>(a.x) + row * a.ldx, hat);
+      sp.load(reinterpret_cast<const T*>(a.dh) + row * a.lddh, c);
+      sp.load(vec(a.pre_w), 0, 1.f, w);
+      if (a.f) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) hat[e] += a.scale * g[e] * b[e];
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        hat[e] = (hat[e] - st.x) * st.y;
+        if constexpr (SUMS & 1) {
+          s_pw[e] += live ? c[e] * hat[e] : 0.f;
+          s_pb[e] += live ? c[e] : 0.f;
+        }
+        c[e] *= w[e];
+        m.x += c[e];
+        m.y += c[e] * hat[e];
+      }
+      m = row_sum2<TPR>(m, red[0]);
+      m.x = a.pre == NORM_LAYER ? m.x * inv_d : 0.f;
+      m.y *= inv_d;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] += (c[e] - m.x - hat[e] * m.y) * st.y;
+    }
+    if (a.dx && live) sp.store(reinterpret_cast<T*>(a.dx) + row * a.lddx, v);
+    if (a.f) {
+      float2 m = make_float2(0.f, 0.f);
+      float dg[VE];
+      if constexpr (TPR == 1024) {
+        sp.load(vec(a.gate), row / a.gate_every * a.ldg, 1.f, g);
+        if (a.post != NORM_NONE) sp.load(vec(a.post_w), 0, 1.f, wt);
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        float du = sp.has(e) ? a.scale * v[e] : 0.f;
+        dg[e] = du * b[e];
+        du *= g[e];
+        if (a.drop.thr) du = kept >> e & 1 ? du * a.drop.scale : 0.f;
+        if constexpr (SUMS & 4) s_g[e] += live ? dg[e] : 0.f;
+        if (a.post != NORM_NONE) {
+          if constexpr (SUMS & 2) {
+            s_qw[e] += live ? du * fh[e] : 0.f;
+            s_qb[e] += live ? du : 0.f;
+          }
+          du *= wt[e];
+          m.x += du;
+          m.y += du * fh[e];
+        }
+        v[e] = du;
+      }
+      if (a.dgate && a.gate_every == 1 && live) {  // a gate for each row: no sum
+        if (a.gate.dt == 1) sp.store(reinterpret_cast<bf16_t*>(a.dgate) + row * a.lddg, dg);
+        else sp.store(reinterpret_cast<float*>(a.dgate) + row * a.lddg, dg);
+      }
+      if (a.post != NORM_NONE) {
+        m = row_sum2<TPR>(m, red[1]);
+        m.x = a.post == NORM_LAYER ? m.x * inv_d : 0.f;
+        m.y *= inv_d;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[e] = (v[e] - m.x - fh[e] * m.y) * st.w;
+      }
+      if (a.df && live) sp.store(reinterpret_cast<T*>(a.df) + row * a.lddf, v);
+    }
+    if constexpr (TPR > 64) __syncthreads();  // red is free again
+  };
+
+  const bool whole_gates = (SUMS & 4) && a.gpart && a.per_gate == 1;
+  const long long step = whole_gates ? a.gate_every : r1 - r0;
+  for (long long b0 = r0; b0 < r1; b0 += step) {
+    const long long b1 = min(b0 + step, r1);
+    for (long long row = b0; row < b1; row += RW) one_row(row + w, row + w < b1);
+    if ((SUMS & 4) && a.gpart)
+      put_sum<TPR, RAGGED>(s_g, a.gpart + (whole_gates ? b0 / a.gate_every : (long long)blockIdx.x) * a.d, sp, lds);
+  }
+  auto put = [&](float (&s)[VE], int k) {
+    if (a.slot[k] >= 0) put_sum<TPR, RAGGED>(s, a.part + ((long long)a.slot[k] * a.parts + blockIdx.x) * a.d, sp, lds);
+  };
+  if constexpr (SUMS & 1) {
+    put(s_pw, kSumPreW);
+    put(s_pb, kSumPreB);
+  }
+  if constexpr (SUMS & 2) {
+    put(s_qw, kSumPostW);
+    put(s_qb, kSumPostB);
+  }
+}
+
+// Rows too long for the registers: the same gradients with every pass reading the row again; the column sums are a
+// second kernel's, from the rows' means kept by this one.
+template <typename T>
+struct ResWide {
+  const ResArgs& a;
+  long long row;
+  float4 st, mean;
+  long long goff;
+  // the branch's elements c .. c + 7: f's normalised values, b = dropout(Npost(f)), and the weight, gate and kept bits
+  __device__ __forceinline__ unsigned branch(int c, float (&fh)[VE], float (&b)[VE], float (&w)[VE], float (&g)[VE]) const {
+    unsigned kept = 0;
+    ld_row(reinterpret_cast<const T*>(a.f) + row * a.ldf, c, a.d, fh);
+    ld_vec(a.gate, goff, c, a.d, 1.f, g);
+    ld_vec(a.post_w, 0, c, a.d, 1.f, w);
+    ld_vec(a.post_b, 0, c, a.d, 0.f, b);
+    float k[VE];
+    if (a.drop.thr) drop8(a.drop, row, c, a.d, k);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      if (a.post != NORM_NONE) {
+        fh[e] = (fh[e] - st.z) * st.w;
+        b[e] += fh[e] * w[e];
+      } else {
+        b[e] = fh[e];
+      }
+      if (a.drop.thr) {
+        b[e] = dropped(b[e], k[e]);
+        kept |= k[e] != 0.f ? 1u << e : 0u;
+      }
+    }
+    return kept;
+  }
+  // y's normalised values, dh and c = dh w
+  __device__ __forceinline__ void pre(int c, float (&hat)[VE], float (&dh)[VE], float (&cw)[VE]) const {
+    float w[VE];
+    ld_row(reinterpret_cast<const T*>(a.x) + row * a.ldx, c, a.d, hat);
+    ld_row(reinterpret_cast<const T*>(a.dh) + row * a.lddh, c, a.d, dh);
+    if (a.f) {
+      float fh[VE], b[VE], g[VE];
+      branch(c, fh, b, w, g);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) hat[e] += a.scale * g[e] * b[e];
+    }
+    ld_vec(a.pre_w, 0, c, a.d, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      hat[e] = (hat[e] - st.x) * st.y;
+      cw[e] = dh[e] * w[e];
+    }
+  }
+  __device__ __forceinline__ void dyt(int c, float (&v)[VE]) const {
+    if (a.dy) ld_row(reinterpret_cast<const T*>(a.dy) + row * a.lddy, c, a.d, v);
+    else
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = 0.f;
+    if (!a.dh) return;
+    float hat[VE], dh[VE], cw[VE];
+    pre(c, hat, dh, cw);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] += (cw[e] - mean.x - hat[e] * mean.y) * st.y;
+  }
+  // v = dyt in; out: f's normalised values, du (v), du w (dw) and the gate's gradient
+  __device__ __forceinline__ void post(int c, float (&v)[VE], float (&fh)[VE], float (&dw)[VE], float (&dg)[VE]) const {
+    float w[VE], b[VE], g[VE];
+    const unsigned kept = branch(c, fh, b, w, g);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      float du = a.scale * v[e];
+      dg[e] = du * b[e];
+      du *= g[e];
+      if (a.drop.thr) du = kept >> e & 1 ? du * a.drop.scale : 0.f;
+      v[e] = du;
+      dw[e] = a.post != NORM_NONE ? du * w[e] : du;
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(1024) residual_norm_backward_wide_kernel(const ResArgs a) {
+  __shared__ float2 red[2][16];
+  const long long row = blockIdx.x;
+  ResWide<T> r{a, row, a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f),
+               row / a.gate_every * a.ldg};
+  const float inv_d = 1.f / (float)a.d;
+  auto each = [&](auto fn) {
+    for (int c = threadIdx.x * VE; c < a.d; c += 1024 * VE) fn(c);
+  };
+  if (a.dh) {
+    float2 m = make_float2(0.f, 0.f);
+    each([&](int c) {
+      float hat[VE], dh[VE], cw[VE];
+      r.pre(c, hat, dh, cw);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        m.x += cw[e];
+        m.y += c + e < a.d ? cw[e] * hat[e] : 0.f;
+      }
+    });
+    m = row_sum2<1024>(m, red[0]);
+    r.mean.x = a.pre == NORM_LAYER ? m.x * inv_d : 0.f;
+    r.mean.y = m.y * inv_d;
+  }
+  if (a.f && a.post != NORM_NONE) {
+    float2 m = make_float2(0.f, 0.f);
+    each([&](int c) {
+      float v[VE], fh[VE], dw[VE], dg[VE];
+      r.dyt(c, v);
+      r.post(c, v, fh, dw, dg);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        m.x += dw[e];
+        m.y += dw[e] * fh[e];
+      }
+    });
+    m = row_sum2<1024>(m, red[1]);
+    r.mean.z = a.post == NORM_LAYER ? m.x * inv_d : 0.f;
+    r.mean.w = m.y * inv_d;
+  }
+  each([&](int c) {
+    float v[VE], fh[VE], dw[VE], dg[VE];
+    r.dyt(c, v);
+    if (a.dx) st_row(reinterpret_cast<T*>(a.dx) + row * a.lddx, c, a.d, v);
+    if (!a.f) return;
+    r.post(c, v, fh, dw, dg);
+    if (a.dgate && a.gate_every == 1) {
+      if (a.gate.dt == 1) st_row(reinterpret_cast<bf16_t*>(a.dgate) + row * a.lddg, c, a.d, dg);
+      else st_row(reinterpret_cast<float*>(a.dgate) + row * a.lddg, c, a.d, dg);
+    }
+    if (a.post != NORM_NONE) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) dw[e] = (dw[e] - r.mean.z - fh[e] * r.mean.w) * r.st.w;
+    }
+    if (a.df) st_row(reinterpret_cast<T*>(a.df) + row * a.lddf, c, a.d, dw);
+  });
+  if (threadIdx.x == 0) a.means[row] = r.mean;
+}
+
+// one workgroup: 2048 columns of `chunk` rows (the same split of the rows as the register kernel's)
+template <typename T>
+__global__ void __launch_bounds__(256) residual_norm_columns_kernel(const ResArgs a, int strips) {
+  const long long wg = blockIdx.x / strips;
+  const int c = ((int)(blockIdx.x % strips) * 256 + threadIdx.x) * VE;
+  if (c >= a.d) return;
+  long long r0, r1;
+  if (a.per_gate > 1) {
+    const long long gate = wg / a.per_gate;
+    r0 = gate * a.gate_every + wg % a.per_gate * a.chunk;
+    r1 = min(r0 + a.chunk, (gate + 1) * a.gate_every);
+  } else {
+    r0 = wg * a.chunk;
+    r1 = min(r0 + a.chunk, a.rows);
+  }
+  float s[4][VE] = {}, sg[VE] = {};
+  for (long long row = r0; row < r1; ++row) {
+    ResWide<T> r{a, row, a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f), a.means[row],
+                 row / a.gate_every * a.ldg};
+    float v[VE];
+    r.dyt(c, v);
+    if (a.dh) {
+      float hat[VE], dh[VE], cw[VE];
+      r.pre(c, hat, dh, cw);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        s[kSumPreW][e] += dh[e] * hat[e];
+        s[kSumPreB][e] += dh[e];
+      }
+    }
+    if (a.f) {
+      float fh[VE], dw[VE], dg[VE];
+      r.post(c, v, fh, dw, dg);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        s[kSumPostW][e] += v[e] * fh[e];
+        s[kSumPostB][e] += v[e];
+        sg[e] += dg[e];
+      }
+      if (a.gpart && (row + 1 == r1 || (a.per_gate == 1 && (row + 1) % a.gate_every == 0))) {
+        st_row(a.gpart + (a.per_gate == 1 ? row / a.gate_every : wg) * a.d, c, a.d, sg);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) sg[e] = 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (a.slot[k] >= 0) st_row(a.part + ((long long)a.slot[k] * a.parts + wg) * a.d, c, a.d, s[k]);
+}
+
+// A workgroup adds 64 columns of one output: wave w the rows w, w + 16, ..., then the 16 sums in order.
+__global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums s) {
+  __shared__ float red[16][64];
+  const int strips = (s.d + 63) / 64;
+  long long i = blockIdx.x / strips;
+  int k = 0;
+  while (i >= s.e[k].groups) i -= s.e[k++].groups;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = (int)(blockIdx.x % strips) * 64 + lane;
+  const float* in = s.e[k].in + i * s.e[k].per * s.d;
+  float v = 0.f;
+  if (c < s.d) {
+#pragma unroll 8
+    for (long long p = w; p < s.e[k].per; p += 16) v += in[p * s.d + c];
+  }
+  red[w][lane] = v;
+  __syncthreads();
+  if (w || c >= s.d) return;
+  for (int q = 1; q < 16; ++q) v += red[q][lane];
+  const long long o = i * s.e[k].ldo + c;
+  if (s.e[k].dt == 1) reinterpret_cast<bf16_t*>(s.e[k].out)[o] = f32_to_bf16(v);
+  else reinterpret_cast<float*>(s.e[k].out)[o] = v;
+}
+
+}  // namespace
+
+void residual_norm_split(ResArgs& a, bool gate_sums) {
+  constexpr long long kTarget = 1024;  // workgroups: four for each CU
+  a.chunk = a.rows > kTarget ? (a.rows + kTarget - 1) / kTarget : 1;
+  const long long at_once = a.d <= 512 ? 4 : a.d <= 1024 ? 2 : 1;
+  a.chunk = (a.chunk + at_once - 1) / at_once * at_once;
+  a.per_gate = 1;
+  if (gate_sums && a.gate_every > 1) {
+    if (a.chunk >= a.gate_every) a.chunk = (a.chunk + a.gate_every - 1) / a.gate_every * a.gate_every;
+    else a.per_gate = (a.gate_every + a.chunk - 1) / a.chunk;
+  }
+  a.parts = a.per_gate > 1 ? a.rows / a.gate_every * a.per_gate : (a.rows + a.chunk - 1) / a.chunk;
+}
+
+template <typename T, int TPR, bool RAGGED>
+static void residual_norm_backward_sized(const ResArgs& a, hipStream_t st) {
+  const bool post = a.slot[kSumPostW] >= 0 || a.slot[kSumPostB] >= 0;
+  const bool any = post || a.gpart || a.slot[kSumPreW] >= 0 || a.slot[kSumPreB] >= 0;
+  const dim3 grid((unsigned)a.parts), block(res_threads(TPR));
+#define PSGDK_RES(SUMS, args) \
+  hipLaunchKernelGGL((residual_norm_backward_kernel<T, TPR, SUMS, RAGGED>), grid, block, 0, st, args)
+  if (!any) {
+    PSGDK_RES(0, a);
+  } else if (!post && !a.gpart) {
+    PSGDK_RES(1, a);
+  } else if constexpr (TPR == 1024) {  // no registers for all sums: the branch's come from a second pass
+    ResArgs q = a;
+    q.dx = q.df = q.dgate = nullptr;
+    q.slot[kSumPreW] = q.slot[kSumPreB] = -1;
+    PSGDK_RES(1, a);
+    PSGDK_RES(6, q);
+  } else if (!a.gpart) {
+    PSGDK_RES(3, a);
+  } else if (!post) {
+    PSGDK_RES(5, a);
+  } else {
+    PSGDK_RES(7, a);
+  }
+#undef PSGDK_RES
+}
+template <typename T, bool RAGGED>
+static void residual_norm_backward_rows(const ResArgs& a, hipStream_t st) {
+  if (a.d <= 512) residual_norm_backward_sized<T, 64, RAGGED>(a, st);
+  else if (a.d <= 1024) residual_norm_backward_sized<T, 128, RAGGED>(a, st);
+  else if (a.d <= 2048) residual_norm_backward_sized<T, 256, RAGGED>(a, st);
+  else if (a.d <= 4096) residual_norm_backward_sized<T, 512, RAGGED>(a, st);
+  else if constexpr (!RAGGED) residual_norm_backward_sized<T, 1024, false>(a, st);
+}
+template <typename T>
+static hipError_t residual_norm_backward_t(const ResArgs& a, hipStream_t st) {
+  if (!res_wide(a.d)) {
+    if (a.d % VE) residual_norm_backward_rows<T, true>(a, st);
+    else residual_norm_backward_rows<T, false>(a, st);
+  } else {
+    hipLaunchKernelGGL(residual_norm_backward_wide_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+    bool any = a.gpart != nullptr;
+    for (int k = 0; k < 4; ++k) any = any || a.slot[k] >= 0;
+    const int strips = (a.d + 256 * VE - 1) / (256 * VE);
+    if (any)
+      hipLaunchKernelGGL(residual_norm_columns_kernel<T>, dim3((unsigned)(a.parts * strips)), dim3(256), 0, st, a, strips);
+  }
+  return hipGetLastError();
+}
+hipError_t residual_norm_backward_launch(const ResArgs& a, hipStream_t st) {
+  return a.dt == 1 ? residual_norm_backward_t<bf16_t>(a, st) : residual_norm_backward_t<float>(a, st);
+}
+
+hipError_t column_sums_launch(const ColumnSums& s, hipStream_t st) {
+  long long groups = 0;
+  for (int k = 0; k < s.n; ++k) groups += s.e[k].groups;
+  if (!groups) return hipSuccess;
+  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)(groups * ((s.d + 63) / 64))), dim3(1024), 0, st, s);
+  return hipGetLastError();
+}
+
+}  // namespace psgdk

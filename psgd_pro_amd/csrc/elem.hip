@@ -1,6 +1,7 @@
 // Elementwise and small reduction kernels of the PSGD-Kron step. All reductions are deterministic: fixed-order
 // partial sums, no float atomics.
 #include "elem.h"
+#include "philox.h"
 
 namespace psgdk {
 
@@ -76,31 +77,12 @@ __device__ __forceinline__ void ew_range8(long long total, int blocks_per, long 
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Standard normals from a counter-based generator: Philox4x32 with 10 rounds (Salmon, Moraes, Dror and Shaw,
-// "Parallel random numbers: as easy as 1, 2, 3", SC 2011), key = the 64-bit seed, counter = (block b of four
-// outputs, as two 32-bit words; the 64-bit stream id as two words). A round multiplies words 0 and 2 by the
-// published constants 0xD2511F53 and 0xCD9E8D57, keeps the low halves and XORs the high halves with words 1, 3 and
-// the key; the key is bumped by the Weyl increments 0x9E3779B9 and 0xBB67AE85 between rounds. Each word x gives
+// Standard normals from the Philox4x32-10 generator (philox.h), key = the 64-bit seed, counter = (block b of four
+// outputs, as two 32-bit words; the 64-bit stream id as two words). Each word x gives
 // the uniform u = (floor(x / 256) + 1/2) 2^-24 in (0, 1), exact in fp32 (so ln u keeps its precision next to 1),
 // and each pair (u0, u1) two normals by the Box-Muller transform,
 // sqrt(-2 ln u0) (cos 2 pi u1, sin 2 pi u1). Output b covers elements 4 b .. 4 b + 3 (fp32, or bf16 rounded from
 // the fp32 value).
-__device__ __forceinline__ void philox4x32_10(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    // one 32 x 32 -> 64-bit product per word (one v_mad_u64_u32) rather than separate low and high multiplies
-    const uint64_t p0 = (uint64_t)0xD2511F53u * c[0], p1 = (uint64_t)0xCD9E8D57u * c[2];
-    const uint32_t lo0 = (uint32_t)p0, hi0 = (uint32_t)(p0 >> 32);
-    const uint32_t lo1 = (uint32_t)p1, hi1 = (uint32_t)(p1 >> 32);
-    c[0] = hi1 ^ c[1] ^ k0;
-    c[1] = lo1;
-    c[2] = hi0 ^ c[3] ^ k1;
-    c[3] = lo0;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-}
-
 // The four normals of output block blk (elements 4 blk .. 4 blk + 3) as normal_fill_kernel computes them, before
 // the storage rounding.
 __device__ __forceinline__ void philox_normals4(unsigned long long blk, uint32_t k0, uint32_t k1, uint32_t s0,

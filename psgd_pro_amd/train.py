@@ -1,0 +1,351 @@
+"""Operators of the training step in front of the optimizer, on the HIP kernels (include/psgdk.h, level 3).
+
+    linear_cross_entropy   the loss of a language model's head from its inputs and vocabulary matrix, logits never kept
+    residual_norm          the residual sum between two blocks of a transformer with its norms, gate, scale and dropout
+    dropout                dropout from the library's counter-based generator, mask never stored
+
+All take CUDA (HIP) tensors in float32 or bfloat16, run on torch's current stream and differentiate once through
+autograd. No counterparts in the reference, which leaves the model to torch.
+"""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+__all__ = ["dropout", "linear_cross_entropy", "residual_norm"]
+
+_NORMS = {None: L.NORM_NONE, "rms": L.NORM_RMS, "layer": L.NORM_LAYER}
+
+
+def _check(t, name, like=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name}: psgd_pro_amd ops take CUDA (HIP) tensors; got " +
+                           (f"a tensor on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{name}: float32 or bfloat16 expected, got {t.dtype}")
+    if like is not None and t.device != like.device:
+        raise RuntimeError(f"{name}: on {t.device}, the input is on {like.device}")
+
+
+def _rows(t):
+    """t as rows of its last dimension, contiguous inside a row (a view where its strides allow)."""
+    r = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
+        r = r.contiguous()
+    return r
+
+
+def _ld(r):
+    return r.stride(0) if r.shape[0] > 1 else r.shape[1]
+
+
+class _on:
+    """The tensor's device made current for the launches (nothing to do where it is)."""
+
+    def __init__(self, t):
+        self.ctx = None if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *e):
+        if self.ctx is not None:
+            self.ctx.__exit__(*e)
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _seed(seed, p):
+    """The generator's 64-bit key; with no seed given, one drawn from torch's CPU generator (as KronWhiten's)."""
+    if seed is None:
+        return int(torch.randint(2 ** 62, ())) if p else 0
+    return int(seed) & (2 ** 64 - 1)
+
+
+def _check_p(p):
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p = {p}: must be in 0..1")
+
+
+# -- dropout ----------------------------------------------------------------------------------------------------------
+
+
+def _dropout_call(x, p, seed, stream):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.numel():
+        r = _rows(x)
+        with _on(x):
+            L.check(L.lib().psgdk_dropout(r.shape[0], r.shape[1], L.dtype_code(x.dtype), r.data_ptr(), _ld(r),
+                                          y.data_ptr(), r.shape[1], p, seed, stream, L.stream_of(x)))
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, stream):
+        ctx.args = p, seed, stream
+        return _dropout_call(x, p, seed, stream)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return _dropout_call(g, *ctx.args), None, None, None
+
+
+def dropout(x, p, *, seed=None, stream=0):
+    """x with each element set to 0 with probability p and the others scaled by 1 / (1 - p).
+
+    p is taken in steps of 2^-16: with t = round(65536 p), element (i, c) of x seen as rows of its last dimension d is
+    kept where the 16-bit number c % 8 of block i ceil(d / 8) + c / 8 of the Philox4x32-10 sequence of (seed, stream) is
+    at least t, and scaled by 65536 / (65536 - t). The mask is made again in the backward pass. The same (seed, stream)
+    and shape give the same mask; seed None draws one from torch's CPU generator. Give each call of a step its own
+    stream (a layer's number, say) under one seed."""
+    _check(x, "x")
+    _check_p(p)
+    if x.dim() == 0:
+        raise RuntimeError("x: at least one dimension expected")
+    seed, stream = _seed(seed, p), int(stream) & (2 ** 64 - 1)
+    if _wants_grad(x):
+        return _Dropout.apply(x, float(p), seed, stream)
+    return _dropout_call(x, float(p), seed, stream)
+
+
+# -- residual_norm ----------------------------------------------------------------------------------------------------
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _res_block(x, f, gate, pw, pb, qw, qb, opt):
+    """psgdk_residual_norm_t of the inputs, and the (possibly copied) tensors it points to."""
+    pre, post, scale, eps, p, seed, stream, gate_rows = opt
+    xr = _rows(x)
+    fr = None if f is None else _rows(f)
+    gr = None if gate is None else _rows(gate)
+    w = [None if t is None else t.contiguous() for t in (pw, pb, qw, qb)]
+    a = L.ResidualNorm()
+    a.rows, a.d = xr.shape
+    a.dtype = L.dtype_code(x.dtype)
+    a.pre, a.post, a.eps, a.scale, a.p, a.seed, a.stream_id, a.gate_rows = pre, post, eps, scale, p, seed, stream, gate_rows
+    a.x, a.ldx = xr.data_ptr(), _ld(xr)
+    if fr is not None:
+        a.f, a.ldf = fr.data_ptr(), _ld(fr)
+    if gr is not None:
+        a.gate, a.ldgate, a.gate_dtype = gr.data_ptr(), _ld(gr), L.dtype_code(gate.dtype)
+    a.pre_w, a.pre_b, a.post_w, a.post_b = (_ptr(t) for t in w)
+    some = next((t for t in w if t is not None), None)
+    a.w_dtype = L.F32 if some is None else L.dtype_code(some.dtype)
+    return a, (xr, fr, gr, w)
+
+
+def _res_forward(x, f, gate, pw, pb, qw, qb, opt, stats):
+    a, keep = _res_block(x, f, gate, pw, pb, qw, qb, opt)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if f is not None else None
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if opt[0] else None
+    st = torch.empty(a.rows, 4, device=x.device) if stats else None
+    a.y, a.ldy, a.h, a.ldh, a.stats = _ptr(y), a.d, _ptr(h), a.d, _ptr(st)
+    if x.numel() and (y is not None or h is not None):
+        with _on(x):
+            L.check(L.lib().psgdk_residual_norm(C.byref(a), L.stream_of(x)))
+    return y, h, st
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, gate, pw, pb, qw, qb, opt):
+        ctx.set_materialize_grads(False)
+        y, h, st = _res_forward(x, f, gate, pw, pb, qw, qb, opt, True)
+        ctx.opt = opt
+        ctx.save_for_backward(x, f, gate, pw, pb, qw, qb, st)
+        if y is None:
+            y = x.view_as(x)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        x, f, gate, pw, pb, qw, qb, st = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        a, keep = _res_block(x, f, gate, pw, pb, qw, qb, ctx.opt)
+        a.stats = _ptr(st)
+        g = L.ResidualNormGrads()
+        for name, t in (("dy", dy), ("dh", dh)):
+            if t is not None:
+                r = _rows(t)
+                keep += (r,)
+                setattr(g, name, r.data_ptr())
+                setattr(g, "ld" + name, _ld(r))
+        outs = [None] * 8
+        for k, (name, like) in enumerate((("dx", x), ("df", f), ("dgate", gate), ("dpre_w", pw), ("dpre_b", pb),
+                                          ("dpost_w", qw), ("dpost_b", qb))):
+            if like is None or not need[k]:
+                continue
+            outs[k] = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+            setattr(g, name, outs[k].data_ptr())
+            if k < 3:
+                setattr(g, "ld" + name, like.shape[-1])
+        if not x.numel():
+            for t in outs:
+                if t is not None:
+                    t.zero_()
+        else:
+            with _on(x):
+                L.call_ws(L.lib().psgdk_residual_norm_backward, C.byref(a), C.byref(g), ws=L.Workspace(),
+                          device=x.device, stream=L.stream_of(x))
+        return tuple(outs)
+
+
+def _gate_rows(gate, x):
+    """Rows of the gate: its leading dimensions are x's first ones, then ones (fewer dimensions: ones in front)."""
+    lead, xs = tuple(gate.shape[:-1]), tuple(x.shape[:-1])
+    bad = f"gate: shape {tuple(gate.shape)} does not go with {tuple(x.shape)} (its last dimension, and its first ones or ones)"
+    if gate.dim() == 0 or gate.shape[-1] != x.shape[-1] or len(lead) > len(xs):
+        raise RuntimeError(bad)
+    lead = (1,) * (len(xs) - len(lead)) + lead
+    n = 0
+    while n < len(xs) and lead[n] == xs[n]:
+        n += 1
+    if any(v != 1 for v in lead[n:]):
+        raise RuntimeError(bad)
+    rows = 1
+    for v in lead:
+        rows *= v
+    return rows
+
+
+def residual_norm(x, f=None, *, pre="rms", post=None, pre_weight=None, pre_bias=None, post_weight=None, post_bias=None,
+                  gate=None, scale=1.0, eps=1e-6, p=0.0, seed=None, stream=0):
+    """(y, h): the residual sum after a block of a transformer and the next block's normalised input, in one pass.
+
+        u = Npost(f);  b = dropout(u, p, seed, stream);  y = x + scale * gate * b;  h = Npre(y)
+
+    x is the residual stream (any shape, norms over the last dimension), f the block's output (None: y is x, as in front
+    of the first block). pre and post choose the norms: "rms" (v / sqrt(mean v^2 + eps) * weight), "layer"
+    ((v - mean) / sqrt(var + eps) * weight + bias) or None (pre None: h is None); weights and biases may be absent and may
+    be float32 beside bfloat16 activations. gate has x's last dimension, and in front of it x's first dimensions followed
+    by ones: (d,) scales channels, (batch, 1, d) each sequence's, x's own shape every element. h is made from the sum
+    before its rounding. Differentiable in x, f, gate and the norms' parameters."""
+    _check(x, "x")
+    _check_p(p)
+    if x.dim() == 0:
+        raise RuntimeError("x: at least one dimension expected")
+    d = x.shape[-1]
+    for name, kind in (("pre", pre), ("post", post)):
+        if kind not in _NORMS:
+            raise ValueError(f"{name} = {kind!r}: 'rms', 'layer' or None")
+    if f is None and (post is not None or gate is not None or p):
+        raise ValueError("post, gate and p need f")
+    if pre is None and f is None:
+        raise ValueError("nothing to compute: neither f nor a norm")
+    if f is not None:
+        _check(f, "f", x)
+        if f.shape != x.shape or f.dtype != x.dtype:
+            raise RuntimeError(f"f: {tuple(f.shape)} {f.dtype} expected as x, {tuple(x.shape)} {x.dtype}")
+    par = (pre_weight, pre_bias, post_weight, post_bias)
+    for name, t, kinds, kind in (("pre_weight", pre_weight, ("rms", "layer"), pre), ("pre_bias", pre_bias, ("layer",), pre),
+                                 ("post_weight", post_weight, ("rms", "layer"), post),
+                                 ("post_bias", post_bias, ("layer",), post)):
+        if t is None:
+            continue
+        _check(t, name, x)
+        if kind not in kinds:
+            raise ValueError(f"{name}: the norm {kind!r} has none")
+        if t.shape != (d,):
+            raise RuntimeError(f"{name}: shape ({d},) expected, got {tuple(t.shape)}")
+        if t.dtype != next(q for q in par if q is not None).dtype:
+            raise RuntimeError("the norms' weights and biases share one dtype")
+    rows = 0
+    if gate is not None:
+        _check(gate, "gate", x)
+        rows = _gate_rows(gate, x)
+    opt = (_NORMS[pre], _NORMS[post], float(scale), float(eps), float(p), _seed(seed, p), int(stream) & (2 ** 64 - 1), rows)
+    if _wants_grad(x, f, gate, *par):
+        return _ResidualNorm.apply(x, f, gate, *par, opt)
+    y, h, _ = _res_forward(x, f, gate, *par, opt, False)
+    return (x if y is None else y), h
+
+
+# -- linear_cross_entropy -----------------------------------------------------------------------------------------------
+
+
+def _lce_call(x, w, target, ignore, row_weight, mean, want_x, want_w):
+    """(losses, their weighted sum, dx, dw)"""
+    xr, wr, t = _rows(x), _rows(w), target.reshape(-1).contiguous()
+    n, d = xr.shape
+    loss = torch.empty(n, device=x.device)
+    total = torch.empty((), device=x.device)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
+    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if want_w else None
+    if not n:
+        return loss, total.zero_(), dx, None if dw is None else dw.zero_()
+    with _on(x):
+        L.call_ws(L.lib().psgdk_linear_cross_entropy, n, d, wr.shape[0], L.dtype_code(x.dtype), xr.data_ptr(), _ld(xr),
+                  wr.data_ptr(), _ld(wr), t.data_ptr(), ignore, _ptr(row_weight), int(mean), loss.data_ptr(),
+                  total.data_ptr(), _ptr(dx), d, _ptr(dw), d, ws=L.Workspace(), device=x.device, stream=L.stream_of(x))
+    return loss, total, dx, dw
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    """A reduced loss has its gradients ready in the forward pass (they cost one third less than with the logits computed
+    again) and hands them over in the backward pass, scaled by the loss's gradient; where the graph is kept for another
+    backward pass they are computed again. The losses of single rows need their gradients' weights first."""
+
+    @staticmethod
+    def forward(ctx, x, w, target, ignore, reduction):
+        reduced = reduction != "none"
+        need = ctx.needs_input_grad
+        loss, total, dx, dw = _lce_call(x, w, target, ignore, None, reduction == "mean", reduced and need[0],
+                                        reduced and need[1])
+        ctx.save_for_backward(x, w, target)
+        ctx.args = ignore, reduction
+        ctx.grads = (dx, dw) if reduced else None
+        return total if reduced else loss.view(target.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, target = ctx.saved_tensors
+        ignore, reduction = ctx.args
+        need = ctx.needs_input_grad
+        if reduction == "none":
+            g = g.reshape(-1).float().contiguous()
+            return (*_lce_call(x, w, target, ignore, g, False, need[0], need[1])[2:], None, None, None)
+        grads, ctx.grads = ctx.grads, None
+        if grads is None:
+            grads = _lce_call(x, w, target, ignore, None, reduction == "mean", need[0], need[1])[2:]
+        ts = [t for t in grads if t is not None and t.numel()]
+        if ts:
+            g = g.float()
+            n = (C.c_int64 * len(ts))(*[t.numel() for t in ts])
+            with _on(x):
+                L.check(L.lib().psgdk_scale_by(len(ts), n, L.dtype_code(x.dtype), L.ptrs(ts), g.data_ptr(), L.stream_of(x)))
+        return (*grads, None, None, None)
+
+
+def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the logits x weight^T, which are never kept: x (..., d), weight (vocabulary, d) in x's
+    dtype, target (...) of int64. Rows whose target is ignore_index have no loss and no gradient, whatever x holds there;
+    another target outside the vocabulary makes the loss NaN. reduction: "mean" over the rows not ignored (0 where there
+    are none), "sum", or "none" (losses in target's shape). Losses are float32; the gradients of x and weight have their
+    dtype."""
+    _check(x, "x")
+    _check(weight, "weight", x)
+    if weight.dtype != x.dtype:
+        raise RuntimeError(f"weight: {x.dtype} expected as x, got {weight.dtype}")
+    if x.dim() == 0 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or not weight.numel():
+        raise RuntimeError(f"x {tuple(x.shape)}, weight {tuple(weight.shape)}: (..., d) and (vocabulary, d) expected")
+    if target.dtype != torch.int64 or target.device != x.device or target.shape != x.shape[:-1]:
+        raise RuntimeError(f"target: int64 {tuple(x.shape[:-1])} on {x.device} expected, got {target.dtype} "
+                           f"{tuple(target.shape)} on {target.device}")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction = {reduction!r}: 'mean', 'sum' or 'none'")
+    if _wants_grad(x, weight):
+        return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), reduction)
+    loss, total, _, _ = _lce_call(x, weight, target, int(ignore_index), None, reduction == "mean", False, False)
+    return loss.view(target.shape) if reduction == "none" else total
