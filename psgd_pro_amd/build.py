@@ -21,7 +21,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpsgdk.so")
-SOURCES = ["gemm_cv.hip", "gemm_bf16.hip", "gemm_small.hip", "nlb.hip", "elem.hip", "block.hip", "xent.hip", "capi.cpp",
+SOURCES = ["gemm_cv.hip", "gemm_bf16.hip", "gemm_small.hip", "nlb.hip", "elem.hip", "block.hip", "xent.hip", "xgemm.hip", "capi.cpp",
            "train_capi.cpp", "noalloc.hip", "measure.hip"]
 HOST_SOURCES = ["capi.cpp", "train_capi.cpp"]  # the C ABI's host code, which the sanitizer build instruments
 ARCH = os.environ.get("PSGDK_ARCH", "gfx950")

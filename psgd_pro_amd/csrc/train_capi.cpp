@@ -137,8 +137,256 @@ int res_args(const psgdk_residual_norm_t* q, ResArgs& a) {
   return PSGDK_OK;
 }
 
-// Rows whose logits (fp32) are in memory at once: up to 1 GiB of them.
+// Rows whose logits (4 bytes each in fp32, 2 on the bf16 path) are in memory at once: up to 1 GiB of them.
 constexpr int64_t kLogitBytes = (int64_t)1 << 30;
+// 256 rows of a product's operand stay within 32-bit byte offsets
+constexpr int64_t kMaxVocab = (int64_t)1 << 22;
+
+struct Lce {
+  int64_t rows, d, vocab;
+  int dtype;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const int64_t* target;
+  int64_t ignore;
+  const float* row_weight;
+  int mean;
+  float *loss, *mean_loss;
+  void* dx;
+  int64_t lddx;
+  void* dw;
+  int64_t lddw;
+  void* ws;
+  size_t* ws_bytes;
+  hipStream_t st;
+};
+
+// The workspace's size (ws null: PSGDK_OK with `done` set) or the check of the caller's.
+int lce_ws(const Lce& p, const Ws& m, bool& done) {
+  done = !p.ws;
+  if (done) *p.ws_bytes = m.off;
+  else if (*p.ws_bytes < m.off) return fail(PSGDK_EWORKSPACE, "workspace %zu < %zu bytes", *p.ws_bytes, m.off);
+  return PSGDK_OK;
+}
+int lce_pointers(const Lce& p) {
+  PSGDK_TRY(check_rows(p.x, p.ldx, p.d, "x"));
+  PSGDK_TRY(check_rows(p.w, p.ldw, p.d, "w"));
+  if (!p.target || !p.loss) return fail(PSGDK_EINVAL, "target, loss: null device pointer");
+  if (p.dx) PSGDK_TRY(check_rows(p.dx, p.lddx, p.d, "dx"));
+  if (p.dw) PSGDK_TRY(check_rows(p.dw, p.lddw, p.d, "dw"));
+  return PSGDK_OK;
+}
+int lce_mean(const Lce& p, const float* weight) {
+  if (!p.mean_loss) return PSGDK_OK;
+  return hip_check(xent_mean_launch(p.loss, p.row_weight, weight, p.rows, p.mean_loss, p.st), "cross entropy mean");
+}
+
+// float32: the logits of a slab of rows by the converting engine, a pass over them, and its products with W and x.
+int lce_f32(const Lce& p) {
+  const bool grad = p.dx || p.dw;
+  const int64_t ldz = (p.vocab + 3) / 4 * 4, slab = std::min(p.rows, std::max<int64_t>(1, kLogitBytes / 4 / ldz));
+  Ws m(p.ws);
+  float* const weight = m.take<float>(1);
+  float* const z = m.take<float>(slab * ldz);
+  float* const xm = m.take<float>(slab * p.d);
+  bool done;
+  PSGDK_TRY(lce_ws(p, m, done));
+  if (done) return PSGDK_OK;
+  PSGDK_TRY(lce_pointers(p));
+  PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
+  for (int64_t r0 = 0; r0 < p.rows; r0 += slab) {
+    const int64_t n = std::min(slab, p.rows - r0);
+    // an ignored row's x must reach nothing: 0 times an infinity is not 0, and a product scales its operands together
+    PSGDK_TRY(hip_check(xent_mask_rows_launch(static_cast<const float*>(p.x) + r0 * p.ldx, p.ldx, xm, p.target + r0,
+                                              p.ignore, n, (int)p.d, p.st), "mask rows"));
+    const void *zc = z, *xc = xm;
+    const psgdk_stream_t st = (psgdk_stream_t)p.st;
+    PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 1, n, p.vocab, p.d, 1.f, PSGDK_F32, PSGDK_F32, 1, &xc, p.d, &p.w, p.ldw, 0.f,
+                         &z, ldz, st));
+    XentRowsArgs a{};
+    a.z = z;
+    a.ldz = ldz;
+    a.rows = n;
+    a.vocab = (int)p.vocab;
+    a.grad = grad;
+    a.ignore = p.ignore;
+    a.target = p.target + r0;
+    a.row_weight = p.row_weight ? p.row_weight + r0 : nullptr;
+    a.weight = weight;
+    a.loss = p.loss + r0;
+    PSGDK_TRY(hip_check(xent_rows_launch(a, p.st), "cross entropy rows"));
+    if (p.dx) {
+      float* out = static_cast<float*>(p.dx) + r0 * p.lddx;
+      PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, p.vocab, 1.f, PSGDK_F32, PSGDK_F32, 1, &zc, ldz, &p.w, p.ldw,
+                           0.f, &out, p.lddx, st));
+    }
+    if (p.dw) {
+      float* out = static_cast<float*>(p.dw);
+      PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 1, 0, p.vocab, p.d, n, 1.f, PSGDK_F32, PSGDK_F32, 1, &zc, ldz, &xc, p.d,
+                           r0 ? 1.f : 0.f, &out, p.lddw, st));
+    }
+  }
+  return lce_mean(p, weight);
+}
+
+// bfloat16, a few rows, losses only
+int lce_few(const Lce& p) {
+  XentFewArgs a{};
+  a.rows = (int)p.rows;
+  a.d = (int)p.d;
+  a.vocab = (int)p.vocab;
+  a.wgs = xent_few_wgs(a.vocab);
+  Ws m(p.ws);
+  float* const weight = m.take<float>(1);
+  a.zt = m.take<float>(64);
+  a.part = m.take<float2>((size_t)a.wgs * 64);
+  bool done;
+  PSGDK_TRY(lce_ws(p, m, done));
+  if (done) return PSGDK_OK;
+  PSGDK_TRY(lce_pointers(p));
+  a.x = static_cast<const bf16_t*>(p.x);
+  a.ldx = p.ldx;
+  a.w = static_cast<const bf16_t*>(p.w);
+  a.ldw = p.ldw;
+  a.ignore = p.ignore;
+  a.target = p.target;
+  a.loss = p.loss;
+  PSGDK_TRY(hip_check(xent_few_launch(a, p.st), "cross entropy of a few rows"));
+  if (!p.mean_loss) return PSGDK_OK;
+  PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
+  return lce_mean(p, weight);
+}
+
+// bfloat16: the logits of a slab of rows as 16-bit codes with the sums of their exponentials (one product), a pass that
+// makes them the logits' gradients, and the products of those with W and x.
+int lce_bf16(const Lce& p) {
+  const bool grad = p.dx || p.dw;
+  const int64_t ld = (p.d + 7) / 8 * 8, ldq = (p.vocab + 63) / 64 * 64;
+  int64_t slab = std::max<int64_t>(kXgRows, kLogitBytes / 2 / ldq / kXgRows * kXgRows);
+  if (slab >= p.rows) slab = p.rows;
+  const int64_t blocks = (slab + kXgRows - 1) / kXgRows, parts = 2 * ((p.vocab + 255) / 256);
+  const bool copy_w = p.d % 8 != 0 || p.ldw % 8 != 0 || p.ldw > kMaxVocab || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
+  const bool sum_w = p.dw && slab < p.rows;
+  const int splits = p.dx ? xgemm_splits(p.d, slab, p.vocab) : 1;
+  Ws m(p.ws);
+  float* const weight = m.take<float>(1);
+  XentBf16Args a{};
+  a.xm = m.take<bf16_t>(slab * ld);
+  a.zt = m.take<float>(slab);
+  a.ref = m.take<float>(slab);
+  a.sum = m.take<float>(slab);
+  a.col = m.take<int>(slab);
+  a.redo = m.take<int>(1 + blocks);
+  a.mark = m.take<int>(blocks);
+  float* const sums = m.take<float>(slab * parts);
+  bf16_t* const wp = m.take<bf16_t>(copy_w ? p.vocab * ld : 0);
+  a.q = m.take<int16_t>(grad ? slab * ldq : 0);
+  float* const dxp = m.take<float>(splits > 1 ? splits * slab * ld : 0);
+  float* const dwf = m.take<float>(sum_w ? p.vocab * ld : 0);
+  bool done;
+  PSGDK_TRY(lce_ws(p, m, done));
+  if (done) return PSGDK_OK;
+  PSGDK_TRY(lce_pointers(p));
+  PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
+  const bf16_t* w = static_cast<const bf16_t*>(p.w);
+  int64_t ldw = p.ldw;
+  if (copy_w) {
+    PSGDK_TRY(hip_check(pad_rows_launch(w, ldw, wp, ld, p.vocab, (int)p.d, p.st), "cross entropy copy"));
+    w = wp;
+    ldw = ld;
+  }
+  a.d = (int)p.d;
+  a.vocab = (int)p.vocab;
+  a.parts = (int)parts;
+  a.ignore = p.ignore;
+  a.w = w;
+  a.ldw = ldw;
+  a.ldx = p.ldx;
+  a.ldm = ld;
+  a.ldq = ldq;
+  a.sums = sums;
+  const float* const alpha = p.mean ? weight : nullptr;
+  for (int64_t r0 = 0; r0 < p.rows; r0 += slab) {
+    const int64_t n = std::min(slab, p.rows - r0);
+    a.rows = n;
+    a.target = p.target + r0;
+    a.row_weight = p.row_weight ? p.row_weight + r0 : nullptr;
+    a.x = static_cast<const bf16_t*>(p.x) + r0 * p.ldx;
+    a.loss = p.loss + r0;
+    PSGDK_TRY(hip_check(xent_prep_launch(a, p.st), "cross entropy rows"));
+    XgArgs g{};
+    g.M = (int)p.vocab;
+    g.N = (int)n;
+    g.K = (int)ld;
+    g.A = w;
+    g.lda = ldw;
+    g.B = a.xm;
+    g.ldb = ld;
+    g.splits = 1;
+    g.q = grad ? a.q : nullptr;
+    g.ldo = ldq;
+    g.ref = a.ref;
+    g.target = a.col;
+    g.sums = sums;
+    PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, p.st), "logits"));
+    PSGDK_TRY(hip_check(xent_join_launch(a, 0, p.st), "cross entropy sums"));
+    // rows whose reference was too low: their maximum, then their blocks once more (nothing where there are none)
+    XgArgs t = g;
+    t.q = nullptr;
+    t.max_only = 1;
+    t.tops = sums;  // of whole blocks, which all get their sums again
+    t.redo = g.redo = a.redo;
+    PSGDK_TRY(hip_check(xgemm_launch(t, XG_LOGITS, p.st), "largest logits"));
+    PSGDK_TRY(hip_check(xent_top_launch(a, p.st), "largest logits of rows"));
+    PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, p.st), "logits again"));
+    PSGDK_TRY(hip_check(xent_join_launch(a, 1, p.st), "cross entropy sums again"));
+    if (!grad) continue;
+    PSGDK_TRY(hip_check(xent_dz_launch(a, p.st), "logits' gradients"));
+    if (p.dx) {
+      bf16_t* const out = static_cast<bf16_t*>(p.dx) + r0 * p.lddx;
+      XgArgs x{};
+      x.M = (int)p.d;
+      x.N = (int)n;
+      x.K = (int)ldq;
+      x.A = w;
+      x.lda = ldw;
+      x.B = reinterpret_cast<const bf16_t*>(a.q);
+      x.ldb = ldq;
+      x.splits = splits;
+      x.out = out;
+      x.ldo = splits > 1 ? ld : p.lddx;
+      x.alpha = alpha;
+      x.outf = splits > 1 ? dxp : nullptr;
+      x.kreal = (int)p.vocab;
+      PSGDK_TRY(hip_check(xgemm_launch(x, XG_DX, p.st), "dx"));
+      if (splits > 1)
+        PSGDK_TRY(hip_check(to_bf16_rows_launch(dxp, splits, ld, alpha, out, p.lddx, n, (int)p.d, p.st), "dx sums"));
+    }
+    if (p.dw) {
+      XgArgs x{};
+      x.M = (int)p.d;
+      x.N = (int)p.vocab;
+      x.K = (int)n;
+      x.A = a.xm;
+      x.lda = ld;
+      x.B = reinterpret_cast<const bf16_t*>(a.q);
+      x.ldb = ldq;
+      x.splits = 1;
+      x.out = static_cast<bf16_t*>(p.dw);
+      x.ldo = sum_w ? ld : p.lddw;
+      x.alpha = alpha;
+      x.outf = sum_w ? dwf : nullptr;
+      x.accumulate = r0 != 0;
+      PSGDK_TRY(hip_check(xgemm_launch(x, XG_DW, p.st), "dw"));
+    }
+  }
+  if (sum_w)
+    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, 1, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab, (int)p.d, p.st),
+                        "dw sums"));
+  return lce_mean(p, weight);
+}
 
 }  // namespace
 
@@ -258,68 +506,15 @@ int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype
   PSGDK_TRY(check_dt(dtype, "dtype"));
   PSGDK_TRY(check_size(rows, 1, (int64_t)1 << 30, "rows"));
   PSGDK_TRY(check_size(d, 1, (int64_t)1 << 20, "d"));
-  PSGDK_TRY(check_size(vocab, 1, (int64_t)1 << 28, "vocab"));
+  PSGDK_TRY(check_size(vocab, 1, kMaxVocab, "vocab"));
   if (!ws_bytes) return fail(PSGDK_EINVAL, "ws_bytes is null");
   if (mean && row_weight) return fail(PSGDK_EINVAL, "mean and row_weight exclude each other");
-  const hipStream_t st = (hipStream_t)stream;
-  const bool grad = dx || dw, cvt = dtype == PSGDK_BF16;
-  const int64_t ldz = (vocab + 3) / 4 * 4, slab = std::min(rows, std::max<int64_t>(1, kLogitBytes / 4 / ldz));
-  Ws m(ws);
-  float* const weight = m.take<float>(1);
-  float* const z = m.take<float>(slab * ldz);
-  float* const dxf = m.take<float>(cvt && dx ? slab * d : 0);
-  float* const dwf = m.take<float>(cvt && dw ? vocab * d : 0);
-  char* const xm = m.take<char>(slab * d * esize(dtype));
-  if (!ws) {
-    *ws_bytes = m.off;
-    return PSGDK_OK;
-  }
-  if (*ws_bytes < m.off) return fail(PSGDK_EWORKSPACE, "workspace %zu < %zu bytes", *ws_bytes, m.off);
-  PSGDK_TRY(check_rows(x, ldx, d, "x"));
-  PSGDK_TRY(check_rows(w, ldw, d, "w"));
-  if (!target || !loss) return fail(PSGDK_EINVAL, "target, loss: null device pointer");
-  if (dx) PSGDK_TRY(check_rows(dx, lddx, d, "dx"));
-  if (dw) PSGDK_TRY(check_rows(dw, lddw, d, "dw"));
-  const int prec = dtype == PSGDK_BF16 ? PSGDK_PREC_BF16 : PSGDK_PREC_F32;
-  PSGDK_TRY(hip_check(xent_weight_launch(target, rows, ignore, mean, weight, st), "cross entropy weight"));
-  for (int64_t r0 = 0; r0 < rows; r0 += slab) {
-    const int64_t n = std::min(slab, rows - r0);
-    const void* xs = static_cast<const char*>(x) + r0 * ldx * esize(dtype);
-    // an ignored row's x must reach nothing: 0 times an infinity is not 0, and a product scales its operands together
-    PSGDK_TRY(hip_check(xent_mask_rows_launch(xs, ldx, xm, target + r0, ignore, n, (int)d, dtype, st), "mask rows"));
-    const void *zc = z, *xc = xm;
-    PSGDK_TRY(psgdk_gemm(prec, 0, 1, n, vocab, d, 1.f, dtype, dtype, 1, &xc, d, &w, ldw, 0.f, &z, ldz, stream));
-    XentRowsArgs a{};
-    a.z = z;
-    a.ldz = ldz;
-    a.rows = n;
-    a.vocab = (int)vocab;
-    a.grad = grad;
-    a.ignore = ignore;
-    a.target = target + r0;
-    a.row_weight = row_weight ? row_weight + r0 : nullptr;
-    a.weight = weight;
-    a.loss = loss + r0;
-    PSGDK_TRY(hip_check(xent_rows_launch(a, st), "cross entropy rows"));
-    if (dx) {
-      float* out = cvt ? dxf : static_cast<float*>(dx) + r0 * lddx;
-      PSGDK_TRY(psgdk_gemm(prec, 0, 0, n, d, vocab, 1.f, PSGDK_F32, dtype, 1, &zc, ldz, &w, ldw, 0.f, &out,
-                           cvt ? d : lddx, stream));
-      if (cvt)
-        PSGDK_TRY(hip_check(to_bf16_rows_launch(dxf, d, static_cast<bf16_t*>(dx) + r0 * lddx, lddx, n, (int)d, st),
-                            "cross entropy dx"));
-    }
-    if (dw) {
-      float* out = cvt ? dwf : static_cast<float*>(dw);
-      PSGDK_TRY(psgdk_gemm(prec, 1, 0, vocab, d, n, 1.f, PSGDK_F32, dtype, 1, &zc, ldz, &xc, d, r0 ? 1.f : 0.f, &out,
-                           cvt ? d : lddw, stream));
-    }
-  }
-  if (cvt && dw)
-    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, d, static_cast<bf16_t*>(dw), lddw, vocab, (int)d, st), "cross entropy dw"));
-  if (mean_loss)
-    PSGDK_TRY(hip_check(xent_mean_launch(loss, row_weight, weight, rows, mean_loss, st), "cross entropy mean"));
-  return PSGDK_OK;
+  if (ldx < d || ldw < d || (dx && lddx < d) || (dw && lddw < d)) return fail(PSGDK_ESHAPE, "row stride < d = %lld", (long long)d);
+  const Lce p{rows, d, vocab, dtype, x, ldx, w, ldw, target, ignore, row_weight, mean, loss, mean_loss, dx, lddx, dw, lddw,
+              ws, ws_bytes, (hipStream_t)stream};
+  if (dtype == PSGDK_F32) return lce_f32(p);
+  // to 64 rows the matrix's bytes bound the call, and tiles of 256 rows would be mostly empty
+  return rows <= 64 && !dx && !dw ? lce_few(p) : lce_bf16(p);
 }
 
 int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const float* scale, psgdk_stream_t stream) {

@@ -1,6 +1,7 @@
 // Softmax cross entropy of a vocabulary's logits: argument blocks and launchers.
 #pragma once
 #include "common.h"
+#include "xgemm.h"
 
 namespace psgdk {
 
@@ -25,12 +26,62 @@ struct XentRowsArgs {
 };
 hipError_t xent_rows_launch(const XentRowsArgs& a, hipStream_t st);
 
-// out (bf16, row stride ldo) = in (fp32, row stride ldi), rows x d
-hipError_t to_bf16_rows_launch(const float* in, long long ldi, bf16_t* out, long long ldo, long long rows, int d,
-                               hipStream_t st);
+// The bf16 path's rows. Reference of row i: r = z_t, the logit of its target, so that the target's exponential is 1 and
+// S = sum of the others' gives loss = log(1 + S), softmax_t - 1 = -S / (1 + S). Rows with S over kSumLimit (their loss is
+// over 31) take their largest logit as r instead, and the target's exponential e_t = e^(z_t - r).
+constexpr float kSumLimit = 2.9e13f;  // e^31: every e^(z - r) below it, z - r within the coded logits' range
+struct XentBf16Args {
+  long long rows;
+  int d, vocab, parts;      // parts: sums of a row (2 tiles of m)
+  int64_t ignore;
+  const int64_t* target;
+  const float* row_weight;  // null: 1 (the mean's weight is the products' alpha)
+  const bf16_t* x;
+  const bf16_t* w;
+  long long ldx, ldw, ldm, ldq;
+  bf16_t* xm;               // x with zeros in ignored rows and behind d, row stride ldm
+  float* zt;                // z_t
+  float* ref;               // r
+  float* sum;               // S
+  int* col;                 // the target's column; -1 for an ignored row, vocab for a foreign target (r is NaN then)
+  int* redo;                // number of blocks of kXgRows rows with a row over the limit, and their numbers
+  int* mark;                // of each block: whether it is listed
+  const float* sums;        // or, for xent_top_launch, the largest logits
+  int16_t* q;               // coded logits, replaced by the logits' gradients in bf16
+  float* loss;
+};
+hipError_t xent_prep_launch(const XentBf16Args& a, hipStream_t st);
+// S and loss of each row from its sums; with `again` only of the rows over the limit, else those are listed in redo
+hipError_t xent_join_launch(const XentBf16Args& a, int again, hipStream_t st);
+// r = the largest logit for the rows over the limit
+hipError_t xent_top_launch(const XentBf16Args& a, hipStream_t st);
+// the logits' gradients (without the mean's weight), zeros in ignored rows and behind the vocabulary
+hipError_t xent_dz_launch(const XentBf16Args& a, hipStream_t st);
+// out (bf16, row stride ldo) = alpha[0] sum over s of in[s] (fp32, rows x d, row stride ldi; alpha null: 1)
+hipError_t to_bf16_rows_launch(const float* in, int splits, long long ldi, const float* alpha, bf16_t* out, long long ldo,
+                               long long rows, int d, hipStream_t st);
+// out (row stride ldo) = in with zeros behind d
+hipError_t pad_rows_launch(const bf16_t* in, long long ldi, bf16_t* out, long long ldo, long long rows, int d,
+                           hipStream_t st);
+
+// Losses of up to 64 rows without gradients: the vocabulary matrix is read once, straight into registers.
+struct XentFewArgs {
+  int rows, d, vocab;
+  long long ldx, ldw;
+  const bf16_t* x;
+  const bf16_t* w;
+  int64_t ignore;
+  const int64_t* target;
+  int wgs;
+  float* zt;     // [rows]
+  float2* part;  // [wgs][64]: largest logit, sum of e^(z - largest), the target left out of both
+  float* loss;
+};
+int xent_few_wgs(int vocab);
+hipError_t xent_few_launch(const XentFewArgs& a, hipStream_t st);
 // out (rows of d) = x, with zeros for the rows whose target is `ignore`
-hipError_t xent_mask_rows_launch(const void* x, long long ldx, void* out, const int64_t* target, int64_t ignore,
-                                 long long rows, int d, int dt, hipStream_t st);
+hipError_t xent_mask_rows_launch(const float* x, long long ldx, float* out, const int64_t* target, int64_t ignore,
+                                 long long rows, int d, hipStream_t st);
 
 // x[b][0 .. n[b]) *= *scale (no access where *scale is 1)
 constexpr int kMaxScale = 4;

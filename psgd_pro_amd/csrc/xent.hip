@@ -85,42 +85,346 @@ hipError_t xent_rows_launch(const XentRowsArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-__global__ void __launch_bounds__(256) to_bf16_rows_kernel(const float* in, long long ldi, bf16_t* out, long long ldo,
+__global__ void __launch_bounds__(256) to_bf16_rows_kernel(const float* in, int splits, long long ldi,
+                                                           const float* alpha, bf16_t* out, long long ldo,
                                                            long long rows, int d) {
-  const long long total = rows * d;
+  const float al = alpha ? *alpha : 1.f;
+  const int per = (d + 3) / 4;
+  const long long total = rows * per;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long r = i / d;
-    const int c = (int)(i - r * d);
-    out[r * ldo + c] = f32_to_bf16(in[r * ldi + c]);
+    const long long r = i / per;
+    const int c = (int)(i - r * per) * 4;
+    float v[4] = {};
+    for (int s = 0; s < splits; ++s) {
+      const float* q = in + (s * rows + r) * ldi + c;
+      if (c + 4 <= d) {
+        float t[4];
+        __builtin_memcpy(t, q, 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += t[e];
+      } else {
+        for (int e = 0; c + e < d; ++e) v[e] += q[e];
+      }
+    }
+    bf16_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = f32_to_bf16(al * v[e]);
+    bf16_t* o = out + r * ldo + c;
+    if (c + 4 <= d) __builtin_memcpy(o, h, 8);
+    else
+      for (int e = 0; c + e < d; ++e) o[e] = h[e];
   }
 }
-hipError_t to_bf16_rows_launch(const float* in, long long ldi, bf16_t* out, long long ldo, long long rows, int d,
-                               hipStream_t st) {
-  const long long want = (rows * d + 255) / 256;
-  hipLaunchKernelGGL(to_bf16_rows_kernel, dim3((unsigned)(want > 8192 ? 8192 : want)), dim3(256), 0, st, in, ldi, out,
-                     ldo, rows, d);
+hipError_t to_bf16_rows_launch(const float* in, int splits, long long ldi, const float* alpha, bf16_t* out, long long ldo,
+                               long long rows, int d, hipStream_t st) {
+  const long long want = (rows * ((d + 3) / 4) + 255) / 256;
+  hipLaunchKernelGGL(to_bf16_rows_kernel, dim3((unsigned)(want > 8192 ? 8192 : want)), dim3(256), 0, st, in, splits, ldi,
+                     alpha, out, ldo, rows, d);
   return hipGetLastError();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) xent_mask_rows_kernel(const T* x, long long ldx, T* out, const int64_t* target,
-                                                             int64_t ignore, long long rows, int d) {
+// 8 consecutive values c .. c + 7 of a row of d (zeros behind it) at any element alignment
+__device__ __forceinline__ uint4 ld8_bits(const bf16_t* row, int c, int d) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (c + 8 <= d) {
+    __builtin_memcpy(&v, row + c, 16);
+  } else {
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < d) w[e / 2] |= (uint32_t)row[c + e] << (16 * (e & 1));
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+__device__ __forceinline__ float dot8(uint4 a, uint4 b, float s) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s += __uint_as_float(x[i] << 16) * __uint_as_float(y[i] << 16);
+    s += __uint_as_float(x[i] & 0xffff0000u) * __uint_as_float(y[i] & 0xffff0000u);
+  }
+  return s;
+}
+
+__global__ void __launch_bounds__(256) pad_rows_kernel(const bf16_t* in, long long ldi, bf16_t* out, long long ldo,
+                                                       long long rows, int d) {
+  const int per = (int)(ldo / 8);
+  const long long total = rows * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    *reinterpret_cast<uint4*>(out + r * ldo + c) = ld8_bits(in + r * ldi, c, d);
+  }
+}
+hipError_t pad_rows_launch(const bf16_t* in, long long ldi, bf16_t* out, long long ldo, long long rows, int d,
+                           hipStream_t st) {
+  const long long want = (rows * (ldo / 8) + 1023) / 1024;
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)(want > 16384 ? 16384 : want)), dim3(256), 0, st, in, ldi, out, ldo,
+                     rows, d);
+  return hipGetLastError();
+}
+
+// One wave a row: r = z_t and the row's copy for the products.
+__global__ void __launch_bounds__(256) xent_prep_kernel(const XentBf16Args a) {
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const int64_t t = a.target[row];
+  const bool skip = t == a.ignore, foreign = !skip && (t < 0 || t >= a.vocab);
+  const bf16_t* x = a.x + row * a.ldx;
+  const bf16_t* w = a.w + (skip || foreign ? 0 : t) * a.ldw;
+  float s = 0.f;
+  for (int c = lane * 8; c < a.ldm; c += 512) {
+    uint4 v = ld8_bits(x, c, a.d);
+    if (skip) v = make_uint4(0, 0, 0, 0);
+    else s = dot8(v, ld8_bits(w, c, a.d), s);
+    *reinterpret_cast<uint4*>(a.xm + row * a.ldm + c) = v;
+  }
+  s = wave_sum(s);
+  if (lane) return;
+  if (foreign) s = NAN;
+  a.zt[row] = s;
+  a.ref[row] = s;
+  a.col[row] = skip ? -1 : foreign ? a.vocab : (int)t;
+  if (row % kXgRows == 0) a.mark[row / kXgRows] = 0;
+  if (row == 0) a.redo[0] = 0;
+}
+hipError_t xent_prep_launch(const XentBf16Args& a, hipStream_t st) {
+  hipLaunchKernelGGL(xent_prep_kernel, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// One wave a row. A NaN sum is under no limit and stays.
+__global__ void __launch_bounds__(256) xent_join_kernel(const XentBf16Args a, int again) {
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.rows || (again && (a.redo[0] == 0 || !(a.sum[row] > kSumLimit)))) return;
+  float s = 0.f;
+  for (int i = lane; i < a.parts; i += 64) s += a.sums[row * a.parts + i];
+  s = wave_sum(s);
+  if (lane) return;
+  a.sum[row] = s;
+  const float under = a.zt[row] - a.ref[row];  // 0 where r is the target's logit
+  a.loss[row] = a.col[row] < 0 ? 0.f : under == 0.f ? log1pf(s) : logf(s + expf(under)) - under;
+  if (!again && s > kSumLimit && a.col[row] >= 0) {
+    const int blk = (int)(row / kXgRows);
+    if (atomicExch(&a.mark[blk], 1) == 0) a.redo[1 + atomicAdd(&a.redo[0], 1)] = blk;  // the list's order is free
+  }
+}
+hipError_t xent_join_launch(const XentBf16Args& a, int again, hipStream_t st) {
+  hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a, again);
+  return hipGetLastError();
+}
+
+__global__ void __launch_bounds__(256) xent_top_kernel(const XentBf16Args a) {
+  if (a.redo[0] == 0) return;
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.rows || a.col[row] < 0 || !(a.sum[row] > kSumLimit)) return;
+  float m = -INFINITY;
+  for (int i = lane; i < a.parts; i += 64) m = fmaxf(m, a.sums[row * a.parts + i]);
+  m = wave_max(m);
+  if (lane == 0) a.ref[row] = m;
+}
+hipError_t xent_top_launch(const XentBf16Args& a, hipStream_t st) {
+  hipLaunchKernelGGL(xent_top_kernel, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// One workgroup a row, in place: the coded logits become softmax - [v = t], each rounded to bf16 once. The step of 2^-9
+// between codes moves a softmax entry by at most 2^-10, half of what that rounding may.
+__global__ void __launch_bounds__(256) xent_dz_kernel(const XentBf16Args a) {
+  const long long row = blockIdx.x;
+  uint4* q = reinterpret_cast<uint4*>(a.q + row * a.ldq);
+  const int n = (int)(a.ldq / 8), t = a.col[row];
+  if (t < 0) {
+    for (int i = threadIdx.x; i < n; i += 256) q[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const float s = a.sum[row], all = s + expf(a.zt[row] - a.ref[row]), g = a.row_weight ? a.row_weight[row] : 1.f;
+  constexpr float L2E = 1.4426950408889634f;
+  const float k0 = (kLogitLow + 64.f) * L2E - log2f(all), k1 = kLogitStep * L2E;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const uint4 v = q[i];
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 8 * i + 2 * j;
+      float lo = g * __builtin_amdgcn_exp2f(__builtin_fmaf((float)(int16_t)(w[j] & 0xffff), k1, k0));
+      float hi = g * __builtin_amdgcn_exp2f(__builtin_fmaf((float)((int32_t)w[j] >> 16), k1, k0));
+      lo = c >= a.vocab ? 0.f : c == t ? -g * (s / all) : lo;
+      hi = c + 1 >= a.vocab ? 0.f : c + 1 == t ? -g * (s / all) : hi;
+      w[j] = pack2(f32_to_bf16(lo), f32_to_bf16(hi));
+    }
+    q[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+hipError_t xent_dz_launch(const XentBf16Args& a, hipStream_t st) {
+  hipLaunchKernelGGL(xent_dz_kernel, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Up to 64 rows, losses only. A wave takes 16 MV rows of the vocabulary at a time against NB blocks of 16 rows of x on
+// 16 x 16 x 32 MFMAs (A: vocabulary, B: x), both operands straight from memory: W's bytes are all that counts. Lane l
+// holds the logits of row l % 16 of x and vocabulary rows 4 (l / 16) .. + 3 of a tile, and keeps a running maximum and
+// the sum of exponentials under it; the lanes' and waves' pairs join at the end.
+template <int MV, int NB>
+__global__ void __launch_bounds__(256) xent_few_kernel(const XentFewArgs a) {
+  __shared__ float2 red[4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  float top[NB], sum[NB];
+  int t[NB];
+  const bf16_t* xr[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int n = b * 16 + r;
+    top[b] = -INFINITY;
+    sum[b] = 0.f;
+    const int64_t tt = n < a.rows ? a.target[n] : -1;
+    t[b] = tt >= 0 && tt < a.vocab ? (int)tt : -1;
+    xr[b] = a.x + (long long)min(n, a.rows - 1) * a.ldx;
+  }
+  for (int v0 = (blockIdx.x * 4 + wave) * 16 * MV; v0 < a.vocab; v0 += gridDim.x * 4 * 16 * MV) {
+    f32x4_t acc[MV][NB];
+#pragma unroll
+    for (int i = 0; i < MV; ++i)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[i][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const bf16_t* wr[MV];
+#pragma unroll
+    for (int i = 0; i < MV; ++i) wr[i] = a.w + (long long)min(v0 + 16 * i + r, a.vocab - 1) * a.ldw;
+    const int whole = a.d & ~31;
+    for (int k = 0; k < whole; k += 32) {
+      bf16x8_t fx[NB], fw[MV];
+#pragma unroll
+      for (int i = 0; i < MV; ++i) __builtin_memcpy(&fw[i], wr[i] + k + 8 * g, 16);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) __builtin_memcpy(&fx[b], xr[b] + k + 8 * g, 16);
+#pragma unroll
+      for (int i = 0; i < MV; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i], fx[b], acc[i][b], 0, 0, 0);
+    }
+    if (whole < a.d) {
+#pragma unroll
+      for (int i = 0; i < MV; ++i) {
+        const uint4 wv = ld8_bits(wr[i], whole + 8 * g, a.d);
+        bf16x8_t fw;
+        __builtin_memcpy(&fw, &wv, 16);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint4 xv = ld8_bits(xr[b], whole + 8 * g, a.d);
+          bf16x8_t fx;
+          __builtin_memcpy(&fx, &xv, 16);
+          acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fx, acc[i][b], 0, 0, 0);
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < MV; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = v0 + 16 * i + 4 * g + e;
+          const float z = acc[i][b][e];
+          if (v == t[b]) {
+            a.zt[b * 16 + r] = z;
+          } else if (v < a.vocab) {
+            if (z != z) sum[b] = NAN;
+            if (z > top[b]) {
+              sum[b] *= expf(top[b] - z);
+              top[b] = z;
+            }
+            if (z > -INFINITY) sum[b] += expf(z - top[b]);
+          }
+        }
+  }
+  auto join = [](float2 p, float2 q) {  // -inf and a sum of 0 (or NaN) where there is nothing
+    const float m = fmaxf(p.x, q.x);
+    const float f = p.x > -INFINITY ? expf(p.x - m) : 1.f, h = q.x > -INFINITY ? expf(q.x - m) : 1.f;
+    return make_float2(m, p.y * f + q.y * h);
+  };
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float2 p = make_float2(top[b], sum[b]);
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) p = join(p, make_float2(__shfl_xor(p.x, o, 64), __shfl_xor(p.y, o, 64)));
+    if (g == 0) red[wave][b * 16 + r] = p;
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 * NB) {
+    float2 p = red[0][threadIdx.x];
+    for (int i = 1; i < 4; ++i) p = join(p, red[i][threadIdx.x]);
+    a.part[(long long)blockIdx.x * 64 + threadIdx.x] = p;
+  }
+}
+__global__ void __launch_bounds__(256) xent_few_join_kernel(const XentFewArgs a) {
+  __shared__ float red[16];
+  const int n = blockIdx.x;
+  const int64_t t = a.target[n];
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < a.wgs; i += 256) top = fmaxf(top, a.part[(long long)i * 64 + n].x);
+  top = block_max(top, red);
+  float s = 0.f;
+  for (int i = threadIdx.x; i < a.wgs; i += 256) {
+    const float2 p = a.part[(long long)i * 64 + n];
+    s += p.x > -INFINITY ? p.y * expf(p.x - top) : p.y;
+  }
+  s = block_sum(s, red);
+  if (threadIdx.x) return;
+  float loss;
+  if (t == a.ignore) {
+    loss = 0.f;
+  } else if (t < 0 || t >= a.vocab) {
+    loss = NAN;
+  } else {
+    const float zt = a.zt[n], m = fmaxf(top, zt), rest = top > -INFINITY ? s * expf(top - m) : s;
+    loss = m == zt ? log1pf(rest) : logf(rest + expf(zt - m)) + (m - zt);
+    if (zt != zt) loss = NAN;
+  }
+  a.loss[n] = loss;
+}
+int xent_few_wgs(int vocab) {
+  const int per = vocab >= 32768 ? 256 : 64;  // vocabulary rows of a workgroup at a time
+  const int want = (vocab + per - 1) / per;
+  return want > 1024 ? 1024 : want;
+}
+hipError_t xent_few_launch(const XentFewArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.wgs);
+#define PSGDK_FEW(MV, NB) hipLaunchKernelGGL((xent_few_kernel<MV, NB>), grid, dim3(256), 0, st, a)
+  if (a.vocab >= 32768) {
+    if (a.rows <= 16) PSGDK_FEW(4, 1);
+    else if (a.rows <= 32) PSGDK_FEW(4, 2);
+    else PSGDK_FEW(4, 4);
+  } else {
+    if (a.rows <= 16) PSGDK_FEW(1, 1);
+    else if (a.rows <= 32) PSGDK_FEW(1, 2);
+    else PSGDK_FEW(1, 4);
+  }
+#undef PSGDK_FEW
+  hipLaunchKernelGGL(xent_few_join_kernel, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+__global__ void __launch_bounds__(256) xent_mask_rows_kernel(const float* x, long long ldx, float* out,
+                                                             const int64_t* target, int64_t ignore, long long rows,
+                                                             int d) {
   const long long total = rows * d;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long r = i / d;
-    out[i] = target[r] == ignore ? from_f32<T>(0.f) : x[r * ldx + (i - r * d)];
+    out[i] = target[r] == ignore ? 0.f : x[r * ldx + (i - r * d)];
   }
 }
-hipError_t xent_mask_rows_launch(const void* x, long long ldx, void* out, const int64_t* target, int64_t ignore,
-                                 long long rows, int d, int dt, hipStream_t st) {
+hipError_t xent_mask_rows_launch(const float* x, long long ldx, float* out, const int64_t* target, int64_t ignore,
+                                 long long rows, int d, hipStream_t st) {
   const long long want = (rows * d + 255) / 256;
-  const dim3 grid((unsigned)(want > 8192 ? 8192 : want));
-  if (dt == 1)
-    hipLaunchKernelGGL(xent_mask_rows_kernel<bf16_t>, grid, dim3(256), 0, st, reinterpret_cast<const bf16_t*>(x), ldx,
-                       reinterpret_cast<bf16_t*>(out), target, ignore, rows, d);
-  else
-    hipLaunchKernelGGL(xent_mask_rows_kernel<float>, grid, dim3(256), 0, st, reinterpret_cast<const float*>(x), ldx,
-                       reinterpret_cast<float*>(out), target, ignore, rows, d);
+  hipLaunchKernelGGL(xent_mask_rows_kernel, dim3((unsigned)(want > 8192 ? 8192 : want)), dim3(256), 0, st, x, ldx, out,
+                     target, ignore, rows, d);
   return hipGetLastError();
 }
 
