@@ -57,22 +57,13 @@ __device__ __forceinline__ void load_wait() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// The order of one k step: the next step's READS LDS reads spread evenly behind this step's MM MFMAs.
-template <int MM, int READS, int G = 0>
-__device__ __forceinline__ void interleave() {
-  if constexpr (G < MM) {
-    constexpr int N = (G + 1) * READS / MM - G * READS / MM;
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x100, N, 0);
-    interleave<MM, READS, G + 1>();
-  }
-}
-
 }  // namespace
 
-// Four waves, 2 x 2, each WTM x WTN of the output. ST stages of BK k in LDS.
+// Four waves, 2 x 2, each WTM x WTN of the output; ST stages of BK k in LDS, and a block of 32 x WTM 16-bit values for
+// each wave's way out. A workgroup takes one tile after the other; the loads of the next tile's first stages are on their
+// way before a tile's results leave.
 template <int WTM, int WTN, int BK, int ST, bool MCA, bool MCB, int KIND, bool OUTF>
-__global__ void __launch_bounds__(256, WTM * WTN > 128 * 64 ? 1 : 2) xgemm_kernel(const XgArgs p) {
+__global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
   constexpr int BM = 2 * WTM, BN = 2 * WTN, FM = WTM / 32, FN = WTN / 32, KS = BK / 16;
   using TA = Tile<BM, BK, MCA>;
   using TB = Tile<BN, BK, MCB>;
@@ -80,17 +71,20 @@ __global__ void __launch_bounds__(256, WTM * WTN > 128 * 64 ? 1 : 2) xgemm_kerne
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 31, hh = lane >> 5, wm = wave >> 1, wn = wave & 1;
+
+  static_assert(BN == kXgRows, "a listed block is a tile of n");
   const int ntiles = p.redo ? p.redo[0] * p.tiles_m : p.tiles_m * p.tiles_n * p.splits;
-  for (int w = blockIdx.x; w < ntiles; w += gridDim.x) {
-  int lane = threadIdx.x & 63;
-  asm volatile("" : "+v"(lane));  // what follows from it is made again for each tile, not kept through the epilogue
-  const int c = lane & 31, hh = lane >> 5;
-  int ti, tj, split = 0;
-  if (p.redo) {
-    ti = w % p.tiles_m;
-    tj = p.redo[1 + w / p.tiles_m];
-  } else {
+  if ((int)blockIdx.x >= ntiles) return;
+  // tile w of the workgroups' order: its m and n tile and its part of k
+  auto where = [&](int w, int& ti, int& tj, int& split) __attribute__((always_inline)) {
+    split = 0;
+    if (p.redo) {
+      ti = w % p.tiles_m;
+      tj = p.redo[1 + w / p.tiles_m];
+      return;
+    }
     // each XCD a contiguous run of tiles, 4 tiles of m by n after n, so that the tiles it runs at once share panels
     constexpr int GM = 4;
     int tile = xcd_run(w, ntiles);
@@ -99,10 +93,7 @@ __global__ void __launch_bounds__(256, WTM * WTN > 128 * 64 ? 1 : 2) xgemm_kerne
     const int grp = tile / (GM * p.tiles_n), r0 = grp * GM, gm = min(GM, p.tiles_m - r0), idx = tile - r0 * p.tiles_n;
     ti = r0 + idx % gm;
     tj = idx / gm;
-  }
-  const int m0 = ti * BM, n0 = tj * BN;
-  const int kb = split * p.kchunk, ke = min(p.K, kb + p.kchunk);
-  const int nk = (ke - kb + BK - 1) / BK;
+  };
 
   // byte offsets of this lane's loads inside a tile
   int va[TA::LOADS], vb[TB::LOADS];
@@ -118,61 +109,86 @@ __global__ void __launch_bounds__(256, WTM * WTN > 128 * 64 ? 1 : 2) xgemm_kerne
     TB::where(wave, lane, i, row, ch);
     vb[i] = (int)((long long)row * p.ldb + ch * 8) * 2;
   }
-  auto issue = [&](int t) {
-    const int k0 = kb + t * BK;
-    const bool live = t < nk;
-    unsigned base = lds0 + (unsigned)(t % ST) * STAGE;
-    const bf16_t* pa = p.A + (MCA ? (long long)k0 * p.lda + m0 : (long long)m0 * p.lda + k0);
-    const bf16_t* pb = p.B + (MCB ? (long long)k0 * p.ldb + n0 : (long long)n0 * p.ldb + k0);
-    i32x4_t ra = rsrc_words(pa, !live ? 0 : 2 * (MCA ? (long long)(min(ke, p.kreal) - k0 - 1) * p.lda + ((p.M - m0 + 7) & ~7)
-                                                           : (long long)(p.M - m0 - 1) * p.lda + (ke - k0)));
-    i32x4_t rb = rsrc_words(pb, !live ? 0 : 2 * (MCB ? (long long)(ke - k0 - 1) * p.ldb + ((p.N - n0 + 7) & ~7)
-                                                           : (long long)(p.N - n0 - 1) * p.ldb + (ke - k0)));
+  // The loads, one k tile after the other and on into the next output tile: plan() moves on to the next (and its stage),
+  // load(i) issues its load i. The buffers begin at the tile and end with the operand: rows behind it read zeros (k behind
+  // the end of a k-contiguous row is the lanes' own check), and behind the last output tile there are only zeros.
+  const bf16_t *pa, *pb;
+  const long long da = MCA ? (long long)BK * p.lda : BK, db = MCB ? (long long)BK * p.ldb : BK;
+  long long ea, eb;
+  int wl = blockIdx.x, kp, kl;
+  unsigned to = lds0;
+  i32x4_t ra, rb;
+  int v[LOADS];
+  auto begin = [&]() __attribute__((always_inline)) {
+    int ti, tj, split;
+    where(wl, ti, tj, split);
+    const int m0 = ti * BM, n0 = tj * BN;
+    kp = split * p.kchunk;
+    kl = min(p.K, kp + p.kchunk);
+    pa = p.A + (MCA ? (long long)kp * p.lda + m0 : (long long)m0 * p.lda + kp);
+    pb = p.B + (MCB ? (long long)kp * p.ldb + n0 : (long long)n0 * p.ldb + kp);
+    ea = MCA ? (long long)(min(kl, p.kreal) - kp - 1) * p.lda + ((p.M - m0 + 7) & ~7)
+             : (long long)(p.M - m0 - 1) * p.lda + (kl - kp);
+    eb = MCB ? (long long)(kl - kp - 1) * p.ldb + ((p.N - n0 + 7) & ~7)
+             : (long long)(p.N - n0 - 1) * p.ldb + (kl - kp);
+  };
+  auto plan = [&](bool first) __attribute__((always_inline)) {
+    if (!first) {
+      to = to + STAGE == lds0 + ST * STAGE ? lds0 : to + STAGE;
+      pa += da;
+      pb += db;
+      ea -= da;
+      eb -= db;
+      kp += BK;
+      if (kp >= kl) {
+        wl += gridDim.x;
+        if (wl < ntiles) {
+          begin();
+        } else {
+          ea = eb = 0;
+          kl = 0;
+        }
+      }
+    }
+    ra = rsrc_words(pa, 2 * ea);
+    rb = rsrc_words(pb, 2 * eb);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const bool isa = i < TA::LOADS;
+      v[i] = isa ? va[i < TA::LOADS ? i : 0] : vb[i < TA::LOADS ? 0 : i - TA::LOADS];
+      if (isa ? !MCA : !MCB) {
+        int row, ch;
+        if (isa) TA::where(wave, lane, i, row, ch);
+        else TB::where(wave, lane, i - TA::LOADS, row, ch);
+        v[i] = kp + ch * 8 < kl ? v[i] : kOob;
+      }
+    }
     // a scalar register that a vector instruction wrote may be read by a load 5 wait states later at the earliest, which
     // the compiler does not see to inside asm statements
-    asm volatile("s_nop 4" : "+s"(ra), "+s"(rb), "+s"(base));
-    const bool whole = k0 + BK <= ke;
-#pragma unroll
-    for (int i = 0; i < TA::LOADS; ++i) {
-      int v = va[i];
-      if (!MCA && !whole) {
-        int row, ch;
-        TA::where(wave, lane, i, row, ch);
-        v = k0 + ch * 8 < ke ? v : kOob;
-      }
-      load_lds(ra, v, base + (unsigned)(wave * TA::LOADS + i) * 1024);
-    }
-#pragma unroll
-    for (int i = 0; i < TB::LOADS; ++i) {
-      int v = vb[i];
-      if (!MCB && !whole) {
-        int row, ch;
-        TB::where(wave, lane, i, row, ch);
-        v = k0 + ch * 8 < ke ? v : kOob;
-      }
-      load_lds(rb, v, base + TA::BYTES + (unsigned)(wave * TB::LOADS + i) * 1024);
-    }
+    asm volatile("s_nop 4" : "+s"(ra), "+s"(rb), "+s"(to));
+  };
+  auto load = [&](int i) __attribute__((always_inline)) {
+    if (i < TA::LOADS) load_lds(ra, v[i], to + (unsigned)(wave * TA::LOADS + i) * 1024);
+    else load_lds(rb, v[i], to + TA::BYTES + (unsigned)(wave * TB::LOADS + i - TA::LOADS) * 1024);
   };
 
-  // LDS offsets of this lane's fragment reads inside a stage: k-contiguous operands by k step, others by 32-block
-  unsigned oa[MCA ? FM : KS], ob[MCB ? FN : KS];
+  // LDS offset of this lane's first fragment read inside a stage. The others differ by a constant, and by an XOR of the
+  // k step (k-contiguous: chunk 2 ks + hh of the row) or of the 32-block (mn-contiguous), which the swizzles let pass.
   const int rr = (lane & 15) >> 2;
-#pragma unroll
-  for (int i = 0; i < (MCA ? FM : KS); ++i)
-    oa[i] = MCA ? (8 * hh + rr) * BM * 2 + ((((wm * WTM + 32 * i) >> 5) ^ TA::swm(8 * hh + rr)) << 6) + (lane >> 4 & 1) * 32 +
-                      (lane & 3) * 8
-                : (wm * WTM + c) * BK * 2 + (((2 * i + hh) ^ TA::swk(c)) << 4);
-#pragma unroll
-  for (int i = 0; i < (MCB ? FN : KS); ++i)
-    ob[i] = TA::BYTES +
-            (MCB ? (8 * hh + rr) * BN * 2 + ((((wn * WTN + 32 * i) >> 5) ^ TB::swm(8 * hh + rr)) << 6) + (lane >> 4 & 1) * 32 +
-                       (lane & 3) * 8
-                 : (wn * WTN + c) * BK * 2 + (((2 * i + hh) ^ TB::swk(c)) << 4));
+  static_assert(WTM % 128 == 0 || !MCA, "the 32-blocks of a wave differ in the lowest bits of their number");
+  static_assert(WTN % 128 == 0 || !MCB, "the 32-blocks of a wave differ in the lowest bits of their number");
+  const unsigned oa = MCA ? (8 * hh + rr) * BM * 2 + (((wm * WTM >> 5) ^ TA::swm(8 * hh + rr)) << 6) + (lane >> 4 & 1) * 32 +
+                                (lane & 3) * 8
+                          : (wm * WTM + c) * BK * 2 + ((hh ^ TA::swk(c)) << 4);
+  const unsigned ob = TA::BYTES +
+                      (MCB ? (8 * hh + rr) * BN * 2 + (((wn * WTN >> 5) ^ TB::swm(8 * hh + rr)) << 6) + (lane >> 4 & 1) * 32 +
+                                 (lane & 3) * 8
+                           : (wn * WTN + c) * BK * 2 + ((hh ^ TB::swk(c)) << 4));
 
-  auto tr = [](unsigned at) {
+  auto tr = [](unsigned at) __attribute__((always_inline)) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4_t*)(uintptr_t)at);
   };
-  auto pair = [&](unsigned at, int pitch4) {
+  auto pair = [&](unsigned at, int pitch4) __attribute__((always_inline)) {
     union {
       s16x4_t h[2];
       bf16x8_t v;
@@ -182,179 +198,212 @@ __global__ void __launch_bounds__(256, WTM * WTN > 128 * 64 ? 1 : 2) xgemm_kerne
     return u.v;
   };
   bf16x8_t fa[2][FM], fb[2][FN];
-  auto frags = [&](int set, unsigned base, int ks) {
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      if constexpr (MCB) fb[set][j] = pair(base + ob[j] + ks * 16 * BN * 2, 4 * BN * 2);
-      else fb[set][j] = *(LDS_AS bf16x8_t*)(uintptr_t)(base + ob[ks] + j * 32 * BK * 2);
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      if constexpr (MCA) fa[set][i] = pair(base + oa[i] + ks * 16 * BM * 2, 4 * BM * 2);
-      else fa[set][i] = *(LDS_AS bf16x8_t*)(uintptr_t)(base + oa[ks] + i * 32 * BK * 2);
+  // fragment f of k step ks: B's FN, then A's FM
+  auto frag = [&](int set, unsigned base, int ks, int f) __attribute__((always_inline)) {
+    if (f < FN) {
+      if constexpr (MCB) fb[set][f] = pair(((base + ob) ^ (f << 6)) + ks * 16 * BN * 2, 4 * BN * 2);
+      else fb[set][f] = *(LDS_AS bf16x8_t*)(uintptr_t)(((base + ob) ^ (ks << 5)) + f * 32 * BK * 2);
+    } else {
+      const int i = f - FN;
+      if constexpr (MCA) fa[set][i] = pair(((base + oa) ^ (i << 6)) + ks * 16 * BM * 2, 4 * BM * 2);
+      else fa[set][i] = *(LDS_AS bf16x8_t*)(uintptr_t)(((base + oa) ^ (ks << 5)) + i * 32 * BK * 2);
     }
   };
 
-  f32x16_t acc[FM][FN];
+  // the state in front of a tile's first step: its ST - 1 first k tiles and the first share of the next are on their way
+  constexpr int MM = FM * FN, FR = FM + FN, PER = KS > 2 ? (LOADS + KS - 2) / (KS - 1) : (LOADS + KS - 1) / KS;
+  begin();
+  for (int t = 0; t < ST; ++t) {
+    plan(t == 0);
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < LOADS; ++i)
+      if (i < PER || t + 1 < ST) load(i);
+  }
+  load_wait<(ST - 2) * LOADS + PER>();
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  for (int f = 0; f < FM + FN; ++f) frag(0, lds0, 0, f);
+  unsigned base = lds0;
 
+  for (int w = blockIdx.x; w < ntiles; w += gridDim.x) {
+    int ti, tj, split;
+    where(w, ti, tj, split);
+    const int nk = (min(p.K - split * p.kchunk, p.kchunk) + BK - 1) / BK;
+    f32x16_t acc[FM][FN];
 #pragma unroll
-  for (int t = 0; t < ST; ++t) issue(t);
-  load_wait<(ST - 1) * LOADS>();
-  frags(0, lds0, 0);
-  static_assert(KS % 2 == 0, "fragment sets alternate over whole tiles");
-  constexpr int READS = FM * (MCA ? 2 : 1) + FN * (MCB ? 2 : 1), MM = FM * FN;
-  for (int kt = 0; kt < nk; ++kt) {
-    const unsigned base = lds0 + (unsigned)(kt % ST) * STAGE, next = lds0 + (unsigned)((kt + 1) % ST) * STAGE;
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int cur = ks & 1;
-      if (ks + 1 < KS) {
-        frags(cur ^ 1, base, ks + 1);
-      } else {
-        load_wait<(ST - 2) * LOADS>();
-        issue(kt + ST);
-        frags(cur ^ 1, next, 0);
-      }
+      for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    static_assert(KS % 2 == 0, "fragment sets alternate over whole tiles");
+    // One k step: its MFMAs, and between them, in an order that the compiler keeps, the reads of the next step's fragments
+    // (early, so that they are there when the step ends) and a share of the loads. The last step of a k tile waits for the
+    // next one before, and begins the loads of the tile that takes this one's stage; the next tile's first steps issue the
+    // rest, all before its last but one. (The loads one after the other kept the MFMAs waiting for half of the time.)
+    constexpr int EARLY = MM * 3 / 4;  // MFMAs over which the reads are spread
+    for (int kt = 0; kt < nk; ++kt) {
+      const unsigned next = base + STAGE == lds0 + ST * STAGE ? lds0 : base + STAGE;
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
+      for (int ks = 0; ks < KS; ++ks) {
+        const int cur = ks & 1;
+        const bool last = ks + 1 == KS;
+        if (last) load_wait<(ST - 2) * LOADS>();
+#pragma unroll
+        for (int g = 0; g < MM; ++g) {
+          const int i = g / FN, j = g % FN;
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[cur][i], fb[cur][j], acc[i][j], 0, 0, 0);
-      interleave<MM, READS>();
-    }
-  }
-  load_wait<0>();  // LDS is the epilogue's now
-
-  // Element e of acc[i][j]: m = 32 i + 8 (e / 4) + 4 hh + e % 4, n = 32 j + c of the wave's block: 4 consecutive m a
-  // lane. The block is put together in LDS (rows n of WTM 16-bit values, 16-byte chunks XORed by n) and leaves in rows of
-  // 16-byte stores.
-  const int mw = m0 + wm * WTM, nw = n0 + wn * WTN;
-  if constexpr (OUTF) {
-    float* const o = p.outf + (long long)split * p.N * p.ldo;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = nw + 32 * j + c;
-      if (n >= p.N) continue;
-      float* const q = o + (long long)n * p.ldo + mw + 4 * hh;
+          for (int f = 0; f < FR; ++f)
+            if (f * EARLY / FR == g) frag(cur ^ 1, last ? next : base, last ? 0 : ks + 1, f);
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int m = 32 * i + 8 * g;
-          if (mw + 4 * hh + m >= p.M) continue;
-          f32x4_t v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-          if (p.accumulate) v += *reinterpret_cast<const f32x4_t*>(q + m);
-          *reinterpret_cast<f32x4_t*>(q + m) = v;
+          for (int l = 0; l < PER; ++l) {
+            const int n = (last ? 0 : ks + 1) * PER + l;
+            if (l * MM / PER == g && n < LOADS) load(n);
+          }
+          if (ks + 2 == KS && g == MM - 2) plan(false);  // for the loads that begin with the last step
+          if (g < MM - 2) __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      base = next;
     }
-    return;
-  }
-  unsigned char* const ep = smem + wave * WTN * WTM * 2;
-  constexpr int CH = WTM / 8;
-  auto slot = [&](int n, int ch) { return ep + n * WTM * 2 + ((ch ^ (n & (CH - 1))) << 4); };
-  if constexpr (KIND == XG_LOGITS) {
+
+    // Element e of acc[i][j]: m = 32 i + 8 (e / 4) + 4 hh + e % 4, n = 32 j + c of the wave's block: 4 consecutive m a
+    // lane. 32 n at a time are put together in the wave's own part of LDS (rows n of WTM 16-bit values, 16-byte chunks
+    // XORed by n) and leave in rows of 16-byte stores.
+    const int mw = ti * BM + wm * WTM, nw = tj * BN + wn * WTN;
+    float ref[FN];
+    int tgt[FN];
+    float al = 1.f;
+    if constexpr (KIND == XG_LOGITS) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int n = nw + 32 * j + c;
+        ref[j] = n < p.N ? p.ref[n] : 0.f;
+        tgt[j] = n < p.N ? p.target[n] : -1;
+      }
+      // these loads' wait belongs here, before the next tile's
+#pragma unroll
+      for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(ref[j]), "+v"(tgt[j]));
+    } else if (!OUTF && p.alpha) {
+      al = p.alpha[0];
+      asm volatile("" : "+v"(al));
+    }
+    if constexpr (OUTF) {
+      float* const o = p.outf + (long long)split * p.N * p.ldo;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int n = nw + 32 * j + c;
+        if (n >= p.N) continue;
+        float* const q = o + (long long)n * p.ldo + mw + 4 * hh;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int m = 32 * i + 8 * g;
+            if (mw + 4 * hh + m >= p.M) continue;
+            f32x4_t x = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            if (p.accumulate) x += *reinterpret_cast<const f32x4_t*>(q + m);
+            *reinterpret_cast<f32x4_t*>(q + m) = x;
+          }
+      }
+      continue;
+    }
+    unsigned char* const ep = smem + ST * STAGE + wave * 32 * WTM * 2;
+    constexpr int CH = WTM / 8;
+    auto slot = [&](int n, int ch) __attribute__((always_inline)) { return ep + n * WTM * 2 + ((ch ^ (n & (CH - 1))) << 4); };
+    uint16_t* const out = KIND == XG_LOGITS ? reinterpret_cast<uint16_t*>(p.q) : p.out;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int n = nw + 32 * j + c;
       const bool row = n < p.N;
-      const float r = row ? p.ref[n] : 0.f;
-      const int t = row ? p.target[n] : -1;
-      const int tl = t - mw - 4 * hh;  // the target as a column of this lane's first group
-      const bool inside = mw + WTM <= p.M && !__any(tl >= -4 && tl < WTM + 4);
-      constexpr float L2E = 1.4426950408889634f;
-      // pknorm: x 32767 to the nearest, clamped; x = ((z - r) - low - 64) / (64 32767 / 32768)
-      constexpr float QS = 32768.f / 32767.f / 64.f;
-      const float e0 = -r * L2E, q0 = (-r - kLogitLow - 64.f) * QS;
-      float s = 0.f, top = -INFINITY;
+      if constexpr (KIND == XG_LOGITS) {
+        const float r = ref[j];
+        const int t = tgt[j];
+        const int tl = t - mw - 4 * hh;  // the target as a column of this lane's first group
+        const bool inside = mw + WTM <= p.M && !__any(tl >= -4 && tl < WTM + 4);
+        constexpr float L2E = 1.4426950408889634f;
+        // pknorm: x 32767 to the nearest, clamped; x = ((z - r) - low - 64) / (64 32767 / 32768)
+        constexpr float QS = 32768.f / 32767.f / 64.f;
+        const float e0 = -r * L2E, q0 = (-r - kLogitLow - 64.f) * QS;
+        float s = 0.f, top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        asm volatile("" : "+a"(acc[i][j]));  // accumulators leave their registers tile by tile, not all at once
+        for (int i = 0; i < FM; ++i) {
+          asm volatile("" : "+a"(acc[i][j]));  // accumulators leave their registers tile by tile, not all at once
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float z[4];
+          for (int g = 0; g < 4; ++g) {
+            float z[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) z[e] = acc[i][j][4 * g + e];
-          const int m = 32 * i + 8 * g + 4 * hh;
-          if (p.max_only) {
+            for (int e = 0; e < 4; ++e) z[e] = acc[i][j][4 * g + e];
+            const int m = 32 * i + 8 * g + 4 * hh;
+            if (p.max_only) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (mw + m + e < p.M) top = fmaxf(top, z[e]);
-          } else if (inside) {
+              for (int e = 0; e < 4; ++e)
+                if (mw + m + e < p.M) top = fmaxf(top, z[e]);
+            } else if (inside) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0));
-          } else {
+              for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0));
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const bool other = mw + m + e < p.M && mw + m + e != t;
-              s += other ? __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0)) : 0.f;
+              for (int e = 0; e < 4; ++e) {
+                const bool other = mw + m + e < p.M && mw + m + e != t;
+                s += other ? __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0)) : 0.f;
+              }
+            }
+            if (p.q) {
+              const auto lo = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[0], QS, q0), __builtin_fmaf(z[1], QS, q0));
+              const auto hi = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[2], QS, q0), __builtin_fmaf(z[3], QS, q0));
+              uint2 x;
+              __builtin_memcpy(&x.x, &lo, 4);
+              __builtin_memcpy(&x.y, &hi, 4);
+              *reinterpret_cast<uint2*>(slot(c, 4 * i + g) + hh * 8) = x;
             }
           }
-          if (p.q) {
-            const auto lo = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[0], QS, q0), __builtin_fmaf(z[1], QS, q0));
-            const auto hi = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[2], QS, q0), __builtin_fmaf(z[3], QS, q0));
-            uint2 w;
-            __builtin_memcpy(&w.x, &lo, 4);
-            __builtin_memcpy(&w.y, &hi, 4);
-            *reinterpret_cast<uint2*>(slot(32 * j + c, 4 * i + g) + hh * 8) = w;
-          }
+        }
+        if (p.max_only) {
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          if (row && hh == 0) p.tops[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = top;
+        } else {
+          s += __shfl_xor(s, 32, 64);
+          if (row && hh == 0) p.sums[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = t < 0 ? 0.f : s;
+        }
+        if (!p.q) continue;
+      } else {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          asm volatile("" : "+a"(acc[i][j]));  // accumulators leave their registers tile by tile, not all at once
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(slot(c, 4 * i + g) + hh * 8) =
+                make_uint2(pack2_bf16(al * acc[i][j][4 * g], al * acc[i][j][4 * g + 1]),
+                           pack2_bf16(al * acc[i][j][4 * g + 2], al * acc[i][j][4 * g + 3]));
         }
       }
-      if (p.max_only) {
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        if (row && hh == 0) p.tops[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = top;
-      } else {
-        s += __shfl_xor(s, 32, 64);
-        if (row && hh == 0) p.sums[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = t < 0 ? 0.f : s;
+#pragma unroll
+      for (int it = 0; it < 32 * CH / 64; ++it) {
+        const int idx = it * 64 + lane, q = idx / CH, ch = idx % CH, m = mw + 8 * ch, no = nw + 32 * j + q;
+        const uint4 x = *reinterpret_cast<const uint4*>(slot(q, ch));
+        if (no >= p.N || m >= p.M) continue;
+        uint16_t* o = out + (long long)no * p.ldo + m;
+        if (m + 8 <= p.M) {
+          __builtin_memcpy(o, &x, 16);
+        } else {
+          uint16_t h[8];
+          __builtin_memcpy(h, &x, 16);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (m + e < p.M) o[e] = h[e];
+        }
       }
     }
-    if (!p.q) continue;
-  } else {
-    const float al = p.alpha ? p.alpha[0] : 1.f;
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        asm volatile("" : "+a"(acc[i][j]));  // accumulators leave their registers tile by tile, not all at once
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint2*>(slot(32 * j + c, 4 * i + g) + hh * 8) =
-              make_uint2(pack2_bf16(al * acc[i][j][4 * g], al * acc[i][j][4 * g + 1]),
-                         pack2_bf16(al * acc[i][j][4 * g + 2], al * acc[i][j][4 * g + 3]));
-      }
   }
-  __syncthreads();
-  uint16_t* const out = KIND == XG_LOGITS ? reinterpret_cast<uint16_t*>(p.q) : p.out;
-#pragma unroll 4
-  for (int it = 0; it < WTN * CH / 64; ++it) {
-    const int idx = it * 64 + lane, n = idx / CH, ch = idx % CH, m = mw + 8 * ch;
-    if (nw + n >= p.N || m >= p.M) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(slot(n, ch));
-    uint16_t* o = out + (long long)(nw + n) * p.ldo + m;
-    if (m + 8 <= p.M) {
-      __builtin_memcpy(o, &v, 16);
-    } else {
-      uint16_t h[8];
-      __builtin_memcpy(h, &v, 16);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (m + e < p.M) o[e] = h[e];
-    }
-  }
-  if constexpr (KIND != XG_LOGITS) return;
-  __syncthreads();  // LDS is the next tile's
-  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup
 }
 
 template <int WTM, int WTN, int BK, int ST, bool MCA, bool MCB, int KIND, bool OUTF = false>
 static hipError_t launch_x(XgArgs& a, hipStream_t st) {
-  constexpr int smem_main = ST * (Tile<2 * WTM, BK, MCA>::BYTES + Tile<2 * WTN, BK, MCB>::BYTES), smem_epi = 4 * WTM * WTN * 2;
-  constexpr int smem = smem_main > smem_epi ? smem_main : smem_epi;
+  constexpr int smem = ST * (Tile<2 * WTM, BK, MCA>::BYTES + Tile<2 * WTN, BK, MCB>::BYTES) + 4 * 32 * WTM * 2;
   void (*fn)(XgArgs) = xgemm_kernel<WTM, WTN, BK, ST, MCA, MCB, KIND, OUTF>;
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -364,8 +413,7 @@ static hipError_t launch_x(XgArgs& a, hipStream_t st) {
   if (!a.kreal) a.kreal = a.K;
   a.kchunk = a.splits > 1 ? ((a.K + a.splits - 1) / a.splits + BK - 1) / BK * BK : a.K;
   const long long tiles = (long long)a.tiles_m * a.tiles_n * a.splits;
-  // tiles to be done again are not known here: one workgroup a CU takes them in turn, and ends at once without any
-  hipLaunchKernelGGL(fn, dim3((unsigned)(a.redo && tiles > 256 ? 256 : tiles)), dim3(256), smem, st, a);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(tiles > 256 ? 256 : tiles)), dim3(256), smem, st, a);  // one a CU
   return hipGetLastError();
 }
 
