@@ -1,4 +1,6 @@
 // The bf16 products of the cross entropy on v_mfma_f32_32x32x16_bf16, operands moved from HBM straight into LDS.
+#include <type_traits>
+
 #include "xgemm.h"
 
 namespace psgdk {
@@ -228,6 +230,19 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     int ti, tj, split;
     where(w, ti, tj, split);
     const int nk = (min(p.K - split * p.kchunk, p.kchunk) + BK - 1) / BK;
+    const int mw = ti * BM + wm * WTM, nw = tj * BN + wn * WTN;  // this wave's block
+    float ref[FN], al = 1.f;
+    int tgt[FN];
+    if constexpr (KIND == XG_LOGITS) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int n = nw + 32 * j + c;
+        ref[j] = n < p.N ? p.ref[n] : 0.f;
+        tgt[j] = n < p.N ? p.target[n] : -1;
+      }
+    } else if (!OUTF && p.alpha) {
+      al = p.alpha[0];
+    }
     f32x16_t acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -272,24 +287,6 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     // Element e of acc[i][j]: m = 32 i + 8 (e / 4) + 4 hh + e % 4, n = 32 j + c of the wave's block: 4 consecutive m a
     // lane. 32 n at a time are put together in the wave's own part of LDS (rows n of WTM 16-bit values, 16-byte chunks
     // XORed by n) and leave in rows of 16-byte stores.
-    const int mw = ti * BM + wm * WTM, nw = tj * BN + wn * WTN;
-    float ref[FN];
-    int tgt[FN];
-    float al = 1.f;
-    if constexpr (KIND == XG_LOGITS) {
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int n = nw + 32 * j + c;
-        ref[j] = n < p.N ? p.ref[n] : 0.f;
-        tgt[j] = n < p.N ? p.target[n] : -1;
-      }
-      // these loads' wait belongs here, before the next tile's
-#pragma unroll
-      for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(ref[j]), "+v"(tgt[j]));
-    } else if (!OUTF && p.alpha) {
-      al = p.alpha[0];
-      asm volatile("" : "+v"(al));
-    }
     if constexpr (OUTF) {
       float* const o = p.outf + (long long)split * p.N * p.ldo;
 #pragma unroll
@@ -328,36 +325,48 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
         constexpr float QS = 32768.f / 32767.f / 64.f;
         const float e0 = -r * L2E, q0 = (-r - kLogitLow - 64.f) * QS;
         float s = 0.f, top = -INFINITY;
+        auto code = [&](int i, int g, const float* z) __attribute__((always_inline)) {
+          const auto lo = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[0], QS, q0), __builtin_fmaf(z[1], QS, q0));
+          const auto hi = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[2], QS, q0), __builtin_fmaf(z[3], QS, q0));
+          uint2 x;
+          __builtin_memcpy(&x.x, &lo, 4);
+          __builtin_memcpy(&x.y, &hi, 4);
+          *reinterpret_cast<uint2*>(slot(c, 4 * i + g) + hh * 8) = x;
+        };
+        auto usual = [&](auto keep) __attribute__((always_inline)) {  // no branches between the 64 exponentials
+          float s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          asm volatile("" : "+a"(acc[i][j]));  // accumulators leave their registers tile by tile, not all at once
+          for (int i = 0; i < FM; ++i) {
+            asm volatile("" : "+a"(acc[i][j]));  // accumulators leave their registers tile by tile, not all at once
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float z[4];
+            for (int g = 0; g < 4; ++g) {
+              const float z[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+              s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[0], L2E, e0));
+              s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(z[1], L2E, e0));
+              s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(z[2], L2E, e0));
+              s3 += __builtin_amdgcn_exp2f(__builtin_fmaf(z[3], L2E, e0));
+              if constexpr (decltype(keep)::value) code(i, g, z);
+            }
+          }
+          s = (s + s1) + (s2 + s3);
+        };
+        if (inside && !p.max_only) {
+          if (p.q) usual(std::true_type{});
+          else usual(std::false_type{});
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = acc[i][j][4 * g + e];
-            const int m = 32 * i + 8 * g + 4 * hh;
-            if (p.max_only) {
+          for (int i = 0; i < FM; ++i) {
+            asm volatile("" : "+a"(acc[i][j]));
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (mw + m + e < p.M) top = fmaxf(top, z[e]);
-            } else if (inside) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0));
-            } else {
+            for (int g = 0; g < 4; ++g) {
+              const float z[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+              const int m = mw + 32 * i + 8 * g + 4 * hh;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const bool other = mw + m + e < p.M && mw + m + e != t;
-                s += other ? __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0)) : 0.f;
+                if (p.max_only) top = fmaxf(top, m + e < p.M ? z[e] : -INFINITY);
+                else s += m + e < p.M && m + e != t ? __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0)) : 0.f;
               }
-            }
-            if (p.q) {
-              const auto lo = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[0], QS, q0), __builtin_fmaf(z[1], QS, q0));
-              const auto hi = __builtin_amdgcn_cvt_pknorm_i16(__builtin_fmaf(z[2], QS, q0), __builtin_fmaf(z[3], QS, q0));
-              uint2 x;
-              __builtin_memcpy(&x.x, &lo, 4);
-              __builtin_memcpy(&x.y, &hi, 4);
-              *reinterpret_cast<uint2*>(slot(c, 4 * i + g) + hh * 8) = x;
+              if (p.q) code(i, g, z);
             }
           }
         }
