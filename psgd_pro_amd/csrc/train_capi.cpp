@@ -269,7 +269,8 @@ int lce_bf16(const Lce& p) {
   const int64_t blocks = (slab + kXgRows - 1) / kXgRows, parts = 2 * ((p.vocab + 255) / 256);
   const bool copy_w = p.d % 8 != 0 || p.ldw % 8 != 0 || p.ldw > kMaxVocab || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
   const bool sum_w = p.dw && slab < p.rows;
-  const int splits = p.dx ? xgemm_splits(p.d, slab, p.vocab) : 1;
+  const XgPlan dx_plan = xgemm_plan(p.d, slab, ldq, true), dw_plan = xgemm_plan(p.d, p.vocab, slab, false);
+  const int splits = p.dx ? dx_plan.splits : 1;
   Ws m(p.ws);
   float* const weight = m.take<float>(1);
   XentBf16Args a{};
@@ -330,7 +331,7 @@ int lce_bf16(const Lce& p) {
     g.ref = a.ref;
     g.target = a.col;
     g.sums = sums;
-    PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, p.st), "logits"));
+    PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, 256, p.st), "logits"));
     PSGDK_TRY(hip_check(xent_join_launch(a, 0, p.st), "cross entropy sums"));
     // rows whose reference was too low: their maximum, then their blocks once more (nothing where there are none)
     XgArgs t = g;
@@ -338,9 +339,9 @@ int lce_bf16(const Lce& p) {
     t.max_only = 1;
     t.tops = sums;  // of whole blocks, which all get their sums again
     t.redo = g.redo = a.redo;
-    PSGDK_TRY(hip_check(xgemm_launch(t, XG_LOGITS, p.st), "largest logits"));
+    PSGDK_TRY(hip_check(xgemm_launch(t, XG_LOGITS, 256, p.st), "largest logits"));
     PSGDK_TRY(hip_check(xent_top_launch(a, p.st), "largest logits of rows"));
-    PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, p.st), "logits again"));
+    PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, 256, p.st), "logits again"));
     PSGDK_TRY(hip_check(xent_join_launch(a, 1, p.st), "cross entropy sums again"));
     if (!grad) continue;
     PSGDK_TRY(hip_check(xent_dz_launch(a, p.st), "logits' gradients"));
@@ -360,7 +361,7 @@ int lce_bf16(const Lce& p) {
       x.alpha = alpha;
       x.outf = splits > 1 ? dxp : nullptr;
       x.kreal = (int)p.vocab;
-      PSGDK_TRY(hip_check(xgemm_launch(x, XG_DX, p.st), "dx"));
+      PSGDK_TRY(hip_check(xgemm_launch(x, XG_DX, dx_plan.bm, p.st), "dx"));
       if (splits > 1)
         PSGDK_TRY(hip_check(to_bf16_rows_launch(dxp, splits, ld, alpha, out, p.lddx, n, (int)p.d, p.st), "dx sums"));
     }
@@ -379,7 +380,7 @@ int lce_bf16(const Lce& p) {
       x.alpha = alpha;
       x.outf = sum_w ? dwf : nullptr;
       x.accumulate = r0 != 0;
-      PSGDK_TRY(hip_check(xgemm_launch(x, XG_DW, p.st), "dw"));
+      PSGDK_TRY(hip_check(xgemm_launch(x, XG_DW, dw_plan.bm, p.st), "dw"));
     }
   }
   if (sum_w)

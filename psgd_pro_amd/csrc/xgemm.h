@@ -41,9 +41,12 @@ enum XgKind : int {
   XG_DX = 1,      // A mn-contiguous, B k-contiguous: m = d (W), n rows (dz), k vocabulary
   XG_DW = 2,      // both mn-contiguous: m = d (x), n vocabulary (dz), k rows
 };
-// sets the tile counts and, for splits > 1, kchunk
-hipError_t xgemm_launch(XgArgs& a, int kind, hipStream_t st);
-// k splits that fill the GPU's CUs
-int xgemm_splits(long long M, long long N, long long K);
+// How a product with out M x N (XG_DX, XG_DW) is cut: 256 or 128 rows of m a tile, and parts of k (1 without can_split)
+struct XgPlan {
+  int bm, splits;
+};
+XgPlan xgemm_plan(long long M, long long N, long long K, bool can_split);
+// sets the tile counts and kchunk; bm: 256 for XG_LOGITS
+hipError_t xgemm_launch(XgArgs& a, int kind, int bm, hipStream_t st);
 
 }  // namespace psgdk

@@ -1,4 +1,5 @@
 // The bf16 products of the cross entropy on v_mfma_f32_32x32x16_bf16, operands moved from HBM straight into LDS.
+#include <cmath>
 #include <type_traits>
 
 #include "xgemm.h"
@@ -177,8 +178,7 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
   // LDS offset of this lane's first fragment read inside a stage. The others differ by a constant, and by an XOR of the
   // k step (k-contiguous: chunk 2 ks + hh of the row) or of the 32-block (mn-contiguous), which the swizzles let pass.
   const int rr = (lane & 15) >> 2;
-  static_assert(WTM % 128 == 0 || !MCA, "the 32-blocks of a wave differ in the lowest bits of their number");
-  static_assert(WTN % 128 == 0 || !MCB, "the 32-blocks of a wave differ in the lowest bits of their number");
+  static_assert((FM & (FM - 1)) == 0 && (FN & (FN - 1)) == 0, "a wave's 32-blocks differ in the lowest bits of their number");
   const unsigned oa = MCA ? (8 * hh + rr) * BM * 2 + (((wm * WTM >> 5) ^ TA::swm(8 * hh + rr)) << 6) + (lane >> 4 & 1) * 32 +
                                 (lane & 3) * 8
                           : (wm * WTM + c) * BK * 2 + ((hh ^ TA::swk(c)) << 4);
@@ -426,18 +426,40 @@ static hipError_t launch_x(XgArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-int xgemm_splits(long long M, long long N, long long K) {
-  const long long tiles = ((M + 255) / 256) * ((N + 255) / 256);
-  long long s = 1;
-  while (s < 16 && tiles * s < 256 && K / (s * 2) >= 512) s *= 2;
-  return (int)s;
+// The time of whole rounds of one workgroup a CU: a CU multiplies a 256 x 256 tile at 5.3 TFLOP/s (4096 x 4096 x 131072:
+// 1360 TFLOP/s) and a 128 x 256 one, whose fragments are read 1.5 times as often, at 4.2 (1080). Small tiles win where
+// large ones fill half a round or pad m: 1531 x 770 x 50021 dw 188 -> 160 us, dx 164 -> 154. A further part of k costs
+// fp32 sums written and read.
+XgPlan xgemm_plan(long long M, long long N, long long K, bool can_split) {
+  XgPlan best{256, 1};
+  double least = 1e30;
+  for (int bm : {256, 128}) {
+    const double tiles = (double)((M + bm - 1) / bm) * (double)((N + 255) / 256);
+    const double tile = 2. * bm * 256 / (bm == 256 ? 5.3e12 : 4.2e12);  // a k
+    for (int s = 1; s <= (can_split ? 32 : 1) && (s == 1 || K / s >= 512); ++s) {
+      const double rounds = std::ceil(tiles * s / 256), t = rounds * tile * (double)((K + s - 1) / s) +
+                            (s > 1 ? 8. * s * (double)M * (double)N / 5e12 + 3e-6 : 0.);
+      if (t < least) {
+        least = t;
+        best = XgPlan{bm, s};
+      }
+    }
+  }
+  return best;
 }
 
-hipError_t xgemm_launch(XgArgs& a, int kind, hipStream_t st) {
+hipError_t xgemm_launch(XgArgs& a, int kind, int bm, hipStream_t st) {
   if (kind == XG_LOGITS) return launch_x<128, 128, 64, 2, false, false, XG_LOGITS>(a, st);
-  if (kind == XG_DX)
+  if (kind == XG_DX) {
+    if (bm == 128)
+      return a.outf ? launch_x<64, 128, 64, 3, true, false, XG_DX, true>(a, st)
+                    : launch_x<64, 128, 64, 3, true, false, XG_DX>(a, st);
     return a.outf ? launch_x<128, 128, 64, 2, true, false, XG_DX, true>(a, st)
                   : launch_x<128, 128, 64, 2, true, false, XG_DX>(a, st);
+  }
+  if (bm == 128)
+    return a.outf ? launch_x<64, 128, 64, 3, true, true, XG_DW, true>(a, st)
+                  : launch_x<64, 128, 64, 3, true, true, XG_DW>(a, st);
   return a.outf ? launch_x<128, 128, 64, 2, true, true, XG_DW, true>(a, st)
                 : launch_x<128, 128, 64, 2, true, true, XG_DW>(a, st);
 }
