@@ -178,9 +178,10 @@ int lce_pointers(const Lce& p) {
   if (p.dw) PSGDK_TRY(check_rows(p.dw, p.lddw, p.d, "dw"));
   return PSGDK_OK;
 }
-int lce_mean(const Lce& p, const float* weight) {
+int lce_mean(const Lce& p) {
   if (!p.mean_loss) return PSGDK_OK;
-  return hip_check(xent_mean_launch(p.loss, p.row_weight, weight, p.rows, p.mean_loss, p.st), "cross entropy mean");
+  return hip_check(xent_mean_launch(p.loss, p.row_weight, p.target, p.rows, p.ignore, p.mean, p.mean_loss, p.st),
+                   "cross entropy mean");
 }
 
 // float32: the logits of a slab of rows by the converting engine, a pass over them, and its products with W and x.
@@ -228,7 +229,7 @@ int lce_f32(const Lce& p) {
                            r0 ? 1.f : 0.f, &out, p.lddw, st));
     }
   }
-  return lce_mean(p, weight);
+  return lce_mean(p);
 }
 
 // bfloat16, a few rows, losses only
@@ -239,7 +240,6 @@ int lce_few(const Lce& p) {
   a.vocab = (int)p.vocab;
   a.wgs = xent_few_wgs(a.vocab);
   Ws m(p.ws);
-  float* const weight = m.take<float>(1);
   a.zt = m.take<float>(64);
   a.part = m.take<float2>((size_t)a.wgs * 64);
   bool done;
@@ -254,9 +254,7 @@ int lce_few(const Lce& p) {
   a.target = p.target;
   a.loss = p.loss;
   PSGDK_TRY(hip_check(xent_few_launch(a, p.st), "cross entropy of a few rows"));
-  if (!p.mean_loss) return PSGDK_OK;
-  PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
-  return lce_mean(p, weight);
+  return lce_mean(p);
 }
 
 // bfloat16: the logits of a slab of rows as 16-bit codes with the sums of their exponentials (one product), a pass that
@@ -290,7 +288,8 @@ int lce_bf16(const Lce& p) {
   PSGDK_TRY(lce_ws(p, m, done));
   if (done) return PSGDK_OK;
   PSGDK_TRY(lce_pointers(p));
-  PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
+  if (grad && p.mean)
+    PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
   const bf16_t* w = static_cast<const bf16_t*>(p.w);
   int64_t ldw = p.ldw;
   if (copy_w) {
@@ -386,7 +385,7 @@ int lce_bf16(const Lce& p) {
   if (sum_w)
     PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, 1, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab, (int)p.d, p.st),
                         "dw sums"));
-  return lce_mean(p, weight);
+  return lce_mean(p);
 }
 
 }  // namespace

@@ -8,9 +8,9 @@ namespace psgdk {
 // weight[0] = mean ? 1 / max(1, rows whose target is not `ignore`) : 1
 hipError_t xent_weight_launch(const int64_t* target, long long rows, int64_t ignore, int mean, float* weight,
                               hipStream_t st);
-// out[0] = sum_i w_i loss[i], w_i = row_weight[i], or weight[0] where row_weight is null; in a fixed order
-hipError_t xent_mean_launch(const float* loss, const float* row_weight, const float* weight, long long rows, float* out,
-                            hipStream_t st);
+// out[0] = sum_i w_i loss[i], w_i = row_weight[i], or where that is null as in xent_weight_launch; in a fixed order
+hipError_t xent_mean_launch(const float* loss, const float* row_weight, const int64_t* target, long long rows,
+                            int64_t ignore, int mean, float* out, hipStream_t st);
 
 // Rows of logits held in memory (fp32, row stride ldz): loss of each row and, with grad, the logits replaced by their
 // gradients.

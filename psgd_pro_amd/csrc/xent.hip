@@ -3,17 +3,22 @@
 
 namespace psgdk {
 
-__global__ void __launch_bounds__(1024) xent_weight_kernel(const int64_t* target, long long rows, int64_t ignore,
-                                                           int mean, float* weight) {
+// of one workgroup: 1 / the number of rows that count, or 1
+__device__ __forceinline__ float count_weight(const int64_t* target, long long rows, int64_t ignore, int mean) {
   __shared__ int total;
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
   int n = 0;
   if (mean)
     for (long long i = threadIdx.x; i < rows; i += 1024) n += target[i] != ignore;
-  atomicAdd(&total, n);  // whole numbers: any order gives the same sum
+  if (n) atomicAdd(&total, n);  // whole numbers: any order gives the same sum
   __syncthreads();
-  if (threadIdx.x == 0) weight[0] = mean ? 1.f / (float)max(total, 1) : 1.f;
+  return mean ? 1.f / (float)max(total, 1) : 1.f;
+}
+__global__ void __launch_bounds__(1024) xent_weight_kernel(const int64_t* target, long long rows, int64_t ignore,
+                                                           int mean, float* weight) {
+  const float w = count_weight(target, rows, ignore, mean);
+  if (threadIdx.x == 0) weight[0] = w;
 }
 hipError_t xent_weight_launch(const int64_t* target, long long rows, int64_t ignore, int mean, float* weight,
                               hipStream_t st) {
@@ -21,17 +26,19 @@ hipError_t xent_weight_launch(const int64_t* target, long long rows, int64_t ign
   return hipGetLastError();
 }
 
-__global__ void __launch_bounds__(1024) xent_mean_kernel(const float* loss, const float* row_weight, const float* weight,
-                                                         long long rows, float* out) {
+__global__ void __launch_bounds__(1024) xent_mean_kernel(const float* loss, const float* row_weight,
+                                                         const int64_t* target, long long rows, int64_t ignore,
+                                                         int mean, float* out) {
   __shared__ float red[16];
+  const float w = row_weight ? 1.f : count_weight(target, rows, ignore, mean);
   float s = 0.f;
   for (long long i = threadIdx.x; i < rows; i += 1024) s += row_weight ? row_weight[i] * loss[i] : loss[i];
   s = block_sum(s, red);
-  if (threadIdx.x == 0) out[0] = row_weight ? s : s * weight[0];
+  if (threadIdx.x == 0) out[0] = s * w;
 }
-hipError_t xent_mean_launch(const float* loss, const float* row_weight, const float* weight, long long rows, float* out,
-                            hipStream_t st) {
-  hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, st, loss, row_weight, weight, rows, out);
+hipError_t xent_mean_launch(const float* loss, const float* row_weight, const int64_t* target, long long rows,
+                            int64_t ignore, int mean, float* out, hipStream_t st) {
+  hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, st, loss, row_weight, target, rows, ignore, mean, out);
   return hipGetLastError();
 }
 
@@ -297,6 +304,7 @@ __global__ void __launch_bounds__(256) xent_few_kernel(const XentFewArgs a) {
 #pragma unroll
     for (int i = 0; i < MV; ++i) wr[i] = a.w + (long long)min(v0 + 16 * i + r, a.vocab - 1) * a.ldw;
     const int whole = a.d & ~31;
+#pragma unroll 4
     for (int k = 0; k < whole; k += 32) {
       bf16x8_t fx[NB], fw[MV];
 #pragma unroll

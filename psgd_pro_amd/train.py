@@ -274,20 +274,20 @@ def residual_norm(x, f=None, *, pre="rms", post=None, pre_weight=None, pre_bias=
 # -- linear_cross_entropy -----------------------------------------------------------------------------------------------
 
 
-def _lce_call(x, w, target, ignore, row_weight, mean, want_x, want_w):
-    """(losses, their weighted sum, dx, dw)"""
+def _lce_call(x, w, target, ignore, row_weight, reduction, want_x, want_w):
+    """(losses, their mean or sum (reduction "none": None), dx, dw)"""
     xr, wr, t = _rows(x), _rows(w), target.reshape(-1).contiguous()
     n, d = xr.shape
     loss = torch.empty(n, device=x.device)
-    total = torch.empty((), device=x.device)
+    total = None if reduction == "none" else torch.empty((), device=x.device)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
     dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if want_w else None
     if not n:
-        return loss, total.zero_(), dx, None if dw is None else dw.zero_()
+        return loss, None if total is None else total.zero_(), dx, None if dw is None else dw.zero_()
     with _on(x):
         L.call_ws(L.lib().psgdk_linear_cross_entropy, n, d, wr.shape[0], L.dtype_code(x.dtype), xr.data_ptr(), _ld(xr),
-                  wr.data_ptr(), _ld(wr), t.data_ptr(), ignore, _ptr(row_weight), int(mean), loss.data_ptr(),
-                  total.data_ptr(), _ptr(dx), d, _ptr(dw), d, ws=L.Workspace(), device=x.device, stream=L.stream_of(x))
+                  wr.data_ptr(), _ld(wr), t.data_ptr(), ignore, _ptr(row_weight), int(reduction == "mean"),
+                  loss.data_ptr(), _ptr(total), _ptr(dx), d, _ptr(dw), d, ws=L.Workspace(), device=x.device, stream=L.stream_of(x))
     return loss, total, dx, dw
 
 
@@ -300,8 +300,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, x, w, target, ignore, reduction):
         reduced = reduction != "none"
         need = ctx.needs_input_grad
-        loss, total, dx, dw = _lce_call(x, w, target, ignore, None, reduction == "mean", reduced and need[0],
-                                        reduced and need[1])
+        loss, total, dx, dw = _lce_call(x, w, target, ignore, None, reduction, reduced and need[0], reduced and need[1])
         ctx.save_for_backward(x, w, target)
         ctx.args = ignore, reduction
         ctx.grads = (dx, dw) if reduced else None
@@ -315,10 +314,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         need = ctx.needs_input_grad
         if reduction == "none":
             g = g.reshape(-1).float().contiguous()
-            return (*_lce_call(x, w, target, ignore, g, False, need[0], need[1])[2:], None, None, None)
+            return (*_lce_call(x, w, target, ignore, g, reduction, need[0], need[1])[2:], None, None, None)
         grads, ctx.grads = ctx.grads, None
         if grads is None:
-            grads = _lce_call(x, w, target, ignore, None, reduction == "mean", need[0], need[1])[2:]
+            grads = _lce_call(x, w, target, ignore, None, reduction, need[0], need[1])[2:]
         ts = [t for t in grads if t is not None and t.numel()]
         if ts:
             g = g.float()
@@ -347,5 +346,5 @@ def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mea
         raise ValueError(f"reduction = {reduction!r}: 'mean', 'sum' or 'none'")
     if _wants_grad(x, weight):
         return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), reduction)
-    loss, total, _, _ = _lce_call(x, weight, target, int(ignore_index), None, reduction == "mean", False, False)
+    loss, total, _, _ = _lce_call(x, weight, target, int(ignore_index), None, reduction, False, False)
     return loss.view(target.shape) if reduction == "none" else total
