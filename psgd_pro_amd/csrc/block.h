@@ -61,13 +61,25 @@ struct ResArgs {
   long long parts;          // workgroups
   long long chunk;          // rows of a workgroup: whole gates' rows, or a part of one gate's
   long long per_gate;       // workgroups that share one gate row (1 where a workgroup has whole gates)
-  float4* means;            // res_wide rows: one float4 each for the column kernel
+  float4* means;            // res_backward_wide: one float4 a row for the column kernel
 };
 enum { kSumPreW = 0, kSumPreB = 1, kSumPostW = 2, kSumPostB = 3 };
 // Rows that do not stay in registers but are read again for each pass: under one vector of 8 elements, over 8192, and
 // (1024 threads have no registers for the masks) over 4096 with an end inside a vector.
 inline bool res_wide(long long d) { return d < 8 || d > 8192 || (d > 4096 && d % 8 != 0); }
 constexpr int kMaxNormD = 1 << 20;
+
+// What a backward call has beside a root-mean-square norm before the next block.
+enum : int { kPost = 1, kGate = 2, kBias = 4 };
+inline int res_has(const ResArgs& a) {
+  return (a.post != NORM_NONE ? kPost : 0) | (a.gate.p ? kGate : 0) |
+         (a.pre == NORM_LAYER || a.post == NORM_LAYER ? kBias : 0);
+}
+// The backward pass also reads rows over 4096 again where it has two of these (registers again).
+inline bool res_backward_wide(const ResArgs& a) {
+  const int h = res_has(a);
+  return res_wide(a.d) || (a.d > 4096 && (h & (h - 1)) != 0);
+}
 
 hipError_t residual_norm_launch(const ResArgs& a, hipStream_t st);
 // rows of one workgroup and the number of workgroups of the backward pass (chunk, per_gate, parts); whole_gates: the

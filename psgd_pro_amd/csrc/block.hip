@@ -70,17 +70,27 @@ struct Span {
     at = RAGGED ? min(c, d - VE) : c;
     move = c - at;
   }
-  __device__ __forceinline__ void zero(float (&v)[VE]) const {
+  // The load in two parts, so that the bits of the next row can be on their way while this one's are used.
+  template <typename T>
+  struct Raw {
+    uint32_t w[VE * sizeof(T) / 4];
+  };
+  template <typename T>
+  __device__ __forceinline__ void fetch(const T* row, Raw<T>& r) const {
+    if (in) {
+      __builtin_memcpy(r.w, row + at, sizeof r.w);
+    } else {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) v[e] = 0.f;
+      for (uint32_t& x : r.w) x = 0;
+    }
   }
   template <typename T>
-  __device__ __forceinline__ void load(const T* row, float (&v)[VE]) const {
-    if (!in) {
-      zero(v);
-      return;
+  __device__ __forceinline__ void use(const Raw<T>& r, float (&v)[VE]) const {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      if constexpr (sizeof(T) == 2) v[e] = __uint_as_float(e & 1 ? r.w[e / 2] & 0xffff0000u : r.w[e / 2] << 16);
+      else v[e] = __uint_as_float(r.w[e]);
     }
-    ld8(row + at, v);
     if constexpr (RAGGED) {
 #pragma unroll
       for (int s = 4; s > 0; s >>= 1) {
@@ -89,6 +99,16 @@ struct Span {
         for (int e = 0; e < VE; ++e) v[e] = m ? (e + s < VE ? v[e + s] : 0.f) : v[e];
       }
     }
+  }
+  __device__ __forceinline__ void zero(float (&v)[VE]) const {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = 0.f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, float (&v)[VE]) const {
+    Raw<T> r;
+    fetch(row, r);
+    use(r, v);
   }
   __device__ __forceinline__ void load(const Vec& w, long long off, float none, float (&v)[VE]) const {
     if (!w.p) {
@@ -161,11 +181,20 @@ namespace {
 
 constexpr int res_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 
+// Sum over a wave, in all lanes: the 16 lanes of each row by DPP moves, then the four rows' sums read as scalars (six
+// shuffles through LDS take several times as long, and a row's time is a chain of these sums).
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = row16_sum(v);
+  const int i = __float_as_int(v);
+  return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
+}
+
 // Sums over the TPR threads of a row, every thread of the workgroup taking part. red holds one value for each wave; its
 // next use has to come after a barrier.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-  v = wave_sum(v);
+  v = lanes_sum(v);
   if constexpr (TPR > 64) {
     const int w = threadIdx.x >> 6, w0 = w / (TPR / 64) * (TPR / 64);
     if ((threadIdx.x & 63) == 0) red[w] = v;
@@ -178,11 +207,8 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 }
 template <int TPR>
 __device__ __forceinline__ float2 row_sum2(float2 v, float2* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    v.x += __shfl_xor(v.x, o, 64);
-    v.y += __shfl_xor(v.y, o, 64);
-  }
+  v.x = lanes_sum(v.x);
+  v.y = lanes_sum(v.y);
   if constexpr (TPR > 64) {
     const int w = threadIdx.x >> 6, w0 = w / (TPR / 64) * (TPR / 64);
     if ((threadIdx.x & 63) == 0) red[w] = v;
@@ -403,15 +429,26 @@ __device__ __forceinline__ void put_sum(float (&s)[VE], float* dst, const Span<R
   sp.zero(s);
 }
 
-// SUMS: column sums in registers (bit 0: of the norm before, bit 1: of the norm after, bit 2: of the gate)
-template <typename T, int TPR, int SUMS, bool RAGGED>
-__global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kernel(const ResArgs a) {
+// HAS: what the call may have (kPost: a norm after the block, kGate, kBias: a layer norm's biases); what it cannot have
+// holds no registers. SUMS: column sums in registers (1: of the norm before, 2: of the norm after, 4: of the gate).
+// Waves a SIMD, by what their registers hold without scratch memory: two workgroups of 512 threads want 128 registers,
+// three of 256 threads 168.
+constexpr int res_waves(int tpr, int has, int esize, bool ragged) {
+  if (tpr == 1024) return 4;
+  if (tpr == 512) return !ragged && (has == 0 || has == kBias || (has == kPost && esize == 2)) ? 4 : 2;
+  return ragged || has == 7 || (has == (kPost | kGate) && esize == 4) ? 2 : 3;
+}
+template <typename T, int TPR, int HAS, int SUMS, bool RAGGED>
+__global__ void __launch_bounds__(res_threads(TPR), res_waves(TPR, HAS, sizeof(T), RAGGED))
+    residual_norm_backward_kernel(const ResArgs a) {
   constexpr int RW = res_threads(TPR) / TPR;  // rows the workgroup has in hand at once
+  constexpr bool AHEAD = TPR < 1024;          // 1024 threads have no registers for the next row's bits
   __shared__ float2 red[2][16];
-  __shared__ float lds[TPR < 256 && SUMS ? VE * 256 : 1];
+  __shared__ float lds[TPR < 256 ? VE * 256 : 1];
   // a row's waves are whole: its number is a scalar, and so are the addresses of its start
   const int t = threadIdx.x % TPR, w = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
-  const Span<RAGGED> sp(t * VE, a.d);
+  using Sp = Span<RAGGED>;
+  const Sp sp(t * VE, a.d);
   // rows r0 .. r1 - 1: `chunk` rows (whole gates), or a part of one gate's
   long long r0, r1;
   if (a.per_gate > 1) {
@@ -424,6 +461,8 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kerne
   }
   float s_pw[VE] = {}, s_pb[VE] = {}, s_qw[VE] = {}, s_qb[VE] = {}, s_g[VE] = {};
   const float inv_d = 1.f / (float)a.d;
+  const bool post = (HAS & kPost) && a.post != NORM_NONE, gated = (HAS & kGate) && a.gate.p;
+  const bool pre_layer = (HAS & kBias) && a.pre == NORM_LAYER, post_layer = (HAS & kBias) && a.post == NORM_LAYER;
 
   // The weights of a row, read again for each row where a thread has no registers left to keep them (1024 threads have
   // 128 each): an empty asm statement hides from the compiler that the addresses stay the same.
@@ -432,19 +471,32 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kerne
     if constexpr (TPR == 1024) asm volatile("" : "+s"(q.p));
     return q;
   };
-  auto one_row = [&](long long want, bool live) {
-    const long long row = live ? want : r0;  // a row behind the last one takes part in the barriers only
-    const float4 st = a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+  struct Bits {
+    typename Sp::template Raw<T> x, f, dy, dh;
+    float4 st;
+  };
+  auto fetch = [&](long long row, Bits& r) {
+    r.st = a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.dy) sp.fetch(reinterpret_cast<const T*>(a.dy) + row * a.lddy, r.dy);
+    if (a.f) sp.fetch(reinterpret_cast<const T*>(a.f) + row * a.ldf, r.f);
+    if (a.dh) {
+      sp.fetch(reinterpret_cast<const T*>(a.x) + row * a.ldx, r.x);
+      sp.fetch(reinterpret_cast<const T*>(a.dh) + row * a.lddh, r.dh);
+    }
+  };
+  auto one_row = [&](long long row, bool live, const Bits& r) {
+    const float4 st = r.st;
     float v[VE], fh[VE], b[VE], g[VE], wt[VE];  // v: dyt, then du
     unsigned kept = 0;
-    if (a.dy) sp.load(reinterpret_cast<const T*>(a.dy) + row * a.lddy, v);
+    if (a.dy) sp.use(r.dy, v);
     else sp.zero(v);
     if (a.f) {  // the branch again: fh = f's normalised values, b = dropout(Npost(f))
-      sp.load(reinterpret_cast<const T*>(a.f) + row * a.ldf, fh);
-      sp.load(vec(a.gate), row / a.gate_every * a.ldg, 1.f, g);
-      if (a.post != NORM_NONE) {
+      sp.use(r.f, fh);
+      if (gated) sp.load(vec(a.gate), row / a.gate_every * a.ldg, 1.f, g);
+      if (post) {
         sp.load(vec(a.post_w), 0, 1.f, wt);
-        sp.load(vec(a.post_b), 0, 0.f, b);
+        if (post_layer) sp.load(vec(a.post_b), 0, 0.f, b);
+        else sp.zero(b);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           fh[e] = (fh[e] - st.z) * st.w;
@@ -465,28 +517,28 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kerne
       }
     }
     if (a.dh) {
-      float hat[VE], c[VE], w[VE];
+      float hat[VE], c[VE], pw[VE];
       float2 m = make_float2(0.f, 0.f);
-      sp.load(reinterpret_cast<const T*>(a.x) + row * a.ldx, hat);
-      sp.load(reinterpret_cast<const T*>(a.dh) + row * a.lddh, c);
-      sp.load(vec(a.pre_w), 0, 1.f, w);
+      sp.use(r.x, hat);
+      sp.use(r.dh, c);
+      sp.load(vec(a.pre_w), 0, 1.f, pw);
       if (a.f) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) hat[e] += a.scale * g[e] * b[e];
+        for (int e = 0; e < VE; ++e) hat[e] += gated ? a.scale * g[e] * b[e] : a.scale * b[e];
       }
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         hat[e] = (hat[e] - st.x) * st.y;
         if constexpr (SUMS & 1) {
           s_pw[e] += live ? c[e] * hat[e] : 0.f;
-          s_pb[e] += live ? c[e] : 0.f;
+          if constexpr (HAS & kBias) s_pb[e] += live ? c[e] : 0.f;
         }
-        c[e] *= w[e];
+        c[e] *= pw[e];
         m.x += c[e];
         m.y += c[e] * hat[e];
       }
       m = row_sum2<TPR>(m, red[0]);
-      m.x = a.pre == NORM_LAYER ? m.x * inv_d : 0.f;
+      m.x = pre_layer ? m.x * inv_d : 0.f;
       m.y *= inv_d;
 #pragma unroll
       for (int e = 0; e < VE; ++e) v[e] += (c[e] - m.x - hat[e] * m.y) * st.y;
@@ -496,20 +548,22 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kerne
       float2 m = make_float2(0.f, 0.f);
       float dg[VE];
       if constexpr (TPR == 1024) {
-        sp.load(vec(a.gate), row / a.gate_every * a.ldg, 1.f, g);
-        if (a.post != NORM_NONE) sp.load(vec(a.post_w), 0, 1.f, wt);
+        if (gated) sp.load(vec(a.gate), row / a.gate_every * a.ldg, 1.f, g);
+        if (post) sp.load(vec(a.post_w), 0, 1.f, wt);
       }
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         float du = sp.has(e) ? a.scale * v[e] : 0.f;
-        dg[e] = du * b[e];
-        du *= g[e];
+        if (gated) {
+          dg[e] = du * b[e];
+          du *= g[e];
+          if constexpr ((SUMS & 4) && (HAS & kGate)) s_g[e] += live ? dg[e] : 0.f;
+        }
         if (a.drop.thr) du = kept >> e & 1 ? du * a.drop.scale : 0.f;
-        if constexpr (SUMS & 4) s_g[e] += live ? dg[e] : 0.f;
-        if (a.post != NORM_NONE) {
-          if constexpr (SUMS & 2) {
+        if (post) {
+          if constexpr ((SUMS & 2) && (HAS & kPost)) {
             s_qw[e] += live ? du * fh[e] : 0.f;
-            s_qb[e] += live ? du : 0.f;
+            if constexpr (HAS & kBias) s_qb[e] += live ? du : 0.f;
           }
           du *= wt[e];
           m.x += du;
@@ -517,13 +571,13 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kerne
         }
         v[e] = du;
       }
-      if (a.dgate && a.gate_every == 1 && live) {  // a gate for each row: no sum
+      if (gated && a.dgate && a.gate_every == 1 && live) {  // a gate for each row: no sum
         if (a.gate.dt == 1) sp.store(reinterpret_cast<bf16_t*>(a.dgate) + row * a.lddg, dg);
         else sp.store(reinterpret_cast<float*>(a.dgate) + row * a.lddg, dg);
       }
-      if (a.post != NORM_NONE) {
+      if (post) {
         m = row_sum2<TPR>(m, red[1]);
-        m.x = a.post == NORM_LAYER ? m.x * inv_d : 0.f;
+        m.x = post_layer ? m.x * inv_d : 0.f;
         m.y *= inv_d;
 #pragma unroll
         for (int e = 0; e < VE; ++e) v[e] = (v[e] - m.x - fh[e] * m.y) * st.w;
@@ -533,12 +587,26 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kerne
     if constexpr (TPR > 64) __syncthreads();  // red is free again
   };
 
-  const bool whole_gates = (SUMS & 4) && a.gpart && a.per_gate == 1;
+  const bool gate_sums = (SUMS & 4) && (HAS & kGate) && a.gpart;
+  const bool whole_gates = gate_sums && a.per_gate == 1;
   const long long step = whole_gates ? a.gate_every : r1 - r0;
   for (long long b0 = r0; b0 < r1; b0 += step) {
     const long long b1 = min(b0 + step, r1);
-    for (long long row = b0; row < b1; row += RW) one_row(row + w, row + w < b1);
-    if ((SUMS & 4) && a.gpart)
+    // a row behind the last one takes part in the barriers only
+    auto row_of = [&](long long row) { return row + w < b1 ? row + w : b1 - 1; };
+    Bits next;
+    if constexpr (AHEAD) fetch(row_of(b0), next);
+    for (long long row = b0; row < b1; row += RW) {
+      Bits now;
+      if constexpr (AHEAD) {
+        now = next;
+        if (row + RW < b1) fetch(row_of(row + RW), next);
+      } else {
+        fetch(row_of(row), now);
+      }
+      one_row(row_of(row), row + w < b1, now);
+    }
+    if (gate_sums)
       put_sum<TPR, RAGGED>(s_g, a.gpart + (whole_gates ? b0 / a.gate_every : (long long)blockIdx.x) * a.d, sp, lds);
   }
   auto put = [&](float (&s)[VE], int k) {
@@ -546,11 +614,11 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_backward_kerne
   };
   if constexpr (SUMS & 1) {
     put(s_pw, kSumPreW);
-    put(s_pb, kSumPreB);
+    if constexpr (HAS & kBias) put(s_pb, kSumPreB);
   }
-  if constexpr (SUMS & 2) {
+  if constexpr ((SUMS & 2) && (HAS & kPost)) {
     put(s_qw, kSumPostW);
-    put(s_qb, kSumPostB);
+    if constexpr (HAS & kBias) put(s_qb, kSumPostB);
   }
 }
 
@@ -769,9 +837,10 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums s) {
 }  // namespace
 
 void residual_norm_split(ResArgs& a, bool gate_sums) {
-  constexpr long long kTarget = 1024;  // workgroups: four for each CU
-  a.chunk = a.rows > kTarget ? (a.rows + kTarget - 1) / kTarget : 1;
+  // as many workgroups as are on the GPU's 256 CUs at once (1024 threads each)
   const long long at_once = a.d <= 512 ? 4 : a.d <= 1024 ? 2 : 1;
+  const long long target = a.d <= 2048 ? 1024 : a.d <= 4096 ? 512 : res_backward_wide(a) ? 1024 : 256;
+  a.chunk = a.rows > target ? (a.rows + target - 1) / target : 1;
   a.chunk = (a.chunk + at_once - 1) / at_once * at_once;
   a.per_gate = 1;
   if (gate_sums && a.gate_every > 1) {
@@ -781,45 +850,52 @@ void residual_norm_split(ResArgs& a, bool gate_sums) {
   a.parts = a.per_gate > 1 ? a.rows / a.gate_every * a.per_gate : (a.rows + a.chunk - 1) / a.chunk;
 }
 
-template <typename T, int TPR, bool RAGGED>
-static void residual_norm_backward_sized(const ResArgs& a, hipStream_t st) {
-  const bool post = a.slot[kSumPostW] >= 0 || a.slot[kSumPostB] >= 0;
-  const bool any = post || a.gpart || a.slot[kSumPreW] >= 0 || a.slot[kSumPreB] >= 0;
+template <typename T, int TPR, int HAS, bool RAGGED>
+static void residual_norm_backward_has(const ResArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)a.parts), block(res_threads(TPR));
 #define PSGDK_RES(SUMS, args) \
-  hipLaunchKernelGGL((residual_norm_backward_kernel<T, TPR, SUMS, RAGGED>), grid, block, 0, st, args)
-  if (!any) {
-    PSGDK_RES(0, a);
-  } else if (!post && !a.gpart) {
-    PSGDK_RES(1, a);
-  } else if constexpr (TPR == 1024) {  // no registers for all sums: the branch's come from a second pass
-    ResArgs q = a;
-    q.dx = q.df = q.dgate = nullptr;
-    q.slot[kSumPreW] = q.slot[kSumPreB] = -1;
-    PSGDK_RES(1, a);
-    PSGDK_RES(6, q);
-  } else if (!a.gpart) {
-    PSGDK_RES(3, a);
-  } else if (!post) {
-    PSGDK_RES(5, a);
-  } else {
+  hipLaunchKernelGGL((residual_norm_backward_kernel<T, TPR, HAS, SUMS, RAGGED>), grid, block, 0, st, args)
+  if constexpr (TPR < 1024) {
     PSGDK_RES(7, a);
+  } else {  // no registers for all sums: the branch's come from a second pass
+    PSGDK_RES(1, a);
+    if constexpr ((HAS & (kPost | kGate)) != 0) {
+      ResArgs q = a;
+      q.dx = q.df = q.dgate = nullptr;
+      q.slot[kSumPreW] = q.slot[kSumPreB] = -1;
+      if (a.gpart || a.slot[kSumPostW] >= 0 || a.slot[kSumPostB] >= 0) PSGDK_RES(6, q);
+    }
   }
 #undef PSGDK_RES
 }
-template <typename T, bool RAGGED>
-static void residual_norm_backward_rows(const ResArgs& a, hipStream_t st) {
-  if (a.d <= 512) residual_norm_backward_sized<T, 64, RAGGED>(a, st);
-  else if (a.d <= 1024) residual_norm_backward_sized<T, 128, RAGGED>(a, st);
-  else if (a.d <= 2048) residual_norm_backward_sized<T, 256, RAGGED>(a, st);
-  else if (a.d <= 4096) residual_norm_backward_sized<T, 512, RAGGED>(a, st);
-  else if constexpr (!RAGGED) residual_norm_backward_sized<T, 1024, false>(a, st);
+template <typename T, int TPR>
+static void residual_norm_backward_sized(const ResArgs& a, hipStream_t st) {
+  if constexpr (TPR < 1024) {
+    if (a.d % VE) return residual_norm_backward_has<T, TPR, kPost | kGate | kBias, true>(a, st);
+  }
+  switch (res_has(a)) {
+    case 0: return residual_norm_backward_has<T, TPR, 0, false>(a, st);
+    case 1: return residual_norm_backward_has<T, TPR, 1, false>(a, st);
+    case 2: return residual_norm_backward_has<T, TPR, 2, false>(a, st);
+    case 4: return residual_norm_backward_has<T, TPR, 4, false>(a, st);
+  }
+  if constexpr (TPR < 1024) {
+    switch (res_has(a)) {
+      case 3: return residual_norm_backward_has<T, TPR, 3, false>(a, st);
+      case 5: return residual_norm_backward_has<T, TPR, 5, false>(a, st);
+      case 6: return residual_norm_backward_has<T, TPR, 6, false>(a, st);
+      default: return residual_norm_backward_has<T, TPR, 7, false>(a, st);
+    }
+  }
 }
 template <typename T>
 static hipError_t residual_norm_backward_t(const ResArgs& a, hipStream_t st) {
-  if (!res_wide(a.d)) {
-    if (a.d % VE) residual_norm_backward_rows<T, true>(a, st);
-    else residual_norm_backward_rows<T, false>(a, st);
+  if (!res_backward_wide(a)) {
+    if (a.d <= 512) residual_norm_backward_sized<T, 64>(a, st);
+    else if (a.d <= 1024) residual_norm_backward_sized<T, 128>(a, st);
+    else if (a.d <= 2048) residual_norm_backward_sized<T, 256>(a, st);
+    else if (a.d <= 4096) residual_norm_backward_sized<T, 512>(a, st);
+    else residual_norm_backward_sized<T, 1024>(a, st);
   } else {
     hipLaunchKernelGGL(residual_norm_backward_wide_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
     bool any = a.gpart != nullptr;

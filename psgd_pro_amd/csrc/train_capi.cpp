@@ -456,7 +456,7 @@ int psgdk_residual_norm_backward(const psgdk_residual_norm_t* q, const psgdk_res
   a.part = w.take<float>((size_t)n * a.parts * a.d);
   a.gpart = w.take<float>(gate_sums ? (size_t)(a.per_gate > 1 ? a.parts : q->gate_rows) * a.d : 0);
   if (!gate_sums) a.gpart = nullptr;
-  a.means = w.take<float4>(res_wide(a.d) ? q->rows : 0);
+  a.means = w.take<float4>(res_backward_wide(a) ? q->rows : 0);
   if (!ws) {
     *ws_bytes = w.off;
     return PSGDK_OK;

@@ -1,4 +1,6 @@
 // Softmax cross entropy: the kernels around the products with the vocabulary matrix.
+#include <type_traits>
+
 #include "xent.h"
 
 namespace psgdk {
@@ -279,6 +281,7 @@ hipError_t xent_dz_launch(const XentBf16Args& a, hipStream_t st) {
 // the sum of exponentials under it; the lanes' and waves' pairs join at the end.
 template <int MV, int NB>
 __global__ void __launch_bounds__(256) xent_few_kernel(const XentFewArgs a) {
+  constexpr int UK = NB == 4 ? 2 : 4;
   __shared__ float2 red[4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
@@ -303,20 +306,29 @@ __global__ void __launch_bounds__(256) xent_few_kernel(const XentFewArgs a) {
     const bf16_t* wr[MV];
 #pragma unroll
     for (int i = 0; i < MV; ++i) wr[i] = a.w + (long long)min(v0 + 16 * i + r, a.vocab - 1) * a.ldw;
+    // U steps of 32 k at a time: their loads all go out before the first product
+    auto steps = [&](auto count, int k) {
+      constexpr int U = decltype(count)::value;
+      bf16x8_t fx[U][NB], fw[U][MV];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < MV; ++i) __builtin_memcpy(&fw[u][i], wr[i] + k + 32 * u + 8 * g, 16);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) __builtin_memcpy(&fx[u][b], xr[b] + k + 32 * u + 8 * g, 16);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < MV; ++i)
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[u][i], fx[u][b], acc[i][b], 0, 0, 0);
+    };
     const int whole = a.d & ~31;
-#pragma unroll 4
-    for (int k = 0; k < whole; k += 32) {
-      bf16x8_t fx[NB], fw[MV];
-#pragma unroll
-      for (int i = 0; i < MV; ++i) __builtin_memcpy(&fw[i], wr[i] + k + 8 * g, 16);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) __builtin_memcpy(&fx[b], xr[b] + k + 8 * g, 16);
-#pragma unroll
-      for (int i = 0; i < MV; ++i)
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i], fx[b], acc[i][b], 0, 0, 0);
-    }
+    int k = 0;
+    for (; k + 32 * UK <= whole; k += 32 * UK) steps(std::integral_constant<int, UK>{}, k);
+    for (; k < whole; k += 32) steps(std::integral_constant<int, 1>{}, k);
     if (whole < a.d) {
 #pragma unroll
       for (int i = 0; i < MV; ++i) {
