@@ -10,8 +10,6 @@ autograd. No counterparts in the reference, which leaves the model to torch.
 import ctypes as C
 
 import torch
-from torch.autograd.function import once_differentiable
-
 from . import _lib as L
 
 __all__ = ["dropout", "linear_cross_entropy", "residual_norm"]
@@ -30,30 +28,39 @@ def _check(t, name, like=None):
 
 
 def _rows(t):
-    """t as rows of its last dimension, contiguous inside a row (a view where its strides allow)."""
-    r = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
+    """(r, ld): t as rows of its last dimension, contiguous inside a row, ld elements from one to the next; r is t itself
+    where its rows lie one after the other, a view where its strides allow, else a copy."""
+    d = t.shape[-1]
+    if t.is_contiguous():
+        return t, d
+    r = t.reshape(-1, d) if t.dim() != 2 else t
+    if (d > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < d):
         r = r.contiguous()
-    return r
+    return r, r.stride(0) if r.shape[0] > 1 else d
 
 
-def _ld(r):
-    return r.stride(0) if r.shape[0] > 1 else r.shape[1]
+def _run(t, fn, *args):
+    """fn(*args, stream) on t's device and its current stream."""
+    i = t.device.index
+    if i == torch.cuda.current_device():
+        L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
+    else:
+        with torch.cuda.device(i):
+            L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
 
 
-class _on:
-    """The tensor's device made current for the launches (nothing to do where it is)."""
+def _run_ws(t, fn, *args):
+    """fn(*args, workspace, its size, stream): the size asked for first, the workspace back with torch's allocator after."""
+    size = C.c_size_t(0)
+    L.check(fn(*args, None, C.byref(size), None))
+    ws = torch.empty(max(size.value, 256), dtype=torch.uint8, device=t.device)
+    _run(t, fn, *args, ws.data_ptr(), C.byref(size))
 
-    def __init__(self, t):
-        self.ctx = None if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *e):
-        if self.ctx is not None:
-            self.ctx.__exit__(*e)
+def _once():
+    """The backward functions' outputs have no graph of their own."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("psgd_pro_amd ops differentiate once: no create_graph through them")
 
 
 def _wants_grad(*ts):
@@ -77,11 +84,10 @@ def _check_p(p):
 
 def _dropout_call(x, p, seed, stream):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if x.numel():
-        r = _rows(x)
-        with _on(x):
-            L.check(L.lib().psgdk_dropout(r.shape[0], r.shape[1], L.dtype_code(x.dtype), r.data_ptr(), _ld(r),
-                                          y.data_ptr(), r.shape[1], p, seed, stream, L.stream_of(x)))
+    n, d = x.numel(), x.shape[-1]
+    if n:
+        r, ld = _rows(x)
+        _run(x, L.lib().psgdk_dropout, n // d, d, L.dtype_code(x.dtype), r.data_ptr(), ld, y.data_ptr(), d, p, seed, stream)
     return y
 
 
@@ -92,8 +98,8 @@ class _Dropout(torch.autograd.Function):
         return _dropout_call(x, p, seed, stream)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _once()
         return _dropout_call(g, *ctx.args), None, None, None
 
 
@@ -125,23 +131,27 @@ def _ptr(t):
 def _res_block(x, f, gate, pw, pb, qw, qb, opt):
     """psgdk_residual_norm_t of the inputs, and the (possibly copied) tensors it points to."""
     pre, post, scale, eps, p, seed, stream, gate_rows = opt
-    xr = _rows(x)
-    fr = None if f is None else _rows(f)
-    gr = None if gate is None else _rows(gate)
-    w = [None if t is None else t.contiguous() for t in (pw, pb, qw, qb)]
+    d = x.shape[-1]
+    w = [t if t is None or t.is_contiguous() else t.contiguous() for t in (pw, pb, qw, qb)]
     a = L.ResidualNorm()
-    a.rows, a.d = xr.shape
+    a.rows, a.d = x.numel() // max(d, 1), d
     a.dtype = L.dtype_code(x.dtype)
     a.pre, a.post, a.eps, a.scale, a.p, a.seed, a.stream_id, a.gate_rows = pre, post, eps, scale, p, seed, stream, gate_rows
-    a.x, a.ldx = xr.data_ptr(), _ld(xr)
-    if fr is not None:
-        a.f, a.ldf = fr.data_ptr(), _ld(fr)
-    if gr is not None:
-        a.gate, a.ldgate, a.gate_dtype = gr.data_ptr(), _ld(gr), L.dtype_code(gate.dtype)
+    xr, a.ldx = _rows(x)
+    a.x = xr.data_ptr()
+    keep = [xr, w]
+    if f is not None:
+        fr, a.ldf = _rows(f)
+        a.f = fr.data_ptr()
+        keep.append(fr)
+    if gate is not None:
+        gr, a.ldgate = _rows(gate)
+        a.gate, a.gate_dtype = gr.data_ptr(), L.dtype_code(gate.dtype)
+        keep.append(gr)
     a.pre_w, a.pre_b, a.post_w, a.post_b = (_ptr(t) for t in w)
     some = next((t for t in w if t is not None), None)
     a.w_dtype = L.F32 if some is None else L.dtype_code(some.dtype)
-    return a, (xr, fr, gr, w)
+    return a, keep
 
 
 def _res_forward(x, f, gate, pw, pb, qw, qb, opt, stats):
@@ -151,8 +161,7 @@ def _res_forward(x, f, gate, pw, pb, qw, qb, opt, stats):
     st = torch.empty(a.rows, 4, device=x.device) if stats else None
     a.y, a.ldy, a.h, a.ldh, a.stats = _ptr(y), a.d, _ptr(h), a.d, _ptr(st)
     if x.numel() and (y is not None or h is not None):
-        with _on(x):
-            L.check(L.lib().psgdk_residual_norm(C.byref(a), L.stream_of(x)))
+        _run(x, L.lib().psgdk_residual_norm, C.byref(a))
     return y, h, st
 
 
@@ -168,19 +177,19 @@ class _ResidualNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh):
+        _once()
         x, f, gate, pw, pb, qw, qb, st = ctx.saved_tensors
         need = ctx.needs_input_grad
         a, keep = _res_block(x, f, gate, pw, pb, qw, qb, ctx.opt)
         a.stats = _ptr(st)
         g = L.ResidualNormGrads()
-        for name, t in (("dy", dy), ("dh", dh)):
-            if t is not None:
-                r = _rows(t)
-                keep += (r,)
-                setattr(g, name, r.data_ptr())
-                setattr(g, "ld" + name, _ld(r))
+        if dy is not None:
+            dy, g.lddy = _rows(dy)
+            g.dy = dy.data_ptr()
+        if dh is not None:
+            dh, g.lddh = _rows(dh)
+            g.dh = dh.data_ptr()
         outs = [None] * 8
         for k, (name, like) in enumerate((("dx", x), ("df", f), ("dgate", gate), ("dpre_w", pw), ("dpre_b", pb),
                                           ("dpost_w", qw), ("dpost_b", qb))):
@@ -195,9 +204,7 @@ class _ResidualNorm(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
         else:
-            with _on(x):
-                L.call_ws(L.lib().psgdk_residual_norm_backward, C.byref(a), C.byref(g), ws=L.Workspace(),
-                          device=x.device, stream=L.stream_of(x))
+            _run_ws(x, L.lib().psgdk_residual_norm_backward, C.byref(a), C.byref(g))
         return tuple(outs)
 
 
@@ -276,18 +283,17 @@ def residual_norm(x, f=None, *, pre="rms", post=None, pre_weight=None, pre_bias=
 
 def _lce_call(x, w, target, ignore, row_weight, reduction, want_x, want_w):
     """(losses, their mean or sum (reduction "none": None), dx, dw)"""
-    xr, wr, t = _rows(x), _rows(w), target.reshape(-1).contiguous()
-    n, d = xr.shape
+    (xr, ldx), (wr, ldw), t = _rows(x), _rows(w), target.contiguous()
+    n, d = t.numel(), x.shape[-1]
     loss = torch.empty(n, device=x.device)
     total = None if reduction == "none" else torch.empty((), device=x.device)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
     dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if want_w else None
     if not n:
         return loss, None if total is None else total.zero_(), dx, None if dw is None else dw.zero_()
-    with _on(x):
-        L.call_ws(L.lib().psgdk_linear_cross_entropy, n, d, wr.shape[0], L.dtype_code(x.dtype), xr.data_ptr(), _ld(xr),
-                  wr.data_ptr(), _ld(wr), t.data_ptr(), ignore, _ptr(row_weight), int(reduction == "mean"),
-                  loss.data_ptr(), _ptr(total), _ptr(dx), d, _ptr(dw), d, ws=L.Workspace(), device=x.device, stream=L.stream_of(x))
+    _run_ws(x, L.lib().psgdk_linear_cross_entropy, n, d, w.shape[0], L.dtype_code(x.dtype), xr.data_ptr(), ldx, wr.data_ptr(),
+            ldw, t.data_ptr(), ignore, _ptr(row_weight), int(reduction == "mean"), loss.data_ptr(), _ptr(total), _ptr(dx), d,
+            _ptr(dw), d)
     return loss, total, dx, dw
 
 
@@ -307,8 +313,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return total if reduced else loss.view(target.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _once()
         x, w, target = ctx.saved_tensors
         ignore, reduction = ctx.args
         need = ctx.needs_input_grad
@@ -322,8 +328,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if ts:
             g = g.float()
             n = (C.c_int64 * len(ts))(*[t.numel() for t in ts])
-            with _on(x):
-                L.check(L.lib().psgdk_scale_by(len(ts), n, L.dtype_code(x.dtype), L.ptrs(ts), g.data_ptr(), L.stream_of(x)))
+            _run(x, L.lib().psgdk_scale_by, len(ts), n, L.dtype_code(x.dtype), L.ptrs(ts), g.data_ptr())
         return (*grads, None, None, None)
 
 
