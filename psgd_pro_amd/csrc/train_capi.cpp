@@ -288,8 +288,6 @@ int lce_bf16(const Lce& p) {
   PSGDK_TRY(lce_ws(p, m, done));
   if (done) return PSGDK_OK;
   PSGDK_TRY(lce_pointers(p));
-  if (grad && p.mean)
-    PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
   const bf16_t* w = static_cast<const bf16_t*>(p.w);
   int64_t ldw = p.ldw;
   if (copy_w) {
@@ -301,6 +299,8 @@ int lce_bf16(const Lce& p) {
   a.vocab = (int)p.vocab;
   a.parts = (int)parts;
   a.ignore = p.ignore;
+  a.all_targets = p.target;
+  a.all_rows = p.rows;
   a.w = w;
   a.ldw = ldw;
   a.ldx = p.ldx;
@@ -331,7 +331,9 @@ int lce_bf16(const Lce& p) {
     g.target = a.col;
     g.sums = sums;
     PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, 256, p.st), "logits"));
+    a.weight = grad && p.mean && r0 == 0 ? weight : nullptr;
     PSGDK_TRY(hip_check(xent_join_launch(a, 0, p.st), "cross entropy sums"));
+    a.weight = nullptr;
     // rows whose reference was too low: their maximum, then their blocks once more (nothing where there are none)
     XgArgs t = g;
     t.q = nullptr;
@@ -341,8 +343,10 @@ int lce_bf16(const Lce& p) {
     PSGDK_TRY(hip_check(xgemm_launch(t, XG_LOGITS, 256, p.st), "largest logits"));
     PSGDK_TRY(hip_check(xent_top_launch(a, p.st), "largest logits of rows"));
     PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, 256, p.st), "logits again"));
-    PSGDK_TRY(hip_check(xent_join_launch(a, 1, p.st), "cross entropy sums again"));
-    if (!grad) continue;
+    if (!grad) {
+      PSGDK_TRY(hip_check(xent_join_launch(a, 1, p.st), "cross entropy sums again"));
+      continue;
+    }
     PSGDK_TRY(hip_check(xent_dz_launch(a, p.st), "logits' gradients"));
     if (p.dx) {
       bf16_t* const out = static_cast<bf16_t*>(p.dx) + r0 * p.lddx;

@@ -46,12 +46,16 @@ struct XentBf16Args {
   int* col;                 // the target's column; -1 for an ignored row, vocab for a foreign target (r is NaN then)
   int* redo;                // number of blocks of kXgRows rows with a row over the limit, and their numbers
   int* mark;                // of each block: whether it is listed
+  float* weight;            // null, or: xent_join_launch makes 1 / the rows of all_targets that count
+  const int64_t* all_targets;
+  long long all_rows;
   const float* sums;        // or, for xent_top_launch, the largest logits
   int16_t* q;               // coded logits, replaced by the logits' gradients in bf16
   float* loss;
 };
 hipError_t xent_prep_launch(const XentBf16Args& a, hipStream_t st);
-// S and loss of each row from its sums; with `again` only of the rows over the limit, else those are listed in redo
+// S and loss of each row from its sums; with `again` only of the rows over the limit, else those are listed in redo.
+// (xent_dz_launch makes those rows' again by itself.)
 hipError_t xent_join_launch(const XentBf16Args& a, int again, hipStream_t st);
 // r = the largest logit for the rows over the limit
 hipError_t xent_top_launch(const XentBf16Args& a, hipStream_t st);

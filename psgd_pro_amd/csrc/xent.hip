@@ -12,7 +12,7 @@ __device__ __forceinline__ float count_weight(const int64_t* target, long long r
   __syncthreads();
   int n = 0;
   if (mean)
-    for (long long i = threadIdx.x; i < rows; i += 1024) n += target[i] != ignore;
+    for (long long i = threadIdx.x; i < rows; i += blockDim.x) n += target[i] != ignore;
   if (n) atomicAdd(&total, n);  // whole numbers: any order gives the same sum
   __syncthreads();
   return mean ? 1.f / (float)max(total, 1) : 1.f;
@@ -204,18 +204,29 @@ hipError_t xent_prep_launch(const XentBf16Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// One wave a row. A NaN sum is under no limit and stays.
-__global__ void __launch_bounds__(256) xent_join_kernel(const XentBf16Args a, int again) {
-  const int lane = threadIdx.x & 63;
-  const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= a.rows || (again && (a.redo[0] == 0 || !(a.sum[row] > kSumLimit)))) return;
+// S and loss of a row from its parts, by one wave
+__device__ __forceinline__ float join_row(const XentBf16Args& a, long long row, int lane) {
   float s = 0.f;
   for (int i = lane; i < a.parts; i += 64) s += a.sums[row * a.parts + i];
   s = wave_sum(s);
+  if (lane == 0) {
+    const float under = a.zt[row] - a.ref[row];  // 0 where r is the target's logit
+    a.loss[row] = a.col[row] < 0 ? 0.f : under == 0.f ? log1pf(s) : logf(s + expf(under)) - under;
+  }
+  return s;
+}
+// One wave a row. A NaN sum is under no limit and stays. Workgroup 0 also makes the mean's weight.
+__global__ void __launch_bounds__(256) xent_join_kernel(const XentBf16Args a, int again) {
+  if (a.weight && blockIdx.x == 0) {
+    const float w = count_weight(a.all_targets, a.all_rows, a.ignore, 1);
+    if (threadIdx.x == 0) a.weight[0] = w;
+  }
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.rows || (again && (a.redo[0] == 0 || !(a.sum[row] > kSumLimit)))) return;
+  const float s = join_row(a, row, lane);
   if (lane) return;
   a.sum[row] = s;
-  const float under = a.zt[row] - a.ref[row];  // 0 where r is the target's logit
-  a.loss[row] = a.col[row] < 0 ? 0.f : under == 0.f ? log1pf(s) : logf(s + expf(under)) - under;
   if (!again && s > kSumLimit && a.col[row] >= 0) {
     const int blk = (int)(row / kXgRows);
     if (atomicExch(&a.mark[blk], 1) == 0) a.redo[1 + atomicAdd(&a.redo[0], 1)] = blk;  // the list's order is free
@@ -251,7 +262,17 @@ __global__ void __launch_bounds__(256) xent_dz_kernel(const XentBf16Args a) {
     for (int i = threadIdx.x; i < n; i += 256) q[i] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const float s = a.sum[row], all = s + expf(a.zt[row] - a.ref[row]), g = a.row_weight ? a.row_weight[row] : 1.f;
+  __shared__ float again;
+  float s = a.sum[row];
+  if (s > kSumLimit) {  // a row whose reference was too low: its sums were made again
+    if (threadIdx.x < 64) {
+      const float q = join_row(a, row, threadIdx.x);
+      if (threadIdx.x == 0) again = q;
+    }
+    __syncthreads();
+    s = again;
+  }
+  const float all = s + expf(a.zt[row] - a.ref[row]), g = a.row_weight ? a.row_weight[row] : 1.f;
   constexpr float L2E = 1.4426950408889634f;
   const float k0 = (kLogitLow + 64.f) * L2E - log2f(all), k1 = kLogitStep * L2E;
   for (int i = threadIdx.x; i < n; i += 256) {
