@@ -192,6 +192,13 @@ int lce_f32(const Lce& p) {
   float* const weight = m.take<float>(1);
   float* const z = m.take<float>(slab * ldz);
   float* const xm = m.take<float>(slab * p.d);
+  // dx is short and narrow with the vocabulary for k: parts of k as problems of one launch, where its 128 x 256 tiles
+  // alone would leave CUs idle (2048 x 512 x 10007: 216 us in one part)
+  const int64_t tiles = ((slab + 127) / 128) * ((p.d + 255) / 256);
+  const int64_t parts = p.dx && tiles < 128 && p.lddx == p.d && p.d % 4 == 0 && (reinterpret_cast<uintptr_t>(p.dx) & 15) == 0
+                            ? std::min<int64_t>({PSGDK_MAXB, 256 / tiles, p.vocab / 512}) : 0;
+  const int64_t part = parts > 1 ? p.vocab / parts / 4 * 4 : 0;
+  float* const dxp = m.take<float>(parts > 1 ? (parts + 1) * slab * p.d : 0);
   bool done;
   PSGDK_TRY(lce_ws(p, m, done));
   if (done) return PSGDK_OK;
@@ -220,8 +227,29 @@ int lce_f32(const Lce& p) {
     PSGDK_TRY(hip_check(xent_rows_launch(a, p.st), "cross entropy rows"));
     if (p.dx) {
       float* out = static_cast<float*>(p.dx) + r0 * p.lddx;
-      PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, p.vocab, 1.f, PSGDK_F32, PSGDK_F32, 1, &zc, ldz, &p.w, p.ldw,
-                           0.f, &out, p.lddx, st));
+      if (parts > 1) {
+        const void *za[PSGDK_MAXB], *wa[PSGDK_MAXB];
+        float* oa[PSGDK_MAXB];
+        for (int64_t i = 0; i < parts; ++i) {
+          za[i] = z + i * part;
+          wa[i] = static_cast<const float*>(p.w) + i * part * p.ldw;
+          oa[i] = dxp + i * n * p.d;
+        }
+        const int64_t done_k = parts * part, rest = p.vocab - done_k;
+        PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, part, 1.f, PSGDK_F32, PSGDK_F32, (int)parts, za, ldz, wa, p.ldw,
+                             0.f, oa, p.d, st));
+        if (rest) {
+          za[0] = z + done_k;
+          wa[0] = static_cast<const float*>(p.w) + done_k * p.ldw;
+          oa[0] = dxp + parts * n * p.d;
+          PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, rest, 1.f, PSGDK_F32, PSGDK_F32, 1, za, ldz, wa, p.ldw, 0.f, oa,
+                               p.d, st));
+        }
+        PSGDK_TRY(hip_check(sum_parts_launch(dxp, (int)(parts + (rest ? 1 : 0)), n * p.d / 4, out, p.st), "dx sums"));
+      } else {
+        PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, p.vocab, 1.f, PSGDK_F32, PSGDK_F32, 1, &zc, ldz, &p.w, p.ldw,
+                             0.f, &out, p.lddx, st));
+      }
     }
     if (p.dw) {
       float* out = static_cast<float*>(p.dw);
@@ -359,6 +387,7 @@ int lce_bf16(const Lce& p) {
       x.B = reinterpret_cast<const bf16_t*>(a.q);
       x.ldb = ldq;
       x.splits = splits;
+      x.kchunk = dx_plan.kchunk;
       x.out = out;
       x.ldo = splits > 1 ? ld : p.lddx;
       x.alpha = alpha;

@@ -15,7 +15,7 @@ hipError_t xent_mean_launch(const float* loss, const float* row_weight, const in
 // Rows of logits held in memory (fp32, row stride ldz): loss of each row and, with grad, the logits replaced by their
 // gradients.
 struct XentRowsArgs {
-  float* z;                 // rows of vocab values, ldz < vocab + 1024
+  float* z;                 // 16-byte aligned; ldz a multiple of 4, less than vocab + 4
   long long ldz, rows;
   int vocab, grad;
   int64_t ignore;
@@ -64,6 +64,8 @@ hipError_t xent_dz_launch(const XentBf16Args& a, hipStream_t st);
 // out (bf16, row stride ldo) = alpha[0] sum over s of in[s] (fp32, rows x d, row stride ldi; alpha null: 1)
 hipError_t to_bf16_rows_launch(const float* in, int splits, long long ldi, const float* alpha, bf16_t* out, long long ldo,
                                long long rows, int d, hipStream_t st);
+// out = the sum of the parts of in, n4 float4 each, in order
+hipError_t sum_parts_launch(const float* in, int parts, long long n4, float* out, hipStream_t st);
 // out (row stride ldo) = in with zeros behind d
 hipError_t pad_rows_launch(const bf16_t* in, long long ldi, bf16_t* out, long long ldo, long long rows, int d,
                            hipStream_t st);

@@ -45,52 +45,84 @@ hipError_t xent_mean_launch(const float* loss, const float* row_weight, const in
 }
 
 // One workgroup a row: its maximum and sum in one pass (each thread keeps a running maximum and the sum of
-// exponentials under it), the gradient in a second one. The target's own term stays out of the sum S of the others:
-// with e_t its exponential, softmax_t - 1 = -S / (S + e_t) and, where the target is the maximum, loss = log(1 + S),
-// both without a difference of near numbers.
+// exponentials under it, four values at a time), the gradient in a second one. The target's own term stays out of the
+// sum S of the others: with e_t its exponential, softmax_t - 1 = -S / (S + e_t) and, where the target is the maximum,
+// loss = log(1 + S), both without a difference of near numbers. (fminf and fmaxf pass over NaN: it is looked for.)
+// The products read whole vectors and take another path where they meet a value that is not finite, also behind the
+// vocabulary's end: no stale memory may lie there.
 __global__ void __launch_bounds__(1024) xent_rows_kernel(const XentRowsArgs a) {
   __shared__ float red[16];
+  constexpr float L2E = 1.4426950408889634f;
   const long long row = blockIdx.x;
-  float* z = a.z + row * a.ldz;
+  float* const z = a.z + row * a.ldz;
+  float4* const z4 = reinterpret_cast<float4*>(z);
+  const int n4 = (int)(a.ldz / 4);
   const int64_t t = a.target[row];
-  // the products read whole vectors and take another path where they meet a value that is not finite, also behind the
-  // vocabulary's end: no stale memory may lie there
-  if (a.grad && threadIdx.x < a.ldz - a.vocab) z[a.vocab + threadIdx.x] = 0.f;
-  if (t == a.ignore) {
-    if (threadIdx.x == 0) a.loss[row] = 0.f;
+  const bool skip = t == a.ignore, foreign = !skip && (t < 0 || t >= a.vocab);
+  if (skip || foreign) {
+    const float fill = skip ? 0.f : NAN;
+    if (threadIdx.x == 0) a.loss[row] = fill;
     if (a.grad)
-      for (int v = threadIdx.x; v < a.vocab; v += 1024) z[v] = 0.f;
-    return;
-  }
-  if (t < 0 || t >= a.vocab) {
-    if (threadIdx.x == 0) a.loss[row] = NAN;
-    if (a.grad)
-      for (int v = threadIdx.x; v < a.vocab; v += 1024) z[v] = NAN;
+      for (int i = threadIdx.x; i < n4; i += 1024) z4[i] = make_float4(fill, fill, fill, fill);
     return;
   }
   const float zt = z[t];
+  auto other = [&](int i, float (&x)[4]) {  // four logits, the target and what lies behind the vocabulary left out
+    const float4 q = z4[i];
+    const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = 4 * i + e < a.vocab && 4 * i + e != t ? v[e] : -INFINITY;
+  };
   float m = -INFINITY, s = 0.f;
-  bool nan = false;
-  for (int v = threadIdx.x; v < a.vocab; v += 1024) {
-    const float x = z[v];
-    nan = nan || x != x;
-    if (x > m) {
-      s *= expf(m - x);
-      m = x;
+  for (int i = threadIdx.x; i < n4; i += 1024) {
+    float x[4];
+    other(i, x);
+    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    if (top > m) {
+      s *= __builtin_amdgcn_exp2f((m - top) * L2E);
+      m = top;
     }
-    if (v != t && x > -INFINITY) s += expf(x - m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += x[e] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[e] - m) * L2E);
   }
-  const float top = block_max(m, red);
-  s = block_sum(nan ? NAN : (m > -INFINITY ? s * expf(m - top) : 0.f), red);
-  const float et = expf(zt - top), all = s + et;
-  if (threadIdx.x == 0) a.loss[row] = zt == top ? log1pf(s) : logf(all) + (top - zt);
+  const float most = fmaxf(block_max(m, red), zt);
+  s = block_sum(m > -INFINITY ? s * __builtin_amdgcn_exp2f((m - most) * L2E) : s, red);
+  const float et = __builtin_amdgcn_exp2f((zt - most) * L2E), all = s + et;
+  if (threadIdx.x == 0) a.loss[row] = zt == most ? log1pf(s) : logf(all) + (most - zt);
   if (!a.grad) return;
   const float w = a.row_weight ? a.row_weight[row] : a.weight[0], q = w / all;
-  __syncthreads();
-  for (int v = threadIdx.x; v < a.vocab; v += 1024) z[v] = v == t ? -s * q : expf(z[v] - top) * q;
+  for (int i = threadIdx.x; i < n4; i += 1024) {
+    const float4 v = z4[i];
+    float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 4 * i + e;
+      x[e] = c >= a.vocab ? 0.f : c == t ? -s * q : __builtin_amdgcn_exp2f((x[e] - most) * L2E) * q;
+    }
+    z4[i] = make_float4(x[0], x[1], x[2], x[3]);
+  }
 }
 hipError_t xent_rows_launch(const XentRowsArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(xent_rows_kernel, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+  return hipGetLastError();
+}
+
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* in, int parts, long long n4, float* out) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
+    float4 v = reinterpret_cast<const float4*>(in)[i];
+    for (int s = 1; s < parts; ++s) {
+      const float4 q = reinterpret_cast<const float4*>(in)[s * n4 + i];
+      v.x += q.x;
+      v.y += q.y;
+      v.z += q.z;
+      v.w += q.w;
+    }
+    reinterpret_cast<float4*>(out)[i] = v;
+  }
+}
+hipError_t sum_parts_launch(const float* in, int parts, long long n4, float* out, hipStream_t st) {
+  const long long want = (n4 + 255) / 256;
+  hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)(want > 4096 ? 4096 : want)), dim3(256), 0, st, in, parts, n4, out);
   return hipGetLastError();
 }
 

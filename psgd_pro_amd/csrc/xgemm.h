@@ -14,7 +14,7 @@ struct XgArgs {
   const bf16_t* B;
   int tiles_m, tiles_n;
   int kreal;           // rows of an mn-contiguous A (0: K); k behind them reads zeros
-  int splits, kchunk;  // split s covers k in [s kchunk, (s + 1) kchunk); splits > 1 need outf
+  int splits, kchunk;  // split s covers k in [s kchunk, (s + 1) kchunk), none of them empty; splits > 1 need outf
   // products with the vocabulary matrix or the rows: out = alpha[0] acc in bf16 (alpha null: 1), or
   bf16_t* out;
   const float* alpha;
@@ -43,10 +43,10 @@ enum XgKind : int {
 };
 // How a product with out M x N (XG_DX, XG_DW) is cut: 256 or 128 rows of m a tile, and parts of k (1 without can_split)
 struct XgPlan {
-  int bm, splits;
+  int bm, splits, kchunk;
 };
 XgPlan xgemm_plan(long long M, long long N, long long K, bool can_split);
-// sets the tile counts and kchunk; bm: 256 for XG_LOGITS
+// sets the tile counts, and kchunk where splits is 1; bm: 256 for XG_LOGITS
 hipError_t xgemm_launch(XgArgs& a, int kind, int bm, hipStream_t st);
 
 }  // namespace psgdk

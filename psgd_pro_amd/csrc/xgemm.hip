@@ -420,7 +420,7 @@ static hipError_t launch_x(XgArgs& a, hipStream_t st) {
   a.tiles_m = (a.M + 2 * WTM - 1) / (2 * WTM);
   a.tiles_n = (a.N + 2 * WTN - 1) / (2 * WTN);
   if (!a.kreal) a.kreal = a.K;
-  a.kchunk = a.splits > 1 ? ((a.K + a.splits - 1) / a.splits + BK - 1) / BK * BK : a.K;
+  if (a.splits == 1) a.kchunk = a.K;
   const long long tiles = (long long)a.tiles_m * a.tiles_n * a.splits;
   hipLaunchKernelGGL(fn, dim3((unsigned)(tiles > 256 ? 256 : tiles)), dim3(256), smem, st, a);  // one a CU
   return hipGetLastError();
@@ -431,7 +431,7 @@ static hipError_t launch_x(XgArgs& a, hipStream_t st) {
 // large ones fill half a round or pad m: 1531 x 770 x 50021 dw 188 -> 160 us, dx 164 -> 154. A further part of k costs
 // fp32 sums written and read.
 XgPlan xgemm_plan(long long M, long long N, long long K, bool can_split) {
-  XgPlan best{256, 1};
+  XgPlan best{256, 1, (int)K};
   double least = 1e30;
   for (int bm : {256, 128}) {
     const double tiles = (double)((M + bm - 1) / bm) * (double)((N + 255) / 256);
@@ -441,7 +441,8 @@ XgPlan xgemm_plan(long long M, long long N, long long K, bool can_split) {
                             (s > 1 ? 8. * s * (double)M * (double)N / 5e12 + 3e-6 : 0.);
       if (t < least) {
         least = t;
-        best = XgPlan{bm, s};
+        const long long chunk = ((K + s - 1) / s + 63) / 64 * 64;  // whole k tiles: the last part may not be there
+        best = XgPlan{bm, (int)((K + chunk - 1) / chunk), s == 1 ? (int)K : (int)chunk};
       }
     }
   }

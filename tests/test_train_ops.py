@@ -444,6 +444,14 @@ def test_cross_entropy_sizes(dtype, n, d, v):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_entropy_parts_of_a_long_vocabulary(dtype):
+    """dx of few rows adds up many parts of the vocabulary: their lengths do not divide it (the last ones short, or not
+    there), with more output tiles than one a CU and with fewer."""
+    for n, d, v in ((64, 256, 16400), (300, 1000, 16447), (1100, 520, 33000)):
+        run_lce(rnd((n, d), 1, dtype), rnd((v, d), 2, dtype, 1.5 / math.sqrt(d)), targets(n, v, 3, 0.2), reductions=("mean",))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_cross_entropy_everything_ignored(dtype):
     x, w = rnd((40, 64), 1, dtype).requires_grad_(), rnd((300, 64), 2, dtype).requires_grad_()
     t = torch.full((40,), 7, device=DEV)
