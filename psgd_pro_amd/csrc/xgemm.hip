@@ -54,6 +54,11 @@ __device__ __forceinline__ void load_lds(i32x4_t rs, int voff, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds)
                : "memory");
 }
+// the same with 4 bytes a lane
+__device__ __forceinline__ void load_lds4(i32x4_t rs, int voff, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds)
+               : "memory");
+}
 // all but the newest N loads into LDS of this wave have arrived, its LDS reads are done, and so for the whole workgroup
 template <int N>
 __device__ __forceinline__ void load_wait() {
@@ -64,8 +69,9 @@ __device__ __forceinline__ void load_wait() {
 
 // Four waves, 2 x 2, each WTM x WTN of the output; ST stages of BK k in LDS, and a block of 32 x WTM 16-bit values for
 // each wave's way out. A workgroup takes one tile after the other; the loads of the next tile's first stages are on their
-// way before a tile's results leave.
-template <int WTM, int WTN, int BK, int ST, bool MCA, bool MCB, int KIND, bool OUTF>
+// way before a tile's results leave. No load that a register waits for may come between: its wait would be for all of them,
+// and for the last tile's stores. (REDO, the listed blocks alone, is an instance of its own for its list's loads.)
+template <int WTM, int WTN, int BK, int ST, bool MCA, bool MCB, int KIND, bool OUTF, bool REDO>
 __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
   constexpr int BM = 2 * WTM, BN = 2 * WTN, FM = WTM / 32, FN = WTN / 32, KS = BK / 16;
   using TA = Tile<BM, BK, MCA>;
@@ -78,12 +84,12 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
   const int c = lane & 31, hh = lane >> 5, wm = wave >> 1, wn = wave & 1;
 
   static_assert(BN == kXgRows, "a listed block is a tile of n");
-  const int ntiles = p.redo ? p.redo[0] * p.tiles_m : p.tiles_m * p.tiles_n * p.splits;
+  const int ntiles = REDO ? p.redo[0] * p.tiles_m : p.tiles_m * p.tiles_n * p.splits;
   if ((int)blockIdx.x >= ntiles) return;
   // tile w of the workgroups' order: its m and n tile and its part of k
   auto where = [&](int w, int& ti, int& tj, int& split) __attribute__((always_inline)) {
     split = 0;
-    if (p.redo) {
+    if constexpr (REDO) {
       ti = w % p.tiles_m;
       tj = p.redo[1 + w / p.tiles_m];
       return;
@@ -94,8 +100,8 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     split = tile / (p.tiles_m * p.tiles_n);
     tile -= split * (p.tiles_m * p.tiles_n);
     const int grp = tile / (GM * p.tiles_n), r0 = grp * GM, gm = min(GM, p.tiles_m - r0), idx = tile - r0 * p.tiles_n;
-    ti = r0 + idx % gm;
-    tj = idx / gm;
+    ti = r0 + (gm == GM ? idx % GM : idx % gm);
+    tj = gm == GM ? idx / GM : idx / gm;
   };
 
   // byte offsets of this lane's loads inside a tile
@@ -225,23 +231,23 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
 #pragma unroll
   for (int f = 0; f < FM + FN; ++f) frag(0, lds0, 0, f);
   unsigned base = lds0;
+  unsigned char* const ep0 = smem + ST * STAGE + wave * 32 * WTM * 2;  // the wave's way out
+  const unsigned ep = lds0 + ST * STAGE + wave * 32 * WTM * 2;
+  const float al = KIND != XG_LOGITS && !OUTF && p.alpha ? p.alpha[0] : 1.f;
 
   for (int w = blockIdx.x; w < ntiles; w += gridDim.x) {
     int ti, tj, split;
     where(w, ti, tj, split);
     const int nk = (min(p.K - split * p.kchunk, p.kchunk) + BK - 1) / BK;
     const int mw = ti * BM + wm * WTM, nw = tj * BN + wn * WTN;  // this wave's block
-    float ref[FN], al = 1.f;
-    int tgt[FN];
-    if constexpr (KIND == XG_LOGITS) {
+    if constexpr (KIND == XG_LOGITS) {  // r and target of the wave's rows, into its way out, for when the products are done
+      i32x4_t rs = rsrc_words(p.ref, 4ll * p.N), ts = rsrc_words(p.target, 4ll * p.N);
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_nop 4" : "+s"(rs), "+s"(ts)::"memory");
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int n = nw + 32 * j + c;
-        ref[j] = n < p.N ? p.ref[n] : 0.f;
-        tgt[j] = n < p.N ? p.target[n] : -1;
+      for (int i = 0; i < WTN; i += 64) {
+        load_lds4(rs, (nw + i + lane) * 4, ep + i * 4);
+        load_lds4(ts, (nw + i + lane) * 4, ep + (WTN + i) * 4);
       }
-    } else if (!OUTF && p.alpha) {
-      al = p.alpha[0];
     }
     f32x16_t acc[FM][FN];
 #pragma unroll
@@ -307,9 +313,17 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
       }
       continue;
     }
-    unsigned char* const ep = smem + ST * STAGE + wave * 32 * WTM * 2;
+    float ref[FN];
+    int tgt[FN];
+    if constexpr (KIND == XG_LOGITS) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        ref[j] = *(LDS_AS float*)(uintptr_t)(ep + (32 * j + c) * 4);
+        tgt[j] = *(LDS_AS int*)(uintptr_t)(ep + (WTN + 32 * j + c) * 4);
+      }
+    }
     constexpr int CH = WTM / 8;
-    auto slot = [&](int n, int ch) __attribute__((always_inline)) { return ep + n * WTM * 2 + ((ch ^ (n & (CH - 1))) << 4); };
+    auto slot = [&](int n, int ch) __attribute__((always_inline)) { return ep0 + n * WTM * 2 + ((ch ^ (n & (CH - 1))) << 4); };
     uint16_t* const out = KIND == XG_LOGITS ? reinterpret_cast<uint16_t*>(p.q) : p.out;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
@@ -350,7 +364,8 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
           }
           s = (s + s1) + (s2 + s3);
         };
-        if (inside && !p.max_only) {
+        const bool max_only = REDO && p.max_only;
+        if (inside && !max_only) {
           if (p.q) usual(std::true_type{});
           else usual(std::false_type{});
         } else {
@@ -363,14 +378,14 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
               const int m = mw + 32 * i + 8 * g + 4 * hh;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                if (p.max_only) top = fmaxf(top, m + e < p.M ? z[e] : -INFINITY);
+                if (max_only) top = fmaxf(top, m + e < p.M ? z[e] : -INFINITY);
                 else s += m + e < p.M && m + e != t ? __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], L2E, e0)) : 0.f;
               }
               if (p.q) code(i, g, z);
             }
           }
         }
-        if (p.max_only) {
+        if (max_only) {
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           if (row && hh == 0) p.tops[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = top;
         } else {
@@ -410,10 +425,10 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup
 }
 
-template <int WTM, int WTN, int BK, int ST, bool MCA, bool MCB, int KIND, bool OUTF = false>
+template <int WTM, int WTN, int BK, int ST, bool MCA, bool MCB, int KIND, bool OUTF = false, bool REDO = false>
 static hipError_t launch_x(XgArgs& a, hipStream_t st) {
   constexpr int smem = ST * (Tile<2 * WTM, BK, MCA>::BYTES + Tile<2 * WTN, BK, MCB>::BYTES) + 4 * 32 * WTM * 2;
-  void (*fn)(XgArgs) = xgemm_kernel<WTM, WTN, BK, ST, MCA, MCB, KIND, OUTF>;
+  void (*fn)(XgArgs) = xgemm_kernel<WTM, WTN, BK, ST, MCA, MCB, KIND, OUTF, REDO>;
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (attr != hipSuccess) return attr;
@@ -450,7 +465,9 @@ XgPlan xgemm_plan(long long M, long long N, long long K, bool can_split) {
 }
 
 hipError_t xgemm_launch(XgArgs& a, int kind, int bm, hipStream_t st) {
-  if (kind == XG_LOGITS) return launch_x<128, 128, 64, 2, false, false, XG_LOGITS>(a, st);
+  if (kind == XG_LOGITS)
+    return a.redo ? launch_x<128, 128, 64, 2, false, false, XG_LOGITS, false, true>(a, st)
+                  : launch_x<128, 128, 64, 2, false, false, XG_LOGITS>(a, st);
   if (kind == XG_DX) {
     if (bm == 128)
       return a.outf ? launch_x<64, 128, 64, 3, true, false, XG_DX, true>(a, st)
