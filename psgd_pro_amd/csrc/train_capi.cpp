@@ -178,9 +178,9 @@ int lce_pointers(const Lce& p) {
   if (p.dw) PSGDK_TRY(check_rows(p.dw, p.lddw, p.d, "dw"));
   return PSGDK_OK;
 }
-int lce_mean(const Lce& p) {
+int lce_mean(const Lce& p, const float* weight) {
   if (!p.mean_loss) return PSGDK_OK;
-  return hip_check(xent_mean_launch(p.loss, p.row_weight, p.target, p.rows, p.ignore, p.mean, p.mean_loss, p.st),
+  return hip_check(xent_mean_launch(p.loss, p.row_weight, weight, p.target, p.rows, p.ignore, p.mean, p.mean_loss, p.st),
                    "cross entropy mean");
 }
 
@@ -257,7 +257,7 @@ int lce_f32(const Lce& p) {
                            r0 ? 1.f : 0.f, &out, p.lddw, st));
     }
   }
-  return lce_mean(p);
+  return lce_mean(p, weight);
 }
 
 // bfloat16, a few rows, losses only
@@ -282,7 +282,7 @@ int lce_few(const Lce& p) {
   a.target = p.target;
   a.loss = p.loss;
   PSGDK_TRY(hip_check(xent_few_launch(a, p.st), "cross entropy of a few rows"));
-  return lce_mean(p);
+  return lce_mean(p, nullptr);
 }
 
 // bfloat16: the logits of a slab of rows as 16-bit codes with the sums of their exponentials (one product), a pass that
@@ -299,6 +299,8 @@ int lce_bf16(const Lce& p) {
   const int splits = p.dx ? dx_plan.splits : 1;
   Ws m(p.ws);
   float* const weight = m.take<float>(1);
+  int* const count = m.take<int>(1);
+  int* const order = m.take<int>(p.rows);
   XentBf16Args a{};
   a.xm = m.take<bf16_t>(slab * ld);
   a.zt = m.take<float>(slab);
@@ -326,9 +328,13 @@ int lce_bf16(const Lce& p) {
   a.d = (int)p.d;
   a.vocab = (int)p.vocab;
   a.parts = (int)parts;
-  a.ignore = p.ignore;
-  a.all_targets = p.target;
-  a.all_rows = p.rows;
+  a.count = count;
+  a.target = p.target;
+  a.row_weight = p.row_weight;
+  a.x = static_cast<const bf16_t*>(p.x);
+  a.loss = p.loss;
+  a.dx = static_cast<bf16_t*>(p.dx);
+  a.lddx = p.lddx;
   a.w = w;
   a.ldw = ldw;
   a.ldx = p.ldx;
@@ -336,13 +342,13 @@ int lce_bf16(const Lce& p) {
   a.ldq = ldq;
   a.sums = sums;
   const float* const alpha = p.mean ? weight : nullptr;
+  PSGDK_TRY(hip_check(xent_order_launch(p.target, p.rows, p.ignore, p.mean, order, count, weight, p.loss, p.st),
+                      "cross entropy order"));
   for (int64_t r0 = 0; r0 < p.rows; r0 += slab) {
     const int64_t n = std::min(slab, p.rows - r0);
     a.rows = n;
-    a.target = p.target + r0;
-    a.row_weight = p.row_weight ? p.row_weight + r0 : nullptr;
-    a.x = static_cast<const bf16_t*>(p.x) + r0 * p.ldx;
-    a.loss = p.loss + r0;
+    a.first = r0;
+    a.order = order + r0;
     PSGDK_TRY(hip_check(xent_prep_launch(a, p.st), "cross entropy rows"));
     XgArgs g{};
     g.M = (int)p.vocab;
@@ -353,15 +359,15 @@ int lce_bf16(const Lce& p) {
     g.B = a.xm;
     g.ldb = ld;
     g.splits = 1;
+    g.count = count;
+    g.first = (int)r0;
     g.q = grad ? a.q : nullptr;
     g.ldo = ldq;
     g.ref = a.ref;
     g.target = a.col;
     g.sums = sums;
     PSGDK_TRY(hip_check(xgemm_launch(g, XG_LOGITS, 256, p.st), "logits"));
-    a.weight = grad && p.mean && r0 == 0 ? weight : nullptr;
     PSGDK_TRY(hip_check(xent_join_launch(a, 0, p.st), "cross entropy sums"));
-    a.weight = nullptr;
     // rows whose reference was too low: their maximum, then their blocks once more (nothing where there are none)
     XgArgs t = g;
     t.q = nullptr;
@@ -377,8 +383,11 @@ int lce_bf16(const Lce& p) {
     }
     PSGDK_TRY(hip_check(xent_dz_launch(a, p.st), "logits' gradients"));
     if (p.dx) {
-      bf16_t* const out = static_cast<bf16_t*>(p.dx) + r0 * p.lddx;
+      bf16_t* const out = static_cast<bf16_t*>(p.dx);
       XgArgs x{};
+      x.count = count;
+      x.first = (int)r0;
+      x.order = a.order;
       x.M = (int)p.d;
       x.N = (int)n;
       x.K = (int)ldq;
@@ -395,10 +404,13 @@ int lce_bf16(const Lce& p) {
       x.kreal = (int)p.vocab;
       PSGDK_TRY(hip_check(xgemm_launch(x, XG_DX, dx_plan.bm, p.st), "dx"));
       if (splits > 1)
-        PSGDK_TRY(hip_check(to_bf16_rows_launch(dxp, splits, ld, alpha, out, p.lddx, n, (int)p.d, p.st), "dx sums"));
+        PSGDK_TRY(hip_check(to_bf16_rows_launch(dxp, splits, ld, alpha, out, p.lddx, n, (int)p.d, a.order, count, r0,
+                                      p.st), "dx sums"));
     }
     if (p.dw) {
       XgArgs x{};
+      x.count = count;
+      x.first = (int)r0;
       x.M = (int)p.d;
       x.N = (int)p.vocab;
       x.K = (int)n;
@@ -416,9 +428,9 @@ int lce_bf16(const Lce& p) {
     }
   }
   if (sum_w)
-    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, 1, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab, (int)p.d, p.st),
-                        "dw sums"));
-  return lce_mean(p);
+    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, 1, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab, (int)p.d,
+                                  nullptr, nullptr, 0, p.st), "dw sums"));
+  return lce_mean(p, weight);
 }
 
 }  // namespace

@@ -8,9 +8,14 @@ namespace psgdk {
 // weight[0] = mean ? 1 / max(1, rows whose target is not `ignore`) : 1
 hipError_t xent_weight_launch(const int64_t* target, long long rows, int64_t ignore, int mean, float* weight,
                               hipStream_t st);
-// out[0] = sum_i w_i loss[i], w_i = row_weight[i], or where that is null as in xent_weight_launch; in a fixed order
-hipError_t xent_mean_launch(const float* loss, const float* row_weight, const int64_t* target, long long rows,
-                            int64_t ignore, int mean, float* out, hipStream_t st);
+// out[0] = sum_i w_i loss[i], w_i = row_weight[i], or where that is null weight[0], or where that is null too as in
+// xent_weight_launch; in a fixed order
+hipError_t xent_mean_launch(const float* loss, const float* row_weight, const float* weight, const int64_t* target,
+                            long long rows, int64_t ignore, int mean, float* out, hipStream_t st);
+// order = the rows whose target is not `ignore`, in their order, then the others, whose losses become 0; count[0] = how
+// many are not; weight as in xent_weight_launch
+hipError_t xent_order_launch(const int64_t* target, long long rows, int64_t ignore, int mean, int* order, int* count,
+                             float* weight, float* loss, hipStream_t st);
 
 // Rows of logits held in memory (fp32, row stride ldz): loss of each row and, with grad, the logits replaced by their
 // gradients.
@@ -31,24 +36,25 @@ hipError_t xent_rows_launch(const XentRowsArgs& a, hipStream_t st);
 // over 31) take their largest logit as r instead, and the target's exponential e_t = e^(z_t - r).
 constexpr float kSumLimit = 2.9e13f;  // e^31: every e^(z - r) below it, z - r within the coded logits' range
 struct XentBf16Args {
-  long long rows;
+  // The rows of a slab are places first .. first + rows - 1 of the order: those before count[0] are there and are numbered
+  // from 0 in everything made here; the others are ignored ones.
+  long long rows, first;
+  const int* order;         // from `first` on
+  const int* count;
   int d, vocab, parts;      // parts: sums of a row (2 tiles of m)
-  int64_t ignore;
-  const int64_t* target;
+  const int64_t* target;    // of all rows, as row_weight, x, dx and loss
   const float* row_weight;  // null: 1 (the mean's weight is the products' alpha)
   const bf16_t* x;
   const bf16_t* w;
-  long long ldx, ldw, ldm, ldq;
-  bf16_t* xm;               // x with zeros in ignored rows and behind d, row stride ldm
+  bf16_t* dx;               // null, or: its ignored rows become zeros
+  long long ldx, ldw, ldm, ldq, lddx;
+  bf16_t* xm;               // x's rows with zeros behind d, row stride ldm
   float* zt;                // z_t
   float* ref;               // r
   float* sum;               // S
-  int* col;                 // the target's column; -1 for an ignored row, vocab for a foreign target (r is NaN then)
+  int* col;                 // the target's column; vocab for a foreign target (r is NaN then)
   int* redo;                // number of blocks of kXgRows rows with a row over the limit, and their numbers
   int* mark;                // of each block: whether it is listed
-  float* weight;            // null, or: xent_join_launch makes 1 / the rows of all_targets that count
-  const int64_t* all_targets;
-  long long all_rows;
   const float* sums;        // or, for xent_top_launch, the largest logits
   int16_t* q;               // coded logits, replaced by the logits' gradients in bf16
   float* loss;
@@ -59,11 +65,12 @@ hipError_t xent_prep_launch(const XentBf16Args& a, hipStream_t st);
 hipError_t xent_join_launch(const XentBf16Args& a, int again, hipStream_t st);
 // r = the largest logit for the rows over the limit
 hipError_t xent_top_launch(const XentBf16Args& a, hipStream_t st);
-// the logits' gradients (without the mean's weight), zeros in ignored rows and behind the vocabulary
+// the logits' gradients (without the mean's weight), zeros behind the vocabulary
 hipError_t xent_dz_launch(const XentBf16Args& a, hipStream_t st);
-// out (bf16, row stride ldo) = alpha[0] sum over s of in[s] (fp32, rows x d, row stride ldi; alpha null: 1)
+// out (bf16, row stride ldo) = alpha[0] sum over s of in[s] (fp32, rows x d, row stride ldi; alpha null: 1); with order,
+// only of the count[0] - first rows that are there, row r to row order[r]
 hipError_t to_bf16_rows_launch(const float* in, int splits, long long ldi, const float* alpha, bf16_t* out, long long ldo,
-                               long long rows, int d, hipStream_t st);
+                               long long rows, int d, const int* order, const int* count, long long first, hipStream_t st);
 // out = the sum of the parts of in, n4 float4 each, in order
 hipError_t sum_parts_launch(const float* in, int parts, long long n4, float* out, hipStream_t st);
 // out (row stride ldo) = in with zeros behind d

@@ -28,19 +28,76 @@ hipError_t xent_weight_launch(const int64_t* target, long long rows, int64_t ign
   return hipGetLastError();
 }
 
-__global__ void __launch_bounds__(1024) xent_mean_kernel(const float* loss, const float* row_weight,
+// One workgroup, 4096 rows a turn (a wave 256 of them, 64 by 64): first how many count, then their places.
+__global__ void __launch_bounds__(1024) xent_order_kernel(const int64_t* target, long long rows, int64_t ignore, int mean,
+                                                          int* order, int* count, float* weight, float* loss) {
+  __shared__ int total, part[2][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  int n = 0;
+  for (long long i = threadIdx.x; i < rows; i += 1024) n += target[i] != ignore;
+  if (n) atomicAdd(&total, n);  // whole numbers: any order gives the same sum
+  __syncthreads();
+  n = total;
+  if (threadIdx.x == 0) {
+    count[0] = n;
+    weight[0] = mean ? 1.f / (float)max(n, 1) : 1.f;
+  }
+  int before = 0;  // rows that count, in front of this turn
+  for (long long r0 = 0; r0 < rows; r0 += 4096) {
+    const int turn = (int)(r0 / 4096 & 1);
+    unsigned long long has[4];
+    int mine = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long long r = r0 + wave * 256 + e * 64 + lane;
+      has[e] = __ballot(r < rows && target[r] != ignore);
+      mine += __popcll(has[e]);
+    }
+    if (lane == 0) part[turn][wave] = mine;
+    __syncthreads();  // (the next turn's values lie beside these: one barrier a turn)
+    int at = before;
+    for (int w = 0; w < 16; ++w) {
+      at += w < wave ? part[turn][w] : 0;
+      before += part[turn][w];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long long r = r0 + wave * 256 + e * 64 + lane;
+      const int rank = at + __popcll(has[e] & ((1ull << lane) - 1));
+      if (r < rows) {
+        if (has[e] >> lane & 1) {
+          order[rank] = (int)r;
+        } else {
+          order[n + (r - rank)] = (int)r;
+          loss[r] = 0.f;
+        }
+      }
+      at += __popcll(has[e]);
+    }
+  }
+}
+hipError_t xent_order_launch(const int64_t* target, long long rows, int64_t ignore, int mean, int* order, int* count,
+                             float* weight, float* loss, hipStream_t st) {
+  hipLaunchKernelGGL(xent_order_kernel, dim3(1), dim3(1024), 0, st, target, rows, ignore, mean, order, count, weight, loss);
+  return hipGetLastError();
+}
+
+__global__ void __launch_bounds__(1024) xent_mean_kernel(const float* loss, const float* row_weight, const float* weight,
                                                          const int64_t* target, long long rows, int64_t ignore,
                                                          int mean, float* out) {
   __shared__ float red[16];
-  const float w = row_weight ? 1.f : count_weight(target, rows, ignore, mean);
+  const float w = row_weight ? 1.f : weight ? weight[0] : count_weight(target, rows, ignore, mean);
   float s = 0.f;
   for (long long i = threadIdx.x; i < rows; i += 1024) s += row_weight ? row_weight[i] * loss[i] : loss[i];
   s = block_sum(s, red);
   if (threadIdx.x == 0) out[0] = s * w;
 }
-hipError_t xent_mean_launch(const float* loss, const float* row_weight, const int64_t* target, long long rows,
-                            int64_t ignore, int mean, float* out, hipStream_t st) {
-  hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, st, loss, row_weight, target, rows, ignore, mean, out);
+hipError_t xent_mean_launch(const float* loss, const float* row_weight, const float* weight, const int64_t* target,
+                            long long rows, int64_t ignore, int mean, float* out, hipStream_t st) {
+  hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, st, loss, row_weight, weight, target, rows, ignore, mean,
+                     out);
   return hipGetLastError();
 }
 
@@ -128,10 +185,11 @@ hipError_t sum_parts_launch(const float* in, int parts, long long n4, float* out
 
 __global__ void __launch_bounds__(256) to_bf16_rows_kernel(const float* in, int splits, long long ldi,
                                                            const float* alpha, bf16_t* out, long long ldo,
-                                                           long long rows, int d) {
+                                                           long long rows, int d, const int* order, const int* count,
+                                                           long long first) {
   const float al = alpha ? *alpha : 1.f;
   const int per = (d + 3) / 4;
-  const long long total = rows * per;
+  const long long total = (order ? min(max(count[0] - first, 0ll), rows) : rows) * per;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long r = i / per;
     const int c = (int)(i - r * per) * 4;
@@ -150,17 +208,18 @@ __global__ void __launch_bounds__(256) to_bf16_rows_kernel(const float* in, int 
     bf16_t h[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = f32_to_bf16(al * v[e]);
-    bf16_t* o = out + r * ldo + c;
+    bf16_t* o = out + (order ? order[r] : r) * ldo + c;
     if (c + 4 <= d) __builtin_memcpy(o, h, 8);
     else
       for (int e = 0; c + e < d; ++e) o[e] = h[e];
   }
 }
 hipError_t to_bf16_rows_launch(const float* in, int splits, long long ldi, const float* alpha, bf16_t* out, long long ldo,
-                               long long rows, int d, hipStream_t st) {
+                               long long rows, int d, const int* order, const int* count, long long first,
+                               hipStream_t st) {
   const long long want = (rows * ((d + 3) / 4) + 255) / 256;
   hipLaunchKernelGGL(to_bf16_rows_kernel, dim3((unsigned)(want > 8192 ? 8192 : want)), dim3(256), 0, st, in, splits, ldi,
-                     alpha, out, ldo, rows, d);
+                     alpha, out, ldo, rows, d, order, count, first);
   return hipGetLastError();
 }
 
@@ -206,20 +265,39 @@ hipError_t pad_rows_launch(const bf16_t* in, long long ldi, bf16_t* out, long lo
   return hipGetLastError();
 }
 
-// One wave a row: r = z_t and the row's copy for the products.
+// rows of a slab that are there
+__device__ __forceinline__ long long live_rows(const XentBf16Args& a) {
+  return min(max(a.count[0] - a.first, 0ll), a.rows);
+}
+
+// One wave a row: r = z_t and the row's copy for the products; zeros for an ignored row's gradient.
 __global__ void __launch_bounds__(256) xent_prep_kernel(const XentBf16Args a) {
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= a.rows) return;
-  const int64_t t = a.target[row];
-  const bool skip = t == a.ignore, foreign = !skip && (t < 0 || t >= a.vocab);
-  const bf16_t* x = a.x + row * a.ldx;
-  const bf16_t* w = a.w + (skip || foreign ? 0 : t) * a.ldw;
+  if (lane == 0) {
+    if (row % kXgRows == 0) a.mark[row / kXgRows] = 0;
+    if (row == 0) a.redo[0] = 0;
+  }
+  const long long from = a.order[row];
+  if (row >= live_rows(a)) {
+    if (!a.dx) return;
+    bf16_t* const o = a.dx + from * a.lddx;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int c = lane * 8; c < a.d; c += 512)
+      if (c + 8 <= a.d) __builtin_memcpy(o + c, &zero, 16);
+      else
+        for (int e = c; e < a.d; ++e) o[e] = 0;
+    return;
+  }
+  const int64_t t = a.target[from];
+  const bool foreign = t < 0 || t >= a.vocab;
+  const bf16_t* x = a.x + from * a.ldx;
+  const bf16_t* w = a.w + (foreign ? 0 : t) * a.ldw;
   float s = 0.f;
   for (int c = lane * 8; c < a.ldm; c += 512) {
-    uint4 v = ld8_bits(x, c, a.d);
-    if (skip) v = make_uint4(0, 0, 0, 0);
-    else s = dot8(v, ld8_bits(w, c, a.d), s);
+    const uint4 v = ld8_bits(x, c, a.d);
+    s = dot8(v, ld8_bits(w, c, a.d), s);
     *reinterpret_cast<uint4*>(a.xm + row * a.ldm + c) = v;
   }
   s = wave_sum(s);
@@ -227,9 +305,7 @@ __global__ void __launch_bounds__(256) xent_prep_kernel(const XentBf16Args a) {
   if (foreign) s = NAN;
   a.zt[row] = s;
   a.ref[row] = s;
-  a.col[row] = skip ? -1 : foreign ? a.vocab : (int)t;
-  if (row % kXgRows == 0) a.mark[row / kXgRows] = 0;
-  if (row == 0) a.redo[0] = 0;
+  a.col[row] = foreign ? a.vocab : (int)t;
 }
 hipError_t xent_prep_launch(const XentBf16Args& a, hipStream_t st) {
   hipLaunchKernelGGL(xent_prep_kernel, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
@@ -243,23 +319,19 @@ __device__ __forceinline__ float join_row(const XentBf16Args& a, long long row, 
   s = wave_sum(s);
   if (lane == 0) {
     const float under = a.zt[row] - a.ref[row];  // 0 where r is the target's logit
-    a.loss[row] = a.col[row] < 0 ? 0.f : under == 0.f ? log1pf(s) : logf(s + expf(under)) - under;
+    a.loss[a.order[row]] = under == 0.f ? log1pf(s) : logf(s + expf(under)) - under;
   }
   return s;
 }
-// One wave a row. A NaN sum is under no limit and stays. Workgroup 0 also makes the mean's weight.
+// One wave a row. A NaN sum is under no limit and stays.
 __global__ void __launch_bounds__(256) xent_join_kernel(const XentBf16Args a, int again) {
-  if (a.weight && blockIdx.x == 0) {
-    const float w = count_weight(a.all_targets, a.all_rows, a.ignore, 1);
-    if (threadIdx.x == 0) a.weight[0] = w;
-  }
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= a.rows || (again && (a.redo[0] == 0 || !(a.sum[row] > kSumLimit)))) return;
+  if (row >= live_rows(a) || (again && (a.redo[0] == 0 || !(a.sum[row] > kSumLimit)))) return;
   const float s = join_row(a, row, lane);
   if (lane) return;
   a.sum[row] = s;
-  if (!again && s > kSumLimit && a.col[row] >= 0) {
+  if (!again && s > kSumLimit) {
     const int blk = (int)(row / kXgRows);
     if (atomicExch(&a.mark[blk], 1) == 0) a.redo[1 + atomicAdd(&a.redo[0], 1)] = blk;  // the list's order is free
   }
@@ -273,7 +345,7 @@ __global__ void __launch_bounds__(256) xent_top_kernel(const XentBf16Args a) {
   if (a.redo[0] == 0) return;
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= a.rows || a.col[row] < 0 || !(a.sum[row] > kSumLimit)) return;
+  if (row >= live_rows(a) || !(a.sum[row] > kSumLimit)) return;
   float m = -INFINITY;
   for (int i = lane; i < a.parts; i += 64) m = fmaxf(m, a.sums[row * a.parts + i]);
   m = wave_max(m);
@@ -289,11 +361,8 @@ hipError_t xent_top_launch(const XentBf16Args& a, hipStream_t st) {
 __global__ void __launch_bounds__(256) xent_dz_kernel(const XentBf16Args a) {
   const long long row = blockIdx.x;
   uint4* q = reinterpret_cast<uint4*>(a.q + row * a.ldq);
+  if (row >= live_rows(a)) return;
   const int n = (int)(a.ldq / 8), t = a.col[row];
-  if (t < 0) {
-    for (int i = threadIdx.x; i < n; i += 256) q[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
   __shared__ float again;
   float s = a.sum[row];
   if (s > kSumLimit) {  // a row whose reference was too low: its sums were made again
@@ -304,7 +373,7 @@ __global__ void __launch_bounds__(256) xent_dz_kernel(const XentBf16Args a) {
     __syncthreads();
     s = again;
   }
-  const float all = s + expf(a.zt[row] - a.ref[row]), g = a.row_weight ? a.row_weight[row] : 1.f;
+  const float all = s + expf(a.zt[row] - a.ref[row]), g = a.row_weight ? a.row_weight[a.order[row]] : 1.f;
   constexpr float L2E = 1.4426950408889634f;
   const float k0 = (kLogitLow + 64.f) * L2E - log2f(all), k1 = kLogitStep * L2E;
   for (int i = threadIdx.x; i < n; i += 256) {

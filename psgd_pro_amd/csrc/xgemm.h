@@ -14,16 +14,20 @@ struct XgArgs {
   const bf16_t* B;
   int tiles_m, tiles_n;
   int kreal;           // rows of an mn-contiguous A (0: K); k behind them reads zeros
+  // the rows that are there: count[0] - first of them (count in device memory), at most N (XG_DW: K)
+  const int* count;
+  int first;
   int splits, kchunk;  // split s covers k in [s kchunk, (s + 1) kchunk), none of them empty; splits > 1 need outf
   // products with the vocabulary matrix or the rows: out = alpha[0] acc in bf16 (alpha null: 1), or
   bf16_t* out;
   const float* alpha;
+  const int* order;    // XG_DX with out: row n goes to row order[n]
   float* outf;         // (where set) split s's acc in fp32 at outf + s N ldo: 16-byte aligned, ldo a multiple of 4
   int accumulate;      // outf += acc
   // logits: m counts the vocabulary, n the rows
   int16_t* q;              // coded logits (see kLogitStep), null: sums only
   const float* ref;        // the row's reference r
-  const int* target;       // the row's target column, -1: none (an ignored row)
+  const int* target;       // the row's target column
   float* sums;             // of each 128 columns, the sum of e^(z - r) over those that are not the target: [N][2 tiles_m]
   float* tops;             // with `max_only` instead of all that: their largest z, same layout
   int max_only;

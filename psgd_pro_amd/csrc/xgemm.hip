@@ -84,8 +84,10 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
   const int c = lane & 31, hh = lane >> 5, wm = wave >> 1, wn = wave & 1;
 
   static_assert(BN == kXgRows, "a listed block is a tile of n");
-  const int ntiles = REDO ? p.redo[0] * p.tiles_m : p.tiles_m * p.tiles_n * p.splits;
-  if ((int)blockIdx.x >= ntiles) return;
+  const int live = __builtin_amdgcn_readfirstlane(min(max(p.count[0] - p.first, 0), KIND == XG_DW ? p.K : p.N));
+  const int N = KIND == XG_DW ? p.N : live, K = KIND == XG_DW ? live : p.K, tiles_n = (N + BN - 1) / BN;
+  const int ntiles = REDO ? p.redo[0] * p.tiles_m : p.tiles_m * tiles_n * p.splits;
+  if ((int)blockIdx.x >= ntiles || (KIND == XG_DW && p.accumulate && K == 0)) return;
   // tile w of the workgroups' order: its m and n tile and its part of k
   auto where = [&](int w, int& ti, int& tj, int& split) __attribute__((always_inline)) {
     split = 0;
@@ -97,9 +99,9 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     // each XCD a contiguous run of tiles, 4 tiles of m by n after n, so that the tiles it runs at once share panels
     constexpr int GM = 4;
     int tile = xcd_run(w, ntiles);
-    split = tile / (p.tiles_m * p.tiles_n);
-    tile -= split * (p.tiles_m * p.tiles_n);
-    const int grp = tile / (GM * p.tiles_n), r0 = grp * GM, gm = min(GM, p.tiles_m - r0), idx = tile - r0 * p.tiles_n;
+    split = tile / (p.tiles_m * tiles_n);
+    tile -= split * (p.tiles_m * tiles_n);
+    const int grp = tile / (GM * tiles_n), r0 = grp * GM, gm = min(GM, p.tiles_m - r0), idx = tile - r0 * tiles_n;
     ti = r0 + (gm == GM ? idx % GM : idx % gm);
     tj = gm == GM ? idx / GM : idx / gm;
   };
@@ -133,13 +135,13 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     where(wl, ti, tj, split);
     const int m0 = ti * BM, n0 = tj * BN;
     kp = split * p.kchunk;
-    kl = min(p.K, kp + p.kchunk);
+    kl = min(K, kp + p.kchunk);
     pa = p.A + (MCA ? (long long)kp * p.lda + m0 : (long long)m0 * p.lda + kp);
     pb = p.B + (MCB ? (long long)kp * p.ldb + n0 : (long long)n0 * p.ldb + kp);
     ea = MCA ? (long long)(min(kl, p.kreal) - kp - 1) * p.lda + ((p.M - m0 + 7) & ~7)
              : (long long)(p.M - m0 - 1) * p.lda + (kl - kp);
-    eb = MCB ? (long long)(kl - kp - 1) * p.ldb + ((p.N - n0 + 7) & ~7)
-             : (long long)(p.N - n0 - 1) * p.ldb + (kl - kp);
+    eb = MCB ? (long long)(kl - kp - 1) * p.ldb + ((N - n0 + 7) & ~7)
+             : (long long)(N - n0 - 1) * p.ldb + (kl - kp);
   };
   auto plan = [&](bool first) __attribute__((always_inline)) {
     if (!first) {
@@ -238,10 +240,11 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
   for (int w = blockIdx.x; w < ntiles; w += gridDim.x) {
     int ti, tj, split;
     where(w, ti, tj, split);
-    const int nk = (min(p.K - split * p.kchunk, p.kchunk) + BK - 1) / BK;
+    int nk = max((min(K - split * p.kchunk, p.kchunk) + BK - 1) / BK, 1);  // (of no rows at all: zeros)
+    asm("" : "+s"(nk));  // known to be at least 1, the loop's registers spill
     const int mw = ti * BM + wm * WTM, nw = tj * BN + wn * WTN;  // this wave's block
     if constexpr (KIND == XG_LOGITS) {  // r and target of the wave's rows, into its way out, for when the products are done
-      i32x4_t rs = rsrc_words(p.ref, 4ll * p.N), ts = rsrc_words(p.target, 4ll * p.N);
+      i32x4_t rs = rsrc_words(p.ref, 4ll * N), ts = rsrc_words(p.target, 4ll * N);
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_nop 4" : "+s"(rs), "+s"(ts)::"memory");
 #pragma unroll
       for (int i = 0; i < WTN; i += 64) {
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const int n = nw + 32 * j + c;
-        if (n >= p.N) continue;
+        if (n >= N) continue;
         float* const q = o + (long long)n * p.ldo + mw + 4 * hh;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
@@ -324,11 +327,17 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     }
     constexpr int CH = WTM / 8;
     auto slot = [&](int n, int ch) __attribute__((always_inline)) { return ep0 + n * WTM * 2 + ((ch ^ (n & (CH - 1))) << 4); };
+    int to_lo = 0, to_hi = 0;  // where rows nw + lane and nw + 64 + lane go
+    if constexpr (KIND == XG_DX) {
+      static_assert(WTN == 128, "two rows a lane");
+      to_lo = p.order[min(nw + lane, N - 1)];
+      to_hi = p.order[min(nw + 64 + lane, N - 1)];
+    }
     uint16_t* const out = KIND == XG_LOGITS ? reinterpret_cast<uint16_t*>(p.q) : p.out;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int n = nw + 32 * j + c;
-      const bool row = n < p.N;
+      const bool row = n < N;
       if constexpr (KIND == XG_LOGITS) {
         const float r = ref[j];
         const int t = tgt[j];
@@ -390,7 +399,7 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
           if (row && hh == 0) p.tops[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = top;
         } else {
           s += __shfl_xor(s, 32, 64);
-          if (row && hh == 0) p.sums[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = t < 0 ? 0.f : s;
+          if (row && hh == 0) p.sums[(long long)n * 2 * p.tiles_m + 2 * ti + wm] = s;
         }
         if (!p.q) continue;
       } else {
@@ -408,8 +417,9 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
       for (int it = 0; it < 32 * CH / 64; ++it) {
         const int idx = it * 64 + lane, q = idx / CH, ch = idx % CH, m = mw + 8 * ch, no = nw + 32 * j + q;
         const uint4 x = *reinterpret_cast<const uint4*>(slot(q, ch));
-        if (no >= p.N || m >= p.M) continue;
-        uint16_t* o = out + (long long)no * p.ldo + m;
+        const int to = KIND == XG_DX ? __shfl(j < 2 ? to_lo : to_hi, (32 * j + q) & 63, 64) : no;
+        if (no >= N || m >= p.M) continue;
+        uint16_t* o = out + (long long)to * p.ldo + m;
         if (m + 8 <= p.M) {
           __builtin_memcpy(o, &x, 16);
         } else {

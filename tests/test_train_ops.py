@@ -482,6 +482,53 @@ def test_cross_entropy_ignored_rows_hold_anything(dtype, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pattern", ["prompt", "padding", "alternate", "one", "first", "last"])
+@pytest.mark.parametrize("n,d,v", [(700, 72, 600), (4500, 24, 130), (65, 40, 300)])
+def test_cross_entropy_patterns_of_ignored_rows(dtype, pattern, n, d, v):
+    """Rows that count are gathered: whichever they are, each loss and gradient lies at its own row, the others are 0."""
+    i = torch.arange(n, device=DEV)
+    keep = {"prompt": i % 97 >= 50, "padding": i < n * 2 // 3, "alternate": i % 2 == 1, "one": i == n // 2, "first": i == 0,
+            "last": i == n - 1}[pattern]
+    x, w = rnd((n, d), 31, dtype).requires_grad_(), rnd((v, d), 32, dtype, std=0.3).requires_grad_()
+    t = targets(n, v, 33).masked_fill(~keep, -100)
+    run_lce(x, w, t)
+    loss = P.linear_cross_entropy(x, w, t, reduction="none")
+    dx, = torch.autograd.grad(loss.sum(), x)
+    assert torch.equal(loss[~keep], torch.zeros_like(loss[~keep])) and torch.equal(dx[~keep], torch.zeros_like(dx[~keep]))
+    if dtype == torch.bfloat16:  # the same bits as from the others alone
+        xs = x.detach()[keep].requires_grad_()
+        alone = P.linear_cross_entropy(xs, w, t[keep], reduction="none")
+        if int(keep.sum()) > 64:  # (up to 64 rows take a kernel of their own where there are no gradients)
+            assert torch.equal(alone, loss[keep])
+        assert torch.equal(torch.autograd.grad(alone.sum(), xs)[0], dx[keep])
+
+
+def test_cross_entropy_slabs_without_a_row_that_counts():
+    """More rows than the logits' memory holds at once: what counts fills the first slabs only."""
+    n, d, v = 12000, 8, 50021
+    x, w = rnd((n, d), 41, torch.bfloat16).requires_grad_(), rnd((v, d), 42, torch.bfloat16, std=0.3).requires_grad_()
+    for kept in (0, 300, 11000):
+        t = targets(n, v, 43)
+        t[:n - kept] = -100  # the last `kept` rows
+        loss = P.linear_cross_entropy(x, w, t, reduction="sum")
+        dx, dw = torch.autograd.grad(loss, (x, w))
+        xs = x.detach()[n - kept:].requires_grad_()
+        if kept:
+            some = P.linear_cross_entropy(xs, w, t[n - kept:], reduction="sum")
+            sx, sw = torch.autograd.grad(some, (xs, w))
+            # the same slabs either way; a single one sums the vocabulary in other parts (rows of softmax - 1: sum below 2)
+            if kept == 11000:
+                assert torch.equal(dx[n - kept:], sx)
+            else:
+                within(dx[n - kept:], sx.double(), 2 * U[torch.bfloat16] * sx.double().abs() + (v + 64) * E * 2 * w.abs().max())
+            assert torch.equal(dw, sw)
+            assert abs(float(loss) - float(some)) <= n * E * float(some)
+        else:
+            assert float(loss) == 0 and not dw.any()
+        assert not dx[:n - kept].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("gain", [1e-3, 30.0, 300.0])
 def test_cross_entropy_sharp_and_flat_rows(dtype, gain):
     """Logits from nearly equal to a spread of a thousand: rows sure of their target (the loss underflows to zero
