@@ -64,9 +64,8 @@ struct ResArgs {
   float4* means;            // res_backward_wide: one float4 a row for the column kernel
 };
 enum { kSumPreW = 0, kSumPreB = 1, kSumPostW = 2, kSumPostB = 3 };
-// Rows that do not stay in registers but are read again for each pass: under one vector of 8 elements, over 8192, and
-// (1024 threads have no registers for the masks) over 4096 with an end inside a vector.
-inline bool res_wide(long long d) { return d < 8 || d > 8192 || (d > 4096 && d % 8 != 0); }
+// Rows that do not stay in registers but are read again for each pass: under one vector of 8 elements and over 8192.
+inline bool res_wide(long long d) { return d < 8 || d > 8192; }
 constexpr int kMaxNormD = 1 << 20;
 
 // What a backward call has beside a root-mean-square norm before the next block.
@@ -75,10 +74,11 @@ inline int res_has(const ResArgs& a) {
   return (a.post != NORM_NONE ? kPost : 0) | (a.gate.p ? kGate : 0) |
          (a.pre == NORM_LAYER || a.post == NORM_LAYER ? kBias : 0);
 }
-// The backward pass also reads rows over 4096 again where it has two of these (registers again).
+// The backward pass has no registers for two of these in rows over 4096 (nor for a gate alone, where fp32 rows end inside a
+// vector): such a row's values are made again from its bits for each pass, the column sums by a kernel of their own.
 inline bool res_backward_wide(const ResArgs& a) {
   const int h = res_has(a);
-  return res_wide(a.d) || (a.d > 4096 && (h & (h - 1)) != 0);
+  return res_wide(a.d) || (a.d > 4096 && ((h & (h - 1)) != 0 || (h == kGate && a.d % 8 != 0 && a.dt == 0)));
 }
 
 hipError_t residual_norm_launch(const ResArgs& a, hipStream_t st);

@@ -46,18 +46,6 @@ __device__ __forceinline__ void st_row(T* row, int c, int d, const float (&v)[VE
       if (c + e < d) row[c + e] = from_f32<T>(v[e]);
   }
 }
-// The same of a vector with a dtype of its own; `none` where it is absent.
-__device__ __forceinline__ void ld_vec(const Vec& w, long long off, int c, int d, float none, float (&v)[VE]) {
-  if (!w.p) {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) v[e] = none;
-  } else if (w.dt == 1) {
-    ld_row(reinterpret_cast<const bf16_t*>(w.p) + off, c, d, v);
-  } else {
-    ld_row(reinterpret_cast<const float*>(w.p) + off, c, d, v);
-  }
-}
-
 // One thread's 8 elements c .. c + 7 of rows of d >= 8 elements. Where the row ends inside them the load starts 8
 // elements before its end and the values move down (zeros behind the end): every lane loads one whole vector. RAGGED:
 // d is no multiple of 8 (else there is nothing to move and to mask).
@@ -91,7 +79,7 @@ struct Span {
       if constexpr (sizeof(T) == 2) v[e] = __uint_as_float(e & 1 ? r.w[e / 2] & 0xffff0000u : r.w[e / 2] << 16);
       else v[e] = __uint_as_float(r.w[e]);
     }
-    if constexpr (RAGGED) {
+    if (RAGGED && __any(move)) {  // (only in the wave that holds the row's end)
 #pragma unroll
       for (int s = 4; s > 0; s >>= 1) {
         const bool m = move & s;
@@ -291,87 +279,248 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_kernel(const R
   if (a.stats && t == 0 && live) a.stats[row] = st;
 }
 
-// Rows too long for the registers, or too short for a vector: every pass reads the row again (from the caches), with
-// the same sums.
+// What a thread has of a row in the kernels for the rest of the lengths (see res_wide): the bits of 8 elements of every
+// tensor, all loaded before any is looked at. A load that starts inside the last 8 elements of a row starts at the first
+// of them, and the values move down (zeros behind the end).
+template <typename T>
+struct Wide {
+  const ResArgs& a;
+  long long row;
+  float4 st, mean;
+  int c, at;
+  uint32_t x[VE * sizeof(T) / 4], f[VE * sizeof(T) / 4], dy[VE * sizeof(T) / 4], dh[VE * sizeof(T) / 4];
+  uint32_t g[VE], pw[VE], pb[VE], qw[VE], qb[VE];
+  __device__ __forceinline__ Wide(const ResArgs& args) : a(args) {}
+  __device__ __forceinline__ void place(int col) {
+    c = col;
+    at = a.d < VE ? 0 : min(c, a.d - VE);
+  }
+  template <typename U, size_t N>
+  __device__ __forceinline__ void bits(const U* p, uint32_t (&w)[N]) const {
+    if (a.d >= VE) {
+      __builtin_memcpy(w, p + at, VE * sizeof(U));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const uint32_t b = e >= a.d ? 0 : sizeof(U) == 4 ? reinterpret_cast<const uint32_t*>(p)[e] : (uint32_t)p[e];
+        if constexpr (sizeof(U) == 4) w[e] = b;
+        else w[e / 2] = e & 1 ? w[e / 2] | b << 16 : b;
+      }
+    }
+  }
+  __device__ __forceinline__ void bits(const Vec& v, long long off, uint32_t (&w)[VE]) const {
+    if (!v.p) return;
+    if (v.dt == 1) bits(reinterpret_cast<const bf16_t*>(v.p) + off, w);
+    else bits(reinterpret_cast<const float*>(v.p) + off, w);
+  }
+  // the row's own tensors (whichever the call has), and the vectors that all rows share
+  __device__ __forceinline__ void fetch_row() {
+    if (a.x) bits(reinterpret_cast<const T*>(a.x) + row * a.ldx, x);
+    if (a.f) bits(reinterpret_cast<const T*>(a.f) + row * a.ldf, f);
+    if (a.dy) bits(reinterpret_cast<const T*>(a.dy) + row * a.lddy, dy);
+    if (a.dh) bits(reinterpret_cast<const T*>(a.dh) + row * a.lddh, dh);
+    bits(a.gate, row / a.gate_every * a.ldg, g);
+  }
+  __device__ __forceinline__ void fetch_shared(bool bias) {
+    bits(a.pre_w, 0, pw);
+    if (bias) bits(a.pre_b, 0, pb);
+    bits(a.post_w, 0, qw);
+    bits(a.post_b, 0, qb);
+  }
+  __device__ __forceinline__ void move_down(float (&v)[VE]) const {
+    if (a.d < VE || !__any(c != at)) return;  // (only in the wave that holds the row's end)
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1) {
+      const bool m = (c - at) & s;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = m ? (e + s < VE ? v[e + s] : 0.f) : v[e];
+    }
+  }
+  template <typename U, size_t N>
+  __device__ __forceinline__ void values(const uint32_t (&w)[N], float (&v)[VE]) const {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      if constexpr (sizeof(U) == 2) v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+      else v[e] = __uint_as_float(w[e]);
+    }
+    move_down(v);
+  }
+  __device__ __forceinline__ void values(const Vec& q, const uint32_t (&w)[VE], float none, float (&v)[VE]) const {
+    if (!q.p) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = none;
+    } else if (q.dt == 1) {
+      values<bf16_t>(w, v);
+    } else {
+      values<float>(w, v);
+    }
+  }
+  // the branch: f's normalised values, b = dropout(Npost(f)) and the elements kept
+  __device__ __forceinline__ unsigned branch(float (&fh)[VE], float (&b)[VE]) const {
+    unsigned kept = 255;
+    values<T>(f, fh);
+    if (a.post != NORM_NONE) {
+      float w[VE];
+      values(a.post_w, qw, 1.f, w);
+      values(a.post_b, qb, 0.f, b);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        fh[e] = (fh[e] - st.z) * st.w;
+        b[e] += fh[e] * w[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) b[e] = fh[e];
+    }
+    if (a.drop.thr) {
+      float k[VE];
+      drop8(a.drop, row, c, a.d, k);
+      kept = 0;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        b[e] = dropped(b[e], k[e]);
+        kept |= k[e] != 0.f ? 1u << e : 0u;
+      }
+    }
+    return kept;
+  }
+  __device__ __forceinline__ void y_of(float (&y)[VE]) const {
+    values<T>(x, y);
+    if (!a.f) return;
+    float fh[VE], b[VE], gate[VE];
+    branch(fh, b);
+    values(a.gate, g, 1.f, gate);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) y[e] += a.scale * gate[e] * b[e];
+  }
+  // y's normalised values, dh and c = dh w
+  __device__ __forceinline__ void pre(float (&hat)[VE], float (&dhv)[VE], float (&cw)[VE]) const {
+    y_of(hat);
+    values<T>(dh, dhv);
+    values(a.pre_w, pw, 1.f, cw);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      hat[e] = (hat[e] - st.x) * st.y;
+      cw[e] *= dhv[e];
+    }
+  }
+  __device__ __forceinline__ void dyt(float (&v)[VE]) const {
+    if (a.dy) values<T>(dy, v);
+    else
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = 0.f;
+    if (!a.dh) return;
+    float hat[VE], dhv[VE], cw[VE];
+    pre(hat, dhv, cw);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] += (cw[e] - mean.x - hat[e] * mean.y) * st.y;
+  }
+  // v = dyt in; out: f's normalised values, du (v), du w (dw) and the gate's gradient
+  __device__ __forceinline__ void post(float (&v)[VE], float (&fh)[VE], float (&dw)[VE], float (&dg)[VE]) const {
+    float gate[VE];
+    const unsigned kept = branch(fh, dg);
+    values(a.gate, g, 1.f, gate);
+    if (a.post != NORM_NONE) {
+      values(a.post_w, qw, 1.f, dw);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) dw[e] = 1.f;
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      float du = a.scale * v[e];
+      dg[e] *= du;
+      du *= gate[e];
+      if (a.drop.thr) du = kept >> e & 1 ? du * a.drop.scale : 0.f;
+      v[e] = du;
+      dw[e] *= du;
+    }
+  }
+};
+// The values made of the bits so far are not kept for later, where they would not fit the registers: an empty asm statement
+// makes the bits new ones to the compiler.
+template <typename... W>
+__device__ __forceinline__ void forget(W&... w) {
+  auto one = [](auto& q) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t& b : q) asm volatile("" : "+v"(b));
+  };
+  (one(w), ...);
+}
+// ONE: the rows fit one vector a thread, whose bits stay for all passes. Else every pass reads the row again, from the
+// caches (branch: only f is looked at).
+template <bool ONE, typename T, typename F>
+__device__ __forceinline__ void wide_pass(Wide<T>& t, bool bias, bool branch, F fn) {
+  if constexpr (ONE) {
+    forget(t.x, t.f, t.dy, t.dh, t.g);
+    t.fetch_shared(bias);
+    if (t.c < t.a.d) fn();
+  } else {
+    for (int c = threadIdx.x * VE; c < t.a.d; c += blockDim.x * VE) {
+      t.place(c);
+      if (branch) {
+        t.bits(reinterpret_cast<const T*>(t.a.f) + t.row * t.a.ldf, t.f);
+      } else {
+        t.fetch_row();
+        t.fetch_shared(bias);
+      }
+      fn();
+    }
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(1024) residual_norm_wide_kernel(const ResArgs a) {
   __shared__ float red[16];
-  const long long row = blockIdx.x;
-  const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
-  const T* fr = reinterpret_cast<const T*>(a.f) + (a.f ? row * a.ldf : 0);
-  const long long goff = row / a.gate_every * a.ldg;
+  Wide<T> t(a);
+  t.row = blockIdx.x;
+  t.st = make_float4(0.f, 0.f, 0.f, 0.f);
+  t.place(threadIdx.x * VE);
   const float inv_d = 1.f / (float)a.d;
-  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto each = [&](auto fn) {
-    for (int c = threadIdx.x * VE; c < a.d; c += 1024 * VE) fn(c);
-  };
-  // y's elements c .. c + 7
-  auto y_of = [&](int c, float (&y)[VE]) {
-    ld_row(xr, c, a.d, y);
-    if (!a.f) return;
-    float b[VE], g[VE];
-    ld_row(fr, c, a.d, b);
-    if (a.post != NORM_NONE) {
-      float w[VE], bs[VE];
-      ld_vec(a.post_w, 0, c, a.d, 1.f, w);
-      ld_vec(a.post_b, 0, c, a.d, 0.f, bs);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) b[e] = (b[e] - st.z) * st.w * w[e] + bs[e];
-    }
-    ld_vec(a.gate, goff, c, a.d, 1.f, g);
-    if (a.drop.thr) {
-      float m[VE];
-      drop8(a.drop, row, c, a.d, m);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) b[e] = dropped(b[e], m[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < VE; ++e) y[e] += a.scale * g[e] * b[e];
-  };
-  auto stats = [&](int kind, auto at) {
+  auto stats = [&](int kind, bool branch, auto at) {
     float mean = 0.f, s = 0.f;
     if (kind == NORM_LAYER) {
-      each([&](int c) {
+      wide_pass<false>(t, false, branch, [&] {
         float v[VE];
-        at(c, v);
+        at(v);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) s += c + e < a.d ? v[e] : 0.f;
+        for (int e = 0; e < VE; ++e) s += t.c + e < a.d ? v[e] : 0.f;
       });
       mean = block_sum(s, red) * inv_d;
       s = 0.f;
     }
-    each([&](int c) {
+    wide_pass<false>(t, false, branch, [&] {
       float v[VE];
-      at(c, v);
+      at(v);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) s += c + e < a.d ? (v[e] - mean) * (v[e] - mean) : 0.f;
+      for (int e = 0; e < VE; ++e) s += t.c + e < a.d ? (v[e] - mean) * (v[e] - mean) : 0.f;
     });
     return make_float2(mean, 1.f / sqrtf(block_sum(s, red) * inv_d + a.eps));
   };
   if (a.f && a.post != NORM_NONE) {
-    const float2 s = stats(a.post, [&](int c, float (&v)[VE]) { ld_row(fr, c, a.d, v); });
-    st.z = s.x;
-    st.w = s.y;
+    const float2 s = stats(a.post, true, [&](float (&v)[VE]) { t.template values<T>(t.f, v); });
+    t.st.z = s.x;
+    t.st.w = s.y;
   }
   if (a.pre != NORM_NONE) {
-    const float2 s = stats(a.pre, y_of);
-    st.x = s.x;
-    st.y = s.y;
+    const float2 s = stats(a.pre, false, [&](float (&v)[VE]) { t.y_of(v); });
+    t.st.x = s.x;
+    t.st.y = s.y;
   }
-  each([&](int c) {
+  wide_pass<false>(t, true, false, [&] {
     float y[VE];
-    y_of(c, y);
-    if (a.y) st_row(reinterpret_cast<T*>(a.y) + row * a.ldy, c, a.d, y);
+    t.y_of(y);
+    if (a.y) st_row(reinterpret_cast<T*>(a.y) + t.row * a.ldy, t.c, a.d, y);
     if (a.pre != NORM_NONE) {
       float w[VE], b[VE];
-      ld_vec(a.pre_w, 0, c, a.d, 1.f, w);
-      ld_vec(a.pre_b, 0, c, a.d, 0.f, b);
+      t.values(a.pre_w, t.pw, 1.f, w);
+      t.values(a.pre_b, t.pb, 0.f, b);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) w[e] = (y[e] - st.x) * st.y * w[e] + b[e];
-      st_row(reinterpret_cast<T*>(a.h) + row * a.ldh, c, a.d, w);
+      for (int e = 0; e < VE; ++e) w[e] = (y[e] - t.st.x) * t.st.y * w[e] + b[e];
+      st_row(reinterpret_cast<T*>(a.h) + t.row * a.ldh, t.c, a.d, w);
     }
   });
-  if (a.stats && threadIdx.x == 0) a.stats[row] = st;
+  if (a.stats && threadIdx.x == 0) a.stats[t.row] = t.st;
 }
 
 }  // namespace
@@ -390,7 +539,7 @@ static hipError_t residual_norm_t(const ResArgs& a, hipStream_t st) {
   else if (a.d <= 1024) residual_norm_sized<T, 128>(a, st);
   else if (a.d <= 2048) residual_norm_sized<T, 256>(a, st);
   else if (a.d <= 4096) residual_norm_sized<T, 512>(a, st);
-  else hipLaunchKernelGGL((residual_norm_kernel<T, 1024, false>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+  else residual_norm_sized<T, 1024>(a, st);
   return hipGetLastError();
 }
 hipError_t residual_norm_launch(const ResArgs& a, hipStream_t st) {
@@ -433,13 +582,13 @@ __device__ __forceinline__ void put_sum(float (&s)[VE], float* dst, const Span<R
 // holds no registers. SUMS: column sums in registers (1: of the norm before, 2: of the norm after, 4: of the gate).
 // Waves a SIMD, by what their registers hold without scratch memory: two workgroups of 512 threads want 128 registers,
 // three of 256 threads 168.
-constexpr int res_waves(int tpr, int has, int esize, bool ragged) {
+constexpr int res_waves(int tpr, int has, int esize) {
   if (tpr == 1024) return 4;
-  if (tpr == 512) return !ragged && (has == 0 || has == kBias || (has == kPost && esize == 2)) ? 4 : 2;
-  return ragged || has == 7 || (has == (kPost | kGate) && esize == 4) ? 2 : 3;
+  if (tpr == 512) return has == 0 || has == kBias || (has == kPost && esize == 2) ? 4 : 2;
+  return has == 7 || (has == (kPost | kGate) && esize == 4) ? 2 : 3;
 }
 template <typename T, int TPR, int HAS, int SUMS, bool RAGGED>
-__global__ void __launch_bounds__(res_threads(TPR), res_waves(TPR, HAS, sizeof(T), RAGGED))
+__global__ void __launch_bounds__(res_threads(TPR), res_waves(TPR, HAS, sizeof(T)))
     residual_norm_backward_kernel(const ResArgs a) {
   constexpr int RW = res_threads(TPR) / TPR;  // rows the workgroup has in hand at once
   constexpr bool AHEAD = TPR < 1024;          // 1024 threads have no registers for the next row's bits
@@ -622,141 +771,68 @@ __global__ void __launch_bounds__(res_threads(TPR), res_waves(TPR, HAS, sizeof(T
   }
 }
 
-// Rows too long for the registers: the same gradients with every pass reading the row again; the column sums are a
-// second kernel's, from the rows' means kept by this one.
-template <typename T>
-struct ResWide {
-  const ResArgs& a;
-  long long row;
-  float4 st, mean;
-  long long goff;
-  // the branch's elements c .. c + 7: f's normalised values, b = dropout(Npost(f)), and the weight, gate and kept bits
-  __device__ __forceinline__ unsigned branch(int c, float (&fh)[VE], float (&b)[VE], float (&w)[VE], float (&g)[VE]) const {
-    unsigned kept = 0;
-    ld_row(reinterpret_cast<const T*>(a.f) + row * a.ldf, c, a.d, fh);
-    ld_vec(a.gate, goff, c, a.d, 1.f, g);
-    ld_vec(a.post_w, 0, c, a.d, 1.f, w);
-    ld_vec(a.post_b, 0, c, a.d, 0.f, b);
-    float k[VE];
-    if (a.drop.thr) drop8(a.drop, row, c, a.d, k);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      if (a.post != NORM_NONE) {
-        fh[e] = (fh[e] - st.z) * st.w;
-        b[e] += fh[e] * w[e];
-      } else {
-        b[e] = fh[e];
-      }
-      if (a.drop.thr) {
-        b[e] = dropped(b[e], k[e]);
-        kept |= k[e] != 0.f ? 1u << e : 0u;
-      }
-    }
-    return kept;
-  }
-  // y's normalised values, dh and c = dh w
-  __device__ __forceinline__ void pre(int c, float (&hat)[VE], float (&dh)[VE], float (&cw)[VE]) const {
-    float w[VE];
-    ld_row(reinterpret_cast<const T*>(a.x) + row * a.ldx, c, a.d, hat);
-    ld_row(reinterpret_cast<const T*>(a.dh) + row * a.lddh, c, a.d, dh);
-    if (a.f) {
-      float fh[VE], b[VE], g[VE];
-      branch(c, fh, b, w, g);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) hat[e] += a.scale * g[e] * b[e];
-    }
-    ld_vec(a.pre_w, 0, c, a.d, 1.f, w);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      hat[e] = (hat[e] - st.x) * st.y;
-      cw[e] = dh[e] * w[e];
-    }
-  }
-  __device__ __forceinline__ void dyt(int c, float (&v)[VE]) const {
-    if (a.dy) ld_row(reinterpret_cast<const T*>(a.dy) + row * a.lddy, c, a.d, v);
-    else
-#pragma unroll
-      for (int e = 0; e < VE; ++e) v[e] = 0.f;
-    if (!a.dh) return;
-    float hat[VE], dh[VE], cw[VE];
-    pre(c, hat, dh, cw);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) v[e] += (cw[e] - mean.x - hat[e] * mean.y) * st.y;
-  }
-  // v = dyt in; out: f's normalised values, du (v), du w (dw) and the gate's gradient
-  __device__ __forceinline__ void post(int c, float (&v)[VE], float (&fh)[VE], float (&dw)[VE], float (&dg)[VE]) const {
-    float w[VE], b[VE], g[VE];
-    const unsigned kept = branch(c, fh, b, w, g);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      float du = a.scale * v[e];
-      dg[e] = du * b[e];
-      du *= g[e];
-      if (a.drop.thr) du = kept >> e & 1 ? du * a.drop.scale : 0.f;
-      v[e] = du;
-      dw[e] = a.post != NORM_NONE ? du * w[e] : du;
-    }
-  }
-};
-
-template <typename T>
-__global__ void __launch_bounds__(1024) residual_norm_backward_wide_kernel(const ResArgs a) {
+// The other lengths (Wide): the same gradients; the column sums are a second kernel's, from the rows' means kept by this
+// one.
+constexpr int res_wide_threads(int esize, bool one) { return one || esize == 2 ? 1024 : 512; }  // (registers)
+template <typename T, bool ONE>
+__global__ void __launch_bounds__(res_wide_threads(sizeof(T), ONE)) residual_norm_backward_wide_kernel(const ResArgs a) {
+  constexpr int TH = res_wide_threads(sizeof(T), ONE);
   __shared__ float2 red[2][16];
-  const long long row = blockIdx.x;
-  ResWide<T> r{a, row, a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f),
-               row / a.gate_every * a.ldg};
+  Wide<T> t(a);
+  t.row = blockIdx.x;
+  t.st = a.stats ? a.stats[t.row] : make_float4(0.f, 0.f, 0.f, 0.f);
+  t.mean = make_float4(0.f, 0.f, 0.f, 0.f);
+  t.place(threadIdx.x * VE);
+  if constexpr (ONE) t.fetch_row();
   const float inv_d = 1.f / (float)a.d;
-  auto each = [&](auto fn) {
-    for (int c = threadIdx.x * VE; c < a.d; c += 1024 * VE) fn(c);
-  };
   if (a.dh) {
     float2 m = make_float2(0.f, 0.f);
-    each([&](int c) {
+    wide_pass<ONE>(t, false, false, [&] {
       float hat[VE], dh[VE], cw[VE];
-      r.pre(c, hat, dh, cw);
+      t.pre(hat, dh, cw);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         m.x += cw[e];
-        m.y += c + e < a.d ? cw[e] * hat[e] : 0.f;
+        m.y += t.c + e < a.d ? cw[e] * hat[e] : 0.f;
       }
     });
-    m = row_sum2<1024>(m, red[0]);
-    r.mean.x = a.pre == NORM_LAYER ? m.x * inv_d : 0.f;
-    r.mean.y = m.y * inv_d;
+    m = row_sum2<TH>(m, red[0]);
+    t.mean.x = a.pre == NORM_LAYER ? m.x * inv_d : 0.f;
+    t.mean.y = m.y * inv_d;
   }
   if (a.f && a.post != NORM_NONE) {
     float2 m = make_float2(0.f, 0.f);
-    each([&](int c) {
+    wide_pass<ONE>(t, false, false, [&] {
       float v[VE], fh[VE], dw[VE], dg[VE];
-      r.dyt(c, v);
-      r.post(c, v, fh, dw, dg);
+      t.dyt(v);
+      t.post(v, fh, dw, dg);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        m.x += dw[e];
-        m.y += dw[e] * fh[e];
+        m.x += t.c + e < a.d ? dw[e] : 0.f;
+        m.y += t.c + e < a.d ? dw[e] * fh[e] : 0.f;
       }
     });
-    m = row_sum2<1024>(m, red[1]);
-    r.mean.z = a.post == NORM_LAYER ? m.x * inv_d : 0.f;
-    r.mean.w = m.y * inv_d;
+    m = row_sum2<TH>(m, red[1]);
+    t.mean.z = a.post == NORM_LAYER ? m.x * inv_d : 0.f;
+    t.mean.w = m.y * inv_d;
   }
-  each([&](int c) {
+  wide_pass<ONE>(t, false, false, [&] {
     float v[VE], fh[VE], dw[VE], dg[VE];
-    r.dyt(c, v);
-    if (a.dx) st_row(reinterpret_cast<T*>(a.dx) + row * a.lddx, c, a.d, v);
+    t.dyt(v);
+    if (a.dx) st_row(reinterpret_cast<T*>(a.dx) + t.row * a.lddx, t.c, a.d, v);
     if (!a.f) return;
-    r.post(c, v, fh, dw, dg);
+    t.post(v, fh, dw, dg);
     if (a.dgate && a.gate_every == 1) {
-      if (a.gate.dt == 1) st_row(reinterpret_cast<bf16_t*>(a.dgate) + row * a.lddg, c, a.d, dg);
-      else st_row(reinterpret_cast<float*>(a.dgate) + row * a.lddg, c, a.d, dg);
+      if (a.gate.dt == 1) st_row(reinterpret_cast<bf16_t*>(a.dgate) + t.row * a.lddg, t.c, a.d, dg);
+      else st_row(reinterpret_cast<float*>(a.dgate) + t.row * a.lddg, t.c, a.d, dg);
     }
     if (a.post != NORM_NONE) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) dw[e] = (dw[e] - r.mean.z - fh[e] * r.mean.w) * r.st.w;
+      for (int e = 0; e < VE; ++e) dw[e] = (dw[e] - t.mean.z - fh[e] * t.mean.w) * t.st.w;
     }
-    if (a.df) st_row(reinterpret_cast<T*>(a.df) + row * a.lddf, c, a.d, dw);
+    if (a.df) st_row(reinterpret_cast<T*>(a.df) + t.row * a.lddf, t.c, a.d, dw);
   });
-  if (threadIdx.x == 0) a.means[row] = r.mean;
+  if (threadIdx.x == 0) a.means[t.row] = t.mean;
 }
 
 // one workgroup: 2048 columns of `chunk` rows (the same split of the rows as the register kernel's)
@@ -775,14 +851,19 @@ __global__ void __launch_bounds__(256) residual_norm_columns_kernel(const ResArg
     r1 = min(r0 + a.chunk, a.rows);
   }
   float s[4][VE] = {}, sg[VE] = {};
-  for (long long row = r0; row < r1; ++row) {
-    ResWide<T> r{a, row, a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f), a.means[row],
-                 row / a.gate_every * a.ldg};
+  Wide<T> t(a);
+  t.place(c);
+  t.fetch_shared(false);
+  for (t.row = r0; t.row < r1; ++t.row) {
+    const long long row = t.row;
+    t.st = a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    t.mean = a.means[row];
+    t.fetch_row();
     float v[VE];
-    r.dyt(c, v);
+    t.dyt(v);
     if (a.dh) {
       float hat[VE], dh[VE], cw[VE];
-      r.pre(c, hat, dh, cw);
+      t.pre(hat, dh, cw);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         s[kSumPreW][e] += dh[e] * hat[e];
@@ -791,7 +872,7 @@ __global__ void __launch_bounds__(256) residual_norm_columns_kernel(const ResArg
     }
     if (a.f) {
       float fh[VE], dw[VE], dg[VE];
-      r.post(c, v, fh, dw, dg);
+      t.post(v, fh, dw, dg);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         s[kSumPostW][e] += v[e] * fh[e];
@@ -868,25 +949,28 @@ static void residual_norm_backward_has(const ResArgs& a, hipStream_t st) {
   }
 #undef PSGDK_RES
 }
-template <typename T, int TPR>
+template <typename T, int TPR, bool RAGGED>
 static void residual_norm_backward_sized(const ResArgs& a, hipStream_t st) {
-  if constexpr (TPR < 1024) {
-    if (a.d % VE) return residual_norm_backward_has<T, TPR, kPost | kGate | kBias, true>(a, st);
-  }
   switch (res_has(a)) {
-    case 0: return residual_norm_backward_has<T, TPR, 0, false>(a, st);
-    case 1: return residual_norm_backward_has<T, TPR, 1, false>(a, st);
-    case 2: return residual_norm_backward_has<T, TPR, 2, false>(a, st);
-    case 4: return residual_norm_backward_has<T, TPR, 4, false>(a, st);
+    case 0: return residual_norm_backward_has<T, TPR, 0, RAGGED>(a, st);
+    case 1: return residual_norm_backward_has<T, TPR, 1, RAGGED>(a, st);
+    case 2:
+      if constexpr (TPR < 1024 || !RAGGED || sizeof(T) == 2) return residual_norm_backward_has<T, TPR, 2, RAGGED>(a, st);
+      break;
+    case 4: return residual_norm_backward_has<T, TPR, 4, RAGGED>(a, st);
   }
   if constexpr (TPR < 1024) {
     switch (res_has(a)) {
-      case 3: return residual_norm_backward_has<T, TPR, 3, false>(a, st);
-      case 5: return residual_norm_backward_has<T, TPR, 5, false>(a, st);
-      case 6: return residual_norm_backward_has<T, TPR, 6, false>(a, st);
-      default: return residual_norm_backward_has<T, TPR, 7, false>(a, st);
+      case 3: return residual_norm_backward_has<T, TPR, 3, RAGGED>(a, st);
+      case 5: return residual_norm_backward_has<T, TPR, 5, RAGGED>(a, st);
+      case 6: return residual_norm_backward_has<T, TPR, 6, RAGGED>(a, st);
+      default: return residual_norm_backward_has<T, TPR, 7, RAGGED>(a, st);
     }
   }
+}
+template <typename T, int TPR>
+static void residual_norm_backward_sized(const ResArgs& a, hipStream_t st) {
+  return a.d % VE ? residual_norm_backward_sized<T, TPR, true>(a, st) : residual_norm_backward_sized<T, TPR, false>(a, st);
 }
 template <typename T>
 static hipError_t residual_norm_backward_t(const ResArgs& a, hipStream_t st) {
@@ -897,7 +981,11 @@ static hipError_t residual_norm_backward_t(const ResArgs& a, hipStream_t st) {
     else if (a.d <= 4096) residual_norm_backward_sized<T, 512>(a, st);
     else residual_norm_backward_sized<T, 1024>(a, st);
   } else {
-    hipLaunchKernelGGL(residual_norm_backward_wide_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+    if (a.d <= 1024 * VE)
+      hipLaunchKernelGGL((residual_norm_backward_wide_kernel<T, true>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+    else
+      hipLaunchKernelGGL((residual_norm_backward_wide_kernel<T, false>), dim3((unsigned)a.rows),
+                         dim3(res_wide_threads(sizeof(T), false)), 0, st, a);
     bool any = a.gpart != nullptr;
     for (int k = 0; k < 4; ++k) any = any || a.slot[k] >= 0;
     const int strips = (a.d + 256 * VE - 1) / (256 * VE);

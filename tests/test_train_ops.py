@@ -248,6 +248,15 @@ def test_residual_norm_long_rows(dtype, d, post, gate):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [2047, 4097, 4101, 6962, 8191])
+@pytest.mark.parametrize("pre,post,gate", [("rms", None, None), ("rms", "rms", None), ("rms", None, "token"), ("layer", None, None),
+                                           ("rms", "rms", "seq"), ("layer", "rms", None), ("layer", "layer", "token")])
+def test_residual_norm_long_rows_that_end_inside_a_vector(dtype, d, pre, post, gate):
+    shape = {None: None, "seq": (2, 1, d), "token": (2, 5, d)}[gate]
+    run_res((2, 5, d), dtype, pre, post, shape, p=0.1 if d % 3 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("gate", ["channel", "ones", "seq", "token"])
 @pytest.mark.parametrize("batch,tokens,d", [(1, 1, 64), (3, 1, 72), (5, 9, 130), (2, 700, 96), (700, 2, 520), (3, 65, 1100)])
 def test_residual_norm_gates(dtype, gate, batch, tokens, d):
