@@ -136,7 +136,9 @@ __device__ __forceinline__ float dropped(float v, float m) { return m == 0.f ? 0
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------------------------
-// y = dropout(x): one Philox block of 128 bits serves 8 elements, 16 bits each (drop probabilities in steps of 2^-16).
+// y = dropout(x): one Philox block of 128 bits serves 8 elements, 16 bits each (drop probabilities in steps of 2^-16), and
+// no mask is stored: the backward pass is the same kernel on the gradient. Bound by memory (2 bytes read and 2 written an
+// element against about 12 instructions): 16384 x 4096 bf16 forward and backward 104-107 us, 5.0-5.2 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_kernel(const DropArgs a) {
   const long long per = (a.d + VE - 1) / VE, total = a.rows * per;
@@ -164,7 +166,9 @@ hipError_t dropout_launch(const DropArgs& a, hipStream_t st) {
 // y = x + scale gate dropout(Npost(f)), h = Npre(y). TPR threads hold a row, 8 elements each; a workgroup of at least
 // 256 threads holds 256 / TPR rows. The waves' sums meet in LDS where a row has more than one. The
 // variance of a layer norm is the mean of the squared centred values, summed from the registers (no difference of large
-// sums). h is made from y before y's rounding.
+// sums). h is made from y before y's rounding. Bound by memory, x and f read once, y and h written once: 16384 rows of 4096
+// bf16 with two rms norms 102 us, 5.3 TB/s (as fast as a copy); 33280 rows of 512 fp32 with a layer norm, a gate and dropout
+// 48 us, 5.7 TB/s.
 namespace {
 
 constexpr int res_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(res_threads(TPR)) residual_norm_kernel(const R
   if (a.stats && t == 0 && live) a.stats[row] = st;
 }
 
-// What a thread has of a row in the kernels for the rest of the lengths (see res_wide): the bits of 8 elements of every
+// What a thread has of a row in the kernels for the other rows (res_wide, res_backward_wide): the bits of 8 elements of every
 // tensor, all loaded before any is looked at. A load that starts inside the last 8 elements of a row starts at the first
 // of them, and the values move down (zeros behind the end).
 template <typename T>
@@ -554,6 +558,10 @@ hipError_t residual_norm_launch(const ResArgs& a, hipStream_t st) {
 //   weights: column sums of dh hat and du fhat, biases: of dh and du
 // A workgroup takes `chunk` consecutive rows and keeps its column sums in registers; they go to one row of `part` each
 // and a second kernel adds those in a fixed order. A gate row whose rows all lie in one workgroup is written at once.
+// Bound by memory where rows are long enough (16384 rows of 4096 bf16, two rms norms: 180 us, 4.5 TB/s; 33280 rows of 512
+// fp32: 92 us, 4.4 TB/s), by the chain of a row's sums on short ragged ones (8481 rows of 770 bf16, everything on: 59 us,
+// 1.5 TB/s): a row's two means are each a wave's sum, a barrier and the waves' sums. The next row's loads are under way
+// meanwhile (without them, and with one workgroup a CU: 410 us in place of 180).
 namespace {
 
 // Stores a workgroup's column sum as a row of the partial sums and starts it again from zero.

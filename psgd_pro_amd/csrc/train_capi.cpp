@@ -137,7 +137,9 @@ int res_args(const psgdk_residual_norm_t* q, ResArgs& a) {
   return PSGDK_OK;
 }
 
-// Rows whose logits (4 bytes each in fp32, 2 on the bf16 path) are in memory at once: up to 1 GiB of them.
+// Rows whose logits (4 bytes each in fp32, 2 on the bf16 path) are in memory at once: up to 1 GiB of them. Fewer rows a
+// slab mean more sums of dw in fp32, more of them nothing (12288 x 2048 x 131072: 20.6 ms with 512 MiB, 18.7 with 1 GiB,
+// 19.4 with 2, whose slabs are uneven there).
 constexpr int64_t kLogitBytes = (int64_t)1 << 30;
 // 256 rows of a product's operand stay within 32-bit byte offsets
 constexpr int64_t kMaxVocab = (int64_t)1 << 22;
@@ -558,8 +560,7 @@ int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype
   const Lce p{rows, d, vocab, dtype, x, ldx, w, ldw, target, ignore, row_weight, mean, loss, mean_loss, dx, lddx, dw, lddw,
               ws, ws_bytes, (hipStream_t)stream};
   if (dtype == PSGDK_F32) return lce_f32(p);
-  // to 64 rows the matrix's bytes bound the call, and tiles of 256 rows would be mostly empty
-  return rows <= 64 && !dx && !dw ? lce_few(p) : lce_bf16(p);
+  return rows <= xent_few_rows(vocab) && !dx && !dw ? lce_few(p) : lce_bf16(p);
 }
 
 int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const float* scale, psgdk_stream_t stream) {

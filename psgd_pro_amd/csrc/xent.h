@@ -77,7 +77,7 @@ hipError_t sum_parts_launch(const float* in, int parts, long long n4, float* out
 hipError_t pad_rows_launch(const bf16_t* in, long long ldi, bf16_t* out, long long ldo, long long rows, int d,
                            hipStream_t st);
 
-// Losses of up to 64 rows without gradients: the vocabulary matrix is read once, straight into registers.
+// Losses of up to xent_few_rows rows without gradients: the vocabulary matrix is read once, straight into registers.
 struct XentFewArgs {
   int rows, d, vocab;
   long long ldx, ldw;
@@ -90,6 +90,10 @@ struct XentFewArgs {
   float2* part;  // [wgs][64]: largest logit, sum of e^(z - largest), the target left out of both
   float* loss;
 };
+// 32, or 64 where the vocabulary is short: to there the matrix's bytes bound the call, and the tiles of 256 rows of the
+// large products would be mostly empty. us, this way / those: 32 rows against 131072 x 4096 227 / 236, 64 rows 362 / 249;
+// 64 rows against 32768 x 1024 35 / 56, against 16384 x 1024 28 / 56; 1 row against 131072 x 4096 207 / 230.
+int xent_few_rows(int64_t vocab);
 int xent_few_wgs(int vocab);
 hipError_t xent_few_launch(const XentFewArgs& a, hipStream_t st);
 // out (rows of d) = x, with zeros for the rows whose target is `ignore`

@@ -490,6 +490,15 @@ def test_cross_entropy_ignored_rows_hold_anything(dtype, n):
     assert torch.equal(res[0][1][::2], torch.zeros_like(x[::2])) and float(res[0][3][::2].abs().sum()) == 0
 
 
+@pytest.mark.parametrize("n", [1, 16, 17, 32, 33, 64, 65])
+@pytest.mark.parametrize("d,v", [(40, 24576), (72, 24575), (33, 49152), (136, 49151), (256, 50001)])
+def test_cross_entropy_losses_of_a_few_rows(n, d, v):
+    x, w = rnd((n, d), 51, torch.bfloat16), rnd((v, d), 52, torch.bfloat16, 1.5 / math.sqrt(d))
+    t = targets(n, v, 53, 0.2)
+    (loss, err), _, _ = lce_ref(x, w, t, -100, torch.ones(n, device=DEV, dtype=torch.float64))
+    within(P.linear_cross_entropy(x, w, t, reduction="none"), loss, err)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("pattern", ["prompt", "padding", "alternate", "one", "first", "last"])
 @pytest.mark.parametrize("n,d,v", [(700, 72, 600), (4500, 24, 130), (65, 40, 300)])
