@@ -144,6 +144,11 @@ constexpr int64_t kLogitBytes = (int64_t)1 << 30;
 // 256 rows of a product's operand stay within 32-bit byte offsets
 constexpr int64_t kMaxVocab = (int64_t)1 << 22;
 
+// To here lce_small's fewer launches win over lce_bf16's fewer bytes and its gathered rows. us (with gradients), small /
+// large: 64 x 256 x 8192 48 / 75, 512 x 1024 x 16384 123 / 134, 256 x 1024 x 32768 132 / 155; beyond: 512 x 1024 x 32768
+// 191 / 183, 1024 x 1024 x 8192 133 / 131, 4096 x 256 x 2048 223 / 132.
+constexpr int64_t kSmallRows = 512, kSmallLogits = (int64_t)1 << 23;
+
 struct Lce {
   int64_t rows, d, vocab;
   int dtype;
@@ -180,10 +185,58 @@ int lce_pointers(const Lce& p) {
   if (p.dw) PSGDK_TRY(check_rows(p.dw, p.lddw, p.d, "dw"));
   return PSGDK_OK;
 }
+// whether the bf16 products cannot read the vocabulary matrix where it is
+bool needs_copy(const Lce& p) {
+  return p.d % 8 != 0 || p.ldw % 8 != 0 || p.ldw > kMaxVocab || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
+}
 int lce_mean(const Lce& p, const float* weight) {
   if (!p.mean_loss) return PSGDK_OK;
   return hip_check(xent_mean_launch(p.loss, p.row_weight, weight, p.target, p.rows, p.ignore, p.mean, p.mean_loss, p.st),
                    "cross entropy mean");
+}
+
+// rows r0 .. r0 + n - 1 of x for the products; with weight what all rows share besides
+int lce_copy(const Lce& p, int64_t r0, int64_t n, void* xm, int64_t ldm, float* weight, int* count, int* ended) {
+  XentCopyArgs a{};
+  a.rows = n;
+  a.ldx = p.ldx;
+  a.ldm = ldm;
+  a.d = (int)p.d;
+  a.mean = p.mean;
+  a.x = static_cast<const char*>(p.x) + r0 * p.ldx * esize(p.dtype);
+  a.xm = xm;
+  a.ignore = p.ignore;
+  a.target = p.target + r0;
+  a.all_targets = p.target;
+  a.all_rows = p.rows;
+  a.weight = weight;
+  a.count = count;
+  a.done = ended;
+  return hip_check(xent_copy_launch(a, p.dtype, p.st), "cross entropy copy");
+}
+// their losses from their logits, and the logits' gradients in their place or in dz; the mean or sum of up to kSmallRows
+// with the last
+int lce_rows(const Lce& p, int64_t r0, int64_t n, float* z, int64_t ldz, bf16_t* dz, int64_t ldq, const float* weight,
+             int* ended) {
+  XentRowsArgs a{};
+  a.z = z;
+  a.ldz = ldz;
+  a.rows = n;
+  a.vocab = (int)p.vocab;
+  a.grad = p.dx || p.dw;
+  a.dz = dz;
+  a.ldq = ldq;
+  a.ignore = p.ignore;
+  a.target = p.target + r0;
+  a.row_weight = p.row_weight ? p.row_weight + r0 : nullptr;
+  a.weight = weight;
+  a.loss = p.loss + r0;
+  a.mean_loss = p.rows <= kSmallRows ? p.mean_loss : nullptr;  // (more rows would queue at the count of those that ended)
+  a.done = ended;
+  a.all_rows = p.rows;
+  a.all_loss = p.loss;
+  a.all_weight = p.row_weight;
+  return hip_check(xent_rows_launch(a, p.st), "cross entropy rows");
 }
 
 // float32: the logits of a slab of rows by the converting engine, a pass over them, and its products with W and x.
@@ -192,6 +245,8 @@ int lce_f32(const Lce& p) {
   const int64_t ldz = (p.vocab + 3) / 4 * 4, slab = std::min(p.rows, std::max<int64_t>(1, kLogitBytes / 4 / ldz));
   Ws m(p.ws);
   float* const weight = m.take<float>(1);
+  int* const count = m.take<int>(1);
+  int* const ended = m.take<int>(1);
   float* const z = m.take<float>(slab * ldz);
   float* const xm = m.take<float>(slab * p.d);
   // dx is short and narrow with the vocabulary for k: parts of k as problems of one launch, where its 128 x 256 tiles
@@ -205,28 +260,15 @@ int lce_f32(const Lce& p) {
   PSGDK_TRY(lce_ws(p, m, done));
   if (done) return PSGDK_OK;
   PSGDK_TRY(lce_pointers(p));
-  PSGDK_TRY(hip_check(xent_weight_launch(p.target, p.rows, p.ignore, p.mean, weight, p.st), "cross entropy weight"));
   for (int64_t r0 = 0; r0 < p.rows; r0 += slab) {
     const int64_t n = std::min(slab, p.rows - r0);
     // an ignored row's x must reach nothing: 0 times an infinity is not 0, and a product scales its operands together
-    PSGDK_TRY(hip_check(xent_mask_rows_launch(static_cast<const float*>(p.x) + r0 * p.ldx, p.ldx, xm, p.target + r0,
-                                              p.ignore, n, (int)p.d, p.st), "mask rows"));
+    PSGDK_TRY(lce_copy(p, r0, n, xm, p.d, r0 ? nullptr : weight, count, ended));
     const void *zc = z, *xc = xm;
     const psgdk_stream_t st = (psgdk_stream_t)p.st;
     PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 1, n, p.vocab, p.d, 1.f, PSGDK_F32, PSGDK_F32, 1, &xc, p.d, &p.w, p.ldw, 0.f,
                          &z, ldz, st));
-    XentRowsArgs a{};
-    a.z = z;
-    a.ldz = ldz;
-    a.rows = n;
-    a.vocab = (int)p.vocab;
-    a.grad = grad;
-    a.ignore = p.ignore;
-    a.target = p.target + r0;
-    a.row_weight = p.row_weight ? p.row_weight + r0 : nullptr;
-    a.weight = weight;
-    a.loss = p.loss + r0;
-    PSGDK_TRY(hip_check(xent_rows_launch(a, p.st), "cross entropy rows"));
+    PSGDK_TRY(lce_rows(p, r0, n, z, ldz, nullptr, 0, weight, ended));
     if (p.dx) {
       float* out = static_cast<float*>(p.dx) + r0 * p.lddx;
       if (parts > 1) {
@@ -259,7 +301,7 @@ int lce_f32(const Lce& p) {
                            r0 ? 1.f : 0.f, &out, p.lddw, st));
     }
   }
-  return lce_mean(p, weight);
+  return p.rows <= kSmallRows ? PSGDK_OK : lce_mean(p, weight);
 }
 
 // bfloat16, a few rows, losses only
@@ -287,6 +329,86 @@ int lce_few(const Lce& p) {
   return lce_mean(p, nullptr);
 }
 
+// bfloat16, rows and vocabulary small: the logits in fp32, a pass over them, and the products of their gradients: half as
+// many launches as the way below.
+int lce_small(const Lce& p) {
+  const bool grad = p.dx || p.dw;
+  const int64_t ld = (p.d + 7) / 8 * 8, ldz = (p.vocab + 3) / 4 * 4, ldq = (p.vocab + 63) / 64 * 64, n = p.rows;
+  const bool copy_w = needs_copy(p);
+  const XgPlan z_plan = xgemm_plan(p.vocab, n, ld, false), dx_plan = xgemm_plan(p.d, n, ldq, true),
+               dw_plan = xgemm_plan(p.d, p.vocab, n, false);
+  const int splits = p.dx ? dx_plan.splits : 1;
+  Ws m(p.ws);
+  float* const weight = m.take<float>(1);
+  int* const count = m.take<int>(1);
+  int* const ended = m.take<int>(1);
+  float* const z = m.take<float>(n * ldz);
+  bf16_t* const xm = m.take<bf16_t>(n * ld);
+  bf16_t* const wp = m.take<bf16_t>(copy_w ? p.vocab * ld : 0);
+  bf16_t* const dz = m.take<bf16_t>(grad ? n * ldq : 0);
+  float* const dxp = m.take<float>(splits > 1 ? splits * n * ld : 0);
+  bool done;
+  PSGDK_TRY(lce_ws(p, m, done));
+  if (done) return PSGDK_OK;
+  PSGDK_TRY(lce_pointers(p));
+  XgArgs g{};
+  g.A = static_cast<const bf16_t*>(p.w);
+  g.lda = p.ldw;
+  if (copy_w) {
+    PSGDK_TRY(hip_check(pad_rows_launch(g.A, p.ldw, wp, ld, p.vocab, (int)p.d, p.st), "cross entropy copy"));
+    g.A = wp;
+    g.lda = ld;
+  }
+  PSGDK_TRY(lce_copy(p, 0, n, xm, ld, weight, count, ended));
+  g.count = count;
+  g.M = (int)p.vocab;
+  g.N = (int)n;
+  g.K = (int)ld;
+  g.B = xm;
+  g.ldb = ld;
+  g.splits = 1;
+  g.outf = z;
+  g.ldo = ldz;
+  XgArgs x = g;
+  PSGDK_TRY(hip_check(xgemm_launch(x, XG_Z, z_plan.bm, p.st), "logits"));
+  PSGDK_TRY(lce_rows(p, 0, n, z, ldz, grad ? dz : nullptr, ldq, weight, ended));
+  const float* const alpha = p.mean ? weight : nullptr;
+  if (p.dx) {
+    x = g;
+    x.M = (int)p.d;
+    x.K = (int)ldq;
+    x.kreal = (int)p.vocab;
+    x.B = dz;
+    x.ldb = ldq;
+    x.splits = splits;
+    x.kchunk = dx_plan.kchunk;
+    x.out = static_cast<bf16_t*>(p.dx);
+    x.ldo = splits > 1 ? ld : p.lddx;
+    x.alpha = alpha;
+    x.outf = splits > 1 ? dxp : nullptr;
+    PSGDK_TRY(hip_check(xgemm_launch(x, XG_DX, dx_plan.bm, p.st), "dx"));
+    if (splits > 1)
+      PSGDK_TRY(hip_check(to_bf16_rows_launch(dxp, splits, ld, alpha, x.out, p.lddx, n, (int)p.d, nullptr, nullptr, 0, p.st),
+                          "dx sums"));
+  }
+  if (p.dw) {
+    x = g;
+    x.M = (int)p.d;
+    x.N = (int)p.vocab;
+    x.K = (int)n;
+    x.A = xm;
+    x.lda = ld;
+    x.B = dz;
+    x.ldb = ldq;
+    x.out = static_cast<bf16_t*>(p.dw);
+    x.ldo = p.lddw;
+    x.alpha = alpha;
+    x.outf = nullptr;
+    PSGDK_TRY(hip_check(xgemm_launch(x, XG_DW, dw_plan.bm, p.st), "dw"));
+  }
+  return PSGDK_OK;
+}
+
 // bfloat16: the logits of a slab of rows as 16-bit codes with the sums of their exponentials (one product), a pass that
 // makes them the logits' gradients, and the products of those with W and x.
 int lce_bf16(const Lce& p) {
@@ -295,7 +417,7 @@ int lce_bf16(const Lce& p) {
   int64_t slab = std::max<int64_t>(kXgRows, kLogitBytes / 2 / ldq / kXgRows * kXgRows);
   if (slab >= p.rows) slab = p.rows;
   const int64_t blocks = (slab + kXgRows - 1) / kXgRows, parts = 2 * ((p.vocab + 255) / 256);
-  const bool copy_w = p.d % 8 != 0 || p.ldw % 8 != 0 || p.ldw > kMaxVocab || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
+  const bool copy_w = needs_copy(p);
   const bool sum_w = p.dw && slab < p.rows;
   const XgPlan dx_plan = xgemm_plan(p.d, slab, ldq, true), dw_plan = xgemm_plan(p.d, p.vocab, slab, false);
   const int splits = p.dx ? dx_plan.splits : 1;
@@ -560,7 +682,8 @@ int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype
   const Lce p{rows, d, vocab, dtype, x, ldx, w, ldw, target, ignore, row_weight, mean, loss, mean_loss, dx, lddx, dw, lddw,
               ws, ws_bytes, (hipStream_t)stream};
   if (dtype == PSGDK_F32) return lce_f32(p);
-  return rows <= xent_few_rows(vocab) && !dx && !dw ? lce_few(p) : lce_bf16(p);
+  if (rows <= xent_few_rows(vocab) && !dx && !dw) return lce_few(p);
+  return rows <= kSmallRows && rows * vocab <= kSmallLogits ? lce_small(p) : lce_bf16(p);
 }
 
 int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const float* scale, psgdk_stream_t stream) {

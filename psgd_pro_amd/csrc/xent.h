@@ -5,15 +5,12 @@
 
 namespace psgdk {
 
-// weight[0] = mean ? 1 / max(1, rows whose target is not `ignore`) : 1
-hipError_t xent_weight_launch(const int64_t* target, long long rows, int64_t ignore, int mean, float* weight,
-                              hipStream_t st);
-// out[0] = sum_i w_i loss[i], w_i = row_weight[i], or where that is null weight[0], or where that is null too as in
-// xent_weight_launch; in a fixed order
+// out[0] = sum_i w_i loss[i] in a fixed order, w_i = row_weight[i], or where that is null weight[0], or where that is null
+// too (mean) 1 / max(1, rows whose target is not `ignore`) or 1
 hipError_t xent_mean_launch(const float* loss, const float* row_weight, const float* weight, const int64_t* target,
                             long long rows, int64_t ignore, int mean, float* out, hipStream_t st);
 // order = the rows whose target is not `ignore`, in their order, then the others, whose losses become 0; count[0] = how
-// many are not; weight as in xent_weight_launch
+// many are not; weight[0] = mean ? 1 / max(1, count[0]) : 1
 hipError_t xent_order_launch(const int64_t* target, long long rows, int64_t ignore, int mean, int* order, int* count,
                              float* weight, float* loss, hipStream_t st);
 
@@ -23,11 +20,19 @@ struct XentRowsArgs {
   float* z;                 // 16-byte aligned; ldz a multiple of 4, less than vocab + 4
   long long ldz, rows;
   int vocab, grad;
+  bf16_t* dz;               // null, or: the gradients go there (rows of ldq, a multiple of 64, zeros behind the vocabulary)
+  long long ldq;            // without the mean's weight
   int64_t ignore;
   const int64_t* target;
   const float* row_weight;  // null: weight[0] for every row
   const float* weight;
   float* loss;
+  // null, or: the workgroup that ends last of all_rows ones (done counts them) adds their losses, all_loss[i] times
+  // all_weight[i] (null: weight[0]), in a fixed order
+  float* mean_loss;
+  int* done;
+  long long all_rows;
+  const float *all_loss, *all_weight;
 };
 hipError_t xent_rows_launch(const XentRowsArgs& a, hipStream_t st);
 
@@ -96,9 +101,22 @@ struct XentFewArgs {
 int xent_few_rows(int64_t vocab);
 int xent_few_wgs(int vocab);
 hipError_t xent_few_launch(const XentFewArgs& a, hipStream_t st);
-// out (rows of d) = x, with zeros for the rows whose target is `ignore`
-hipError_t xent_mask_rows_launch(const float* x, long long ldx, float* out, const int64_t* target, int64_t ignore,
-                                 long long rows, int d, hipStream_t st);
+// The rows of x (of a slab) for the products: row stride ldm, zeros in the rows whose target is `ignore` and (bf16, ldm a
+// multiple of 8) behind d. With weight also, for all rows: weight[0] = mean ? 1 / max(1, those not ignored) : 1,
+// count[0] = rows, done[0] = 0.
+struct XentCopyArgs {
+  long long rows, ldx, ldm;
+  int d, mean;
+  const void* x;
+  void* xm;
+  int64_t ignore;
+  const int64_t* target;
+  const int64_t* all_targets;
+  long long all_rows;
+  float* weight;
+  int *count, *done;
+};
+hipError_t xent_copy_launch(const XentCopyArgs& a, int dt, hipStream_t st);
 
 // x[b][0 .. n[b]) *= *scale (no access where *scale is 1)
 constexpr int kMaxScale = 4;

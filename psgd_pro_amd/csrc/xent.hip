@@ -11,23 +11,14 @@ __device__ __forceinline__ float count_weight(const int64_t* target, long long r
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
   int n = 0;
-  if (mean)
+  if (mean) {
+#pragma unroll 8
     for (long long i = threadIdx.x; i < rows; i += blockDim.x) n += target[i] != ignore;
+  }
   if (n) atomicAdd(&total, n);  // whole numbers: any order gives the same sum
   __syncthreads();
   return mean ? 1.f / (float)max(total, 1) : 1.f;
 }
-__global__ void __launch_bounds__(1024) xent_weight_kernel(const int64_t* target, long long rows, int64_t ignore,
-                                                           int mean, float* weight) {
-  const float w = count_weight(target, rows, ignore, mean);
-  if (threadIdx.x == 0) weight[0] = w;
-}
-hipError_t xent_weight_launch(const int64_t* target, long long rows, int64_t ignore, int mean, float* weight,
-                              hipStream_t st) {
-  hipLaunchKernelGGL(xent_weight_kernel, dim3(1), dim3(1024), 0, st, target, rows, ignore, mean, weight);
-  return hipGetLastError();
-}
-
 // The ignored rows' share of the products is saved by numbering the rows that count (1531 x 770 x 50021, half of them
 // ignored: 542 -> 420 us in all). One workgroup, 4096 rows a turn (a wave 256 of them, 64 by 64): first how many count, then their places.
 __global__ void __launch_bounds__(1024) xent_order_kernel(const int64_t* target, long long rows, int64_t ignore, int mean,
@@ -37,6 +28,7 @@ __global__ void __launch_bounds__(1024) xent_order_kernel(const int64_t* target,
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
   int n = 0;
+#pragma unroll 8
   for (long long i = threadIdx.x; i < rows; i += 1024) n += target[i] != ignore;
   if (n) atomicAdd(&total, n);  // whole numbers: any order gives the same sum
   __syncthreads();
@@ -109,20 +101,26 @@ hipError_t xent_mean_launch(const float* loss, const float* row_weight, const fl
 // written: 5.1 TB/s).
 // The products read whole vectors and take another path where they meet a value that is not finite, also behind the
 // vocabulary's end: no stale memory may lie there.
-__global__ void __launch_bounds__(1024) xent_rows_kernel(const XentRowsArgs a) {
-  __shared__ float red[16];
+template <int TH>
+__device__ __forceinline__ void xent_row(const XentRowsArgs& a, long long row, float* red) {
   constexpr float L2E = 1.4426950408889634f;
-  const long long row = blockIdx.x;
   float* const z = a.z + row * a.ldz;
   float4* const z4 = reinterpret_cast<float4*>(z);
   const int n4 = (int)(a.ldz / 4);
   const int64_t t = a.target[row];
   const bool skip = t == a.ignore, foreign = !skip && (t < 0 || t >= a.vocab);
+  // (agent scope: the workgroup that adds the losses may be on another XCD)
+  auto put_loss = [&](float v) { __hip_atomic_store(a.loss + row, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  auto put = [&](int i, const float (&x)[4]) {
+    if (a.dz) *reinterpret_cast<uint2*>(a.dz + row * a.ldq + 4 * i) = make_uint2(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]));
+    else z4[i] = make_float4(x[0], x[1], x[2], x[3]);
+  };
+  const int out4 = a.dz ? (int)(a.ldq / 4) : n4;
   if (skip || foreign) {
-    const float fill = skip ? 0.f : NAN;
-    if (threadIdx.x == 0) a.loss[row] = fill;
+    const float fill = skip ? 0.f : NAN, x[4] = {fill, fill, fill, fill};
+    if (threadIdx.x == 0) put_loss(fill);
     if (a.grad)
-      for (int i = threadIdx.x; i < n4; i += 1024) z4[i] = make_float4(fill, fill, fill, fill);
+      for (int i = threadIdx.x; i < out4; i += TH) put(i, x);
     return;
   }
   const float zt = z[t];
@@ -133,7 +131,7 @@ __global__ void __launch_bounds__(1024) xent_rows_kernel(const XentRowsArgs a) {
     for (int e = 0; e < 4; ++e) x[e] = 4 * i + e < a.vocab && 4 * i + e != t ? v[e] : -INFINITY;
   };
   float m = -INFINITY, s = 0.f;
-  for (int i = threadIdx.x; i < n4; i += 1024) {
+  for (int i = threadIdx.x; i < n4; i += TH) {
     float x[4];
     other(i, x);
     const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
@@ -147,22 +145,43 @@ __global__ void __launch_bounds__(1024) xent_rows_kernel(const XentRowsArgs a) {
   const float most = fmaxf(block_max(m, red), zt);
   s = block_sum(m > -INFINITY ? s * __builtin_amdgcn_exp2f((m - most) * L2E) : s, red);
   const float et = __builtin_amdgcn_exp2f((zt - most) * L2E), all = s + et;
-  if (threadIdx.x == 0) a.loss[row] = zt == most ? log1pf(s) : logf(all) + (most - zt);
+  if (threadIdx.x == 0) put_loss(zt == most ? log1pf(s) : logf(all) + (most - zt));
   if (!a.grad) return;
-  const float w = a.row_weight ? a.row_weight[row] : a.weight[0], q = w / all;
-  for (int i = threadIdx.x; i < n4; i += 1024) {
-    const float4 v = z4[i];
+  const float w = a.row_weight ? a.row_weight[row] : a.dz ? 1.f : a.weight[0], q = w / all;
+  for (int i = threadIdx.x; i < out4; i += TH) {
+    const float4 v = i < n4 ? z4[i] : make_float4(0.f, 0.f, 0.f, 0.f);
     float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int c = 4 * i + e;
       x[e] = c >= a.vocab ? 0.f : c == t ? -s * q : __builtin_amdgcn_exp2f((x[e] - most) * L2E) * q;
     }
-    z4[i] = make_float4(x[0], x[1], x[2], x[3]);
+    put(i, x);
   }
 }
+template <int TH>
+__global__ void __launch_bounds__(TH) xent_rows_kernel(const XentRowsArgs a) {
+  __shared__ float red[16];
+  __shared__ bool last;
+  xent_row<TH>(a, blockIdx.x, red);
+  if (!a.mean_loss) return;
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(a.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == a.all_rows;
+  __syncthreads();
+  if (!last) return;
+  float s = 0.f;
+  for (long long i = threadIdx.x; i < a.all_rows; i += TH) {
+    const float v = __hip_atomic_load(a.all_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s += a.all_weight ? a.all_weight[i] * v : v;
+  }
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) a.mean_loss[0] = a.all_weight ? s : s * a.weight[0];
+}
+// Threads a row: 1024 from 4096 columns on, else 256.
 hipError_t xent_rows_launch(const XentRowsArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(xent_rows_kernel, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+  const dim3 grid((unsigned)a.rows);
+  if (a.vocab >= 4096) hipLaunchKernelGGL(xent_rows_kernel<1024>, grid, dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL(xent_rows_kernel<256>, grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -570,20 +589,42 @@ hipError_t xent_few_launch(const XentFewArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-__global__ void __launch_bounds__(256) xent_mask_rows_kernel(const float* x, long long ldx, float* out,
-                                                             const int64_t* target, int64_t ignore, long long rows,
-                                                             int d) {
-  const long long total = rows * d;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long r = i / d;
-    out[i] = target[r] == ignore ? 0.f : x[r * ldx + (i - r * d)];
+// one wave a row
+template <typename T>
+__global__ void __launch_bounds__(256) xent_copy_kernel(const XentCopyArgs a) {
+  if (a.weight && blockIdx.x == 0) {
+    const float w = count_weight(a.all_targets, a.all_rows, a.ignore, a.mean);
+    if (threadIdx.x == 0) {
+      a.weight[0] = w;
+      a.count[0] = (int)a.rows;
+      a.done[0] = 0;
+    }
+  }
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const bool skip = a.target[row] == a.ignore;
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+  T* m = reinterpret_cast<T*>(a.xm) + row * a.ldm;
+  if constexpr (sizeof(T) == 2) {
+    for (int c = lane * 8; c < a.ldm; c += 512)
+      *reinterpret_cast<uint4*>(m + c) = skip ? make_uint4(0, 0, 0, 0) : ld8_bits(x, c, a.d);
+  } else {
+    for (int c = lane * 4; c < a.d; c += 256) {
+      float v[4] = {};
+      if (c + 4 <= a.d) {
+        if (!skip) __builtin_memcpy(v, x + c, 16);
+        __builtin_memcpy(m + c, v, 16);
+      } else {
+        for (int e = c; e < a.d; ++e) m[e] = skip ? 0.f : x[e];
+      }
+    }
   }
 }
-hipError_t xent_mask_rows_launch(const float* x, long long ldx, float* out, const int64_t* target, int64_t ignore,
-                                 long long rows, int d, hipStream_t st) {
-  const long long want = (rows * d + 255) / 256;
-  hipLaunchKernelGGL(xent_mask_rows_kernel, dim3((unsigned)(want > 8192 ? 8192 : want)), dim3(256), 0, st, x, ldx, out,
-                     target, ignore, rows, d);
+hipError_t xent_copy_launch(const XentCopyArgs& a, int dt, hipStream_t st) {
+  const dim3 grid((unsigned)((a.rows + 3) / 4));
+  if (dt == 1) hipLaunchKernelGGL(xent_copy_kernel<bf16_t>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(xent_copy_kernel<float>, grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -21,7 +21,7 @@ struct XgArgs {
   // products with the vocabulary matrix or the rows: out = alpha[0] acc in bf16 (alpha null: 1), or
   bf16_t* out;
   const float* alpha;
-  const int* order;    // XG_DX with out: row n goes to row order[n]
+  const int* order;    // XG_DX with out: row n goes to row order[n] (null: n)
   float* outf;         // (where set) split s's acc in fp32 at outf + s N ldo: 16-byte aligned, ldo a multiple of 4
   int accumulate;      // outf += acc
   // logits: m counts the vocabulary, n the rows
@@ -44,6 +44,7 @@ enum XgKind : int {
   XG_LOGITS = 0,  // both operands k-contiguous: m vocabulary (W), n rows (x), k = d
   XG_DX = 1,      // A mn-contiguous, B k-contiguous: m = d (W), n rows (dz), k vocabulary
   XG_DW = 2,      // both mn-contiguous: m = d (x), n vocabulary (dz), k rows
+  XG_Z = 3,       // as XG_LOGITS with outf: the logits themselves
 };
 // How a product with out M x N (XG_DX, XG_DW) is cut: 256 or 128 rows of m a tile, and parts of k (1 without can_split)
 struct XgPlan {

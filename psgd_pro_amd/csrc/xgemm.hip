@@ -335,8 +335,12 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     int to_lo = 0, to_hi = 0;  // where rows nw + lane and nw + 64 + lane go
     if constexpr (KIND == XG_DX) {
       static_assert(WTN == 128, "two rows a lane");
-      to_lo = p.order[min(nw + lane, N - 1)];
-      to_hi = p.order[min(nw + 64 + lane, N - 1)];
+      to_lo = nw + lane;
+      to_hi = nw + 64 + lane;
+      if (p.order) {
+        to_lo = p.order[min(to_lo, N - 1)];
+        to_hi = p.order[min(to_hi, N - 1)];
+      }
     }
     uint16_t* const out = KIND == XG_LOGITS ? reinterpret_cast<uint16_t*>(p.q) : p.out;
 #pragma unroll
@@ -483,6 +487,9 @@ hipError_t xgemm_launch(XgArgs& a, int kind, int bm, hipStream_t st) {
   if (kind == XG_LOGITS)
     return a.redo ? launch_x<128, 128, 64, 2, false, false, XG_LOGITS, false, true>(a, st)
                   : launch_x<128, 128, 64, 2, false, false, XG_LOGITS>(a, st);
+  if (kind == XG_Z)
+    return bm == 128 ? launch_x<64, 128, 64, 3, false, false, XG_Z, true>(a, st)
+                     : launch_x<128, 128, 64, 2, false, false, XG_Z, true>(a, st);
   if (kind == XG_DX) {
     if (bm == 128)
       return a.outf ? launch_x<64, 128, 64, 3, true, false, XG_DX, true>(a, st)

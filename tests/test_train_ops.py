@@ -513,12 +513,68 @@ def test_cross_entropy_patterns_of_ignored_rows(dtype, pattern, n, d, v):
     loss = P.linear_cross_entropy(x, w, t, reduction="none")
     dx, = torch.autograd.grad(loss.sum(), x)
     assert torch.equal(loss[~keep], torch.zeros_like(loss[~keep])) and torch.equal(dx[~keep], torch.zeros_like(dx[~keep]))
-    if dtype == torch.bfloat16:  # the same bits as from the others alone
+    kept = int(keep.sum())
+    if dtype == torch.bfloat16 and (n > 512) == (kept > 512):  # the same bits as from the others alone (the same kernels)
         xs = x.detach()[keep].requires_grad_()
         alone = P.linear_cross_entropy(xs, w, t[keep], reduction="none")
-        if int(keep.sum()) > 64:  # (up to 64 rows take a kernel of their own where there are no gradients)
+        if kept > 64:  # (up to 64 rows take a kernel of their own where there are no gradients)
             assert torch.equal(alone, loss[keep])
         assert torch.equal(torch.autograd.grad(alone.sum(), xs)[0], dx[keep])
+
+
+# Up to 512 rows and 2^23 logits have kernels of their own: both sides of each limit, and what the smaller tests look at once
+# more with more rows.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,v", [(511, 40, 700), (512, 96, 257), (513, 96, 257), (512, 24, 16384), (512, 24, 16385), (2, 16, 4194304),
+                                   (3, 16, 4194304), (1500, 33, 4095), (1500, 64, 4096)])
+def test_cross_entropy_sizes_at_the_limits(dtype, n, d, v):
+    if v > 1 << 20 and dtype == torch.float32:
+        v //= 4
+    x, w = rnd((n, d), 61, dtype), rnd((v, d), 62, dtype, 1.5 / math.sqrt(d))
+    run_lce(x, w, targets(n, v, 63, 0.2))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gain", [1e-3, 30.0, 300.0])
+@pytest.mark.parametrize("n", [520, 1030])
+def test_cross_entropy_many_sharp_and_flat_rows(dtype, gain, n):
+    d, v = 64, 1500
+    w = rnd((v, d), 2, dtype, 1.0 / math.sqrt(d))
+    t = targets(n, v, 3)
+    x = rnd((n, d), 1, dtype)
+    x[::3] = (w[t[::3]].float() * 8 / w[t[::3]].float().square().sum(1, keepdim=True)).to(dtype)
+    x[1::3] = -x[1::3]
+    run_lce((x.float() * gain).to(dtype), w, t, reductions=("mean", "none"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_entropy_many_rows_in_other_layouts(dtype):
+    n = 700
+    x, w, t = rnd((n, 200), 1, dtype), rnd((530, 200), 2, dtype, 0.1), targets(n, 530, 3, 0.3)
+
+    def padded(q, pad):
+        b = torch.full((q.shape[0], q.shape[1] + pad), math.nan, device=DEV, dtype=q.dtype)
+        b[:, :q.shape[1]] = q
+        return b[:, :q.shape[1]]
+
+    for xs, ws in ((padded(x, 8), padded(w, 24)), (padded(x, 3), padded(w, 1)), (x.t().contiguous().t(), w.t().contiguous().t())):
+        run_lce(xs, ws, t, reductions=("mean",))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [40, 700])
+def test_cross_entropy_foreign_targets_stay_in_their_rows(dtype, n):
+    """A target outside the vocabulary makes its own loss and dx NaN, no other row's, and dw."""
+    x, w = rnd((n, 32), 1, dtype).requires_grad_(), rnd((50, 32), 2, dtype).requires_grad_()
+    t = targets(n, 50, 3)
+    t[3], t[n // 2], t[5] = 50, -1, -100
+    foreign = torch.zeros(n, dtype=torch.bool, device=DEV)
+    foreign[3] = foreign[n // 2] = True
+    loss = P.linear_cross_entropy(x, w, t, reduction="none")
+    assert torch.equal(torch.isnan(loss), foreign)
+    dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+    assert torch.equal(torch.isnan(dx).all(1), foreign) and torch.equal(torch.isnan(dx).any(1), foreign)
+    assert torch.isnan(dw).all() and not dx[5].any()
 
 
 def test_cross_entropy_slabs_without_a_row_that_counts():
