@@ -1,5 +1,7 @@
 // Dropout, and the residual sum between two blocks of a transformer with its norms, gate, scale and dropout. Both are
 // bound by memory: every tensor passes once, a row stays in registers between its statistics and its use, sums are fp32.
+#include <algorithm>
+
 #include "block.h"
 #include "philox.h"
 
@@ -559,8 +561,8 @@ hipError_t residual_norm_launch(const ResArgs& a, hipStream_t st) {
 // A workgroup takes `chunk` consecutive rows and keeps its column sums in registers; they go to one row of `part` each
 // and a second kernel adds those in a fixed order. A gate row whose rows all lie in one workgroup is written at once.
 // Bound by memory where rows are long enough (16384 rows of 4096 bf16, two rms norms: 180 us, 4.5 TB/s; 33280 rows of 512
-// fp32: 92 us, 4.4 TB/s), by the chain of a row's sums on short ragged ones (8481 rows of 770 bf16, everything on: 59 us,
-// 1.5 TB/s): a row's two means are each a wave's sum, a barrier and the waves' sums. The next row's loads are under way
+// fp32: 86 us, 4.7 TB/s), by the chain of a row's sums on short ragged ones (8481 rows of 770 bf16, everything on: 51 us,
+// 1.8 TB/s): a row's two means are each a wave's sum, a barrier and the waves' sums. The next row's loads are under way
 // meanwhile (without them, and with one workgroup a CU: 410 us in place of 180).
 namespace {
 
@@ -588,12 +590,11 @@ __device__ __forceinline__ void put_sum(float (&s)[VE], float* dst, const Span<R
 
 // HAS: what the call may have (kPost: a norm after the block, kGate, kBias: a layer norm's biases); what it cannot have
 // holds no registers. SUMS: column sums in registers (1: of the norm before, 2: of the norm after, 4: of the gate).
-// Waves a SIMD, by what their registers hold without scratch memory: two workgroups of 512 threads want 128 registers,
-// three of 256 threads 168.
+// Waves a SIMD, by what their registers hold without scratch memory (512, 168 and 128 registers a lane for 1 to 2, 3 and 4
+// of them); the rows are cut for so many workgroups at once.
 constexpr int res_waves(int tpr, int has, int esize) {
-  if (tpr == 1024) return 4;
-  if (tpr == 512) return has == 0 || has == kBias || (has == kPost && esize == 2) ? 4 : 2;
-  return has == 7 || (has == (kPost | kGate) && esize == 4) ? 2 : 3;
+  if (tpr == 1024 || has == 0 || has == kBias || (tpr == 512 && has == kPost && esize == 2)) return 4;
+  return tpr == 512 || has == 7 || (has == (kPost | kGate) && esize == 4) ? 2 : 3;
 }
 template <typename T, int TPR, int HAS, int SUMS, bool RAGGED>
 __global__ void __launch_bounds__(res_threads(TPR), res_waves(TPR, HAS, sizeof(T)))
@@ -926,15 +927,22 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums s) {
 }  // namespace
 
 void residual_norm_split(ResArgs& a, bool gate_sums) {
-  // as many workgroups as are on the GPU's 256 CUs at once (1024 threads each)
+  // as many workgroups as are on the GPU's 256 CUs at once: one more would begin when all the others
+  // end (1024 of them where 512 or 768 fit: 16384 rows of 1024 bf16 58 us in place of 47, 33280 of 512 fp32 102 / 87)
   const long long at_once = a.d <= 512 ? 4 : a.d <= 1024 ? 2 : 1;
-  const long long target = a.d <= 2048 ? 1024 : a.d <= 4096 ? 512 : res_backward_wide(a) ? 1024 : 256;
+  const int waves = res_waves(a.d <= 2048 ? 256 : a.d <= 4096 ? 512 : 1024, res_has(a), a.dt == 1 ? 2 : 4);
+  const long long target = res_backward_wide(a) ? 1024 : a.d <= 2048 ? 256 * waves : a.d <= 4096 ? 128 * waves : 256;
   a.chunk = a.rows > target ? (a.rows + target - 1) / target : 1;
   a.chunk = (a.chunk + at_once - 1) / at_once * at_once;
   a.per_gate = 1;
   if (gate_sums && a.gate_every > 1) {
     if (a.chunk >= a.gate_every) a.chunk = (a.chunk + a.gate_every - 1) / a.gate_every * a.gate_every;
-    else a.per_gate = (a.gate_every + a.chunk - 1) / a.chunk;
+    else {
+      const long long parts = std::max(1ll, target / (a.rows / a.gate_every));  // of each gate's rows
+      a.chunk = (a.gate_every + parts - 1) / parts;
+      a.chunk = std::min((a.chunk + at_once - 1) / at_once * at_once, a.gate_every);
+      a.per_gate = (a.gate_every + a.chunk - 1) / a.chunk;
+    }
   }
   a.parts = a.per_gate > 1 ? a.rows / a.gate_every * a.per_gate : (a.rows + a.chunk - 1) / a.chunk;
 }
