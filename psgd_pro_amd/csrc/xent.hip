@@ -5,16 +5,24 @@
 
 namespace psgdk {
 
+// a thread's share of the rows that count, eight loads at a time
+__device__ __forceinline__ int count_rows(const int64_t* target, long long rows, int64_t ignore) {
+  int n = 0;
+  for (long long r0 = threadIdx.x; r0 < rows; r0 += 8 * (long long)blockDim.x) {
+    int64_t t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = target[min(r0 + k * (long long)blockDim.x, rows - 1)];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) n += r0 + k * (long long)blockDim.x < rows && t[k] != ignore;
+  }
+  return n;
+}
 // of one workgroup: 1 / the number of rows that count, or 1
 __device__ __forceinline__ float count_weight(const int64_t* target, long long rows, int64_t ignore, int mean) {
   __shared__ int total;
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
-  int n = 0;
-  if (mean) {
-#pragma unroll 8
-    for (long long i = threadIdx.x; i < rows; i += blockDim.x) n += target[i] != ignore;
-  }
+  const int n = mean ? count_rows(target, rows, ignore) : 0;
   if (n) atomicAdd(&total, n);  // whole numbers: any order gives the same sum
   __syncthreads();
   return mean ? 1.f / (float)max(total, 1) : 1.f;
@@ -27,9 +35,7 @@ __global__ void __launch_bounds__(1024) xent_order_kernel(const int64_t* target,
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
-  int n = 0;
-#pragma unroll 8
-  for (long long i = threadIdx.x; i < rows; i += 1024) n += target[i] != ignore;
+  int n = count_rows(target, rows, ignore);
   if (n) atomicAdd(&total, n);  // whole numbers: any order gives the same sum
   __syncthreads();
   n = total;
@@ -41,11 +47,13 @@ __global__ void __launch_bounds__(1024) xent_order_kernel(const int64_t* target,
   for (long long r0 = 0; r0 < rows; r0 += 4096) {
     const int turn = (int)(r0 / 4096 & 1);
     unsigned long long has[4];
+    int64_t t[4];
     int mine = 0;
 #pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = target[min(r0 + wave * 256 + e * 64 + lane, rows - 1)];
+#pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const long long r = r0 + wave * 256 + e * 64 + lane;
-      has[e] = __ballot(r < rows && target[r] != ignore);
+      has[e] = __ballot(r0 + wave * 256 + e * 64 + lane < rows && t[e] != ignore);
       mine += __popcll(has[e]);
     }
     if (lane == 0) part[turn][wave] = mine;
@@ -611,9 +619,11 @@ __global__ void __launch_bounds__(256) xent_copy_kernel(const XentCopyArgs a) {
       *reinterpret_cast<uint4*>(m + c) = skip ? make_uint4(0, 0, 0, 0) : ld8_bits(x, c, a.d);
   } else {
     for (int c = lane * 4; c < a.d; c += 256) {
-      float v[4] = {};
       if (c + 4 <= a.d) {
-        if (!skip) __builtin_memcpy(v, x + c, 16);
+        float v[4];
+        __builtin_memcpy(v, x + c, 16);
+#pragma unroll
+        for (float& e : v) e = skip ? 0.f : e;
         __builtin_memcpy(m + c, v, 16);
       } else {
         for (int e = c; e < a.d; ++e) m[e] = skip ? 0.f : x[e];
