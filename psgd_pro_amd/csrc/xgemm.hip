@@ -72,7 +72,7 @@ __device__ __forceinline__ void load_wait() {
 // way before a tile's results leave. No load that a register waits for may come between: its wait would be for all of them,
 // and for the last tile's stores. (REDO, the listed blocks alone, is an instance of its own for its list's loads.)
 // Bound by the matrix cores at the clock that their power leaves (1.7-1.8 GHz): 4096 x 4096 x 131072 (4.4 TFLOP a product),
-// logits 3.56 ms (1240 TFLOP/s), dx 3.17 (1390), dw 3.32 (1325), the MFMA pipe busy 64, 75 and 72% of the cycles; the
+// logits 3.70 ms (1190 TFLOP/s), dx 3.26 (1350), dw 3.35 (1310), the MFMA pipe busy 64, 75 and 72% of the cycles; the
 // logits' exponentials and stores are the rest of theirs. Why one workgroup of four 128 x 128 waves a CU: two of 128 x 256
 // (logits / dx / dw) 4.60 / 4.09 / 3.53 ms, eight waves of 128 x 64 4.02 / 3.32 / 3.44, k tiles of 32 in four stages
 // 4.06 / 3.32 / 3.61.
