@@ -241,7 +241,6 @@ int lce_rows(const Lce& p, int64_t r0, int64_t n, float* z, int64_t ldz, bf16_t*
 
 // float32: the logits of a slab of rows by the converting engine, a pass over them, and its products with W and x.
 int lce_f32(const Lce& p) {
-  const bool grad = p.dx || p.dw;
   const int64_t ldz = (p.vocab + 3) / 4 * 4, slab = std::min(p.rows, std::max<int64_t>(1, kLogitBytes / 4 / ldz));
   Ws m(p.ws);
   float* const weight = m.take<float>(1);
