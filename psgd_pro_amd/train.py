@@ -17,14 +17,18 @@ __all__ = ["dropout", "linear_cross_entropy", "residual_norm"]
 _NORMS = {None: L.NORM_NONE, "rms": L.NORM_RMS, "layer": L.NORM_LAYER}
 
 
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
 def _check(t, name, like=None):
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPES and (like is None or t.get_device() == like.get_device()):
+        return
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name}: psgd_pro_amd ops take CUDA (HIP) tensors; got " +
                            (f"a tensor on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
-    if t.dtype not in (torch.float32, torch.bfloat16):
+    if t.dtype not in _DTYPES:
         raise RuntimeError(f"{name}: float32 or bfloat16 expected, got {t.dtype}")
-    if like is not None and t.device != like.device:
-        raise RuntimeError(f"{name}: on {t.device}, the input is on {like.device}")
+    raise RuntimeError(f"{name}: on {t.device}, the input is on {like.device}")
 
 
 def _rows(t):
@@ -41,8 +45,8 @@ def _rows(t):
 
 def _run(t, fn, *args):
     """fn(*args, stream) on t's device and its current stream."""
-    i = t.device.index
-    if i == torch.cuda.current_device():
+    i = t.get_device()
+    if i == torch._C._cuda_getDevice():
         L.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
     else:
         with torch.cuda.device(i):
@@ -83,7 +87,7 @@ def _check_p(p):
 
 
 def _dropout_call(x, p, seed, stream):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     n, d = x.numel(), x.shape[-1]
     if n:
         r, ld = _rows(x)
@@ -156,8 +160,8 @@ def _res_block(x, f, gate, pw, pb, qw, qb, opt):
 
 def _res_forward(x, f, gate, pw, pb, qw, qb, opt, stats):
     a, keep = _res_block(x, f, gate, pw, pb, qw, qb, opt)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if f is not None else None
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if opt[0] else None
+    y = x.new_empty(x.shape) if f is not None else None
+    h = x.new_empty(x.shape) if opt[0] else None
     st = torch.empty(a.rows, 4, device=x.device) if stats else None
     a.y, a.ldy, a.h, a.ldh, a.stats = _ptr(y), a.d, _ptr(h), a.d, _ptr(st)
     if x.numel() and (y is not None or h is not None):
@@ -195,7 +199,7 @@ class _ResidualNorm(torch.autograd.Function):
                                           ("dpost_w", qw), ("dpost_b", qb))):
             if like is None or not need[k]:
                 continue
-            outs[k] = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+            outs[k] = like.new_empty(like.shape)
             setattr(g, name, outs[k].data_ptr())
             if k < 3:
                 setattr(g, "ld" + name, like.shape[-1])
@@ -287,8 +291,8 @@ def _lce_call(x, w, target, ignore, row_weight, reduction, want_x, want_w):
     n, d = t.numel(), x.shape[-1]
     loss = torch.empty(n, device=x.device)
     total = None if reduction == "none" else torch.empty((), device=x.device)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if want_w else None
+    dx = x.new_empty(x.shape) if want_x else None
+    dw = w.new_empty(w.shape) if want_w else None
     if not n:
         return loss, None if total is None else total.zero_(), dx, None if dw is None else dw.zero_()
     _run_ws(x, L.lib().psgdk_linear_cross_entropy, n, d, w.shape[0], L.dtype_code(x.dtype), xr.data_ptr(), ldx, wr.data_ptr(),
