@@ -417,8 +417,8 @@ int lce_bf16(const Lce& p) {
   if (slab >= p.rows) slab = p.rows;
   const int64_t blocks = (slab + kXgRows - 1) / kXgRows, parts = 2 * ((p.vocab + 255) / 256);
   const bool copy_w = needs_copy(p);
-  const bool sum_w = p.dw && slab < p.rows;
-  const XgPlan dx_plan = xgemm_plan(p.d, slab, ldq, true), dw_plan = xgemm_plan(p.d, p.vocab, slab, false);
+  const XgPlan dx_plan = xgemm_plan(p.d, slab, ldq, true), dw_plan = xgemm_plan(p.d, p.vocab, slab, true);
+  const bool sum_w = p.dw && (slab < p.rows || dw_plan.splits > 1);
   const int splits = p.dx ? dx_plan.splits : 1;
   Ws m(p.ws);
   float* const weight = m.take<float>(1);
@@ -436,7 +436,7 @@ int lce_bf16(const Lce& p) {
   bf16_t* const wp = m.take<bf16_t>(copy_w ? p.vocab * ld : 0);
   a.q = m.take<int16_t>(grad ? slab * ldq : 0);
   float* const dxp = m.take<float>(splits > 1 ? splits * slab * ld : 0);
-  float* const dwf = m.take<float>(sum_w ? p.vocab * ld : 0);
+  float* const dwf = m.take<float>(sum_w ? dw_plan.splits * p.vocab * ld : 0);
   bool done;
   PSGDK_TRY(lce_ws(p, m, done));
   if (done) return PSGDK_OK;
@@ -541,7 +541,8 @@ int lce_bf16(const Lce& p) {
       x.lda = ld;
       x.B = reinterpret_cast<const bf16_t*>(a.q);
       x.ldb = ldq;
-      x.splits = 1;
+      x.splits = dw_plan.splits;  // (of few rows that count, the last ones have none and add zeros)
+      x.kchunk = dw_plan.kchunk;
       x.out = static_cast<bf16_t*>(p.dw);
       x.ldo = sum_w ? ld : p.lddw;
       x.alpha = alpha;
@@ -551,7 +552,7 @@ int lce_bf16(const Lce& p) {
     }
   }
   if (sum_w)
-    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, 1, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab, (int)p.d,
+    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, dw_plan.splits, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab, (int)p.d,
                                   nullptr, nullptr, 0, p.st), "dw sums"));
   return lce_mean(p, weight);
 }

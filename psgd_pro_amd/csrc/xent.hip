@@ -91,7 +91,17 @@ __global__ void __launch_bounds__(1024) xent_mean_kernel(const float* loss, cons
   __shared__ float red[16];
   const float w = row_weight ? 1.f : weight ? weight[0] : count_weight(target, rows, ignore, mean);
   float s = 0.f;
-  for (long long i = threadIdx.x; i < rows; i += 1024) s += row_weight ? row_weight[i] * loss[i] : loss[i];
+  for (long long r0 = threadIdx.x; r0 < rows; r0 += 8 * 1024) {  // eight loads at a time
+    float v[8], g[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const long long i = min(r0 + k * 1024, rows - 1);
+      v[k] = loss[i];
+      g[k] = row_weight ? row_weight[i] : 1.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += r0 + k * 1024 < rows ? g[k] * v[k] : 0.f;
+  }
   s = block_sum(s, red);
   if (threadIdx.x == 0) out[0] = s * w;
 }

@@ -17,7 +17,7 @@ struct XgArgs {
   // the rows that are there: count[0] - first of them (count in device memory), at most N (XG_DW: K)
   const int* count;
   int first;
-  int splits, kchunk;  // split s covers k in [s kchunk, (s + 1) kchunk), none of them empty; splits > 1 need outf
+  int splits, kchunk;  // split s covers k in [s kchunk, (s + 1) kchunk), none empty but by count; splits > 1 need outf
   // products with the vocabulary matrix or the rows: out = alpha[0] acc in bf16 (alpha null: 1), or
   bf16_t* out;
   const float* alpha;

@@ -577,6 +577,17 @@ def test_cross_entropy_foreign_targets_stay_in_their_rows(dtype, n):
     assert torch.isnan(dw).all() and not dx[5].any()
 
 
+@pytest.mark.parametrize("kept", [1, 700, 6000])
+@pytest.mark.parametrize("d,v", [(40, 200), (136, 1000)])
+def test_cross_entropy_parts_of_many_rows(kept, d, v):
+    """dw of a small vocabulary adds up parts of the rows; where few of them count the last parts are empty."""
+    n = 6000
+    x, w = rnd((n, d), 71, torch.bfloat16), rnd((v, d), 72, torch.bfloat16, 1.0 / math.sqrt(d))
+    t = targets(n, v, 73)
+    t[kept:] = -100
+    run_lce(x, w, t)
+
+
 def test_cross_entropy_slabs_without_a_row_that_counts():
     """More rows than the logits' memory holds at once: what counts fills the first slabs only."""
     n, d, v = 12000, 8, 50021
