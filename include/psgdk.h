@@ -376,7 +376,7 @@ int psgdk_residual_norm_backward(const psgdk_residual_norm_t* a, const psgdk_res
  * sum_i row_weight[i] loss[i] under the same rule. An ignored row's x reaches no result, its dx is 0, and the bf16
  * products leave it out. rows up to 2^30, d up to 2^20, vocab up to 2^22. The logits are never in memory in fp32 with bf16 inputs; of a slab of rows (up to 1 GiB) they
  * are there as 16-bit codes while the gradients are made (fp32 inputs: 1 GiB of fp32 logits). The workspace's size
- * depends on w's alignment: the size query is made with the same w. */
+ * depends on the alignment of w, dx and dw: the size query is made with the same pointers. */
 int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype, const void* x, int64_t ldx,
                                const void* w, int64_t ldw, const int64_t* target, int64_t ignore,
                                const float* row_weight, int mean, float* loss, float* mean_loss, void* dx,

@@ -239,6 +239,38 @@ int lce_rows(const Lce& p, int64_t r0, int64_t n, float* z, int64_t ldz, bf16_t*
   return hip_check(xent_rows_launch(a, p.st), "cross entropy rows");
 }
 
+// An m x d product with a long k has few of the 128 x 256 tiles that fill the CUs: parts of k as problems of one launch then
+// (0: one part). 2048 x 512 x 10007: dx 216 us in one part, 115 + 16 in parts; 65536 x 256 x 1024: dw 1160 in one part, 321 + 7 in parts.
+int64_t f32_parts(int64_t m, int64_t d, int64_t k, const void* out, int64_t ldo) {
+  const int64_t tiles = ((m + 127) / 128) * ((d + 255) / 256);
+  if (tiles >= 128 || ldo != d || d % 4 || (reinterpret_cast<uintptr_t>(out) & 15)) return 0;
+  const int64_t parts = std::min<int64_t>({PSGDK_MAXB, 256 / tiles, k / 512});
+  return parts > 1 ? parts : 0;
+}
+// out (m x d) = z w (z: m x k) or, with ta, z^T w (z: k x m), w: k x d; sums: room for parts + 1 of them
+int f32_split_k(const Lce& p, int ta, int64_t m, int64_t k, int parts, const float* z, int64_t ldz, const float* w, int64_t ldw,
+                float* sums, float* out) {
+  const int64_t part = k / parts / 4 * 4, done = parts * part, step = ta ? ldz : 1;
+  const psgdk_stream_t st = (psgdk_stream_t)p.st;
+  const void *za[PSGDK_MAXB], *wa[PSGDK_MAXB];
+  float* oa[PSGDK_MAXB];
+  for (int64_t i = 0; i < parts; ++i) {
+    za[i] = z + i * part * step;
+    wa[i] = w + i * part * ldw;
+    oa[i] = sums + i * m * p.d;
+  }
+  PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, ta, 0, m, p.d, part, 1.f, PSGDK_F32, PSGDK_F32, parts, za, ldz, wa, ldw, 0.f, oa, p.d,
+                       st));
+  if (done < k) {
+    za[0] = z + done * step;
+    wa[0] = w + done * ldw;
+    oa[0] = sums + parts * m * p.d;
+    PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, ta, 0, m, p.d, k - done, 1.f, PSGDK_F32, PSGDK_F32, 1, za, ldz, wa, ldw, 0.f, oa,
+                         p.d, st));
+  }
+  return hip_check(sum_parts_launch(sums, parts + (done < k ? 1 : 0), m * p.d / 4, out, p.st), "sums of parts");
+}
+
 // float32: the logits of a slab of rows by the converting engine, a pass over them, and its products with W and x.
 int lce_f32(const Lce& p) {
   const int64_t ldz = (p.vocab + 3) / 4 * 4, slab = std::min(p.rows, std::max<int64_t>(1, kLogitBytes / 4 / ldz));
@@ -248,13 +280,10 @@ int lce_f32(const Lce& p) {
   int* const ended = m.take<int>(1);
   float* const z = m.take<float>(slab * ldz);
   float* const xm = m.take<float>(slab * p.d);
-  // dx is short and narrow with the vocabulary for k: parts of k as problems of one launch, where its 128 x 256 tiles
-  // alone would leave CUs idle (2048 x 512 x 10007: 216 us in one part)
-  const int64_t tiles = ((slab + 127) / 128) * ((p.d + 255) / 256);
-  const int64_t parts = p.dx && tiles < 128 && p.lddx == p.d && p.d % 4 == 0 && (reinterpret_cast<uintptr_t>(p.dx) & 15) == 0
-                            ? std::min<int64_t>({PSGDK_MAXB, 256 / tiles, p.vocab / 512}) : 0;
-  const int64_t part = parts > 1 ? p.vocab / parts / 4 * 4 : 0;
-  float* const dxp = m.take<float>(parts > 1 ? (parts + 1) * slab * p.d : 0);
+  const int64_t dx_parts = p.dx ? f32_parts(slab, p.d, p.vocab, p.dx, p.lddx) : 0;
+  const int64_t dw_parts = p.dw && slab == p.rows ? f32_parts(p.vocab, p.d, p.rows, p.dw, p.lddw) : 0;
+  float* const sums = m.take<float>(std::max(dx_parts ? (dx_parts + 1) * slab * p.d : 0,
+                                             dw_parts ? (dw_parts + 1) * p.vocab * p.d : 0));
   bool done;
   PSGDK_TRY(lce_ws(p, m, done));
   if (done) return PSGDK_OK;
@@ -270,34 +299,19 @@ int lce_f32(const Lce& p) {
     PSGDK_TRY(lce_rows(p, r0, n, z, ldz, nullptr, 0, weight, ended));
     if (p.dx) {
       float* out = static_cast<float*>(p.dx) + r0 * p.lddx;
-      if (parts > 1) {
-        const void *za[PSGDK_MAXB], *wa[PSGDK_MAXB];
-        float* oa[PSGDK_MAXB];
-        for (int64_t i = 0; i < parts; ++i) {
-          za[i] = z + i * part;
-          wa[i] = static_cast<const float*>(p.w) + i * part * p.ldw;
-          oa[i] = dxp + i * n * p.d;
-        }
-        const int64_t done_k = parts * part, rest = p.vocab - done_k;
-        PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, part, 1.f, PSGDK_F32, PSGDK_F32, (int)parts, za, ldz, wa, p.ldw,
-                             0.f, oa, p.d, st));
-        if (rest) {
-          za[0] = z + done_k;
-          wa[0] = static_cast<const float*>(p.w) + done_k * p.ldw;
-          oa[0] = dxp + parts * n * p.d;
-          PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, rest, 1.f, PSGDK_F32, PSGDK_F32, 1, za, ldz, wa, p.ldw, 0.f, oa,
-                               p.d, st));
-        }
-        PSGDK_TRY(hip_check(sum_parts_launch(dxp, (int)(parts + (rest ? 1 : 0)), n * p.d / 4, out, p.st), "dx sums"));
-      } else {
+      if (dx_parts)
+        PSGDK_TRY(f32_split_k(p, 0, n, p.vocab, (int)dx_parts, z, ldz, static_cast<const float*>(p.w), p.ldw, sums, out));
+      else
         PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 0, 0, n, p.d, p.vocab, 1.f, PSGDK_F32, PSGDK_F32, 1, &zc, ldz, &p.w, p.ldw,
                              0.f, &out, p.lddx, st));
-      }
     }
     if (p.dw) {
       float* out = static_cast<float*>(p.dw);
-      PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 1, 0, p.vocab, p.d, n, 1.f, PSGDK_F32, PSGDK_F32, 1, &zc, ldz, &xc, p.d,
-                           r0 ? 1.f : 0.f, &out, p.lddw, st));
+      if (dw_parts)
+        PSGDK_TRY(f32_split_k(p, 1, p.vocab, n, (int)dw_parts, z, ldz, xm, p.d, sums, out));
+      else
+        PSGDK_TRY(psgdk_gemm(PSGDK_PREC_F32, 1, 0, p.vocab, p.d, n, 1.f, PSGDK_F32, PSGDK_F32, 1, &zc, ldz, &xc, p.d,
+                             r0 ? 1.f : 0.f, &out, p.lddw, st));
     }
   }
   return p.rows <= kSmallRows ? PSGDK_OK : lce_mean(p, weight);
@@ -552,8 +566,8 @@ int lce_bf16(const Lce& p) {
     }
   }
   if (sum_w)
-    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, dw_plan.splits, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab, (int)p.d,
-                                  nullptr, nullptr, 0, p.st), "dw sums"));
+    PSGDK_TRY(hip_check(to_bf16_rows_launch(dwf, dw_plan.splits, ld, alpha, static_cast<bf16_t*>(p.dw), p.lddw, p.vocab,
+                                            (int)p.d, nullptr, nullptr, 0, p.st), "dw sums"));
   return lce_mean(p, weight);
 }
 

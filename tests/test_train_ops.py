@@ -588,6 +588,12 @@ def test_cross_entropy_parts_of_many_rows(kept, d, v):
     run_lce(x, w, t)
 
 
+@pytest.mark.parametrize("n,d,v", [(6001, 40, 200), (3000, 136, 1000), (1025, 256, 130), (2050, 33, 260)])
+def test_cross_entropy_parts_of_many_rows_in_float32(n, d, v):
+    x, w = rnd((n, d), 81), rnd((v, d), 82, std=1.0 / math.sqrt(d))
+    run_lce(x, w, targets(n, v, 83, 0.1))
+
+
 def test_cross_entropy_slabs_without_a_row_that_counts():
     """More rows than the logits' memory holds at once: what counts fills the first slabs only."""
     n, d, v = 12000, 8, 50021
