@@ -162,7 +162,7 @@ def _res_forward(x, f, gate, pw, pb, qw, qb, opt, stats):
     a, keep = _res_block(x, f, gate, pw, pb, qw, qb, opt)
     y = x.new_empty(x.shape) if f is not None else None
     h = x.new_empty(x.shape) if opt[0] else None
-    st = torch.empty(a.rows, 4, device=x.device) if stats else None
+    st = torch.empty(a.rows, 4, device=x.device, dtype=torch.float32) if stats else None
     a.y, a.ldy, a.h, a.ldh, a.stats = _ptr(y), a.d, _ptr(h), a.d, _ptr(st)
     if x.numel() and (y is not None or h is not None):
         _run(x, L.lib().psgdk_residual_norm, C.byref(a))
@@ -289,8 +289,8 @@ def _lce_call(x, w, target, ignore, row_weight, reduction, want_x, want_w):
     """(losses, their mean or sum (reduction "none": None), dx, dw)"""
     (xr, ldx), (wr, ldw), t = _rows(x), _rows(w), target.contiguous()
     n, d = t.numel(), x.shape[-1]
-    loss = torch.empty(n, device=x.device)
-    total = None if reduction == "none" else torch.empty((), device=x.device)
+    loss = torch.empty(n, device=x.device, dtype=torch.float32)
+    total = None if reduction == "none" else torch.empty((), device=x.device, dtype=torch.float32)
     dx = x.new_empty(x.shape) if want_x else None
     dw = w.new_empty(w.shape) if want_w else None
     if not n:
