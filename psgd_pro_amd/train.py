@@ -5,11 +5,12 @@
     dropout                dropout from the library's counter-based generator, mask never stored
 
 All take CUDA (HIP) tensors in float32 or bfloat16, run on torch's current stream and differentiate once through
-autograd. No counterparts in the reference, which leaves the model to torch.
+autograd (not in forward mode, which is refused). No counterparts in the reference, which leaves the model to torch.
 """
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from . import _lib as L
 
 __all__ = ["dropout", "linear_cross_entropy", "residual_norm"]
@@ -68,6 +69,10 @@ def _once():
 
 
 def _wants_grad(*ts):
+    # (the plain call would leave a tangent behind without a word, and grad mode says nothing about forward mode)
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError("psgd_pro_amd ops have no forward-mode derivatives")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 

@@ -2,6 +2,7 @@
 made (outputs hold nothing)."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import psgd_pro_amd as P
 from psgd_pro_amd import train as T
@@ -42,3 +43,36 @@ def test_row_statistics_are_float32_under_any_default_dtype(calls, default_dtype
     assert y.dtype == h.dtype == torch.float32 and len(calls) == 1
     stats = y.grad_fn.saved_tensors[-1]
     assert stats.shape == (6, 4) and stats.dtype == torch.float32
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_is_refused(calls, grad, no_grad):
+    """A tangent would be lost without a word. It is refused whichever input carries it, also where no input requires grad,
+    and the same call without tangents goes through inside a dual level."""
+    x, w = torch.ones(4, 8), torch.ones(5, 8)
+    v, t = torch.ones(8), torch.zeros(4, dtype=torch.int64)
+    ops = {
+        "dropout": (lambda x: P.dropout(x, 0.5, seed=1), (x,)),
+        "residual_norm": (lambda x, f, pw, pb, qw, qb, g: P.residual_norm(
+            x, f, pre="layer", post="layer", pre_weight=pw, pre_bias=pb, post_weight=qw, post_bias=qb, gate=g),
+            (x, x.clone(), v, v.clone(), v.clone(), v.clone(), v.clone())),
+        "linear_cross_entropy": (lambda x, w: P.linear_cross_entropy(x, w, t), (x, w)),
+    }
+    with fwAD.dual_level(), torch.set_grad_enabled(not no_grad):
+        for name, (op, args) in ops.items():
+            args = [a.clone().requires_grad_(grad) for a in args]
+            for k, a in enumerate(args):
+                dual = fwAD.make_dual(a, torch.ones_like(a))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    op(*args[:k], dual, *args[k + 1:])
+            assert not calls, name
+            op(*args)
+            assert len(calls) == 1, name
+            calls.clear()
+
+
+def test_forward_mode_transform_is_refused(calls):
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: P.dropout(x, 0.5, seed=1), (torch.ones(4, 8),), (torch.ones(4, 8),))
+    assert not calls
