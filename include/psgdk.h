@@ -372,7 +372,8 @@ int psgdk_residual_norm_backward(const psgdk_residual_norm_t* a, const psgdk_res
  *   loss[i] = log sum_v exp(x_i . w_v) - x_i . w_t,  t = target[i];  0 where target[i] == ignore
  * and, where dx or dw is non-NULL, that gradient of sum_i row_weight[i] loss[i], in the dtype of x and w; row_weight
  * NULL: 1 for every row (mean 0) or 1 / (number of rows not ignored) (mean 1). A target outside 0 .. vocab - 1 that is
- * not `ignore` gives a NaN loss (and NaN gradients of its row). mean_loss (optional, one float) receives
+ * not `ignore` gives a NaN loss (and NaN gradients of its row), and so does a logit of +inf or NaN; a target's logit of
+ * -inf beside a finite one gives a loss of +inf. mean_loss (optional, one float) receives
  * sum_i row_weight[i] loss[i] under the same rule. An ignored row's x reaches no result, its dx is 0, and the bf16
  * products leave it out. rows up to 2^30, d up to 2^20, vocab up to 2^22. The logits are never in memory in fp32 with bf16 inputs; of a slab of rows (up to 1 GiB) they
  * are there as 16-bit codes while the gradients are made (fp32 inputs: 1 GiB of fp32 logits). The workspace's size

@@ -38,7 +38,7 @@ hipError_t xent_rows_launch(const XentRowsArgs& a, hipStream_t st);
 
 // The bf16 path's rows. Reference of row i: r = z_t, the logit of its target, so that the target's exponential is 1 and
 // S = sum of the others' gives loss = log(1 + S), softmax_t - 1 = -S / (1 + S). Rows with S over kSumLimit (their loss is
-// over 31) take their largest logit as r instead, and the target's exponential e_t = e^(z_t - r).
+// over 31, or z_t is -inf) take their largest logit as r instead, and the target's exponential e_t = e^(z_t - r).
 constexpr float kSumLimit = 2.9e13f;  // e^31: every e^(z - r) below it, z - r within the coded logits' range
 struct XentBf16Args {
   // The rows of a slab are places first .. first + rows - 1 of the order: those before count[0] are there and are numbered

@@ -163,7 +163,8 @@ __device__ __forceinline__ void xent_row(const XentRowsArgs& a, long long row, f
   const float most = fmaxf(block_max(m, red), zt);
   s = block_sum(m > -INFINITY ? s * __builtin_amdgcn_exp2f((m - most) * L2E) : s, red);
   const float et = __builtin_amdgcn_exp2f((zt - most) * L2E), all = s + et;
-  if (threadIdx.x == 0) put_loss(zt == most ? log1pf(s) : logf(all) + (most - zt));
+  const float over = most - zt;  // (an infinite logit that is both has no loss: inf - inf)
+  if (threadIdx.x == 0) put_loss(over == 0.f ? log1pf(s) : logf(all) + over);
   if (!a.grad) return;
   const float w = a.row_weight ? a.row_weight[row] : a.dz ? 1.f : a.weight[0], q = w / all;
   for (int i = threadIdx.x; i < out4; i += TH) {
@@ -367,8 +368,10 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const XentBf16Args a, in
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= live_rows(a) || (again && (a.redo[0] == 0 || !(a.sum[row] > kSumLimit)))) return;
-  const float s = join_row(a, row, lane);
+  float s = join_row(a, row, lane);
   if (lane) return;
+  // a target of -inf is no reference: others of -inf made this sum a NaN
+  if (!again && a.zt[row] == -INFINITY) s = INFINITY;
   a.sum[row] = s;
   if (!again && s > kSumLimit) {
     const int blk = (int)(row / kXgRows);
@@ -569,9 +572,8 @@ __global__ void __launch_bounds__(256) xent_few_join_kernel(const XentFewArgs a)
   } else if (t < 0 || t >= a.vocab) {
     loss = NAN;
   } else {
-    const float zt = a.zt[n], m = fmaxf(top, zt), rest = top > -INFINITY ? s * expf(top - m) : s;
-    loss = m == zt ? log1pf(rest) : logf(rest + expf(zt - m)) + (m - zt);
-    if (zt != zt) loss = NAN;
+    const float zt = a.zt[n], m = fmaxf(top, zt), over = m - zt, rest = top > -INFINITY ? s * expf(top - m) : s;
+    loss = over == 0.f ? log1pf(rest) : logf(rest + expf(zt - m)) + over;  // (NaN where over is: inf - inf, or a NaN z_t)
   }
   a.loss[n] = loss;
 }

@@ -1,0 +1,77 @@
+"""The training operators on the GPU where a step goes wrong: infinite logits. References in float64, bounds as in test_train_ops.py."""
+import math
+
+import pytest
+import torch
+
+import psgd_pro_amd as P
+from test_train_ops import DEV, DTYPES, E, U, lce_ref, rnd, targets, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _lib(hip):
+    return hip
+
+
+# -- logits that overflow -----------------------------------------------------------------------------------------------
+
+BIG = 2.0 ** 100  # its square overflows float32
+
+
+def overflowing(n, v, dtype, kind):
+    """Every third row has an infinite logit: (x, w, targets, those rows). Column 0 of w holds BIG or -BIG at one place
+    of the vocabulary and -BIG at another, column 1 -BIG everywhere, and only the rows meant have BIG in x there."""
+    d = 24
+    x, w, t = rnd((n, d), 91, dtype), rnd((v, d), 92, dtype, 0.3), targets(n, v, 93)
+    x[:, :2], w[:, 0], w[:, 1] = 0, 0, -BIG
+    hit = torch.arange(n, device=DEV) % 3 == 1
+    at, other = v // 2, 3
+    t = torch.where(t == at, at + 1, t)
+    t[hit] = at if kind != "another +inf" else at + 1
+    x[hit, 1 if kind == "all -inf" else 0] = BIG
+    w[at, 0] = BIG if "+inf" in kind else -BIG
+    if kind == "target and another -inf":
+        w[other, 0] = -BIG
+    return x, w, t, hit
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v", [(3, 70), (40, 1100), (600, 1100)])
+@pytest.mark.parametrize("kind,loss_is", [("target +inf", math.nan), ("another +inf", math.nan), ("target -inf", math.inf),
+                                          ("target and another -inf", math.inf), ("all -inf", math.nan)])
+def test_cross_entropy_of_infinite_logits(dtype, n, v, kind, loss_is):
+    """inf - inf is NaN and stays in its row, whichever kernels the sizes choose; a target of -inf costs infinitely much."""
+    x, w, t, hit = overflowing(n, v, dtype, kind)
+
+    def check(loss, what):
+        got = loss[hit]
+        assert bool((torch.isnan(got) if math.isnan(loss_is) else got == loss_is).all()), (what, got)
+
+    (ref, err), (rx, rx_err), _ = lce_ref(x[~hit], w, t[~hit], -100, torch.ones(int((~hit).sum()), device=DEV, dtype=torch.float64))
+    plain = P.linear_cross_entropy(x, w, t, reduction="none")
+    check(plain, "loss without gradients")
+    within(plain[~hit], ref, err, "other rows' losses")
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = P.linear_cross_entropy(xs, ws, t, reduction="none")
+    check(loss.detach(), "loss")
+    within(loss.detach()[~hit], ref, err, "other rows' losses with gradients")
+    dx, dw = torch.autograd.grad(loss, (xs, ws), torch.ones_like(loss))
+    within(dx[~hit], rx, rx_err, "other rows' dx")
+    if math.isnan(loss_is):
+        assert torch.isnan(dx[hit]).all() and torch.isnan(dw).all()
+    else:  # softmax - 1 with the target's share 0: z of the others as if it were not there
+        W = w.double()
+        z = (x.double() @ W.t())[hit]
+        gone = z < -1e20
+        assert bool(gone[:, v // 2].all())
+        p = torch.softmax(z.masked_fill(gone, -math.inf), 1)
+        p[:, v // 2] = -1.0
+        zerr = ((24 + 64) * E * (x[hit, 2:].double().abs() @ W[:, 2:].abs().t())).amax(1, keepdim=True)
+        rel = 4 * zerr + 2 * U[dtype] + (2 * v + 192) * E
+        within(dx[hit], p @ W, rel * (p.abs() @ W.abs()) + U[dtype] * (p @ W).abs() + v * 2.0 ** -126 * W.abs().sum(0), "dx")
+        assert torch.isfinite(dw[:, 2:]).all()
+    for red in ("sum", "mean"):
+        total = float(P.linear_cross_entropy(x, w, t, reduction=red))
+        assert math.isnan(total) if math.isnan(loss_is) else total == math.inf
