@@ -900,28 +900,34 @@ __global__ void __launch_bounds__(256) residual_norm_columns_kernel(const ResArg
     if (a.slot[k] >= 0) st_row(a.part + ((long long)a.slot[k] * a.parts + wg) * a.d, c, a.d, s[k]);
 }
 
-// A workgroup adds 64 columns of one output: wave w the rows w, w + 16, ..., then the 16 sums in order.
-__global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums s) {
+// A workgroup adds 64 columns of one output: wave w the rows w, w + 16, ..., then the 16 sums in order. It takes one such
+// strip after the other: a gate for every few rows has millions of them, and a launch holds less than 2^32 threads (one of
+// exactly that many is accepted and runs nothing).
+__global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums s, long long total) {
   __shared__ float red[16][64];
   const int strips = (s.d + 63) / 64;
-  long long i = blockIdx.x / strips;
-  int k = 0;
-  while (i >= s.e[k].groups) i -= s.e[k++].groups;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = (int)(blockIdx.x % strips) * 64 + lane;
-  const float* in = s.e[k].in + i * s.e[k].per * s.d;
-  float v = 0.f;
-  if (c < s.d) {
+  for (long long at = blockIdx.x; at < total; at += gridDim.x) {
+    long long i = at / strips;
+    int k = 0;
+    while (i >= s.e[k].groups) i -= s.e[k++].groups;
+    const int c = (int)(at % strips) * 64 + lane;
+    const float* in = s.e[k].in + i * s.e[k].per * s.d;
+    float v = 0.f;
+    if (c < s.d) {
 #pragma unroll 8
-    for (long long p = w; p < s.e[k].per; p += 16) v += in[p * s.d + c];
+      for (long long p = w; p < s.e[k].per; p += 16) v += in[p * s.d + c];
+    }
+    red[w][lane] = v;
+    __syncthreads();
+    if (w == 0 && c < s.d) {
+      for (int q = 1; q < 16; ++q) v += red[q][lane];
+      const long long o = i * s.e[k].ldo + c;
+      if (s.e[k].dt == 1) reinterpret_cast<bf16_t*>(s.e[k].out)[o] = f32_to_bf16(v);
+      else reinterpret_cast<float*>(s.e[k].out)[o] = v;
+    }
+    __syncthreads();  // red is free again
   }
-  red[w][lane] = v;
-  __syncthreads();
-  if (w || c >= s.d) return;
-  for (int q = 1; q < 16; ++q) v += red[q][lane];
-  const long long o = i * s.e[k].ldo + c;
-  if (s.e[k].dt == 1) reinterpret_cast<bf16_t*>(s.e[k].out)[o] = f32_to_bf16(v);
-  else reinterpret_cast<float*>(s.e[k].out)[o] = v;
 }
 
 }  // namespace
@@ -1018,7 +1024,8 @@ hipError_t column_sums_launch(const ColumnSums& s, hipStream_t st) {
   long long groups = 0;
   for (int k = 0; k < s.n; ++k) groups += s.e[k].groups;
   if (!groups) return hipSuccess;
-  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)(groups * ((s.d + 63) / 64))), dim3(1024), 0, st, s);
+  const long long total = groups * ((s.d + 63) / 64);
+  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)std::min(total, 1ll << 16)), dim3(1024), 0, st, s, total);
   return hipGetLastError();
 }
 

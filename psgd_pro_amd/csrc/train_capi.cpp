@@ -85,7 +85,8 @@ int res_args(const psgdk_residual_norm_t* q, ResArgs& a) {
   if (!q) return fail(PSGDK_EINVAL, "null argument block");
   PSGDK_TRY(check_dt(q->dtype, "dtype"));
   PSGDK_TRY(check_size(q->d, 1, kMaxNormD, "d"));
-  // the launches hold at most 2^32 threads: one for each 8 elements of a row, 1024 for res_wide rows
+  // A launch holds less than 2^32 threads: these are the forward and backward kernels' of a row, one for each 8 elements,
+  // 1024 for res_wide rows. The other launches' grids do not grow with the rows.
   const int64_t threads = res_wide(q->d) ? 1024 : q->d <= 512 ? 64 : q->d <= 1024 ? 128 :
                           q->d <= 2048 ? 256 : q->d <= 4096 ? 512 : 1024;
   PSGDK_TRY(check_size(q->rows, 0, (((int64_t)1 << 32) - 1024) / threads, "rows"));

@@ -1,11 +1,12 @@
-"""The training operators on the GPU where a step goes wrong: infinite logits. References in float64, bounds as in test_train_ops.py."""
+"""The training operators on the GPU where a step goes wrong or is unusually large: infinite logits, and more gates than one
+launch holds workgroups for. References in float64, bounds as in test_train_ops.py."""
 import math
 
 import pytest
 import torch
 
 import psgd_pro_amd as P
-from test_train_ops import DEV, DTYPES, E, U, lce_ref, rnd, targets, within
+from test_train_ops import DEV, DTYPES, E, U, lce_ref, res_ref, rnd, targets, within
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,28 @@ def test_cross_entropy_of_infinite_logits(dtype, n, v, kind, loss_is):
     for red in ("sum", "mean"):
         total = float(P.linear_cross_entropy(x, w, t, reduction=red))
         assert math.isnan(total) if math.isnan(loss_is) else total == math.inf
+
+
+# -- launches of the largest calls --------------------------------------------------------------------------------------
+
+
+def test_residual_norm_of_four_million_gates():
+    """A gate for every two rows, so many that one workgroup for each would pass the 2^32 threads of a launch."""
+    gates, d = 1 << 22, 8
+    x, f, g = rnd((gates, 2, d), 1), rnd((gates, 2, d), 2), rnd((gates, 1, d), 3, std=0.5, mean=0.5)
+    w = rnd(d, 4, std=0.1, mean=1.0)
+    dy, dh = rnd((gates, 2, d), 5), rnd((gates, 2, d), 6)
+    leaves = [q.requires_grad_() for q in (x, f, g, w)]
+    y, h = P.residual_norm(x, f, gate=g, pre_weight=w, scale=0.5, eps=1e-5)
+    grads = torch.autograd.grad((y, h), leaves, (dy, dh))
+    step = gates // 4
+    for a in range(0, gates, step):  # (the reference in parts; the weight's gradient is the other tests')
+        rows = [q.detach()[a:a + step].expand(step, 2, d).reshape(2 * step, d) for q in (x, f, g, dy, dh, y, h, grads[0], grads[1])]
+        ref = res_ref(rows[0], rows[1], {"pre_weight": w.detach()}, "rms", None, rows[2], 0.5, 1e-5,
+                      torch.ones_like(rows[0], dtype=torch.float64), rows[3], rows[4], U[torch.float32])
+        for name, out in zip(("y", "h", "x", "f"), rows[5:]):
+            within(out.detach(), *ref[name], name)
+        dyt, dyt_err = ref["x"]  # the gate's gradient: the sum of scale dyt f over its two rows
+        b = 0.5 * (dyt_err * rows[1].abs() + 10 * E * (dyt * rows[1]).abs()).view(step, 2, d).sum(1)
+        v = 0.5 * (dyt * rows[1]).view(step, 2, d).sum(1)
+        within(grads[2][a:a + step].view(step, d), v, b + U[torch.float32] * v.abs(), "gate")
