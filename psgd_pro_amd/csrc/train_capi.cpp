@@ -142,6 +142,9 @@ int res_args(const psgdk_residual_norm_t* q, ResArgs& a) {
 // slab mean more sums of dw in fp32, more of them nothing (12288 x 2048 x 131072: 20.6 ms with 512 MiB, 18.7 with 1 GiB,
 // 19.4 with 2, whose slabs are uneven there).
 constexpr int64_t kLogitBytes = (int64_t)1 << 30;
+// and no more than this many: xent_rows_launch has 256 threads or more for each, and a launch less than 2^32 (the bf16 path's
+// codes lie in rows of at least 64: 2^23 rows of 256 threads)
+constexpr int64_t kSlabRows = (int64_t)1 << 22;
 // 256 rows of a product's operand stay within 32-bit byte offsets
 constexpr int64_t kMaxVocab = (int64_t)1 << 22;
 
@@ -274,7 +277,7 @@ int f32_split_k(const Lce& p, int ta, int64_t m, int64_t k, int parts, const flo
 
 // float32: the logits of a slab of rows by the converting engine, a pass over them, and its products with W and x.
 int lce_f32(const Lce& p) {
-  const int64_t ldz = (p.vocab + 3) / 4 * 4, slab = std::min(p.rows, std::max<int64_t>(1, kLogitBytes / 4 / ldz));
+  const int64_t ldz = (p.vocab + 3) / 4 * 4, slab = std::min({p.rows, kSlabRows, std::max<int64_t>(1, kLogitBytes / 4 / ldz)});
   Ws m(p.ws);
   float* const weight = m.take<float>(1);
   int* const count = m.take<int>(1);

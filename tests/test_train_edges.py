@@ -1,5 +1,5 @@
-"""The training operators on the GPU where a step goes wrong or is unusually large: infinite logits, and more gates than one
-launch holds workgroups for. References in float64, bounds as in test_train_ops.py."""
+"""The training operators on the GPU where a step goes wrong or is unusually large: infinite logits, and more rows or
+gates than one launch holds workgroups for. References in float64, bounds as in test_train_ops.py."""
 import math
 
 import pytest
@@ -101,3 +101,28 @@ def test_residual_norm_of_four_million_gates():
         b = 0.5 * (dyt_err * rows[1].abs() + 10 * E * (dyt * rows[1]).abs()).view(step, 2, d).sum(1)
         v = 0.5 * (dyt * rows[1]).view(step, 2, d).sum(1)
         within(grads[2][a:a + step].view(step, d), v, b + U[torch.float32] * v.abs(), "gate")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_entropy_of_sixteen_million_rows(dtype):
+    """Two classes and so many rows that one workgroup for each would pass the 2^32 threads of a launch."""
+    n, d, v = (1 << 24) + 5, 1, 2
+    x, w, t = rnd((n, d), 1, dtype).requires_grad_(), rnd((v, d), 2, dtype).requires_grad_(), targets(n, v, 3, 0.1)
+    loss = P.linear_cross_entropy(x, w, t, reduction="none")
+    gx, gw = torch.autograd.grad(loss, (x, w), torch.ones_like(loss))
+    (ref, err), (rx, rx_err), (rw, _) = lce_ref(x.detach(), w.detach(), t, -100, torch.ones(n, device=DEV, dtype=torch.float64))
+    within(loss.detach(), ref, err, "loss")
+    within(gx, rx, rx_err, "dx")
+    # n roundings of partial sums, each within E of the terms' sum and either way: their sum grows with sqrt(n) (the bound
+    # for roundings that all go one way would not see a lost part of the rows)
+    terms = torch.stack([(p.abs() * x.detach().double().abs()[:, 0]).sum() for p in _dz(x.detach(), w.detach(), t)])[:, None]
+    # (bf16: each logit's gradient is rounded, after its code's step of 2^-9, and so is the sum)
+    within(gw, rw, (64 * math.sqrt(n) * E + (0 if dtype == torch.float32 else 3 * U[dtype])) * terms, "dw")
+
+
+def _dz(x, w, t):
+    """The logits' gradients of two classes in float64, a class at a time."""
+    z = x.double() @ w.double().t()
+    p = torch.softmax(z, 1)
+    for c in (0, 1):
+        yield torch.where(t == -100, 0.0, p[:, c] - (t == c).double())
