@@ -10,6 +10,10 @@ namespace {
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+// A wave's way out holds one after the other what its loads wrote, 16-bit results and rows of them: its numbers are read by
+// types that may alias all of those, so that no read moves past a write of another type to the same bytes.
+typedef float lds_float __attribute__((may_alias));
+typedef int lds_int __attribute__((may_alias));
 #define LDS_AS __attribute__((address_space(3)))
 
 // One operand's tile of R rows (m or n) x BK k in LDS, filled by loads that write LDS directly (16 bytes a lane, 1 KB a
@@ -326,8 +330,8 @@ __global__ void __launch_bounds__(256, 1) xgemm_kernel(const XgArgs p) {
     if constexpr (KIND == XG_LOGITS) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        ref[j] = *(LDS_AS float*)(uintptr_t)(ep + (32 * j + c) * 4);
-        tgt[j] = *(LDS_AS int*)(uintptr_t)(ep + (WTN + 32 * j + c) * 4);
+        ref[j] = *(LDS_AS lds_float*)(uintptr_t)(ep + (32 * j + c) * 4);
+        tgt[j] = *(LDS_AS lds_int*)(uintptr_t)(ep + (WTN + 32 * j + c) * 4);
       }
     }
     constexpr int CH = WTM / 8;
