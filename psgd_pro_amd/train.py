@@ -316,23 +316,25 @@ class _LinearCrossEntropy(torch.autograd.Function):
         reduced = reduction != "none"
         need = ctx.needs_input_grad
         loss, total, dx, dw = _lce_call(x, w, target, ignore, None, reduction, reduced and need[0], reduced and need[1])
-        ctx.save_for_backward(x, w, target)
+        ctx.save_for_backward(x, w, target, dx, dw)  # all of them: hooks on saved tensors move or drop the gradients too
         ctx.args = ignore, reduction
-        ctx.grads = (dx, dw) if reduced else None
+        ctx.handed_over = False
         return total if reduced else loss.view(target.shape)
 
     @staticmethod
     def backward(ctx, g):
         _once()
-        x, w, target = ctx.saved_tensors
+        x, w, target, *grads = ctx.saved_tensors
         ignore, reduction = ctx.args
         need = ctx.needs_input_grad
         if reduction == "none":
             g = g.reshape(-1).float().contiguous()
             return (*_lce_call(x, w, target, ignore, g, reduction, need[0], need[1])[2:], None, None, None)
-        grads, ctx.grads = ctx.grads, None
-        if grads is None:
+        if ctx.handed_over:
             grads = _lce_call(x, w, target, ignore, None, reduction, need[0], need[1])[2:]
+        else:  # (.data: what the caller does to them in place is no change of a saved tensor)
+            grads = [None if t is None else t.data for t in grads]
+            ctx.handed_over = True
         ts = [t for t in grads if t is not None and t.numel()]
         if ts:
             g = g.float()

@@ -1,9 +1,10 @@
-"""The training operators on the GPU where a step goes wrong or is unusually large: infinite logits, and more rows or
-gates than one launch holds workgroups for. References in float64, bounds as in test_train_ops.py."""
+"""The training operators on the GPU where a step goes wrong or is unusually large: infinite logits, more rows or
+gates than one launch holds workgroups for, forward passes that are run again. References in float64, bounds as in test_train_ops.py."""
 import math
 
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 import psgd_pro_amd as P
 from test_train_ops import DEV, DTYPES, E, U, lce_ref, res_ref, rnd, targets, within
@@ -126,3 +127,31 @@ def _dz(x, w, t):
     p = torch.softmax(z, 1)
     for c in (0, 1):
         yield torch.where(t == -100, 0.0, p[:, c] - (t == c).double())
+
+
+# -- saved tensors ------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("way", ["checkpoint", "reentrant checkpoint", "on the host"])
+def test_operators_under_checkpoints_and_saved_tensor_hooks(dtype, way):
+    """The same bits where the forward pass is run again in the backward pass, and where saved tensors wait on the host."""
+    x, f, w, t = rnd((600, 256), 1, dtype), rnd((600, 256), 2, dtype), rnd((1000, 256), 3, dtype, 0.1), targets(600, 1000, 4, 0.2)
+
+    def loss(x, f, w):
+        y, h = P.residual_norm(x, f, post="rms", p=0.1, seed=3)
+        return P.linear_cross_entropy(P.dropout(h, 0.2, seed=4), w, t) / 3 + y.float().square().mean()
+
+    def run(call):
+        leaves = [q.detach().clone().requires_grad_() for q in (x, f, w)]
+        out = call(*leaves)
+        out.backward()
+        return (out.detach(), *(q.grad for q in leaves))
+
+    ref = run(loss)
+    if way == "on the host":
+        with torch.autograd.graph.save_on_cpu():
+            out = run(loss)
+    else:
+        out = run(lambda *a: checkpoint(loss, *a, use_reentrant=way.startswith("reentrant")))
+    assert all(torch.equal(p, q) for p, q in zip(ref, out))

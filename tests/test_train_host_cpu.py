@@ -1,5 +1,7 @@
 """The training operators' Python side without a GPU: the entry points on CPU tensors, their launches recorded instead of
 made (outputs hold nothing)."""
+import weakref
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -76,3 +78,34 @@ def test_forward_mode_transform_is_refused(calls):
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda x: P.dropout(x, 0.5, seed=1), (torch.ones(4, 8),), (torch.ones(4, 8),))
     assert not calls
+
+
+@pytest.mark.parametrize("need", [(True, True), (True, False), (False, True)])
+def test_gradients_made_ahead_are_saved_tensors(calls, need):
+    """Hooks that move saved tensors away or drop them get the gradients that a reduced loss made in its forward pass, and
+    nothing else keeps them."""
+    x, w = (torch.ones(n, 8).requires_grad_(q) for n, q in zip((4, 5), need))
+    t, held = torch.zeros(4, dtype=torch.int64), []
+
+    def pack(q):
+        held.append((q.shape, weakref.ref(q.untyped_storage())))
+        return q.shape, q.dtype
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda q: torch.full(q[0], 7, dtype=q[1])):
+        out = P.linear_cross_entropy(x, w, t)
+    made = [shape for shape, storage in held if storage() is None]  # (x, w and the targets are still here)
+    wanted = [q for q in (x, w) if q.requires_grad]
+    assert made == [q.shape for q in wanted]
+    for g, q in zip(torch.autograd.grad(out, wanted), wanted):
+        assert torch.equal(g, torch.full_like(q, 7))
+    assert [c[0] for c in calls] == ["psgdk_linear_cross_entropy", "psgdk_scale_by"]
+
+
+def test_a_second_backward_pass_makes_the_gradients_again(calls):
+    x = torch.ones(4, 8, requires_grad=True)
+    out = P.linear_cross_entropy(x, torch.ones(5, 8), torch.zeros(4, dtype=torch.int64))
+    a, = torch.autograd.grad(out, x, retain_graph=True)
+    a.mul_(2)  # the caller's to change
+    b, = torch.autograd.grad(out, x)
+    assert a.data_ptr() != b.data_ptr()
+    assert [c[0] for c in calls] == ["psgdk_linear_cross_entropy", "psgdk_scale_by"] * 2
