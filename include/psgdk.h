@@ -307,7 +307,7 @@ int psgdk_fill_normal(void* out, int64_t n, int dtype, uint64_t seed, uint64_t s
 /* ---------------------------------------------------------------------------------------------------------------
  * Level 3: operators of the training step in front of the optimizer. Rows are stored with the last dimension
  * contiguous; ld* are row strides in elements. Storage dtypes are PSGDK_F32 or PSGDK_BF16; statistics, sums and
- * accumulators are fp32 and every output is rounded once. No counterparts in the reference.
+ * accumulators are fp32 and every output is rounded once from its fp32 value. No counterparts in the reference.
  * ------------------------------------------------------------------------------------------------------------ */
 
 /* y = dropout(x) over rows x d. Element (i, c) is kept where the 16-bit number c % 8 (low half of a word first) of
@@ -373,11 +373,19 @@ int psgdk_residual_norm_backward(const psgdk_residual_norm_t* a, const psgdk_res
  * and, where dx or dw is non-NULL, that gradient of sum_i row_weight[i] loss[i], in the dtype of x and w; row_weight
  * NULL: 1 for every row (mean 0) or 1 / (number of rows not ignored) (mean 1). A target outside 0 .. vocab - 1 that is
  * not `ignore` gives a NaN loss (and NaN gradients of its row), and so does a logit of +inf or NaN; a target's logit of
- * -inf beside a finite one gives a loss of +inf. mean_loss (optional, one float) receives
- * sum_i row_weight[i] loss[i] under the same rule. An ignored row's x reaches no result, its dx is 0, and the bf16
- * products leave it out. rows up to 2^30, d up to 2^20, vocab up to 2^22. The logits are never in memory in fp32 with bf16 inputs; of a slab of rows (up to 1 GiB) they
- * are there as 16-bit codes while the gradients are made (fp32 inputs: 1 GiB of fp32 logits). The workspace's size
- * depends on the alignment of w, dx and dw: the size query is made with the same pointers. */
+ * -inf beside a finite one gives a loss of +inf. mean_loss (optional, one float) receives sum_i row_weight[i] loss[i]
+ * under the same rule. An ignored row's x reaches no result and its dx is 0. rows up to 2^30, d up to 2^20, vocab up to
+ * 2^22.
+ * Precision: losses and sums are fp32. With bf16 inputs the logits' gradients are rounded to bf16 before the products
+ * that make dx and dw, where the matrix cores take them, and with many rows the logits behind them are held as 16-bit
+ * numbers of steps of 2^-9; fp32 inputs keep 24 bits throughout.
+ * The workspace holds, of a slab of rows at a time, the logits while the gradients are made and a copy of the rows of x.
+ * A slab's logits take up to 1 GiB (or what 256 rows take, fp32 one row), in fp32 with fp32 inputs and in 16 bits with
+ * bf16 ones, except that up to 512 rows and 2^23 logits of those are there in fp32 as well. Many bf16 rows are gathered
+ * first, so that the ignored ones cost no products; few rows and fp32 ones are multiplied as zeros. Besides: a copy of a
+ * bf16 w whose rows are not 16-byte aligned, and fp32 sums of dx and dw, one for each of the parts (up to 32) in which
+ * they are made where their tiles alone leave CUs idle, one of dw for several slabs of bf16 rows. The size depends on the
+ * alignment of w, dx and dw: the size query is made with the same pointers. */
 int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype, const void* x, int64_t ldx,
                                const void* w, int64_t ldw, const int64_t* target, int64_t ignore,
                                const float* row_weight, int mean, float* loss, float* mean_loss, void* dx,
@@ -385,7 +393,8 @@ int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype
                                psgdk_stream_t stream);
 
 /* x[b][i] *= *scale (device memory, one float) for the n[b] elements of nb (1 .. 4) tensors of one dtype; nothing but
- * the scale is read, and nothing written, where it is 1. n and x are host arrays. */
+ * the scale is read, and nothing written, where it is 1; bf16 values are rounded again, which changes nothing where it is
+ * a power of two. n and x are host arrays. */
 int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const float* scale, psgdk_stream_t stream);
 
 /* Launch profiling (diagnostic, per host thread): after psgdk_profile_start every MFMA-engine launch the thread makes is

@@ -20,8 +20,10 @@ struct XentRowsArgs {
   float* z;                 // 16-byte aligned; ldz a multiple of 4, less than vocab + 4
   long long ldz, rows;
   int vocab, grad;
-  bf16_t* dz;               // null, or: the gradients go there (rows of ldq, a multiple of 64, zeros behind the vocabulary)
-  long long ldq;            // without the mean's weight
+  // null, or: the gradients go there, without the mean's weight, rounded to bf16 for the matrix cores of the bf16 products
+  // that follow (rows of ldq, a multiple of 64, zeros behind the vocabulary)
+  bf16_t* dz;
+  long long ldq;
   int64_t ignore;
   const int64_t* target;
   const float* row_weight;  // null: weight[0] for every row

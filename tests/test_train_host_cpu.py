@@ -1,5 +1,6 @@
 """The training operators' Python side without a GPU: the entry points on CPU tensors, their launches recorded instead of
 made (outputs hold nothing)."""
+import ctypes as C
 import weakref
 
 import pytest
@@ -7,6 +8,7 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 import psgd_pro_amd as P
+from psgd_pro_amd import _lib as L
 from psgd_pro_amd import train as T
 
 
@@ -109,3 +111,23 @@ def test_a_second_backward_pass_makes_the_gradients_again(calls):
     b, = torch.autograd.grad(out, x)
     assert a.data_ptr() != b.data_ptr()
     assert [c[0] for c in calls] == ["psgdk_linear_cross_entropy", "psgdk_scale_by"] * 2
+
+
+@pytest.mark.parametrize("rows,d,vocab", [(500000, 4096, 1000), (1 << 20, 1024, 16), (4096, 4096, 131072), (1531, 770, 50021),
+                                          (512, 1024, 16384), (65536, 256, 1024), (1 << 25, 1, 2), (3, 16, 1 << 22)])
+@pytest.mark.parametrize("dtype", [L.F32, L.BF16])
+@pytest.mark.parametrize("grad", [False, True])
+def test_cross_entropy_workspace_is_what_the_header_says(rows, d, vocab, dtype, grad):
+    """A slab's logits and its copy of x, a copy of an unaligned head, parts of the gradients."""
+    size, ptr = C.c_size_t(0), 0x10000
+    out = ptr if grad else None
+    assert L.lib().psgdk_linear_cross_entropy(rows, d, vocab, dtype, ptr, d, ptr, d, ptr, -100, None, 1, ptr, None, out, d, out, d,
+                                              None, C.byref(size), None) == L.OK
+    e, ld, up = (2, -(-d // 8) * 8, -(-vocab // 64) * 64) if dtype == L.BF16 else (4, d, -(-vocab // 4) * 4)
+    slab = min(rows, max(256 if dtype == L.BF16 else 1, (1 << 30) // (up * e)), 1 << (23 if dtype == L.BF16 else 22))
+    small = dtype == L.BF16 and rows <= 512 and rows * vocab <= 1 << 23
+    logits = slab * up * (e + 4 * small) if grad or small or dtype == L.F32 else 0
+    parts = 32 * min(slab, 4096) * ld * 4 + 32 * vocab * ld * 4 if grad else 0
+    copies = slab * ld * e + (vocab * ld * e if dtype == L.BF16 and d % 8 else 0)
+    each = rows * 4 + slab * 64 + slab * -(-vocab // 256) * 8 + (1 << 20)  # the order, what a row keeps, sums of 128 columns
+    assert size.value <= logits + copies + parts + each
