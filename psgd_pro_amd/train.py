@@ -311,8 +311,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     again) and hands them over in the backward pass, scaled by the loss's gradient; where the graph is kept for another
     backward pass they are computed again. bfloat16 gradients are rounded a second time by that scaling: it costs them less
     than the float32 ones between the passes would take in memory (twice dx and dw) or a third set of products in time, and
-    nothing where the scale is a power of two. The losses of single rows need their gradients' weights first, and are
-    rounded once."""
+    nothing where the scale is a power of two. The losses of single rows need their gradients' weights first."""
 
     @staticmethod
     def forward(ctx, x, w, target, ignore, reduction):
@@ -351,9 +350,8 @@ def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mea
     dtype, target (...) of int64. Rows whose target is ignore_index have no loss and no gradient, whatever x holds there;
     another target outside the vocabulary makes the loss NaN. reduction: "mean" over the rows not ignored (0 where there
     are none), "sum", or "none" (losses in target's shape). Losses are float32; the gradients of x and weight have their
-    dtype. With bfloat16 they are sums over logits' gradients rounded to bfloat16 (float32: not rounded), and where the
-    loss is scaled afterwards by other than a power of two they are rounded again: "none" takes the weights of its rows in
-    before that."""
+    dtype. With bfloat16 they are sums over logits' gradients rounded to bfloat16 ("none": weighted and rounded), and where
+    a mean or sum is scaled afterwards by other than a power of two they are rounded again; float32 keeps its bits."""
     _check(x, "x")
     _check(weight, "weight", x)
     if weight.dtype != x.dtype:
