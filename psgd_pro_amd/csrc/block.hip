@@ -559,10 +559,10 @@ hipError_t residual_norm_launch(const ResArgs& a, hipStream_t st) {
 //   dgate = sum over its rows of scale dyt b;  du = scale gate dropout'(dyt);  df from du and f as dyt from dh and y
 //   weights: column sums of dh hat and du fhat, biases: of dh and du
 // A workgroup takes `chunk` consecutive rows and keeps its column sums in registers; they go to one row of `part` each
-// and a second kernel adds those in a fixed order. A gate row whose rows all lie in one workgroup is written at once.
+// and a second kernel adds those in a fixed order. A gate whose rows all lie in one workgroup has one such row.
 // Bound by memory where rows are long enough (16384 rows of 4096 bf16, two rms norms: 180 us, 4.5 TB/s; 33280 rows of 512
 // fp32: 86 us, 4.7 TB/s), by the chain of a row's sums on short ragged ones (8481 rows of 770 bf16, everything on: 51 us,
-// 1.8 TB/s): a row's two means are each a wave's sum, a barrier and the waves' sums. The next row's loads are under way
+// 1.5 TB/s): a row's two means are each a wave's sum, a barrier and the waves' sums. The next row's loads are under way
 // meanwhile (without them, and with one workgroup a CU: 410 us in place of 180).
 namespace {
 
@@ -590,8 +590,8 @@ __device__ __forceinline__ void put_sum(float (&s)[VE], float* dst, const Span<R
 
 // HAS: what the call may have (kPost: a norm after the block, kGate, kBias: a layer norm's biases); what it cannot have
 // holds no registers. SUMS: column sums in registers (1: of the norm before, 2: of the norm after, 4: of the gate).
-// Waves a SIMD, by what their registers hold without scratch memory (512, 168 and 128 registers a lane for 1 to 2, 3 and 4
-// of them); the rows are cut for so many workgroups at once.
+// Waves a SIMD, by what their registers hold without scratch memory (256, 168 and 128 registers a lane for 2, 3 and 4 of
+// them); the rows are cut for so many workgroups at once.
 constexpr int res_waves(int tpr, int has, int esize) {
   if (tpr == 1024 || has == 0 || has == kBias || (tpr == 512 && has == kPost && esize == 2)) return 4;
   return tpr == 512 || has == 7 || (has == (kPost | kGate) && esize == 4) ? 2 : 3;
