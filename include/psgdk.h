@@ -325,7 +325,8 @@ enum { PSGDK_NORM_NONE = 0, PSGDK_NORM_RMS = 1, PSGDK_NORM_LAYER = 2 };
  * NULL: 1, 0); NONE as post: u = f, as pre: no h. f NULL: y = x. The gate has gate_rows rows (0: no gate), row i of x
  * taking gate row i / (rows / gate_rows); gate_rows divides rows. */
 typedef struct psgdk_residual_norm {
-  int64_t rows, d;          /* d up to 2^20 */
+  int64_t rows, d;          /* d up to 2^20; rows under 2^26 up to 512 elements, half for each doubling of d to 2^22 over
+                               4096, and 2^22 under 8 */
   int32_t dtype;            /* x, f, y, h, and the gradients dy, dh, dx, df */
   int32_t pre, post;        /* PSGDK_NORM_* */
   int32_t w_dtype;          /* the norms' weights and biases, and their gradients */
