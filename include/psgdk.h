@@ -28,9 +28,9 @@ extern "C" {
 typedef struct ihipStream_t* psgdk_stream_t; /* hipStream_t */
 typedef struct ihipEvent_t* psgdk_event_t;   /* hipEvent_t */
 
-/* 6: level 3 (the training step's operators). 5: option 8 chooses how fp32 products are summed (in 4: whether a k-contiguous fp32 kernel is taken), option 13, kernel
+/* 7: attention, norms of queries and keys, AdamW. 6: level 3 (the training step's operators). 5: option 8 chooses how fp32 products are summed (in 4: whether a k-contiguous fp32 kernel is taken), option 13, kernel
  * ids 6000 and 8000 (in 4: other engines' ids below 5000 and at 6000), smaller workspaces of psgdk_trmm_ws. */
-#define PSGDK_VERSION 6
+#define PSGDK_VERSION 7
 #define PSGDK_MAXB 16 /* problems per grouped call */
 #define PSGDK_MAX_GROUPS 64 /* groups per psgdk_kron2d_update_groups call */
 #define PSGDK_NLB_K 32 /* rows of the random start of the norm lower bounds */
@@ -397,6 +397,41 @@ int psgdk_linear_cross_entropy(int64_t rows, int64_t d, int64_t vocab, int dtype
  * the scale is read, and nothing written, where it is 1; bf16 values are rounded again, which changes nothing where it is
  * a power of two. n and x are host arrays. */
 int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const float* scale, psgdk_stream_t stream);
+
+/* Attention of grouped heads under a causal mask with a sliding window and first tokens that stay visible. Query i of sequence b
+ * is at position p = starts[b] + i (starts NULL: m - n + i, the last of the m tokens) and sees key j where
+ *   0 <= p < length,  j <= p  and  (p - j < window or j < sinks),   length = lengths[b] (NULL: m; clamped to 0 .. m);
+ * window 0: all of them. o = sum_j softmax_j(scale q . k_j) v_j, 0 where nothing is seen; query head h takes the keys of head
+ * h / (heads / kv_heads). Keys and values from `length` on, and queries and their gradients that see nothing, may hold anything.
+ * Sums are added in an order that the sizes alone set. With bf16 the probabilities and, backward, the scores' gradients are
+ * rounded to bf16 before the matrix cores take them.
+ * d: a multiple of 8 up to 128; n and m up to 2^28, n heads / kv_heads under 2^31 - 256. */
+typedef struct psgdk_heads { /* (batch, tokens, heads, d), d contiguous; strides in elements, whole 16 bytes and up to 2^21 for
+                                tokens and (up to 128 heads; in inverse proportion for more) heads; 16-byte aligned */
+  const void* p;
+  int64_t batch_stride, token_stride, head_stride;
+} psgdk_heads_t;
+typedef struct psgdk_window_attention {
+  int64_t batch, n, m;      /* n queries and m keys a sequence */
+  int32_t heads, kv_heads, d, dtype;
+  int64_t window, sinks;
+  float scale;              /* positive */
+  psgdk_heads_t q, k, v;
+  const int64_t *lengths, *starts; /* device memory, one a sequence */
+  void* o;                  /* (batch, n, heads, d), contiguous: output of the forward call, input of the backward call */
+  float* lse;               /* [batch][kv_heads][n][heads / kv_heads]: log2 of the row's sum of e^score, output of the forward
+                               call (NULL: not stored), input of the backward call */
+} psgdk_window_attention_t;
+int psgdk_window_attention(const psgdk_window_attention_t* a, void* ws, size_t* ws_bytes, psgdk_stream_t stream);
+
+/* Gradients of q, k and v from o's, contiguous; those that are NULL are not computed. The workspace depends on which of them are
+ * asked for: the size query is made with the same pointers. */
+typedef struct psgdk_window_attention_grads {
+  psgdk_heads_t dout;
+  void *dq, *dk, *dv;
+} psgdk_window_attention_grads_t;
+int psgdk_window_attention_backward(const psgdk_window_attention_t* a, const psgdk_window_attention_grads_t* g, void* ws,
+                                    size_t* ws_bytes, psgdk_stream_t stream);
 
 /* Launch profiling (diagnostic, per host thread): after psgdk_profile_start every MFMA-engine launch the thread makes is
  * bracketed by a pair of HIP events on its stream. psgdk_profile_stop ends the recording and, with out non-NULL,

@@ -73,6 +73,24 @@ class ResidualNormGrads(C.Structure):
                 ("dpost_b", C.c_void_p)]
 
 
+class Heads(C.Structure):
+    """psgdk_heads_t"""
+    _fields_ = [("p", C.c_void_p), ("batch_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class WindowAttention(C.Structure):
+    """psgdk_window_attention_t"""
+    _fields_ = [("batch", C.c_int64), ("n", C.c_int64), ("m", C.c_int64), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("d", C.c_int32), ("dtype", C.c_int32), ("window", C.c_int64), ("sinks", C.c_int64), ("scale", C.c_float),
+                ("q", Heads), ("k", Heads), ("v", Heads), ("lengths", C.c_void_p), ("starts", C.c_void_p), ("o", C.c_void_p),
+                ("lse", C.c_void_p)]
+
+
+class WindowAttentionGrads(C.Structure):
+    """psgdk_window_attention_grads_t"""
+    _fields_ = [("dout", Heads), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p)]
+
+
 class ProfRecord(C.Structure):
     _fields_ = [("kernel_id", C.c_int32), ("tri", C.c_int32), ("nb", C.c_int32), ("ms", C.c_float),
                 ("flops", C.c_double), ("bytes", C.c_double), ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
@@ -128,6 +146,8 @@ _SIGS = {
     "psgdk_linear_cross_entropy": (_i32, [_i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _vp,
                                           _vp, _i64, _vp, _i64, _vp, _szp, _vp]),
     "psgdk_scale_by": (_i32, [_i32, C.POINTER(C.c_int64), _i32, _vpa, _vp, _vp]),
+    "psgdk_window_attention": (_i32, [C.POINTER(WindowAttention), _vp, _szp, _vp]),
+    "psgdk_window_attention_backward": (_i32, [C.POINTER(WindowAttention), C.POINTER(WindowAttentionGrads), _vp, _szp, _vp]),
     "psgdk_set_option": (_i32, [_i32, _i32]),
     "psgdk_get_option": (_i32, [_i32, C.POINTER(C.c_int)]),
     "psgdk_profile_start": (_i32, []),
@@ -136,7 +156,7 @@ _SIGS = {
 }
 
 EXPORTED = tuple(_SIGS)
-ABI_VERSION = 6  # PSGDK_VERSION of include/psgdk.h that these signatures and structures follow
+ABI_VERSION = 7  # PSGDK_VERSION of include/psgdk.h that these signatures and structures follow
 
 _lib = None
 

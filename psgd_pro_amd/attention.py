@@ -1,0 +1,123 @@
+"""Attention of a transformer's block on the HIP kernels (include/psgdk.h, level 3).
+
+    window_attention   softmax attention with grouped heads, a sliding window and first tokens that stay visible
+
+CUDA (HIP) tensors in float32 or bfloat16, on torch's current stream, differentiable once through autograd. No counterparts in
+the reference, which leaves the model to torch.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib as L
+from .train import _check, _once, _ptr, _run_ws, _wants_grad
+
+__all__ = ["window_attention"]
+
+_MAX_STRIDE = 1 << 21  # of tokens and heads, in elements
+
+
+def _heads(t):
+    """(psgdk_heads_t of t, the tensor it points to): t itself where its rows are aligned, else a copy."""
+    unit = 16 // t.element_size()
+    sb, sn, sh, sd = t.stride()
+    if (sd != 1 or t.data_ptr() % 16 or sb % unit or sn % unit or sh % unit or sn > _MAX_STRIDE
+            or sh * max(t.shape[2], 128) > _MAX_STRIDE * 128):
+        t = t.clone(memory_format=torch.contiguous_format)
+        sb, sn, sh, _ = t.stride()
+    return L.Heads(t.data_ptr(), sb, sn, sh), t
+
+
+def _attn_block(q, k, v, lengths, starts, o, lse, opt):
+    """psgdk_window_attention_t of the inputs, and the (possibly copied) tensors it points to."""
+    window, sinks, scale = opt
+    a = L.WindowAttention(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], L.dtype_code(q.dtype), window,
+                          sinks, scale)
+    (a.q, q), (a.k, k), (a.v, v) = _heads(q), _heads(k), _heads(v)
+    a.lengths, a.starts, a.o, a.lse = _ptr(lengths), _ptr(starts), o.data_ptr(), _ptr(lse)
+    return a, (q, k, v)
+
+
+def _attn_forward(q, k, v, lengths, starts, opt, stats):
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32) if stats else None
+    if not q.numel():
+        return o, lse
+    if not k.numel():  # no key to see
+        return o.zero_(), None if lse is None else lse.zero_()
+    a, keep = _attn_block(q, k, v, lengths, starts, o, lse, opt)
+    _run_ws(q, L.lib().psgdk_window_attention, C.byref(a))
+    return o, lse
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, starts, opt):
+        o, lse = _attn_forward(q, k, v, lengths, starts, opt, True)
+        ctx.opt = opt
+        ctx.save_for_backward(q, k, v, lengths, starts, o, lse)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        _once()
+        q, k, v, lengths, starts, o, lse = ctx.saved_tensors
+        outs = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if need else None
+                for t, need in zip((q, k, v), ctx.needs_input_grad)]
+        if not q.numel() or not k.numel():
+            for t in outs:
+                if t is not None:
+                    t.zero_()
+            return (*outs, None, None, None)
+        a, keep = _attn_block(q, k, v, lengths, starts, o, lse, ctx.opt)
+        g = L.WindowAttentionGrads()
+        g.dout, do = _heads(do)
+        g.dq, g.dk, g.dv = (_ptr(t) for t in outs)
+        _run_ws(q, L.lib().psgdk_window_attention_backward, C.byref(a), C.byref(g))
+        return (*outs, None, None, None)
+
+
+def window_attention(q, k, v, *, window=None, sinks=0, scale=None, lengths=None, starts=None):
+    """Causal attention: q (batch, n, heads, d), k and v (batch, m, kv_heads, d), heads a multiple of kv_heads (query head h takes
+    the keys of head h // (heads // kv_heads)), d a multiple of 8 up to 128; any strides (rows that are not 16-byte aligned are
+    copied). Returns (batch, n, heads, d).
+
+    Query i of sequence b is at position p = starts[b] + i, and sees key j where 0 <= p < lengths[b], j <= p, and (with a window)
+    p - j < window or j < sinks. lengths and starts are int64 tensors (batch,); absent, every sequence has m tokens and its
+    queries are the last n of them, so that
+
+        window_attention(q, k, v)                                    trains on whole sequences,
+        window_attention(q, k, v, lengths=n_tokens)                  on a batch padded on the right,
+        window_attention(q, kc, vc, lengths=n_tokens, starts=n_tokens - n)    reads the caches kc, vc of m places for the
+                                                                     last n tokens of each sequence.
+
+    A query that sees nothing has output 0 and no gradient; keys and values from lengths[b] on, and queries and gradients of
+    positions outside the sequence, may hold anything. scale: 1 / sqrt(d) if not given. Differentiable in q, k and v."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check(t, name, None if t is q else q)
+        if t.dim() != 4 or t.dtype != q.dtype:
+            raise RuntimeError(f"{name}: (batch, tokens, heads, d) in {q.dtype} expected, got {tuple(t.shape)} in {t.dtype}")
+    b, n, h, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise RuntimeError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: batch and d of q, k and v alike expected")
+    if not h or not k.shape[2] or h % k.shape[2]:
+        raise RuntimeError(f"{h} query heads: a multiple of the {k.shape[2]} key heads expected")
+    if not 8 <= d <= 128 or d % 8:
+        raise RuntimeError(f"d = {d}: a multiple of 8 up to 128 expected")
+    if window is not None and not window >= 1:
+        raise ValueError(f"window = {window}: at least 1, or None")
+    if not sinks >= 0:
+        raise ValueError(f"sinks = {sinks}: must be >= 0")
+    scale = 1 / math.sqrt(d) if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale = {scale}: must be positive")
+    tell = []
+    for name, t in (("lengths", lengths), ("starts", starts)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.device != q.device or t.shape != (b,)):
+            raise RuntimeError(f"{name}: an int64 tensor ({b},) on {q.device} expected")
+        tell.append(t if t is None else t.contiguous())
+    opt = (min(int(window), 1 << 40) if window is not None else 0, min(int(sinks), 1 << 40), scale)
+    if _wants_grad(q, k, v):
+        return _WindowAttention.apply(q, k, v, *tell, opt)
+    return _attn_forward(q, k, v, *tell, opt, False)[0]

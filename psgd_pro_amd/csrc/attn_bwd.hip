@@ -1,0 +1,361 @@
+// Attention backward, two passes without atomics: for 128 rows over their keys (delta, dq), for 128 keys over their rows
+// (dk, dv), each making the probabilities again from the scores and the forward pass's sums.
+#include <algorithm>
+
+#include "attn_dev.h"
+
+namespace psgdk {
+
+namespace {
+
+// With P the probabilities, dP = dO V^T, delta = sum of o dO over a row:  dS = P (dP - delta),  dQ = scale dS K.
+// Transposed as the forward pass: a lane has one row, dS^T is the last product's operand where it is made.
+template <typename T, int DP, int BK>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_dq_kernel(const AttnArgs a, int row_tiles) {
+  using R = Rows<T, DP>;
+  constexpr int LOADS = R::loads(BK, 4), TILE = BK * R::PITCH, KT = BK / 32, DC = DP / 16, DT = DP / 32;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 31, h = lane >> 5;
+
+  const int work = xcd_run(blockIdx.x, gridDim.x), pair = work / row_tiles, row0 = (row_tiles - 1 - (work - pair * row_tiles)) * 128;
+  const int b = pair / a.kv, head = pair - b * a.kv;
+  const Seq s = sequence(a, b);
+  const int lo = s.start + row_token(a, row0), hi = s.start + row_token(a, min(row0 + 128, a.rows) - 1);
+  const KeyTiles tiles = key_tiles<BK>(a, s, lo, hi);
+
+  const int r = row0 + wave * 32 + c, tok = row_token(a, r), g = r - tok * a.group;
+  const bool there = r < a.rows;
+  const int pos = there && s.start + tok >= 0 && s.start + tok < s.len ? s.start + tok : -1;
+  const long long qh = head * a.group + g;
+  const T* const qp = static_cast<const T*>(a.q.p) + b * a.q.sb + tok * a.q.sn + qh * a.q.sh;
+  const T* const gp = static_cast<const T*>(a.dout.p) + b * a.dout.sb + tok * a.dout.sn + qh * a.dout.sh;
+  const T* const op = static_cast<const T*>(a.o.p) + b * a.o.sb + tok * a.o.sn + qh * a.o.sh;
+  frag_t<T> qf[DC], gf[DC];
+  float delta = 0.f;
+#pragma unroll
+  for (int i = 0; i < DC; ++i) {
+    qf[i] = row_frag<T>(qp, 16 * i + 8 * h, a.d, pos >= 0);
+    gf[i] = row_frag<T>(gp, 16 * i + 8 * h, a.d, pos >= 0);
+    const frag_t<T> of = row_frag<T>(op, 16 * i + 8 * h, a.d, pos >= 0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) delta += (float)gf[i][e] * (float)of[e];
+  }
+  delta += other_half(delta);
+  const long long at = (long long)pair * a.rows + r;
+  if (there && h == 0) a.delta[at] = delta;
+  if (!a.dq) return;
+  const float lse = there ? a.lse[at] : 0.f;
+
+  int vk[LOADS], vv[LOADS], lrow[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    int chunk;
+    R::where(wave * LOADS + i, lane, lrow[i], chunk);
+    const bool in = chunk * R::PER < a.d;
+    vk[i] = in ? (int)(lrow[i] * a.k.sn * R::E) + chunk * 16 : kOob;
+    vv[i] = in ? (int)(lrow[i] * a.v.sn * R::E) + chunk * 16 : kOob;
+  }
+  const T* const kp = static_cast<const T*>(a.k.p) + b * a.k.sb + head * a.k.sh;
+  const T* const vp = static_cast<const T*>(a.v.p) + b * a.v.sb + head * a.v.sh;
+  auto load = [&](int t) __attribute__((always_inline)) {
+    const int j0 = tiles.tile(t) * BK;
+    i32x4_t rk = rsrc_words(kp + j0 * a.k.sn, 0x7fffffff), rv = rsrc_words(vp + j0 * a.v.sn, 0x7fffffff);
+    unsigned to = uniform(lds0 + (t & 1) * 2 * TILE + wave * LOADS * 1024);
+    asm volatile("s_nop 4" : "+s"(rk), "+s"(rv), "+s"(to));  // (as in the forward pass)
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const bool in = j0 + lrow[i] < s.len;
+      load_lds(rk, in ? vk[i] : kOob, to + i * 1024);
+      load_lds(rv, in ? vv[i] : kOob, to + TILE + i * 1024);
+    }
+  };
+
+  f32x16_t dq[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) dq[i] = zero16();
+  if (tiles.count) load(0);
+  for (int t = 0; t < tiles.count; ++t) {
+    const int j0 = tiles.tile(t) * BK;
+    load_wait<0>();
+    if (t + 1 < tiles.count) load(t + 1);
+    const unsigned kt = lds0 + (t & 1) * 2 * TILE, vt = kt + TILE;
+    const bool look = j0 + BK - 1 > lo || hi >= s.len || (hi - j0 >= a.window && j0 + BK > a.sinks);
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      f32x16_t x = zero16(), dp = zero16();
+#pragma unroll
+      for (int k = 0; k < DC; ++k) {
+        x = mma(R::straight(kt, 32 * i + c, k, h), qf[k], x);
+        dp = mma(R::straight(vt, 32 * i + c, k, h), gf[k], dp);
+      }
+      if (look) {
+        const int j = j0 + 32 * i + 4 * h;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = j + 8 * (e >> 2) + (e & 3);
+          if (!(key <= pos && (pos - key < a.window || key < a.sinks))) x[e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse)) * (dp[e] - delta);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const frag_t<T> ds = crossed<T>(x, u);
+#pragma unroll
+        for (int k = 0; k < DT; ++k) dq[k] = mma(R::transposed(kt, 32 * i + 16 * u, k, lane), ds, dq[k]);
+      }
+    }
+  }
+  if (!there) return;
+  T* const out = static_cast<T*>(a.dq) + (((long long)b * a.n + tok) * a.kv * a.group + qh) * a.d;
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int col = 32 * i + 2 * e + 4 * h;
+      if (col >= a.d) continue;
+      const float y0 = dq[i][e] * a.scale, y1 = dq[i][e + 1] * a.scale, y2 = dq[i][e + 2] * a.scale, y3 = dq[i][e + 3] * a.scale;
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + col) = make_uint2(pack2_bf16(y0, y1), pack2_bf16(y2, y3));
+      else *reinterpret_cast<f32x4_t*>(out + col) = f32x4_t{y0, y1, y2, y3};
+    }
+}
+
+// 4 values of dk or dv of one key
+template <typename T>
+__device__ __forceinline__ void store4(T* out, float y0, float y1, float y2, float y3) {
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out) = make_uint2(pack2_bf16(y0, y1), pack2_bf16(y2, y3));
+  else *reinterpret_cast<f32x4_t*>(out) = f32x4_t{y0, y1, y2, y3};
+}
+
+// dV = P^T dO, dK = scale dS^T Q for 128 keys, 32 of each wave, over the rows that see any of them: all the key head's query
+// heads are among them, so that shared heads' gradients need no further sum. S = Q K^T has a key in each lane, P and dS are
+// the second products' operands where they are made (dV^T = dO^T P, dK^T = Q^T dS), and a tile of rows serves straight and
+// transposed. Key tiles that hold sinks are seen by all rows: their rows are cut in parts, whose sums attn_dkv_sum adds.
+template <typename T, int DP, int BR>
+__global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) attn_dkv_kernel(const AttnArgs a, int key_tiles) {
+  using R = Rows<T, DP>;
+  constexpr int LOADS = R::loads(BR, 4), TILE = BR * R::PITCH, STAGE = 2 * TILE + 512, RT = BR / 32, DC = DP / 16, DT = DP / 32;
+  static_assert(BR <= 64, "a load of 64 floats");
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 31, h = lane >> 5;
+
+  const int sinks = a.sink_tiles * a.sink_parts, per = sinks + (key_tiles - a.sink_tiles) * a.rest_parts;
+  const int work = xcd_run(blockIdx.x, gridDim.x), pair = work / per, rest = work - pair * per;
+  const bool sink = rest < sinks;
+  const int parts = sink ? a.sink_parts : a.rest_parts, part = sink ? rest % parts : (rest - sinks) % parts;
+  const int tile = sink ? rest / parts : a.sink_tiles + (rest - sinks) / parts, j0 = tile * kAttnKeys;
+  const int b = pair / a.kv, head = pair - b * a.kv;
+  const Seq s = sequence(a, b);
+  // tokens that see any of the keys, and their rows' tiles
+  const int from = max(0, j0 - s.start);
+  int to = min(a.n, s.len - s.start);
+  if (!sink && j0 >= a.sinks) to = min(to, j0 + kAttnKeys - 1 + a.window - s.start);
+  const int first = (int)((long long)from * a.group / BR), tiles = to > from ? (int)(((long long)to * a.group + BR - 1) / BR) - first : 0;
+  const int t0 = part_begin(tiles, part, parts), t1 = part_begin(tiles, part + 1, parts);
+
+  const int key = j0 + wave * 32 + c;
+  const T* const kp = static_cast<const T*>(a.k.p) + b * a.k.sb + key * a.k.sn + head * a.k.sh;
+  const T* const vp = static_cast<const T*>(a.v.p) + b * a.v.sb + key * a.v.sn + head * a.v.sh;
+  frag_t<T> kf[DC], vf[DC];
+#pragma unroll
+  for (int i = 0; i < DC; ++i) {
+    kf[i] = row_frag<T>(kp, 16 * i + 8 * h, a.d, key < s.len);
+    vf[i] = row_frag<T>(vp, 16 * i + 8 * h, a.d, key < s.len);
+  }
+
+  const T* const qp = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)head * a.group * a.q.sh;
+  const T* const gp = static_cast<const T*>(a.dout.p) + b * a.dout.sb + (long long)head * a.group * a.dout.sh;
+  auto load = [&](int t) __attribute__((always_inline)) {
+    const int r0 = (first + t) * BR, tok0 = row_token(a, r0);
+    i32x4_t rq = rsrc_words(qp + tok0 * a.q.sn, 0x7fffffff), rg = rsrc_words(gp + tok0 * a.dout.sn, 0x7fffffff);
+    i32x4_t rs = rsrc_words((wave == 0 ? a.lse : a.delta) + (long long)pair * a.rows + r0, 0x7fffffff);
+    unsigned at = uniform(lds0 + (t & 1) * STAGE + wave * LOADS * 1024);
+    unsigned st = uniform(lds0 + (t & 1) * STAGE + 2 * TILE + wave * 256);
+    asm volatile("s_nop 4" : "+s"(rq), "+s"(rg), "+s"(rs), "+s"(at), "+s"(st));  // (as in the forward pass)
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int lrow, chunk;
+      R::where(wave * LOADS + i, lane, lrow, chunk);
+      const int r = r0 + lrow, tok = row_token(a, r), g = r - tok * a.group;
+      const bool in = chunk * R::PER < a.d && tok >= from && tok < to;
+      load_lds(rq, in ? (int)(((tok - tok0) * a.q.sn + g * a.q.sh) * R::E) + chunk * 16 : kOob, at + i * 1024);
+      load_lds(rg, in ? (int)(((tok - tok0) * a.dout.sn + g * a.dout.sh) * R::E) + chunk * 16 : kOob, at + TILE + i * 1024);
+    }
+    if (wave < 2) load_lds4(rs, lane < BR && r0 + lane < a.rows ? lane * 4 : kOob, st);
+  };
+
+  f32x16_t dk[DT], dv[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) dk[i] = dv[i] = zero16();
+  if (t0 < t1) load(t0);
+  for (int t = t0; t < t1; ++t) {
+    load_wait<0>();
+    if (t + 1 < t1) load(t + 1);
+    const unsigned qt = lds0 + (t & 1) * STAGE, gt = qt + TILE, st = gt + TILE;
+    const int r0 = (first + t) * BR, lo = s.start + row_token(a, r0), hi = s.start + row_token(a, r0 + BR - 1);
+    const bool look = lo < j0 + kAttnKeys - 1 || hi >= s.len || hi >= s.start + a.n ||
+                      (hi - j0 >= a.window && j0 + kAttnKeys > a.sinks);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      f32x16_t x = zero16(), dp = zero16();
+#pragma unroll
+      for (int k = 0; k < DC; ++k) {
+        x = mma(R::straight(qt, 32 * i + c, k, h), kf[k], x);
+        dp = mma(R::straight(gt, 32 * i + c, k, h), vf[k], dp);
+      }
+      f32x4_t lse[4], delta[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lse[e] = *(LDS_AS f32x4_t*)(uintptr_t)(st + (32 * i + 8 * e + 4 * h) * 4);
+        delta[e] = *(LDS_AS f32x4_t*)(uintptr_t)(st + 256 + (32 * i + 8 * e + 4 * h) * 4);
+      }
+      if (look) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int tok = row_token(a, r0 + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3)), pos = s.start + tok;
+          if (!(tok < to && key <= pos && (pos - key < a.window || key < a.sinks))) x[e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse[e >> 2][e & 3]));
+        dp[e] = x[e] * (dp[e] - delta[e >> 2][e & 3]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const frag_t<T> p = crossed<T>(x, u), ds = crossed<T>(dp, u);
+#pragma unroll
+        for (int k = 0; k < DT; ++k) {
+          dv[k] = mma(R::transposed(gt, 32 * i + 16 * u, k, lane), p, dv[k]);
+          dk[k] = mma(R::transposed(qt, 32 * i + 16 * u, k, lane), ds, dk[k]);
+        }
+      }
+    }
+  }
+
+  if (parts > 1) {
+    const long long at = sink ? ((long long)pair * a.sink_tiles + tile) * parts + part
+                              : (a.sink_parts > 1 ? (long long)a.batch * a.kv * sinks : 0) +
+                                    ((long long)pair * (key_tiles - a.sink_tiles) + tile - a.sink_tiles) * parts + part;
+    float* const out = a.part_kv + (at * 2 * kAttnKeys + wave * 32 + c) * DP;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int col = 32 * i + 2 * e + 4 * h;
+        *reinterpret_cast<f32x4_t*>(out + col) = f32x4_t{dk[i][e], dk[i][e + 1], dk[i][e + 2], dk[i][e + 3]};
+        *reinterpret_cast<f32x4_t*>(out + kAttnKeys * DP + col) = f32x4_t{dv[i][e], dv[i][e + 1], dv[i][e + 2], dv[i][e + 3]};
+      }
+    return;
+  }
+  if (key >= a.m) return;
+  const long long at = (((long long)b * a.m + key) * a.kv + head) * a.d;
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int col = 32 * i + 2 * e + 4 * h;
+      if (col >= a.d) continue;
+      if (a.dk) store4(static_cast<T*>(a.dk) + at + col, dk[i][e] * a.scale, dk[i][e + 1] * a.scale, dk[i][e + 2] * a.scale,
+                       dk[i][e + 3] * a.scale);
+      if (a.dv) store4(static_cast<T*>(a.dv) + at + col, dv[i][e], dv[i][e + 1], dv[i][e + 2], dv[i][e + 3]);
+    }
+}
+
+// the parts' sums of the key tiles that have several, in order; a thread has 4 columns of a key's dk or dv
+template <typename T>
+__global__ void __launch_bounds__(256) attn_dkv_sum_kernel(const AttnArgs a, int first_tile, int tiles, int parts, int dp,
+                                                           long long base) {
+  const int quads = kAttnKeys * dp / 4, per = 2 * quads / 256;  // workgroups of a tile (dp a multiple of 32)
+  const int at = blockIdx.x / per, in = (blockIdx.x - at * per) * 256 + threadIdx.x;
+  const int pair = at / tiles, tile = at - pair * tiles, which = in / quads, q = in - which * quads;
+  const int row = q / (dp / 4), col = (q - row * (dp / 4)) * 4, key = (first_tile + tile) * kAttnKeys + row;
+  void* const to = which ? a.dv : a.dk;
+  if (key >= a.m || col >= a.d || !to) return;
+  const float* from = a.part_kv + ((base + (long long)at * parts) * 2 + which) * kAttnKeys * dp + row * dp + col;
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(from + (long long)p * 2 * kAttnKeys * dp);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += x[e];
+  }
+  const float by = which ? 1.f : a.scale;
+  const int b = pair / a.kv, head = pair - b * a.kv;
+  store4(static_cast<T*>(to) + (((long long)b * a.m + key) * a.kv + head) * a.d + col, sum[0] * by, sum[1] * by, sum[2] * by,
+         sum[3] * by);
+}
+
+template <typename T>
+constexpr int kTileRows = sizeof(T) == 2 ? 64 : 32;  // of a tile in LDS, keys or rows
+
+template <typename T, int DP>
+hipError_t launch_dq(const AttnArgs& a, hipStream_t st) {
+  constexpr int BK = kTileRows<T>, smem = 4 * BK * Rows<T, DP>::PITCH;
+  const auto fn = attn_dq_kernel<T, DP, BK>;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (attr != hipSuccess) return attr;
+  const int row_tiles = (a.rows + 127) / 128;
+  hipLaunchKernelGGL(fn, dim3(a.batch * a.kv * row_tiles), dim3(256), smem, st, a, row_tiles);
+  return hipGetLastError();
+}
+template <typename T, int DP>
+hipError_t launch_dkv(const AttnArgs& a, hipStream_t st) {
+  constexpr int BR = kTileRows<T>, smem = 2 * (2 * BR * Rows<T, DP>::PITCH + 512);
+  const auto fn = attn_dkv_kernel<T, DP, BR>;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (attr != hipSuccess) return attr;
+  const int tiles = (a.m + kAttnKeys - 1) / kAttnKeys, rest = tiles - a.sink_tiles, pairs = a.batch * a.kv;
+  hipLaunchKernelGGL(fn, dim3(pairs * (a.sink_tiles * a.sink_parts + rest * a.rest_parts)), dim3(256), smem, st, a, tiles);
+  hipError_t e = hipGetLastError();
+  const unsigned per = 2 * kAttnKeys * DP / 4 / 256;
+  if (e == hipSuccess && a.sink_parts > 1) {
+    hipLaunchKernelGGL(attn_dkv_sum_kernel<T>, dim3(pairs * a.sink_tiles * per), dim3(256), 0, st, a, 0, a.sink_tiles, a.sink_parts,
+                       DP, 0ll);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && a.rest_parts > 1 && rest) {
+    const long long base = a.sink_parts > 1 ? (long long)pairs * a.sink_tiles * a.sink_parts : 0;
+    hipLaunchKernelGGL(attn_dkv_sum_kernel<T>, dim3(pairs * rest * per), dim3(256), 0, st, a, a.sink_tiles, rest, a.rest_parts, DP,
+                       base);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+}  // namespace
+
+// Parts so that there are about 512 workgroups, none of fewer than 4 tiles of rows; key tiles with sinks, which all rows see,
+// in as many as leave each about the rows of another tile's.
+void attn_backward_parts(AttnArgs& a) {
+  const long long br = a.dt == 0 ? 32 : 64, pairs = (long long)a.batch * a.kv, tiles = (a.m + kAttnKeys - 1) / kAttnKeys;
+  const long long all = (a.rows + br - 1) / br;
+  const long long seen = std::min(all, ((long long)(a.window + kAttnKeys - 1) * a.group + br - 1) / br + 1);
+  a.sink_tiles = a.sinks && seen < all ? (int)((std::min(a.sinks, a.m) + kAttnKeys - 1) / kAttnKeys) : 0;
+  const long long rest = tiles - a.sink_tiles;
+  a.rest_parts = (int)std::max<long long>(1, std::min<long long>({rest ? 512 / (pairs * rest) : 1, seen / 4, 64}));
+  const long long share = std::max<long long>(seen / a.rest_parts, 8);
+  a.sink_parts = 1;
+  if (a.sink_tiles)  // (4096 parts' sums are 512 MiB)
+    a.sink_parts = (int)std::max<long long>(1, std::min<long long>({all / share, 64, 4096 / (pairs * a.sink_tiles)}));
+}
+long long attn_part_tiles(const AttnArgs& a) {
+  const long long pairs = (long long)a.batch * a.kv, rest = (a.m + kAttnKeys - 1) / kAttnKeys - a.sink_tiles;
+  return pairs * ((a.sink_parts > 1 ? (long long)a.sink_tiles * a.sink_parts : 0) + (a.rest_parts > 1 ? rest * a.rest_parts : 0));
+}
+
+#define PSGDK_BY_D(fn)                            \
+  switch (attn_dp(a.d)) {                         \
+    case 32: return a.dt == 0 ? fn<float, 32>(a, st) : fn<bf16_t, 32>(a, st);   \
+    case 64: return a.dt == 0 ? fn<float, 64>(a, st) : fn<bf16_t, 64>(a, st);   \
+    case 96: return a.dt == 0 ? fn<float, 96>(a, st) : fn<bf16_t, 96>(a, st);   \
+    default: return a.dt == 0 ? fn<float, 128>(a, st) : fn<bf16_t, 128>(a, st); \
+  }
+hipError_t attn_dq_launch(const AttnArgs& a, hipStream_t st) { PSGDK_BY_D(launch_dq) }
+hipError_t attn_dkv_launch(const AttnArgs& a, hipStream_t st) { PSGDK_BY_D(launch_dkv) }
+
+}  // namespace psgdk

@@ -4,47 +4,16 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 
 #include "../../include/psgdk.h"
 #include "block.h"
+#include "capi_util.h"
 #include "xent.h"
-
-namespace psgdk {
-int set_error(int code, const char* msg);
-}
 
 using namespace psgdk;
 
 namespace {
 
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  return set_error(code, buf);
-}
-int hip_check(hipError_t e, const char* what) {
-  return e == hipSuccess ? PSGDK_OK : fail(PSGDK_EHIP, "%s: %s", what, hipGetErrorString(e));
-}
-#define PSGDK_TRY(expr)              \
-  do {                               \
-    const int _rc = (expr);          \
-    if (_rc != PSGDK_OK) return _rc; \
-  } while (0)
-
-int check_dt(int dt, const char* name) {
-  if (dt != PSGDK_F32 && dt != PSGDK_BF16) return fail(PSGDK_EINVAL, "%s = %d", name, dt);
-  return PSGDK_OK;
-}
-int check_size(int64_t v, int64_t lo, int64_t hi, const char* name) {
-  if (v < lo || v > hi)
-    return fail(PSGDK_ESHAPE, "%s = %lld: must be in %lld..%lld", name, (long long)v, (long long)lo, (long long)hi);
-  return PSGDK_OK;
-}
 // a tensor of rows: present, row stride at least d
 int check_rows(const void* p, int64_t ld, int64_t d, const char* name) {
   if (!p) return fail(PSGDK_EINVAL, "%s: null device pointer", name);
@@ -63,22 +32,6 @@ int make_drop(float p, uint64_t seed, uint64_t stream_id, Drop& d) {
   d.scale = d.thr < 65536 ? (float)(65536.0 / (65536 - d.thr)) : 0.f;
   return PSGDK_OK;
 }
-
-size_t esize(int dt) { return dt == PSGDK_BF16 ? 2 : 4; }
-
-// Bump allocator over the caller's workspace; with base == nullptr it only measures.
-struct Ws {
-  char* base;
-  size_t off = 0;
-  explicit Ws(void* b) : base(static_cast<char*>(b)) {}
-  template <typename T>
-  T* take(size_t count) {
-    off = (off + 255) & ~size_t(255);
-    T* p = base ? reinterpret_cast<T*>(base + off) : nullptr;
-    off += count * sizeof(T);
-    return p;
-  }
-};
 
 // the argument checks and the kernels' argument block of both residual_norm calls
 int res_args(const psgdk_residual_norm_t* q, ResArgs& a) {

@@ -2,19 +2,17 @@
 #include <cmath>
 #include <type_traits>
 
+#include "lds.h"
 #include "xgemm.h"
 
 namespace psgdk {
 
 namespace {
 
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 // A wave's way out holds one after the other what its loads wrote, 16-bit results and rows of them: its numbers are read by
 // types that may alias all of those, so that no read moves past a write of another type to the same bytes.
 typedef float lds_float __attribute__((may_alias));
 typedef int lds_int __attribute__((may_alias));
-#define LDS_AS __attribute__((address_space(3)))
 
 // One operand's tile of R rows (m or n) x BK k in LDS, filled by loads that write LDS directly (16 bytes a lane, 1 KB a
 // wave in lane order), so any reordering against bank conflicts is in which global chunk a lane asks for.
@@ -44,30 +42,6 @@ struct Tile {
     }
   }
 };
-
-// make_rsrc's words, in scalar registers
-__device__ __forceinline__ i32x4_t rsrc_words(const void* p, long long bytes) {
-  const uint64_t at = (uint64_t)(uintptr_t)p;
-  const int n = bytes > 0x7fffffffLL ? 0x7fffffff : bytes < 0 ? 0 : (int)bytes;
-  return i32x4_t{__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
-                 __builtin_amdgcn_readfirstlane(n), 0x00020000};
-}
-// 16 bytes a lane from the buffer to LDS at `lds` (wave-uniform) + 16 lane; lanes beyond the buffer write zeros. Not the
-// builtin: with it the compiler waits for every such load before any LDS read. The waits are load_wait's.
-__device__ __forceinline__ void load_lds(i32x4_t rs, int voff, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds)
-               : "memory");
-}
-// the same with 4 bytes a lane
-__device__ __forceinline__ void load_lds4(i32x4_t rs, int voff, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds)
-               : "memory");
-}
-// all but the newest N loads into LDS of this wave have arrived, its LDS reads are done, and so for the whole workgroup
-template <int N>
-__device__ __forceinline__ void load_wait() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
 
 }  // namespace
 
