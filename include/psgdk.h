@@ -433,6 +433,67 @@ typedef struct psgdk_window_attention_grads {
 int psgdk_window_attention_backward(const psgdk_window_attention_t* a, const psgdk_window_attention_grads_t* g, void* ws,
                                     size_t* ws_bytes, psgdk_stream_t stream);
 
+/* Queries and keys of each head normalised, weighted and rotated by their position:
+ *   u = N(x) * w  (PSGDK_NORM_* over the head's d, no bias; w NULL: 1; NONE: u = x),   y = R(p) u:
+ * pair i of the first rotary_dim elements, (i, i + rotary_dim / 2) or interleaved (2 i, 2 i + 1), becomes
+ * (a cos t - b sin t, b cos t + a sin t) with t = p theta^(-2 i / rotary_dim) for position p; the others stay. The angle is kept
+ * as a 64-bit fraction of a turn, so that far positions lose nothing. positions NULL: a token's index in its sequence. */
+typedef struct psgdk_qk_norm_rope {
+  int64_t batch, n;           /* batch * n up to 2^30 */
+  int32_t heads, kv_heads;    /* kv_heads 0: no keys */
+  int32_t d, rotary_dim;      /* even, d up to 512 */
+  int32_t dtype, w_dtype;     /* of q, k and their gradients; of the weights and theirs */
+  int32_t norm, interleaved;
+  float eps;
+  double theta;               /* at least 1 */
+  const int64_t* positions;   /* device memory, sequence b's n at positions + b * positions_stride */
+  int64_t positions_stride;
+  psgdk_heads_t q, k;         /* any alignment of whole elements */
+  const void *q_w, *k_w;      /* d of them */
+} psgdk_qk_norm_rope_t;
+/* outputs qo (batch, n, heads, d) and ko (batch, n, kv_heads, d), contiguous */
+int psgdk_qk_norm_rope(const psgdk_qk_norm_rope_t* a, void* qo, void* ko, psgdk_stream_t stream);
+
+/* Gradients of q, k (contiguous) and of the weights from those of qo and ko (p NULL: zero); NULL outputs are not computed. Sums
+ * over tokens and heads are added in a fixed order. */
+typedef struct psgdk_qk_norm_rope_grads {
+  psgdk_heads_t dqo, dko;
+  void *dq, *dk, *dqw, *dkw;
+} psgdk_qk_norm_rope_grads_t;
+int psgdk_qk_norm_rope_backward(const psgdk_qk_norm_rope_t* a, const psgdk_qk_norm_rope_grads_t* g, void* ws, size_t* ws_bytes,
+                                psgdk_stream_t stream);
+
+/* One AdamW step over nb tensors (any number; host arrays of device pointers), elements stored one after the other:
+ *   g = c gradient, c = min(1, max_norm / norm of all gradients) (max_norm 0: 1)
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ * Parameters and gradients in dtype[t]; arithmetic in fp32, squares of the norm in fp64, parameters rounded to nearest.
+ * bits 32: m and v are fp32. bits 8: m holds e4m3 codes of the first moment and v those of the second's root, each with one
+ * scale byte for 256 elements (m_scale, v_scale: ceil(n / 256) bytes a tensor; value 2^(byte - 127), byte 0 with codes 0: zeros,
+ * 255: NaN). The scale puts a block's largest magnitude into e4m3's top binade; a magnitude is rounded to one of the codes
+ * around it by chance, so that its expected value is its own: element i of tensor t takes the 16-bit number i % 8 (low half of a
+ * word first) of block i / 8 of Philox4x32-10 (key seed; upper counter words step, t), and the magnitude's bits below the code
+ * plus 16 times that number carry or not. A root that is not 0 gets no code 0. Zeroed codes and scales are zero states.
+ * p NULL: nothing but the norm. Tensors may begin anywhere (whole elements). norm: optional, one float in device memory.
+ * Two runs with the same inputs give the same bits. */
+typedef struct psgdk_adamw {
+  int64_t nb;
+  int32_t bits;             /* of the states: 8 or 32 */
+  const int64_t* n;         /* elements */
+  const int32_t* dtype;     /* of p and g */
+  void* const* p;
+  const void* const* g;
+  void* const* m;
+  void* const* v;
+  void* const* m_scale;     /* 8 bits only */
+  void* const* v_scale;
+  double lr, beta1, beta2, eps, weight_decay, max_norm;
+  int64_t step;             /* from 1 */
+  uint64_t seed;
+  float* norm;
+} psgdk_adamw_t;
+int psgdk_adamw(const psgdk_adamw_t* a, void* ws, size_t* ws_bytes, psgdk_stream_t stream);
+
 /* Launch profiling (diagnostic, per host thread): after psgdk_profile_start every MFMA-engine launch the thread makes is
  * bracketed by a pair of HIP events on its stream. psgdk_profile_stop ends the recording and, with out non-NULL,
  * waits for the recorded events and fills one record per launch: the kernel instantiation id

@@ -7,10 +7,11 @@ HipOps is the drop-in for its arithmetic plugin (kernels/ops.py make_ops). linea
 dropout are operators of the training step in front of the optimizer. All run on libpsgdk.so, built with
 `python -m psgd_pro_amd.build`.
 """
-from .attention import window_attention
+from .adamw import AdamW, adamw_state, adamw_step
+from .attention import qk_norm_rope, window_attention
 from .kron import KronWhiten
 from .ops import EagerOps, HipOps, make_ops
 from .train import dropout, linear_cross_entropy, residual_norm
 
-__all__ = ["KronWhiten", "EagerOps", "HipOps", "make_ops", "dropout", "linear_cross_entropy", "residual_norm",
-           "window_attention"]
+__all__ = ["KronWhiten", "EagerOps", "HipOps", "make_ops", "AdamW", "adamw_state", "adamw_step", "dropout",
+           "linear_cross_entropy", "qk_norm_rope", "residual_norm", "window_attention"]

@@ -91,6 +91,29 @@ class WindowAttentionGrads(C.Structure):
     _fields_ = [("dout", Heads), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p)]
 
 
+class QkNormRope(C.Structure):
+    """psgdk_qk_norm_rope_t"""
+    _fields_ = [("batch", C.c_int64), ("n", C.c_int64), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("d", C.c_int32),
+                ("rotary_dim", C.c_int32), ("dtype", C.c_int32), ("w_dtype", C.c_int32), ("norm", C.c_int32),
+                ("interleaved", C.c_int32), ("eps", C.c_float), ("theta", C.c_double), ("positions", C.c_void_p),
+                ("positions_stride", C.c_int64), ("q", Heads), ("k", Heads), ("q_w", C.c_void_p), ("k_w", C.c_void_p)]
+
+
+class QkNormRopeGrads(C.Structure):
+    """psgdk_qk_norm_rope_grads_t"""
+    _fields_ = [("dqo", Heads), ("dko", Heads), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dqw", C.c_void_p),
+                ("dkw", C.c_void_p)]
+
+
+class AdamW(C.Structure):
+    """psgdk_adamw_t"""
+    _fields_ = [("nb", C.c_int64), ("bits", C.c_int32), ("n", C.c_void_p), ("dtype", C.c_void_p), ("p", C.c_void_p),
+                ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("max_norm", C.c_double), ("step", C.c_int64), ("seed", C.c_uint64),
+                ("norm", C.c_void_p)]
+
+
 class ProfRecord(C.Structure):
     _fields_ = [("kernel_id", C.c_int32), ("tri", C.c_int32), ("nb", C.c_int32), ("ms", C.c_float),
                 ("flops", C.c_double), ("bytes", C.c_double), ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
@@ -148,6 +171,9 @@ _SIGS = {
     "psgdk_scale_by": (_i32, [_i32, C.POINTER(C.c_int64), _i32, _vpa, _vp, _vp]),
     "psgdk_window_attention": (_i32, [C.POINTER(WindowAttention), _vp, _szp, _vp]),
     "psgdk_window_attention_backward": (_i32, [C.POINTER(WindowAttention), C.POINTER(WindowAttentionGrads), _vp, _szp, _vp]),
+    "psgdk_qk_norm_rope": (_i32, [C.POINTER(QkNormRope), _vp, _vp, _vp]),
+    "psgdk_qk_norm_rope_backward": (_i32, [C.POINTER(QkNormRope), C.POINTER(QkNormRopeGrads), _vp, _szp, _vp]),
+    "psgdk_adamw": (_i32, [C.POINTER(AdamW), _vp, _szp, _vp]),
     "psgdk_set_option": (_i32, [_i32, _i32]),
     "psgdk_get_option": (_i32, [_i32, C.POINTER(C.c_int)]),
     "psgdk_profile_start": (_i32, []),

@@ -1,5 +1,6 @@
 """Attention of a transformer's block on the HIP kernels (include/psgdk.h, level 3).
 
+    qk_norm_rope       norms of queries and keys for each head and their rotation by position, one pass
     window_attention   softmax attention with grouped heads, a sliding window and first tokens that stay visible
 
 CUDA (HIP) tensors in float32 or bfloat16, on torch's current stream, differentiable once through autograd. No counterparts in
@@ -11,9 +12,9 @@ import math
 import torch
 
 from . import _lib as L
-from .train import _check, _once, _ptr, _run_ws, _wants_grad
+from .train import _NORMS, _check, _once, _ptr, _run, _run_ws, _wants_grad
 
-__all__ = ["window_attention"]
+__all__ = ["qk_norm_rope", "window_attention"]
 
 _MAX_STRIDE = 1 << 21  # of tokens and heads, in elements
 
@@ -121,3 +122,121 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, lengths=None,
     if _wants_grad(q, k, v):
         return _WindowAttention.apply(q, k, v, *tell, opt)
     return _attn_forward(q, k, v, *tell, opt, False)[0]
+
+
+# -- qk_norm_rope -----------------------------------------------------------------------------------------------------------
+
+
+def _dense(t):
+    """(psgdk_heads_t of t, the tensor it points to): any strides, a head's elements one after the other."""
+    if t.stride(3) != 1 and t.shape[3] > 1:
+        t = t.contiguous()
+    return L.Heads(t.data_ptr(), *t.stride()[:3]), t
+
+
+def _rope_block(q, k, qw, kw, pos, opt):
+    """psgdk_qk_norm_rope_t of the inputs, and the (possibly copied) tensors it points to."""
+    norm, eps, theta, rot, interleaved = opt
+    w = [t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(memory_format=torch.contiguous_format)
+         for t in (qw, kw)]
+    some = qw if qw is not None else kw
+    a = L.QkNormRope(q.shape[0], q.shape[1], q.shape[2], 0 if k is None else k.shape[2], q.shape[3], rot, L.dtype_code(q.dtype),
+                     L.F32 if some is None else L.dtype_code(some.dtype), norm, interleaved, eps, theta, _ptr(pos),
+                     0 if pos is None or pos.dim() == 1 else pos.shape[1])
+    a.q, q = _dense(q)
+    if k is not None:
+        a.k, k = _dense(k)
+    a.q_w, a.k_w = (_ptr(t) for t in w)
+    return a, (q, k, w)
+
+
+def _rope_forward(q, k, qw, kw, pos, opt):
+    a, keep = _rope_block(q, k, qw, kw, pos, opt)
+    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    ko = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    if qo.numel():
+        _run(q, L.lib().psgdk_qk_norm_rope, C.byref(a), qo.data_ptr(), _ptr(ko))
+    return qo, ko
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, pos, opt):
+        ctx.set_materialize_grads(False)
+        ctx.opt = opt
+        ctx.save_for_backward(q, k, qw, kw, pos)
+        return _rope_forward(q, k, qw, kw, pos, opt)
+
+    @staticmethod
+    def backward(ctx, dqo, dko):
+        _once()
+        q, k, qw, kw, pos = ctx.saved_tensors
+        outs = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if t is not None and need else None
+                for t, need in zip((q, k, qw, kw), ctx.needs_input_grad)]
+        if not q.numel():
+            for t in outs:
+                if t is not None:
+                    t.zero_()
+            return (*outs, None, None)
+        a, keep = _rope_block(q, k, qw, kw, pos, ctx.opt)
+        g = L.QkNormRopeGrads()
+        if dqo is not None:
+            g.dqo, dqo = _dense(dqo)
+        if dko is not None:
+            g.dko, dko = _dense(dko)
+        g.dq, g.dk, g.dqw, g.dkw = (_ptr(t) for t in outs)
+        _run_ws(q, L.lib().psgdk_qk_norm_rope_backward, C.byref(a), C.byref(g))
+        return (*outs, None, None)
+
+
+def qk_norm_rope(q, k=None, *, norm="rms", q_weight=None, k_weight=None, eps=1e-6, positions=None, theta=10000.0,
+                 rotary_dim=None, interleaved=False):
+    """(q', k'): queries q (batch, n, heads, d) and keys k (batch, n, kv_heads, d; None: k' is None) normalised over each head's
+    d, times their weights (d,), and rotated by their tokens' positions, in one pass.
+
+        u = N(x) * w;  pair (a, b) of u becomes (a cos t - b sin t, b cos t + a sin t),  t = p theta^(-2 i / rotary_dim)
+
+    norm: "rms" (v / sqrt(mean v^2 + eps)), "layer" ((v - mean) / sqrt(var + eps)) or None (no weights then); weights may be
+    absent and may be float32 beside bfloat16 inputs. Pair i of the first rotary_dim elements (d if not given; even) is
+    (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved; the elements behind are not rotated. positions: int64 (n,) or
+    (batch, n); a token's index in its sequence if not given. Angles are exact to float32's rounding at any position. d is even
+    and up to 512, q and k may have any strides; q' and k' are contiguous. Differentiable in q, k and the weights."""
+    if norm not in _NORMS:
+        raise ValueError(f"norm = {norm!r}: 'rms', 'layer' or None")
+    _check(q, "q")
+    for name, t in (("q", q), ("k", k)):
+        if t is None:
+            continue
+        _check(t, name, q)
+        if t.dim() != 4 or t.dtype != q.dtype or t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3]:
+            raise RuntimeError(f"{name}: (batch, n, heads, d) in {q.dtype} expected, batch, n and d as q's, got {tuple(t.shape)} in "
+                               f"{t.dtype}")
+        if not t.shape[2]:
+            raise RuntimeError(f"{name}: at least one head expected")
+    d = q.shape[3]
+    if not 2 <= d <= 512 or d % 2:
+        raise RuntimeError(f"d = {d}: even and up to 512 expected")
+    for name, t, of in (("q_weight", q_weight, q), ("k_weight", k_weight, k)):
+        if t is None:
+            continue
+        _check(t, name, q)
+        if norm is None or of is None:
+            raise ValueError(f"{name}: " + ("the norm None has none" if norm is None else "needs k"))
+        if t.shape != (d,) or (q_weight is not None and t.dtype != q_weight.dtype):
+            raise RuntimeError(f"{name}: shape ({d},) expected, and one dtype for both weights; got {tuple(t.shape)} in {t.dtype}")
+    rot = d if rotary_dim is None else int(rotary_dim)
+    if not 0 <= rot <= d or rot % 2:
+        raise ValueError(f"rotary_dim = {rotary_dim}: even and in 0..{d}")
+    if not (theta >= 1 and math.isfinite(theta)):
+        raise ValueError(f"theta = {theta}: must be at least 1")
+    if not eps >= 0:
+        raise ValueError(f"eps = {eps}: must be >= 0")
+    if positions is not None:
+        if (not isinstance(positions, torch.Tensor) or positions.dtype != torch.int64 or positions.device != q.device
+                or tuple(positions.shape) not in (tuple(q.shape[1:2]), tuple(q.shape[:2]))):
+            raise RuntimeError(f"positions: an int64 tensor ({q.shape[1]},) or ({q.shape[0]}, {q.shape[1]}) on {q.device} expected")
+        positions = positions.contiguous()
+    opt = (_NORMS[norm], float(eps), float(theta), rot, int(bool(interleaved)))
+    if _wants_grad(q, k, q_weight, k_weight):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, positions, opt)
+    return _rope_forward(q, k, q_weight, k_weight, positions, opt)

@@ -22,8 +22,9 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpsgdk.so")
 SOURCES = ["gemm_cv.hip", "gemm_bf16.hip", "gemm_small.hip", "nlb.hip", "elem.hip", "block.hip", "xent.hip", "xgemm.hip",
-           "attn_fwd.hip", "attn_bwd.hip", "capi.cpp", "train_capi.cpp", "attn_capi.cpp", "noalloc.hip", "measure.hip"]
-HOST_SOURCES = ["capi.cpp", "train_capi.cpp", "attn_capi.cpp"]  # the C ABI's host code, which the sanitizer build instruments
+           "attn_fwd.hip", "attn_bwd.hip", "rope.hip", "adamw.hip", "capi.cpp", "train_capi.cpp", "attn_capi.cpp", "adamw_capi.cpp",
+           "noalloc.hip", "measure.hip"]
+HOST_SOURCES = ["capi.cpp", "train_capi.cpp", "attn_capi.cpp", "adamw_capi.cpp"]  # the C ABI's host code, which the sanitizer build instruments
 ARCH = os.environ.get("PSGDK_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 

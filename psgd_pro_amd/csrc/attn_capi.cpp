@@ -1,10 +1,11 @@
-// The C ABI of attention (include/psgdk.h, level 3): argument validation, workspace layout and launches. Host code only; every
+// The C ABI of attention and of the norms and rotation in front of it (include/psgdk.h, level 3): argument validation, workspace layout and launches. Host code only; every
 // launch goes to the caller's stream, nothing synchronizes.
 #include <algorithm>
 #include <cmath>
 
 #include "attn.h"
 #include "capi_util.h"
+#include "rope.h"
 
 using namespace psgdk;
 
@@ -83,9 +84,125 @@ int attn_pointers(const psgdk_window_attention_t* q, AttnArgs& a) {
   return PSGDK_OK;
 }
 
+// the argument checks and the kernels' argument block of both calls; `aligned` says for which vectors base and strides are
+struct Aligned {
+  bool by16 = true, by8 = true;
+  void add(const void* p, const int64_t (&s)[3], size_t e) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p) | s[0] * e | s[1] * e | s[2] * e;
+    by16 = by16 && !(all & 15);
+    by8 = by8 && !(all & 7);
+  }
+};
+RopeSide rope_side(const psgdk_heads_t& t, int64_t batch, int64_t tokens, int64_t heads, int dt, Aligned& al) {
+  const int64_t s[3] = {batch > 1 ? t.batch_stride : 0, tokens > 1 ? t.token_stride : 0, heads > 1 ? t.head_stride : 0};
+  if (t.p) al.add(t.p, s, esize(dt));
+  return RopeSide{t.p, s[0], s[1], s[2]};
+}
+int rope_args(const psgdk_qk_norm_rope_t* q, RopeArgs& a, Aligned& al) {
+  if (!q) return fail(PSGDK_EINVAL, "null argument block");
+  PSGDK_TRY(check_dt(q->dtype, "dtype"));
+  PSGDK_TRY(check_size(q->batch, 1, (int64_t)1 << 30, "batch"));
+  PSGDK_TRY(check_size(q->n, 1, (int64_t)1 << 30, "n"));
+  PSGDK_TRY(check_size(q->batch * q->n, 1, (int64_t)1 << 30, "batch * n"));
+  PSGDK_TRY(check_size(q->heads, 1, 1 << 16, "heads"));
+  PSGDK_TRY(check_size(q->kv_heads, 0, 1 << 16, "kv_heads"));
+  PSGDK_TRY(check_size(q->d, 2, kRopeMaxD, "d"));
+  PSGDK_TRY(check_size(q->rotary_dim, 0, q->d, "rotary_dim"));
+  if (q->d % 2 || q->rotary_dim % 2) return fail(PSGDK_ESHAPE, "d = %d, rotary_dim = %d: must be even", q->d, q->rotary_dim);
+  if (q->norm < PSGDK_NORM_NONE || q->norm > PSGDK_NORM_LAYER) return fail(PSGDK_EINVAL, "norm = %d", q->norm);
+  if (!(q->eps >= 0.f)) return fail(PSGDK_EINVAL, "eps = %g: must be >= 0", (double)q->eps);
+  if (!(q->theta >= 1.0 && std::isfinite(q->theta))) return fail(PSGDK_EINVAL, "theta = %g: must be at least 1", q->theta);
+  if (q->norm == PSGDK_NORM_NONE && (q->q_w || q->k_w)) return fail(PSGDK_EINVAL, "weight of a norm that has none");
+  if (q->q_w || q->k_w) PSGDK_TRY(check_dt(q->w_dtype, "w_dtype"));
+  if (!q->q.p || (q->kv_heads && !q->k.p)) return fail(PSGDK_EINVAL, "q, k: null device pointer");
+  if (!q->kv_heads && q->k_w) return fail(PSGDK_EINVAL, "k_w needs keys");
+  a = RopeArgs{};
+  a.tokens = q->batch * q->n;
+  a.n = (int)q->n;
+  a.heads = q->heads;
+  a.all = q->heads + q->kv_heads;
+  a.d = q->d;
+  a.rot = q->rotary_dim;
+  a.dt = q->dtype;
+  a.norm = q->norm;
+  a.eps = q->eps;
+  a.pos = q->positions;
+  a.pos_sb = q->positions_stride;
+  double p = q->rotary_dim ? std::pow(q->theta, -2.0 / q->rotary_dim) : 1.0;
+  for (int k = 0; k < kRopePowers; ++k, p *= p) a.ratio[k] = p;
+  a.interleaved = q->interleaved != 0;
+  a.x[0] = rope_side(q->q, q->batch, q->n, q->heads, a.dt, al);
+  if (q->kv_heads) a.x[1] = rope_side(q->k, q->batch, q->n, q->kv_heads, a.dt, al);
+  a.w[0] = Vec{q->q_w, q->w_dtype};
+  a.w[1] = Vec{q->k_w, q->w_dtype};
+  const int64_t none[3] = {0, 0, 0};
+  for (const void* w : {q->q_w, q->k_w})
+    if (w) al.add(w, none, 1);
+  return PSGDK_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int psgdk_qk_norm_rope(const psgdk_qk_norm_rope_t* q, void* qo, void* ko, psgdk_stream_t stream) {
+  RopeArgs a;
+  Aligned al;
+  PSGDK_TRY(rope_args(q, a, al));
+  if (!qo || (q->kv_heads && !ko)) return fail(PSGDK_EINVAL, "qo, ko: null device pointer");
+  a.y[0] = qo;
+  a.y[1] = ko;
+  const int64_t none[3] = {0, 0, 0};
+  for (const void* p : {qo, ko})
+    if (p) al.add(p, none, 1);
+  rope_plan(a, al.by16, al.by8);
+  return hip_check(rope_launch(a, false, (hipStream_t)stream), "qk_norm_rope");
+}
+
+int psgdk_qk_norm_rope_backward(const psgdk_qk_norm_rope_t* q, const psgdk_qk_norm_rope_grads_t* g, void* ws, size_t* ws_bytes,
+                                psgdk_stream_t stream) {
+  RopeArgs a;
+  Aligned al;
+  PSGDK_TRY(rope_args(q, a, al));
+  if (!g) return fail(PSGDK_EINVAL, "null gradient block");
+  if (!ws_bytes) return fail(PSGDK_EINVAL, "ws_bytes is null");
+  if ((g->dqw && !q->q_w) || (g->dkw && !q->k_w)) return fail(PSGDK_EINVAL, "gradient of a weight that is absent");
+  if (g->dk && !q->kv_heads) return fail(PSGDK_EINVAL, "gradient of keys that are absent");
+  a.dy[0] = rope_side(g->dqo, q->batch, q->n, q->heads, a.dt, al);
+  if (q->kv_heads) a.dy[1] = rope_side(g->dko, q->batch, q->n, q->kv_heads, a.dt, al);
+  a.dx[0] = g->dq;
+  a.dx[1] = g->dk;
+  const int64_t none[3] = {0, 0, 0};
+  for (const void* p : {g->dq, g->dk})
+    if (p) al.add(p, none, 1);
+  rope_plan(a, al.by16, al.by8);
+  const bool sums = g->dqw || g->dkw;
+  Ws m(ws);
+  // (room for the most parts there are, whatever the pointers' alignment)
+  if (sums) a.part = m.take<float>((size_t)2 * kRopeParts * a.d);
+  if (!ws) {
+    *ws_bytes = m.off;
+    return PSGDK_OK;
+  }
+  if (*ws_bytes < m.off) return fail(PSGDK_EWORKSPACE, "workspace %zu < %zu bytes", *ws_bytes, m.off);
+  if (!g->dq && !g->dk && !sums) return PSGDK_OK;
+  PSGDK_TRY(hip_check(rope_launch(a, true, (hipStream_t)stream), "qk_norm_rope backward"));
+  if (!sums) return PSGDK_OK;
+  ColumnSums s{};
+  s.d = a.d;
+  void* const out[2] = {g->dqw, g->dkw};
+  for (int k = 0; k < 2; ++k) {
+    if (!out[k]) continue;
+    auto& e = s.e[s.n++];
+    e.in = a.part + (size_t)k * a.parts * a.d;
+    e.out = out[k];
+    e.dt = q->w_dtype;
+    e.groups = 1;
+    e.per = a.parts;
+    e.ldo = a.d;
+  }
+  return hip_check(column_sums_launch(s, (hipStream_t)stream), "column sums");
+}
 
 int psgdk_window_attention(const psgdk_window_attention_t* q, void* ws, size_t* ws_bytes, psgdk_stream_t stream) {
   AttnArgs a;
