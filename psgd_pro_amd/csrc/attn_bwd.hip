@@ -14,6 +14,7 @@ template <typename T, int DP, int BK>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_dq_kernel(const AttnArgs a, int row_tiles) {
   using R = Rows<T, DP>;
   constexpr int LOADS = R::loads(BK, 4), TILE = BK * R::PITCH, KT = BK / 32, DC = DP / 16, DT = DP / 32;
+  constexpr int AHEAD = sizeof(T) == 2 && DT > 1 ? 4 : 2;  // at most 2 DT
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -46,7 +47,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_d
   const long long at = (long long)pair * a.rows + r;
   if (there && h == 0) a.delta[at] = delta;
   if (!a.dq) return;
-  const float lse = there ? a.lse[at] : 0.f;
+  float lse = there ? a.lse[at] : 0.f;
+  arrived(lse);
+#pragma unroll
+  for (int i = 0; i < DC; ++i) {
+    arrived(qf[i]);
+    arrived(gf[i]);
+  }
 
   int vk[LOADS], vv[LOADS], lrow[LOADS];
 #pragma unroll
@@ -80,32 +87,41 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_d
     const int j0 = tiles.tile(t) * BK;
     load_wait<0>();
     if (t + 1 < tiles.count) load(t + 1);
-    const unsigned kt = lds0 + (t & 1) * 2 * TILE, vt = kt + TILE;
+    const unsigned kt = lds0 + (t & 1) * 2 * TILE;
+    const Straight<T, DP> keys(kt, lane), values(kt + TILE, lane);
+    const Transposed<T, DP> columns(kt, lane);
     const bool look = j0 + BK - 1 > lo || hi >= s.len || (hi - j0 >= a.window && j0 + BK > a.sinks);
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
       f32x16_t x = zero16(), dp = zero16();
-#pragma unroll
-      for (int k = 0; k < DC; ++k) {
-        x = mma(R::straight(kt, 32 * i + c, k, h), qf[k], x);
-        dp = mma(R::straight(vt, 32 * i + c, k, h), gf[k], dp);
-      }
+      frag_t<T> f[AHEAD];
+      const auto row_frags = [&](int s) __attribute__((always_inline)) { return s % 2 ? values(i, s / 2) : keys(i, s / 2); };
+      first_loads<T>(f, row_frags);
+      __builtin_amdgcn_s_setprio(1);
+      ahead<T, 2 * DC>(f, row_frags, [&](int s, frag_t<T> y) __attribute__((always_inline)) {
+        if (s % 2) dp = mma(y, gf[s / 2], dp);
+        else x = mma(y, qf[s / 2], x);
+      });
+      __builtin_amdgcn_s_setprio(0);
+      const auto key_frags = [&](int s) __attribute__((always_inline)) { return columns(2 * i + s / DT, s % DT); };
+      first_loads<T>(f, key_frags);
       if (look) {
         const int j = j0 + 32 * i + 4 * h;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int key = j + 8 * (e >> 2) + (e & 3);
-          if (!(key <= pos && (pos - key < a.window || key < a.sinks))) x[e] = -INFINITY;
+          x[e] = (key <= pos) & ((pos - key < a.window) | (key < a.sinks)) ? x[e] : -INFINITY;
         }
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse)) * (dp[e] - delta);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const frag_t<T> ds = crossed<T>(x, u);
-#pragma unroll
-        for (int k = 0; k < DT; ++k) dq[k] = mma(R::transposed(kt, 32 * i + 16 * u, k, lane), ds, dq[k]);
-      }
+      const frag_t<T> ds[2] = {crossed<T>(x, 0), crossed<T>(x, 1)};
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      ahead<T, 2 * DT>(f, key_frags, [&](int s, frag_t<T> y) __attribute__((always_inline)) {
+        dq[s % DT] = mma(y, ds[s / DT], dq[s % DT]);
+      });
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   if (!there) return;
@@ -136,7 +152,8 @@ __device__ __forceinline__ void store4(T* out, float y0, float y1, float y2, flo
 template <typename T, int DP, int BR>
 __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) attn_dkv_kernel(const AttnArgs a, int key_tiles) {
   using R = Rows<T, DP>;
-  constexpr int LOADS = R::loads(BR, 4), TILE = BR * R::PITCH, STAGE = 2 * TILE + 512, RT = BR / 32, DC = DP / 16, DT = DP / 32;
+  constexpr int LOADS = R::loads(BR, 4), TILE = BR * R::PITCH, STAGE = 2 * TILE + 1024, RT = BR / 32, DC = DP / 16, DT = DP / 32;
+  constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2;  // at most 4 DT
   static_assert(BR <= 64, "a load of 64 floats");
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
@@ -165,6 +182,11 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
   for (int i = 0; i < DC; ++i) {
     kf[i] = row_frag<T>(kp, 16 * i + 8 * h, a.d, key < s.len);
     vf[i] = row_frag<T>(vp, 16 * i + 8 * h, a.d, key < s.len);
+  }
+#pragma unroll
+  for (int i = 0; i < DC; ++i) {
+    arrived(kf[i]);
+    arrived(vf[i]);
   }
 
   const T* const qp = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)head * a.group * a.q.sh;
@@ -196,28 +218,39 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
     load_wait<0>();
     if (t + 1 < t1) load(t + 1);
     const unsigned qt = lds0 + (t & 1) * STAGE, gt = qt + TILE, st = gt + TILE;
+    const Straight<T, DP> queries(qt, lane), grads(gt, lane);
+    const Transposed<T, DP> query_cols(qt, lane), grad_cols(gt, lane);
     const int r0 = (first + t) * BR, lo = s.start + row_token(a, r0), hi = s.start + row_token(a, r0 + BR - 1);
     const bool look = lo < j0 + kAttnKeys - 1 || hi >= s.len || hi >= s.start + a.n ||
                       (hi - j0 >= a.window && j0 + kAttnKeys > a.sinks);
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       f32x16_t x = zero16(), dp = zero16();
-#pragma unroll
-      for (int k = 0; k < DC; ++k) {
-        x = mma(R::straight(qt, 32 * i + c, k, h), kf[k], x);
-        dp = mma(R::straight(gt, 32 * i + c, k, h), vf[k], dp);
-      }
+      frag_t<T> f[AHEAD];
+      const auto row_frags = [&](int s) __attribute__((always_inline)) { return s % 2 ? grads(i, s / 2) : queries(i, s / 2); };
+      first_loads<T>(f, row_frags);
+      __builtin_amdgcn_s_setprio(1);
+      ahead<T, 2 * DC>(f, row_frags, [&](int s, frag_t<T> y) __attribute__((always_inline)) {
+        if (s % 2) dp = mma(y, vf[s / 2], dp);
+        else x = mma(y, kf[s / 2], x);
+      });
       f32x4_t lse[4], delta[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         lse[e] = *(LDS_AS f32x4_t*)(uintptr_t)(st + (32 * i + 8 * e + 4 * h) * 4);
         delta[e] = *(LDS_AS f32x4_t*)(uintptr_t)(st + 256 + (32 * i + 8 * e + 4 * h) * 4);
       }
+      __builtin_amdgcn_s_setprio(0);
+      // 16 rows' dO, then their Q, then the next 16 rows'
+      const auto col_frags = [&](int s) __attribute__((always_inline)) {
+        return s / DT % 2 ? query_cols(2 * i + s / (2 * DT), s % DT) : grad_cols(2 * i + s / (2 * DT), s % DT);
+      };
+      first_loads<T>(f, col_frags);
       if (look) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int tok = row_token(a, r0 + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3)), pos = s.start + tok;
-          if (!(tok < to && key <= pos && (pos - key < a.window || key < a.sinks))) x[e] = -INFINITY;
+          x[e] = (tok < to) & (key <= pos) & ((pos - key < a.window) | (key < a.sinks)) ? x[e] : -INFINITY;
         }
       }
 #pragma unroll
@@ -225,15 +258,14 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
         x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse[e >> 2][e & 3]));
         dp[e] = x[e] * (dp[e] - delta[e >> 2][e & 3]);
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const frag_t<T> p = crossed<T>(x, u), ds = crossed<T>(dp, u);
-#pragma unroll
-        for (int k = 0; k < DT; ++k) {
-          dv[k] = mma(R::transposed(gt, 32 * i + 16 * u, k, lane), p, dv[k]);
-          dk[k] = mma(R::transposed(qt, 32 * i + 16 * u, k, lane), ds, dk[k]);
-        }
-      }
+      const frag_t<T> p[2] = {crossed<T>(x, 0), crossed<T>(x, 1)}, ds[2] = {crossed<T>(dp, 0), crossed<T>(dp, 1)};
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      ahead<T, 4 * DT>(f, col_frags, [&](int s, frag_t<T> y) __attribute__((always_inline)) {
+        if (s / DT % 2) dk[s % DT] = mma(y, ds[s / (2 * DT)], dk[s % DT]);
+        else dv[s % DT] = mma(y, p[s / (2 * DT)], dv[s % DT]);
+      });
+      __builtin_amdgcn_s_setprio(0);
     }
   }
 
@@ -305,7 +337,7 @@ hipError_t launch_dq(const AttnArgs& a, hipStream_t st) {
 }
 template <typename T, int DP>
 hipError_t launch_dkv(const AttnArgs& a, hipStream_t st) {
-  constexpr int BR = kTileRows<T>, smem = 2 * (2 * BR * Rows<T, DP>::PITCH + 512);
+  constexpr int BR = kTileRows<T>, smem = 2 * (2 * BR * Rows<T, DP>::PITCH + 1024);
   const auto fn = attn_dkv_kernel<T, DP, BR>;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (attr != hipSuccess) return attr;

@@ -48,6 +48,20 @@ __device__ __forceinline__ frag_t<T> crossed(const f32x16_t& c, int u) {
   }
 }
 
+// sum + the 8 values
+__device__ __forceinline__ float sum_of(bf16x8_t f, float sum) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{f[2 * i], f[2 * i + 1]}, one, sum, false);
+  return sum;
+}
+__device__ __forceinline__ float sum_of(Frag<float>::type f, float sum) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += f[i];
+  return sum;
+}
+
 // R rows of DP elements in LDS, each row's 16-byte chunks XORed by a function of the row. With bf16: the 16 rows of a quarter
 // wave's fragment read lie in 16 different 16-byte bank groups, and so do the 4 rows x 64 bytes of half a transposed read
 // (its low two bits from row / 4, the others, which choose among a 64-byte block's places, from row % 4). With fp32 the same
@@ -72,41 +86,88 @@ struct Rows {
     row = c / CPR;
     chunk = (c % CPR) ^ swz(row);
   }
-  // k along the row: row `row` (already this lane's), k = 16 c + 8 h ..
-  static __device__ __forceinline__ frag_t<T> straight(unsigned base, int row, int c, int h) {
-    if constexpr (E == 2) {
-      return *(LDS_AS frag_t<T>*)(uintptr_t)(base + at(row, 2 * c + h));
+};
+
+// Fragments of Rows tiles: a tile's address with the lane's part once, then constants. What the swizzle lets pass as an XOR of
+// the address where rows are a power of two long (tiles begin at multiples of 1024) is one there; else the chunk's upper bits,
+// which the swizzle leaves alone, are added.
+// k along the row: row 32 block + lane % 32, k = 16 c + 8 h ..
+template <typename T, int DP>
+struct Straight {
+  using R = Rows<T, DP>;
+  unsigned at;
+  __device__ __forceinline__ Straight(unsigned base, int lane)
+      : at(base + (lane & 31) * R::PITCH + (((R::E == 2 ? 1 : 2) * (lane >> 5) ^ R::swz(lane & 31)) << 4)) {}
+  __device__ __forceinline__ frag_t<T> operator()(int block, int c) const {
+    constexpr bool POW2 = (DP & (DP - 1)) == 0;
+    if constexpr (R::E == 2) {
+      const unsigned p = POW2 ? at ^ c << 5 : (at ^ (c & 1) << 5) + (c >> 1) * 64;
+      return *(LDS_AS frag_t<T>*)(uintptr_t)(p + block * 32 * R::PITCH);
     } else {
-      const f32x4_t x = *(LDS_AS f32x4_t*)(uintptr_t)(base + at(row, 4 * c + 2 * h));
-      const f32x4_t y = *(LDS_AS f32x4_t*)(uintptr_t)(base + at(row, 4 * c + 2 * h + 1));
+      const unsigned p = POW2 ? at ^ c << 6 : (at ^ (c & 1) << 6) + (c >> 1) * 128, q = p + block * 32 * R::PITCH;
+      const f32x4_t x = *(LDS_AS f32x4_t*)(uintptr_t)q, y = *(LDS_AS f32x4_t*)(uintptr_t)(q ^ 16);
       return frag_t<T>{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     }
   }
-  // k along the column: column 32 t + lane % 32, rows r0 + 4 h .. and r0 + 8 + 4 h ..  (r0 a multiple of 16)
-  static __device__ __forceinline__ frag_t<T> transposed(unsigned base, int r0, int t, int lane) {
+};
+// k along the column: column 32 t + lane % 32, rows 16 u + 4 h .. and 16 u + 8 + 4 h ..
+template <typename T, int DP>
+struct Transposed {
+  using R = Rows<T, DP>;
+  unsigned at, sw;
+  __device__ __forceinline__ Transposed(unsigned base, int lane) {
     const int h = lane >> 5;
-    if constexpr (E == 2) {
+    if constexpr (R::E == 2) {
       // of 16 lanes lane i names the 8 bytes of row i / 4, columns 4 (i % 4) .., and receives column i of the 4 rows
-      const int i = lane & 15, col = 32 * t + (lane & 16) + 4 * (i & 3), row = r0 + 4 * h + (i >> 2);
+      const int i = lane & 15, row = 4 * h + (i >> 2);
+      at = base + row * R::PITCH + ((((lane >> 3 & 2) + (i >> 1 & 1)) ^ R::swz(row)) << 4) + (i & 1) * 8;
+    } else {
+      at = base + 4 * h * R::PITCH + (lane & 3) * 4;
+      sw = (lane >> 2 & 7) ^ R::swz(4 * h);
+    }
+  }
+  __device__ __forceinline__ frag_t<T> operator()(int u, int t) const {
+    constexpr bool XOR = DP == 64 || DP == 128;
+    if constexpr (R::E == 2) {
       union {
         s16x4_t v[2];
         frag_t<T> f;
-      } u;
+      } w;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        u.v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (LDS_AS s16x4_t*)(uintptr_t)(base + at(row + 8 * x, col >> 3) + (col & 4) * 2));
-      return u.f;
+      for (int x = 0; x < 2; ++x) {  // (8 rows on, row / 4 differs by 2)
+        const unsigned p = XOR ? at ^ (t << 6 | x << 5) : (at ^ x << 5) + t * 64;
+        w.v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4_t*)(uintptr_t)(p + (16 * u + 8 * x) * R::PITCH));
+      }
+      return w.f;
     } else {
-      const int col = 32 * t + (lane & 31);
       frag_t<T> f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        f[e] = *(LDS_AS float*)(uintptr_t)(base + at(r0 + (e & 4) * 2 + 4 * h + (e & 3), col >> 2) + (col & 3) * 4);
+      for (int e = 0; e < 8; ++e) {  // (the swizzle is linear: a row's is the XOR of its parts')
+        const int row = (e & 4) * 2 + (e & 3);
+        f[e] = *(LDS_AS float*)(uintptr_t)(at + (16 * u + row) * R::PITCH + ((sw ^ R::swz(row) ^ 8 * t) << 4));
+      }
       return f;
     }
   }
 };
+
+// N steps of load(i) and use(i, fragment), each load D steps ahead of its use (left to itself the compiler loads, waits and
+// multiplies one after the other)
+template <typename T, int N, int D, typename Load, typename Use>
+__device__ __forceinline__ void ahead(frag_t<T> (&f)[D], Load load, Use use) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    use(i, f[i % D]);
+    if (i + D < N) f[i % D] = load(i + D);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+template <typename T, int D, typename Load>
+__device__ __forceinline__ void first_loads(frag_t<T> (&f)[D], Load load) {
+#pragma unroll
+  for (int i = 0; i < D; ++i) f[i] = load(i);
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // 8 elements at p + k for k = 16 c + 8 h, zeros from d on (d a multiple of 8) or where !ok, times `by`
 template <typename T>
@@ -124,6 +185,12 @@ __device__ __forceinline__ frag_t<T> row_frag(const T* p, int k, int d, bool ok)
     for (int e = 0; e < 8; ++e) f[e] = 0;
   }
   return f;
+}
+
+// Waits for what loads x: in front of a loop whose loads into LDS are on their way, where a wait for x would wait for those too.
+template <typename X>
+__device__ __forceinline__ void arrived(X& x) {
+  asm volatile("" : "+v"(x));
 }
 
 __device__ __forceinline__ f32x16_t zero16() {

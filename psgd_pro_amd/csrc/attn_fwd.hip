@@ -14,6 +14,7 @@ template <typename T, int DP, int WQ, int WK, int BK>
 __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP == 128 ? 1 : 2) attn_forward_kernel(const AttnArgs a, int row_tiles) {
   using R = Rows<T, DP>;
   constexpr int W = WQ * WK, LOADS = R::loads(BK, W), TILE = BK * R::PITCH, KT = BK / WK / 32, DC = DP / 16, DT = DP / 32;
+  constexpr int AHEAD = DT < 4 ? 2 : sizeof(T) == 2 ? 4 : 2;  // at most KT DC and 2 KT DT
   static_assert(LOADS * W * 1024 == TILE && KT * WK * 32 == BK, "whole loads, whole blocks of keys");
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
@@ -37,6 +38,8 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
   frag_t<T> qf[DC];
 #pragma unroll
   for (int i = 0; i < DC; ++i) qf[i] = row_frag<T>(qp, 16 * i + 8 * h, a.d, pos >= 0);
+#pragma unroll
+  for (int i = 0; i < DC; ++i) arrived(qf[i]);
 
   int vk[LOADS], vv[LOADS], lrow[LOADS];
 #pragma unroll
@@ -74,15 +77,23 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
     const int stage = (t - t0) & 1, j0 = tiles.tile(t) * BK;
     load_wait<0>();
     if (t + 1 < t1) load(t + 1, stage ^ 1);
-    const unsigned kt = lds0 + stage * 2 * TILE + wk * (32 * KT) * R::PITCH, vt = kt + TILE;
+    const unsigned kt = lds0 + stage * 2 * TILE + wk * (32 * KT) * R::PITCH;
+    const Straight<T, DP> keys(kt, lane);
+    const Transposed<T, DP> values(kt + TILE, lane);
 
     f32x16_t x[KT];
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      x[i] = zero16();
-#pragma unroll
-      for (int k = 0; k < DC; ++k) x[i] = mma(R::straight(kt, 32 * i + c, k, h), qf[k], x[i]);
-    }
+    for (int i = 0; i < KT; ++i) x[i] = zero16();
+    frag_t<T> f[AHEAD];
+    const auto key_frag = [&](int i) __attribute__((always_inline)) { return keys(i / DC, i % DC); };
+    first_loads<T>(f, key_frag);
+    __builtin_amdgcn_s_setprio(1);
+    ahead<T, KT * DC>(f, key_frag, [&](int i, frag_t<T> y) __attribute__((always_inline)) {
+      x[i / DC] = mma(y, qf[i % DC], x[i / DC]);
+    });
+    const auto value_frag = [&](int i) __attribute__((always_inline)) { return values(i / DT, i % DT); };
+    __builtin_amdgcn_s_setprio(0);
+    first_loads<T>(f, value_frag);
     // all keys of the tile are visible to all rows, or each is looked at
     if (j0 + BK - 1 > lo || hi >= s.len || (hi - j0 >= a.window && j0 + BK > a.sinks)) {
       const int j = j0 + wk * 32 * KT + 4 * h;
@@ -91,7 +102,7 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int key = j + 32 * i + 8 * (e >> 2) + (e & 3);
-          if (!(key <= pos && (pos - key < a.window || key < a.sinks))) x[i][e] = -INFINITY;
+          x[i][e] = (key <= pos) & ((pos - key < a.window) | (key < a.sinks)) ? x[i][e] : -INFINITY;
         }
     }
     float top = x[0][0];
@@ -117,17 +128,20 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         x[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], a.scale2, -mu));
-        sum += x[i][e];
       }
-    // (bf16: the probabilities are rounded for the matrix cores, their sum is not)
+    // (bf16: the probabilities are rounded for the matrix cores, and their sum is of the rounded ones)
+    frag_t<T> p[2 * KT];
 #pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const frag_t<T> p = crossed<T>(x[i], u);
-#pragma unroll
-        for (int k = 0; k < DT; ++k) o[k] = mma(R::transposed(vt, 32 * i + 16 * u, k, lane), p, o[k]);
-      }
+    for (int i = 0; i < 2 * KT; ++i) {
+      p[i] = crossed<T>(x[i / 2], i % 2);
+      sum = sum_of(p[i], sum);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    ahead<T, 2 * KT * DT>(f, value_frag, [&](int i, frag_t<T> y) __attribute__((always_inline)) {
+      o[i % DT] = mma(y, p[i / DT], o[i % DT]);
+    });
+    __builtin_amdgcn_s_setprio(0);
   }
   sum += other_half(sum);
 
