@@ -19,60 +19,15 @@ from .train import _run_ws
 __all__ = ["AdamW", "adamw_state", "adamw_step"]
 
 _BLOCK = 256  # elements that share a scale
-_DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
-def _addresses(ts):
-    return (C.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
-
-
-def _check_params(params):
-    """Their elements and dtypes as host arrays."""
-    device = params[0].device if isinstance(params[0], torch.Tensor) else None
-    for i, p in enumerate(params):
-        if not isinstance(p, torch.Tensor) or not p.is_cuda or p.device != device:
-            raise RuntimeError(f"parameter {i}: CUDA (HIP) tensors on one device expected; got " +
-                               (f"one on {p.device}" if isinstance(p, torch.Tensor) else type(p).__name__))
-        if p.dtype not in _DTYPES:
-            raise TypeError(f"parameter {i}: float32 or bfloat16 expected, got {p.dtype}")
-        if not p.is_contiguous():
-            raise RuntimeError(f"parameter {i}: contiguous storage expected, its strides are {p.stride()}")
-    if len({p.data_ptr() for p in params if p.numel()}) < sum(p.numel() > 0 for p in params):
-        raise RuntimeError("a parameter is there twice")
-    return (C.c_int64 * len(params))(*[p.numel() for p in params]), (C.c_int32 * len(params))(*[_DTYPES[p.dtype] for p in params])
-
-
-def _check_grads(params, grads):
-    """The gradients, contiguous."""
-    if len(grads) != len(params):
-        raise RuntimeError(f"{len(grads)} gradients for {len(params)} parameters")
-    out = []
-    for i, (p, g) in enumerate(zip(params, grads)):
-        if not isinstance(g, torch.Tensor) or g.shape != p.shape or g.dtype != p.dtype or g.get_device() != p.get_device():
-            raise RuntimeError(f"gradient {i}: {tuple(p.shape)} in {p.dtype} on {p.device} expected as its parameter, got " +
-                               (f"{tuple(g.shape)} in {g.dtype} on {g.device}" if isinstance(g, torch.Tensor) else type(g).__name__))
-        out.append(g if g.is_contiguous() else g.contiguous())
-    return out
-
-
-def _check_states(params, states, name):
-    """(32 or 8, the states' addresses, their scales')."""
-    if len(states) != len(params):
-        raise RuntimeError(f"{len(states)} {name} for {len(params)} parameters")
-    pair = isinstance(states[0], (tuple, list))
-    for i, (p, s) in enumerate(zip(params, states)):
-        n = p.numel()
-        if pair != isinstance(s, (tuple, list)):
-            raise RuntimeError(f"{name}: states of 32 and of 8 bits in one call")
-        parts = ((s, torch.float32, n),) if not pair else tuple(zip(s, (_CODES, _SCALES), (n, -(-n // _BLOCK))))
-        for t, dt, size in parts:
-            if (not isinstance(t, torch.Tensor) or t.dtype != dt or t.numel() != size or t.get_device() != p.get_device()
-                    or not t.is_contiguous()):
-                raise RuntimeError(f"{name} {i}: {size} elements in {dt} on {p.device}, contiguous, expected")
-    if not pair:
-        return 32, _addresses(states), None
-    return 8, _addresses([s[0] for s in states]), _addresses([s[1] for s in states])
+def _tables(params, grads, ms, vs):
+    """The host arrays of psgdk_adamw_t for lists of tensors, checked (csrc/tables.cpp): (their buffer, the states' bits, copies of
+    gradients that had to be made contiguous)."""
+    from . import _tables as T  # (after torch; built beside the library)
+    buf = (C.c_int64 * (8 * len(params)))()
+    return (buf, *T.adamw(params, grads, ms, vs, C.addressof(buf)))
 
 
 def _check_numbers(step, lr, betas, eps, weight_decay, max_norm):
@@ -88,14 +43,15 @@ def _check_numbers(step, lr, betas, eps, weight_decay, max_norm):
         raise ValueError(f"max_norm = {max_norm}: must be positive, or None")
 
 
-def _launch(params, tables, grads, bits, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, seed):
+def _launch(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm, seed):
+    buf, bits, keep = _tables(params, grads, ms, vs)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("psgd_pro_amd: an AdamW step is not captured into a graph (its number would stay the same)")
-    n, dt, p = tables
-    g = _addresses(grads)
     norm = torch.empty((), device=params[0].device, dtype=torch.float32) if max_norm is not None else None
-    a = L.AdamW(len(params), bits, *(C.cast(x, C.c_void_p) for x in (n, dt, p, g, m, v)), C.cast(ms, C.c_void_p), C.cast(vs, C.c_void_p),
-                lr, betas[0], betas[1], eps, weight_decay, max_norm or 0.0, step, seed, None if norm is None else norm.data_ptr())
+    at, n = C.addressof(buf), 8 * len(params)
+    scales = (at + 6 * n, at + 7 * n) if bits == 8 else (None, None)
+    a = L.AdamW(len(params), bits, at, at + n, at + 2 * n, at + 3 * n, at + 4 * n, at + 5 * n, *scales, lr, betas[0], betas[1], eps,
+                weight_decay, max_norm or 0.0, step, seed, None if norm is None else norm.data_ptr())
     _run_ws(params[0], L.lib().psgdk_adamw, C.byref(a))
     return norm
 
@@ -128,16 +84,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     bfloat16 parameters are rounded to nearest. Tensors may begin anywhere in their storage, parameters and states are contiguous.
     Returns the gradients' norm before clipping (a 0-d float32 tensor) where max_norm is given. Capture into a graph is refused."""
     _check_numbers(step, lr, betas, eps, weight_decay, max_norm)
-    params, exp_avgs, exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)
-    if not params:
-        raise RuntimeError("no parameters")
-    n, dt = _check_params(params)
-    grads = _check_grads(params, list(grads))
-    bits, m, ms = _check_states(params, exp_avgs, "exp_avgs")
-    bits2, v, vs = _check_states(params, exp_avg_sqs, "exp_avg_sqs")
-    if bits != bits2:
-        raise RuntimeError("exp_avgs and exp_avg_sqs: states of 32 and of 8 bits in one call")
-    return _launch(params, (n, dt, _addresses(params)), grads, bits, m, v, ms, vs, int(step), float(lr), tuple(map(float, betas)),
+    return _launch(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), int(step), float(lr), tuple(map(float, betas)),
                    float(eps), float(weight_decay), max_norm, int(seed) & (2 ** 64 - 1))
 
 
@@ -166,24 +113,16 @@ class AdamW:
         self._bits = state_bits
         self._seed = (int(torch.randint(2 ** 62, ())) if seed is None else int(seed)) & (2 ** 64 - 1)
         self._step = 0
-        self._n, self._dt = _check_params(self._params_with_grad)
         self._ms = [adamw_state(p, state_bits) for p in self._params_with_grad]
         self._vs = [adamw_state(p, state_bits) for p in self._params_with_grad]
-        self._tables = [_check_states(self._params_with_grad, s, "states")[1:] for s in (self._ms, self._vs)]
+        _tables(*([p.detach() for p in self._params_with_grad],) * 2, self._ms, self._vs)  # (refuses what a step would)
 
     @torch.no_grad()
     def step_math(self, grads):
         """One step with the gradients given."""
-        params = self._params_with_grad
         _check_numbers(self._step + 1, self.lr_params, self.betas, self.eps, self.weight_decay, self.max_norm)
-        grads = _check_grads(params, grads)
-        (m, ms), (v, vs) = self._tables
-        # (a parameter's storage may have been exchanged: p.data = ...)
-        if any(p.numel() != n or _DTYPES.get(p.dtype) != dt or not p.is_contiguous() for p, n, dt in zip(params, self._n, self._dt)):
-            raise RuntimeError("a parameter's size, dtype or layout has changed since the optimizer was made")
-        norm = _launch(params, (self._n, self._dt, _addresses(params)), grads, self._bits, m, v, ms, vs, self._step + 1,
-                       float(self.lr_params), tuple(map(float, self.betas)), float(self.eps), float(self.weight_decay), self.max_norm,
-                       self._seed)
+        norm = _launch(self._params_with_grad, list(grads), self._ms, self._vs, self._step + 1, float(self.lr_params),
+                       tuple(map(float, self.betas)), float(self.eps), float(self.weight_decay), self.max_norm, self._seed)
         self._step += 1
         if norm is not None:
             self.norm = norm
@@ -228,5 +167,5 @@ class AdamW:
         for k, v in st["hyper"].items():
             setattr(self, k, v)
         self._step, self._seed = st["step"], st["seed"]
-        for x, y in pairs:  # into the existing buffers: the tables hold their addresses
+        for x, y in pairs:
             (x if x.dtype == torch.float32 else x.view(torch.uint8)).copy_(y if y.dtype == torch.float32 else y.view(torch.uint8))

@@ -1,4 +1,5 @@
-"""Builds psgd_pro_amd/libpsgdk.so (gfx950) from psgd_pro_amd/csrc with hipcc, in the source tree.
+"""Builds psgd_pro_amd/libpsgdk.so (gfx950) from psgd_pro_amd/csrc with hipcc, and psgd_pro_amd/_tables.so (a small Python module,
+host code against torch's headers) with g++, in the source tree.
 
     python -m psgd_pro_amd.build [--jobs N]
 
@@ -21,6 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpsgdk.so")
+TABLES = os.path.join(HERE, "_tables.so")  # a Python module against torch's headers (csrc/tables.cpp), host code only
 SOURCES = ["gemm_cv.hip", "gemm_bf16.hip", "gemm_small.hip", "nlb.hip", "elem.hip", "block.hip", "xent.hip", "xgemm.hip",
            "attn_fwd.hip", "attn_bwd.hip", "rope.hip", "adamw.hip", "capi.cpp", "train_capi.cpp", "attn_capi.cpp", "adamw_capi.cpp",
            "noalloc.hip", "measure.hip"]
@@ -80,11 +82,30 @@ def build_asan(objects):
     return ASAN_LIB
 
 
+def build_tables():
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    inc = [f for d in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"]) for f in ("-isystem", d)]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = TABLES + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *inc, os.path.join(CSRC, "tables.cpp"), "-o", tmp, "-L", libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"build failed: {' '.join(cmd)}\n{r.stderr}")
+    os.replace(tmp, TABLES)
+    return TABLES
+
+
 def build(jobs=None, verbose=False, asan=False):
     os.makedirs(BUILD, exist_ok=True)
     jobs = jobs or min(len(SOURCES), os.cpu_count() or 1)
-    with cf.ThreadPoolExecutor(jobs) as ex:
+    with cf.ThreadPoolExecutor(jobs + 1) as ex:
+        tables = ex.submit(build_tables)
         results = list(ex.map(_compile, SOURCES))
+        tables.result()
     for _, err in results:
         if err.strip() and verbose:
             print(err, file=sys.stderr)

@@ -149,19 +149,22 @@ __device__ __forceinline__ void store4(T* out, float y0, float y1, float y2, flo
 // heads are among them, so that shared heads' gradients need no further sum. S = Q K^T has a key in each lane, P and dS are
 // the second products' operands where they are made (dV^T = dO^T P, dK^T = Q^T dS), and a tile of rows serves straight and
 // transposed. Key tiles that hold sinks are seen by all rows: their rows are cut in parts, whose sums attn_dkv_sum adds.
-template <typename T, int DP, int BR>
-__global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) attn_dkv_kernel(const AttnArgs a, int key_tiles) {
+// KV: the tile's keys and values are fragments in registers; else the values are in LDS (bf16 heads of 128 then fit two waves
+// a SIMD: 1750 -> 1400 us of 4 x 4096 tokens with 32 / 8 heads; 1050 with the tiles of the most rows first).
+template <typename T, int DP, int BR, bool KV>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_dkv_kernel(const AttnArgs a, int key_tiles) {
   using R = Rows<T, DP>;
   constexpr int LOADS = R::loads(BR, 4), TILE = BR * R::PITCH, STAGE = 2 * TILE + 1024, RT = BR / 32, DC = DP / 16, DT = DP / 32;
-  constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2;  // at most 4 DT
+  constexpr int AHEAD = sizeof(T) == 4 ? 2 : KV ? 4 : 3, VALUES = KV ? 0 : kAttnKeys * R::PITCH;  // AHEAD: at most 4 DT
   static_assert(BR <= 64, "a load of 64 floats");
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
 
-  const int sinks = a.sink_tiles * a.sink_parts, per = sinks + (key_tiles - a.sink_tiles) * a.rest_parts;
-  const int work = xcd_run(blockIdx.x, gridDim.x), pair = work / per, rest = work - pair * per;
+  const int sinks = a.sink_tiles * a.sink_parts;
+  // the tiles with the most rows first, a pair's on one XCD where there are 8 pairs or a multiple of them
+  const int pairs = a.batch * a.kv, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
   const bool sink = rest < sinks;
   const int parts = sink ? a.sink_parts : a.rest_parts, part = sink ? rest % parts : (rest - sinks) % parts;
   const int tile = sink ? rest / parts : a.sink_tiles + (rest - sinks) / parts, j0 = tile * kAttnKeys;
@@ -175,37 +178,63 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
   const int t0 = part_begin(tiles, part, parts), t1 = part_begin(tiles, part + 1, parts);
 
   const int key = j0 + wave * 32 + c;
-  const T* const kp = static_cast<const T*>(a.k.p) + b * a.k.sb + key * a.k.sn + head * a.k.sh;
-  const T* const vp = static_cast<const T*>(a.v.p) + b * a.v.sb + key * a.v.sn + head * a.v.sh;
-  frag_t<T> kf[DC], vf[DC];
+  const T* const kp = static_cast<const T*>(a.k.p) + b * a.k.sb + head * a.k.sh;
+  const T* const vp = static_cast<const T*>(a.v.p) + b * a.v.sb + head * a.v.sh;
+  frag_t<T> kf[DC], vf[KV ? DC : 1];
 #pragma unroll
   for (int i = 0; i < DC; ++i) {
-    kf[i] = row_frag<T>(kp, 16 * i + 8 * h, a.d, key < s.len);
-    vf[i] = row_frag<T>(vp, 16 * i + 8 * h, a.d, key < s.len);
+    kf[i] = row_frag<T>(kp + key * a.k.sn, 16 * i + 8 * h, a.d, key < s.len);
+    if constexpr (KV) vf[i] = row_frag<T>(vp + key * a.v.sn, 16 * i + 8 * h, a.d, key < s.len);
   }
 #pragma unroll
   for (int i = 0; i < DC; ++i) {
     arrived(kf[i]);
-    arrived(vf[i]);
+    if constexpr (KV) arrived(vf[i]);
+  }
+  if constexpr (!KV) {
+    i32x4_t rv = rsrc_words(vp + (long long)j0 * a.v.sn, 0x7fffffff);
+    asm volatile("s_nop 4" : "+s"(rv));  // (as in the forward pass)
+#pragma unroll
+    for (int i = 0; i < R::loads(kAttnKeys, 4); ++i) {
+      int row, chunk;
+      R::where(wave * R::loads(kAttnKeys, 4) + i, lane, row, chunk);
+      const bool in = chunk * R::PER < a.d && j0 + row < s.len;
+      load_lds(rv, in ? (int)(row * a.v.sn * R::E) + chunk * 16 : kOob, lds0 + (wave * R::loads(kAttnKeys, 4) + i) * 1024);
+    }
   }
 
   const T* const qp = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)head * a.group * a.q.sh;
   const T* const gp = static_cast<const T*>(a.dout.p) + b * a.dout.sb + (long long)head * a.group * a.dout.sh;
-  auto load = [&](int t) __attribute__((always_inline)) {
-    const int r0 = (first + t) * BR, tok0 = row_token(a, r0);
-    i32x4_t rq = rsrc_words(qp + tok0 * a.q.sn, 0x7fffffff), rg = rsrc_words(gp + tok0 * a.dout.sn, 0x7fffffff);
-    i32x4_t rs = rsrc_words((wave == 0 ? a.lse : a.delta) + (long long)pair * a.rows + r0, 0x7fffffff);
-    unsigned at = uniform(lds0 + (t & 1) * STAGE + wave * LOADS * 1024);
-    unsigned st = uniform(lds0 + (t & 1) * STAGE + 2 * TILE + wave * 256);
-    asm volatile("s_nop 4" : "+s"(rq), "+s"(rg), "+s"(rs), "+s"(at), "+s"(st));  // (as in the forward pass)
+  // where this lane's rows are, from the token of the tile's first row: the same in every tile where tokens are not cut
+  int tok[LOADS], oq[LOADS], og[LOADS];
+  auto place = [&](int r0) __attribute__((always_inline)) {
+    const int tok0 = row_token(a, r0);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      int lrow, chunk;
-      R::where(wave * LOADS + i, lane, lrow, chunk);
-      const int r = r0 + lrow, tok = row_token(a, r), g = r - tok * a.group;
-      const bool in = chunk * R::PER < a.d && tok >= from && tok < to;
-      load_lds(rq, in ? (int)(((tok - tok0) * a.q.sn + g * a.q.sh) * R::E) + chunk * 16 : kOob, at + i * 1024);
-      load_lds(rg, in ? (int)(((tok - tok0) * a.dout.sn + g * a.dout.sh) * R::E) + chunk * 16 : kOob, at + TILE + i * 1024);
+      int row, chunk;
+      R::where(wave * LOADS + i, lane, row, chunk);
+      const int t = row_token(a, r0 + row), g = r0 + row - t * a.group;
+      tok[i] = chunk * R::PER < a.d ? t - tok0 : 1 << 30;
+      oq[i] = (int)(((t - tok0) * a.q.sn + g * a.q.sh) * R::E) + chunk * 16;
+      og[i] = (int)(((t - tok0) * a.dout.sn + g * a.dout.sh) * R::E) + chunk * 16;
+    }
+  };
+  const bool whole = BR % a.group == 0;
+  place(0);
+  auto load = [&](int t) __attribute__((always_inline)) {
+    const int r0 = (first + t) * BR, tok0 = uniform(row_token(a, r0));
+    if (!whole) place(r0);
+    i32x4_t rq = rsrc_words(qp + tok0 * a.q.sn, 0x7fffffff), rg = rsrc_words(gp + tok0 * a.dout.sn, 0x7fffffff);
+    i32x4_t rs = rsrc_words((wave == 0 ? a.lse : a.delta) + (long long)pair * a.rows + r0, 0x7fffffff);
+    unsigned at = uniform(lds0 + VALUES + (t & 1) * STAGE + wave * LOADS * 1024);
+    unsigned st = uniform(lds0 + VALUES + (t & 1) * STAGE + 2 * TILE + wave * 256);
+    asm volatile("s_nop 4" : "+s"(rq), "+s"(rg), "+s"(rs), "+s"(at), "+s"(st));
+    const int lo = from - tok0, hi = to - tok0;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const bool in = (tok[i] >= lo) & (tok[i] < hi);
+      load_lds(rq, in ? oq[i] : kOob, at + i * 1024);
+      load_lds(rg, in ? og[i] : kOob, at + TILE + i * 1024);
     }
     if (wave < 2) load_lds4(rs, lane < BR && r0 + lane < a.rows ? lane * 4 : kOob, st);
   };
@@ -213,11 +242,12 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
   f32x16_t dk[DT], dv[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) dk[i] = dv[i] = zero16();
+  const Straight<T, DP> values(lds0 + (KV ? 0 : wave * 32 * R::PITCH), lane);
   if (t0 < t1) load(t0);
   for (int t = t0; t < t1; ++t) {
     load_wait<0>();
     if (t + 1 < t1) load(t + 1);
-    const unsigned qt = lds0 + (t & 1) * STAGE, gt = qt + TILE, st = gt + TILE;
+    const unsigned qt = lds0 + VALUES + (t & 1) * STAGE, gt = qt + TILE, st = gt + TILE;
     const Straight<T, DP> queries(qt, lane), grads(gt, lane);
     const Transposed<T, DP> query_cols(qt, lane), grad_cols(gt, lane);
     const int r0 = (first + t) * BR, lo = s.start + row_token(a, r0), hi = s.start + row_token(a, r0 + BR - 1);
@@ -227,18 +257,27 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
     for (int i = 0; i < RT; ++i) {
       f32x16_t x = zero16(), dp = zero16();
       frag_t<T> f[AHEAD];
-      const auto row_frags = [&](int s) __attribute__((always_inline)) { return s % 2 ? grads(i, s / 2) : queries(i, s / 2); };
-      first_loads<T>(f, row_frags);
-      __builtin_amdgcn_s_setprio(1);
-      ahead<T, 2 * DC>(f, row_frags, [&](int s, frag_t<T> y) __attribute__((always_inline)) {
-        if (s % 2) dp = mma(y, vf[s / 2], dp);
-        else x = mma(y, kf[s / 2], x);
-      });
-      f32x4_t lse[4], delta[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        lse[e] = *(LDS_AS f32x4_t*)(uintptr_t)(st + (32 * i + 8 * e + 4 * h) * 4);
-        delta[e] = *(LDS_AS f32x4_t*)(uintptr_t)(st + 256 + (32 * i + 8 * e + 4 * h) * 4);
+      if constexpr (KV) {
+        const auto row_frags = [&](int s) __attribute__((always_inline)) { return s % 2 ? grads(i, s / 2) : queries(i, s / 2); };
+        first_loads<T>(f, row_frags);
+        __builtin_amdgcn_s_setprio(1);
+        ahead<T, 2 * DC>(f, row_frags, [&](int s, frag_t<T> y) __attribute__((always_inline)) {
+          if (s % 2) dp = mma(y, vf[s / 2], dp);
+          else x = mma(y, kf[s / 2], x);
+        });
+      } else {
+        // a query's, a gradient's and a value's fragment in turn
+        const auto row_frags = [&](int s) __attribute__((always_inline)) {
+          return s % 3 == 0 ? queries(i, s / 3) : s % 3 == 1 ? grads(i, s / 3) : values(0, s / 3);
+        };
+        frag_t<T> held;
+        first_loads<T>(f, row_frags);
+        __builtin_amdgcn_s_setprio(1);
+        ahead<T, 3 * DC>(f, row_frags, [&](int s, frag_t<T> y) __attribute__((always_inline)) {
+          if (s % 3 == 0) x = mma(y, kf[s / 3], x);
+          else if (s % 3 == 1) held = y;
+          else dp = mma(held, y, dp);
+        });
       }
       __builtin_amdgcn_s_setprio(0);
       // 16 rows' dO, then their Q, then the next 16 rows'
@@ -249,14 +288,19 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
       if (look) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int tok = row_token(a, r0 + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3)), pos = s.start + tok;
-          x[e] = (tok < to) & (key <= pos) & ((pos - key < a.window) | (key < a.sinks)) ? x[e] : -INFINITY;
+          const int at = row_token(a, r0 + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3)), pos = s.start + at;
+          x[e] = (at < to) & (key <= pos) & ((pos - key < a.window) | (key < a.sinks)) ? x[e] : -INFINITY;
         }
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale2, -lse[e >> 2][e & 3]));
-        dp[e] = x[e] * (dp[e] - delta[e >> 2][e & 3]);
+      for (int e = 0; e < 16; e += 4) {
+        const f32x4_t lse = *(LDS_AS f32x4_t*)(uintptr_t)(st + (32 * i + 2 * e + 4 * h) * 4);
+        const f32x4_t delta = *(LDS_AS f32x4_t*)(uintptr_t)(st + 256 + (32 * i + 2 * e + 4 * h) * 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          x[e + q] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + q], a.scale2, -lse[q]));
+          dp[e + q] = x[e + q] * (dp[e + q] - delta[q]);
+        }
       }
       const frag_t<T> p[2] = {crossed<T>(x, 0), crossed<T>(x, 1)}, ds[2] = {crossed<T>(dp, 0), crossed<T>(dp, 1)};
       __builtin_amdgcn_sched_barrier(0);
@@ -268,6 +312,8 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 4 ? 32 : 64) ? 1 : 2) 
       __builtin_amdgcn_s_setprio(0);
     }
   }
+  // (no load of values may reach LDS after the workgroup)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   if (parts > 1) {
     const long long at = sink ? ((long long)pair * a.sink_tiles + tile) * parts + part
@@ -337,8 +383,9 @@ hipError_t launch_dq(const AttnArgs& a, hipStream_t st) {
 }
 template <typename T, int DP>
 hipError_t launch_dkv(const AttnArgs& a, hipStream_t st) {
-  constexpr int BR = kTileRows<T>, smem = 2 * (2 * BR * Rows<T, DP>::PITCH + 1024);
-  const auto fn = attn_dkv_kernel<T, DP, BR>;
+  constexpr bool KV = sizeof(T) == 4 || DP < 128;
+  constexpr int BR = KV ? kTileRows<T> : 32, smem = (KV ? 0 : kAttnKeys * Rows<T, DP>::PITCH) + 2 * (2 * BR * Rows<T, DP>::PITCH + 1024);
+  const auto fn = attn_dkv_kernel<T, DP, BR, KV>;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (attr != hipSuccess) return attr;
   const int tiles = (a.m + kAttnKeys - 1) / kAttnKeys, rest = tiles - a.sink_tiles, pairs = a.batch * a.kv;
@@ -359,19 +406,32 @@ hipError_t launch_dkv(const AttnArgs& a, hipStream_t st) {
   return e;
 }
 
+// rows of a tile of the dk, dv pass
+int attn_dkv_rows(const AttnArgs& a) { return a.dt == 0 || a.d > 96 ? 32 : 64; }
+
 }  // namespace
 
-// Parts so that there are about 512 workgroups, none of fewer than 4 tiles of rows; key tiles with sinks, which all rows see,
-// in as many as leave each about the rows of another tile's.
+// Key tiles with sinks, which all rows see, are cut in as many parts as leave each about the rows of another tile's. The others
+// are cut where a round of workgroups would otherwise leave CUs idle: 512 (256 where a wave has a SIMD's registers to itself) run
+// at once, and 564 of equal work take as long as 1024 (16384 tokens, window 1024, 16 / 4 heads of 64: 340 us uncut, XX cut). A
+// part costs about 8 tiles of rows for its keys, its sums and their addition.
 void attn_backward_parts(AttnArgs& a) {
-  const long long br = a.dt == 0 ? 32 : 64, pairs = (long long)a.batch * a.kv, tiles = (a.m + kAttnKeys - 1) / kAttnKeys;
+  const long long br = attn_dkv_rows(a), pairs = (long long)a.batch * a.kv, tiles = (a.m + kAttnKeys - 1) / kAttnKeys;
   const long long all = (a.rows + br - 1) / br;
   const long long seen = std::min(all, ((long long)(a.window + kAttnKeys - 1) * a.group + br - 1) / br + 1);
   a.sink_tiles = a.sinks && seen < all ? (int)((std::min(a.sinks, a.m) + kAttnKeys - 1) / kAttnKeys) : 0;
-  const long long rest = tiles - a.sink_tiles;
-  a.rest_parts = (int)std::max<long long>(1, std::min<long long>({rest ? 512 / (pairs * rest) : 1, seen / 4, 64}));
+  const long long rest = pairs * (tiles - a.sink_tiles), slots = a.dt == 0 && a.d > 32 ? 256 : 512, over = 8;
+  long long best = 0;
+  a.rest_parts = a.sink_parts = 1;
+  for (int parts = 1; parts <= 64 && rest && (parts == 1 || (seen / parts >= 4 && rest * parts <= 4096)); ++parts) {
+    const long long per = (seen + parts - 1) / parts;
+    const long long cost = (rest * parts + pairs * a.sink_tiles * (all / per + 1) + slots - 1) / slots * (per + over) + (parts > 1 ? over : 0);
+    if (!best || cost < best) {
+      best = cost;
+      a.rest_parts = parts;
+    }
+  }
   const long long share = std::max<long long>(seen / a.rest_parts, 8);
-  a.sink_parts = 1;
   if (a.sink_tiles)  // (4096 parts' sums are 512 MiB)
     a.sink_parts = (int)std::max<long long>(1, std::min<long long>({all / share, 64, 4096 / (pairs * a.sink_tiles)}));
 }

@@ -85,11 +85,11 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
 #pragma unroll
     for (int i = 0; i < KT; ++i) x[i] = zero16();
     frag_t<T> f[AHEAD];
-    const auto key_frag = [&](int i) __attribute__((always_inline)) { return keys(i / DC, i % DC); };
+    const auto key_frag = [&](int i) __attribute__((always_inline)) { return keys(i % KT, i / KT); };
     first_loads<T>(f, key_frag);
     __builtin_amdgcn_s_setprio(1);
     ahead<T, KT * DC>(f, key_frag, [&](int i, frag_t<T> y) __attribute__((always_inline)) {
-      x[i / DC] = mma(y, qf[i % DC], x[i / DC]);
+      x[i % KT] = mma(y, qf[i / KT], x[i % KT]);
     });
     const auto value_frag = [&](int i) __attribute__((always_inline)) { return values(i / DT, i % DT); };
     __builtin_amdgcn_s_setprio(0);
