@@ -1,4 +1,6 @@
 // Norms of queries and keys for each head, their weights and the position rotation, one pass each way.
+#include <type_traits>
+
 #include "rope.h"
 
 namespace psgdk {
@@ -62,7 +64,12 @@ __device__ __forceinline__ void turn(uint64_t t, float& c, float& s) {
 
 // sum over `lanes` (a power of two) lanes that lie together, every lane getting it
 __device__ __forceinline__ float lanes_sum(float v, int lanes) {
-  for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, 64);
+  if (lanes > 1) v += dpp<0xB1>(v);
+  if (lanes > 2) v += dpp<0x4E>(v);
+  if (lanes > 4) v += dpp<0x141>(v);
+  if (lanes > 8) v += dpp<0x140>(v);
+  if (lanes > 16) v += __shfl_xor(v, 16, 64);
+  if (lanes > 32) v += __shfl_xor(v, 32, 64);
   return v;
 }
 
@@ -79,7 +86,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int sub = lane & (a.lanes - 1), slot = lane / a.lanes, at_once = 64 / a.lanes;
   const int half = a.rot / 2, pairs = a.d / 2;
-  const int steps = (a.all + at_once - 1) / at_once;
+  const int q_steps = (a.heads + at_once - 1) / at_once, steps = q_steps + (a.all - a.heads + at_once - 1) / at_once;
   const float inv_d = 1.f / (float)a.d;
 
   int e0[S], e1[S];
@@ -146,12 +153,13 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
 #pragma unroll
       for (int v = 0; v < V; ++v) turn(pos * rate[s][v], cs[s][v], sn[s][v]);
 
-    for (int it = part * steps / a.waves; it < (part + 1) * steps / a.waves; ++it) {
-      const int hh = it * at_once + slot, k = hh >= a.heads, head = hh - (k ? a.heads : 0);
-      const bool there = hh < a.all;
-      const T* const xp = k ? head_of<T>(a.x[1], b, i, head) : head_of<T>(a.x[0], b, i, head);
+    // heads `head` of the queries (K 0) or keys (K 1)
+    auto heads = [&](auto which, int head) __attribute__((always_inline)) {
+      constexpr int K = decltype(which)::value;
+      const bool there = head < (K ? a.all - a.heads : a.heads);
+      const T* const xp = head_of<T>(a.x[K], b, i, head);
       const T* gp = nullptr;
-      if constexpr (BACK) gp = k ? head_of<T>(a.dy[1], b, i, head) : head_of<T>(a.dy[0], b, i, head);
+      if constexpr (BACK) gp = head_of<T>(a.dy[K], b, i, head);
       float x[S][2 * V], g[S][2 * V];
       float sum = 0.f, sq = 0.f;
 #pragma unroll
@@ -200,7 +208,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const int p = first(v), q = second(v);
-            const float u0 = x[s][p] * rstd * (k ? w[1][s][p] : w[0][s][p]), u1 = x[s][q] * rstd * (k ? w[1][s][q] : w[0][s][q]);
+            const float u0 = x[s][p] * rstd * w[K][s][p], u1 = x[s][q] * rstd * w[K][s][q];
             out[s][p] = u0 * cs[s][v] - u1 * sn[s][v];
             out[s][q] = u1 * cs[s][v] + u0 * sn[s][v];
           }
@@ -215,12 +223,10 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
             x[s][p] *= rstd;  // the normalised values
             x[s][q] *= rstd;
             const float t0 = u0 * x[s][p], t1 = u1 * x[s][q];
-            dw[0][s][p] += k ? 0.f : t0;
-            dw[0][s][q] += k ? 0.f : t1;
-            dw[1][s][p] += k ? t0 : 0.f;
-            dw[1][s][q] += k ? t1 : 0.f;
-            g[s][p] = u0 * (k ? w[1][s][p] : w[0][s][p]);
-            g[s][q] = u1 * (k ? w[1][s][q] : w[0][s][q]);
+            dw[K][s][p] += t0;
+            dw[K][s][q] += t1;
+            g[s][p] = u0 * w[K][s][p];
+            g[s][q] = u1 * w[K][s][q];
             dot += g[s][p] * x[s][p] + g[s][q] * x[s][q];
             csum += g[s][p] + g[s][q];
           }
@@ -232,9 +238,9 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
 #pragma unroll
           for (int e = 0; e < 2 * V; ++e) out[s][e] = (g[s][e] - x[s][e] * dot - cmean) * rstd;
       }
-      T* const base = static_cast<T*>(BACK ? (k ? a.dx[1] : a.dx[0]) : (k ? a.y[1] : a.y[0]));
+      T* const base = static_cast<T*>(BACK ? a.dx[K] : a.y[K]);
       if (there && base) {
-        T* const op = base + (token * (k ? a.all - a.heads : a.heads) + head) * a.d;
+        T* const op = base + (token * (K ? a.all - a.heads : a.heads) + head) * a.d;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           if (!in[s]) continue;
@@ -248,6 +254,10 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
           st_vec<T, V>(op + e1[s], hi);
         }
       }
+    };
+    for (int it = part * steps / a.waves; it < (part + 1) * steps / a.waves; ++it) {
+      if (it < q_steps) heads(std::integral_constant<int, 0>{}, it * at_once + slot);
+      else heads(std::integral_constant<int, 1>{}, (it - q_steps) * at_once + slot);
     }
   }
 
@@ -298,7 +308,8 @@ void rope_plan(RopeArgs& a, bool aligned16, bool aligned8) {
   a.lanes = 1;
   while (a.lanes < need && a.lanes < 64) a.lanes *= 2;
   // all heads of a token on one wave where there are tokens enough to fill the GPU
-  const int steps = (a.all + 64 / a.lanes - 1) / (64 / a.lanes);
+  const int at_once = 64 / a.lanes;
+  const int steps = (a.heads + at_once - 1) / at_once + (a.all - a.heads + at_once - 1) / at_once;
   a.waves = (int)std::max<long long>(1, std::min<long long>(steps, 8192 / std::max<long long>(a.tokens, 1)));
   a.parts = (int)std::min<long long>((a.tokens * a.waves + 3) / 4, kRopeParts);
 }
