@@ -155,7 +155,7 @@ int psgdk_qk_norm_rope(const psgdk_qk_norm_rope_t* q, void* qo, void* ko, psgdk_
   const int64_t none[3] = {0, 0, 0};
   for (const void* p : {qo, ko})
     if (p) al.add(p, none, 1);
-  rope_plan(a, al.by16, al.by8);
+  rope_plan(a, false, al.by16, al.by8);
   return hip_check(rope_launch(a, false, (hipStream_t)stream), "qk_norm_rope");
 }
 
@@ -175,11 +175,10 @@ int psgdk_qk_norm_rope_backward(const psgdk_qk_norm_rope_t* q, const psgdk_qk_no
   const int64_t none[3] = {0, 0, 0};
   for (const void* p : {g->dq, g->dk})
     if (p) al.add(p, none, 1);
-  rope_plan(a, al.by16, al.by8);
+  rope_plan(a, true, al.by16, al.by8);
   const bool sums = g->dqw || g->dkw;
   Ws m(ws);
-  // (room for the most parts there are, whatever the pointers' alignment)
-  if (sums) a.part = m.take<float>((size_t)2 * kRopeParts * a.d);
+  if (sums) a.part = m.take<float>((size_t)2 * kRopeParts * a.d);  // (the parts go by alignment: room for the most there are)
   if (!ws) {
     *ws_bytes = m.off;
     return PSGDK_OK;

@@ -36,7 +36,7 @@ struct RopeArgs {
   int waves;             // waves of a token
 };
 // pairs_lane, lanes, waves and parts; aligned16: every base and stride is a multiple of 16 bytes
-void rope_plan(RopeArgs& a, bool aligned16, bool aligned8);
+void rope_plan(RopeArgs& a, bool backward, bool aligned16, bool aligned8);
 hipError_t rope_launch(const RopeArgs& a, bool backward, hipStream_t st);
 
 }  // namespace psgdk
