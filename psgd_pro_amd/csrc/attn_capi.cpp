@@ -27,6 +27,11 @@ int check_side(const psgdk_heads_t& t, int dt, int64_t tokens, int64_t heads, co
   out = AttnSide{t.p, t.batch_stride, tokens > 1 ? t.token_stride : 0, heads > 1 ? t.head_stride : 0};
   return PSGDK_OK;
 }
+int check_launch(int64_t pairs, int64_t tiles, int64_t limit, const char* name) {
+  if (pairs * tiles >= limit)
+    return fail(PSGDK_ESHAPE, "batch * kv_heads = %lld with %lld tiles of %s each: too many for a launch", (long long)pairs, (long long)tiles, name);
+  return PSGDK_OK;
+}
 int attn_args(const psgdk_window_attention_t* q, AttnArgs& a) {
   if (!q) return fail(PSGDK_EINVAL, "null argument block");
   PSGDK_TRY(check_dt(q->dtype, "dtype"));
@@ -65,14 +70,9 @@ int attn_args(const psgdk_window_attention_t* q, AttnArgs& a) {
   a.lengths = q->lengths;
   a.starts = q->starts;
   a.lse = q->lse;
-  // A launch holds less than 2^32 threads: a forward workgroup of 32 rows has 128, one of 128 keys backward 256. (More than one
-  // for a tile of keys or rows there are only where the tiles are few.)
-  const int64_t pairs = q->batch * a.kv;
   a.parts = 1;
-  if (pairs * ((rows + 31) / 32) >= (int64_t)1 << 24 || pairs * ((q->m + 127) / 128) >= (int64_t)1 << 23)
-    return fail(PSGDK_ESHAPE, "batch * kv_heads = %lld with %lld rows and %lld keys each: too many for a launch", (long long)pairs,
-                (long long)rows, (long long)q->m);
-  return PSGDK_OK;
+  // a launch holds less than 2^32 threads: a workgroup of 32 rows has 128 (several for one tile only where tiles are few)
+  return check_launch(q->batch * a.kv, (rows + 31) / 32, (int64_t)1 << 24, "rows");
 }
 int attn_pointers(const psgdk_window_attention_t* q, AttnArgs& a) {
   PSGDK_TRY(check_side(q->q, a.dt, q->n, q->heads, "q", a.q));
@@ -229,6 +229,7 @@ int psgdk_window_attention_backward(const psgdk_window_attention_t* q, const psg
   PSGDK_TRY(attn_args(q, a));
   if (!g) return fail(PSGDK_EINVAL, "null gradient block");
   if (!ws_bytes) return fail(PSGDK_EINVAL, "ws_bytes is null");
+  PSGDK_TRY(check_launch(q->batch * a.kv, (q->m + kAttnKeys - 1) / kAttnKeys, (int64_t)1 << 23, "keys"));  // (256 threads each)
   attn_backward_parts(a);
   a.dq = g->dq;
   a.dk = g->dk;
