@@ -55,38 +55,47 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_d
     arrived(gf[i]);
   }
 
-  int vk[LOADS], vv[LOADS], lrow[LOADS];
+  int vk[LOADS], vv[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
-    int chunk;
-    R::where(wave * LOADS + i, lane, lrow[i], chunk);
+    int row, chunk;
+    R::where(wave * LOADS + i, lane, row, chunk);
     const bool in = chunk * R::PER < a.d;
-    vk[i] = in ? (int)(lrow[i] * a.k.sn * R::E) + chunk * 16 : kOob;
-    vv[i] = in ? (int)(lrow[i] * a.v.sn * R::E) + chunk * 16 : kOob;
+    vk[i] = in ? (int)(row * a.k.sn * R::E) + chunk * 16 : kOob;
+    vv[i] = in ? (int)(row * a.v.sn * R::E) + chunk * 16 : kOob;
   }
   const T* const kp = static_cast<const T*>(a.k.p) + b * a.k.sb + head * a.k.sh;
   const T* const vp = static_cast<const T*>(a.v.p) + b * a.v.sb + head * a.v.sh;
-  auto load = [&](int t) __attribute__((always_inline)) {
+  // (as in the forward pass)
+  i32x4_t rk, rv;
+  unsigned to;
+  auto plan = [&](int t) __attribute__((always_inline)) {
     const int j0 = tiles.tile(t) * BK;
-    i32x4_t rk = rsrc_words(kp + j0 * a.k.sn, 0x7fffffff), rv = rsrc_words(vp + j0 * a.v.sn, 0x7fffffff);
-    unsigned to = uniform(lds0 + (t & 1) * 2 * TILE + wave * LOADS * 1024);
-    asm volatile("s_nop 4" : "+s"(rk), "+s"(rv), "+s"(to));  // (as in the forward pass)
+    rk = rsrc_words(kp + j0 * a.k.sn, ((s.len - j0 - 1) * a.k.sn + a.d) * R::E);
+    rv = rsrc_words(vp + j0 * a.v.sn, ((s.len - j0 - 1) * a.v.sn + a.d) * R::E);
+    to = uniform(lds0 + (t & 1) * 2 * TILE + wave * LOADS * 1024);
+    asm volatile("s_nop 4" : "+s"(rk), "+s"(rv), "+s"(to));
+  };
+  auto load = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const bool in = j0 + lrow[i] < s.len;
-      load_lds(rk, in ? vk[i] : kOob, to + i * 1024);
-      load_lds(rv, in ? vv[i] : kOob, to + TILE + i * 1024);
+      load_lds(rk, vk[i], to + i * 1024);
+      load_lds(rv, vv[i], to + TILE + i * 1024);
     }
   };
 
   f32x16_t dq[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) dq[i] = zero16();
-  if (tiles.count) load(0);
+  if (tiles.count) {
+    plan(0);
+    load();
+  }
   for (int t = 0; t < tiles.count; ++t) {
     const int j0 = tiles.tile(t) * BK;
+    plan(t + 1);
     load_wait<0>();
-    if (t + 1 < tiles.count) load(t + 1);
+    if (t + 1 < tiles.count) load();
     const unsigned kt = lds0 + (t & 1) * 2 * TILE;
     const Straight<T, DP> keys(kt, lane), values(kt + TILE, lane);
     const Transposed<T, DP> columns(kt, lane);
@@ -221,33 +230,45 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_d
   };
   const bool whole = BR % a.group == 0;
   place(0);
-  auto load = [&](int t) __attribute__((always_inline)) {
-    const int r0 = (first + t) * BR, tok0 = uniform(row_token(a, r0));
-    if (!whole) place(r0);
-    i32x4_t rq = rsrc_words(qp + tok0 * a.q.sn, 0x7fffffff), rg = rsrc_words(gp + tok0 * a.dout.sn, 0x7fffffff);
-    i32x4_t rs = rsrc_words((wave == 0 ? a.lse : a.delta) + (long long)pair * a.rows + r0, 0x7fffffff);
-    unsigned at = uniform(lds0 + VALUES + (t & 1) * STAGE + wave * LOADS * 1024);
-    unsigned st = uniform(lds0 + VALUES + (t & 1) * STAGE + 2 * TILE + wave * 256);
-    asm volatile("s_nop 4" : "+s"(rq), "+s"(rg), "+s"(rs), "+s"(at), "+s"(st));
-    const int lo = from - tok0, hi = to - tok0;
+  i32x4_t rq, rg, rs;
+  unsigned ring, sums;
+  int lo_tok, hi_tok, next0;
+  auto plan = [&](int t) __attribute__((always_inline)) {
+    next0 = (first + t) * BR;
+    const int tok0 = uniform(row_token(a, next0));
+    if (!whole) place(next0);
+    rq = rsrc_words(qp + tok0 * a.q.sn, 0x7fffffff);
+    rg = rsrc_words(gp + tok0 * a.dout.sn, 0x7fffffff);
+    rs = rsrc_words((wave == 0 ? a.lse : a.delta) + (long long)pair * a.rows + next0, 0x7fffffff);
+    ring = uniform(lds0 + VALUES + (t & 1) * STAGE + wave * LOADS * 1024);
+    sums = uniform(lds0 + VALUES + (t & 1) * STAGE + 2 * TILE + wave * 256);
+    asm volatile("s_nop 4" : "+s"(rq), "+s"(rg), "+s"(rs), "+s"(ring), "+s"(sums));
+    lo_tok = from - tok0;
+    hi_tok = to - tok0;
+  };
+  auto load = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const bool in = (tok[i] >= lo) & (tok[i] < hi);
-      load_lds(rq, in ? oq[i] : kOob, at + i * 1024);
-      load_lds(rg, in ? og[i] : kOob, at + TILE + i * 1024);
+      const bool in = (tok[i] >= lo_tok) & (tok[i] < hi_tok);
+      load_lds(rq, in ? oq[i] : kOob, ring + i * 1024);
+      load_lds(rg, in ? og[i] : kOob, ring + TILE + i * 1024);
     }
-    if (wave < 2) load_lds4(rs, lane < BR && r0 + lane < a.rows ? lane * 4 : kOob, st);
+    if (wave < 2) load_lds4(rs, lane < BR && next0 + lane < a.rows ? lane * 4 : kOob, sums);
   };
 
   f32x16_t dk[DT], dv[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) dk[i] = dv[i] = zero16();
   const Straight<T, DP> values(lds0 + (KV ? 0 : wave * 32 * R::PITCH), lane);
-  if (t0 < t1) load(t0);
+  if (t0 < t1) {
+    plan(t0);
+    load();
+  }
   for (int t = t0; t < t1; ++t) {
+    plan(t + 1);
     load_wait<0>();
-    if (t + 1 < t1) load(t + 1);
-    const unsigned qt = lds0 + VALUES + (t & 1) * STAGE, gt = qt + TILE, st = gt + TILE;
+    if (t + 1 < t1) load();
+    const unsigned qt = lds0 + VALUES + (t & 1) * STAGE, gt = qt + TILE, ls = gt + TILE;
     const Straight<T, DP> queries(qt, lane), grads(gt, lane);
     const Transposed<T, DP> query_cols(qt, lane), grad_cols(gt, lane);
     const int r0 = (first + t) * BR, lo = s.start + row_token(a, r0), hi = s.start + row_token(a, r0 + BR - 1);
@@ -294,8 +315,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_d
       }
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        const f32x4_t lse = *(LDS_AS f32x4_t*)(uintptr_t)(st + (32 * i + 2 * e + 4 * h) * 4);
-        const f32x4_t delta = *(LDS_AS f32x4_t*)(uintptr_t)(st + 256 + (32 * i + 2 * e + 4 * h) * 4);
+        const f32x4_t lse = *(LDS_AS f32x4_t*)(uintptr_t)(ls + (32 * i + 2 * e + 4 * h) * 4);
+        const f32x4_t delta = *(LDS_AS f32x4_t*)(uintptr_t)(ls + 256 + (32 * i + 2 * e + 4 * h) * 4);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           x[e + q] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + q], a.scale2, -lse[q]));

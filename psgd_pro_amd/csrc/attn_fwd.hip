@@ -41,29 +41,35 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
 #pragma unroll
   for (int i = 0; i < DC; ++i) arrived(qf[i]);
 
-  int vk[LOADS], vv[LOADS], lrow[LOADS];
+  int vk[LOADS], vv[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
-    int chunk;
-    R::where(wave * LOADS + i, lane, lrow[i], chunk);
+    int row, chunk;
+    R::where(wave * LOADS + i, lane, row, chunk);
     const bool in = chunk * R::PER < a.d;
-    vk[i] = in ? (int)(lrow[i] * a.k.sn * R::E) + chunk * 16 : kOob;
-    vv[i] = in ? (int)(lrow[i] * a.v.sn * R::E) + chunk * 16 : kOob;
+    vk[i] = in ? (int)(row * a.k.sn * R::E) + chunk * 16 : kOob;
+    vv[i] = in ? (int)(row * a.v.sn * R::E) + chunk * 16 : kOob;
   }
   const T* const kp = static_cast<const T*>(a.k.p) + b * a.k.sb + head * a.k.sh;
   const T* const vp = static_cast<const T*>(a.v.p) + b * a.v.sb + head * a.v.sh;
-  auto load = [&](int t, int stage) __attribute__((always_inline)) {
+  // The next tile's loads: where from, found out in front of the wait for the last ones, and the loads themselves.
+  i32x4_t rk, rv;
+  unsigned to;
+  auto plan = [&](int t, int stage) __attribute__((always_inline)) {
     const int j0 = tiles.tile(t) * BK;
-    i32x4_t rk = rsrc_words(kp + j0 * a.k.sn, 0x7fffffff), rv = rsrc_words(vp + j0 * a.v.sn, 0x7fffffff);
-    unsigned to = uniform(lds0 + stage * 2 * TILE + wave * LOADS * 1024);
+    // (rows behind the sequence, whatever they hold, are behind the buffer's end and read as zeros)
+    rk = rsrc_words(kp + j0 * a.k.sn, ((s.len - j0 - 1) * a.k.sn + a.d) * R::E);
+    rv = rsrc_words(vp + j0 * a.v.sn, ((s.len - j0 - 1) * a.v.sn + a.d) * R::E);
+    to = uniform(lds0 + stage * 2 * TILE + wave * LOADS * 1024);
     // a scalar register that a vector instruction wrote may be read by a load 5 wait states later at the earliest, which
     // the compiler does not see to inside asm statements
     asm volatile("s_nop 4" : "+s"(rk), "+s"(rv), "+s"(to));
+  };
+  auto load = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {  // (rows behind the sequence, whatever they hold, read as zeros)
-      const bool in = j0 + lrow[i] < s.len;
-      load_lds(rk, in ? vk[i] : kOob, to + i * 1024);
-      load_lds(rv, in ? vv[i] : kOob, to + TILE + i * 1024);
+    for (int i = 0; i < LOADS; ++i) {
+      load_lds(rk, vk[i], to + i * 1024);
+      load_lds(rv, vv[i], to + TILE + i * 1024);
     }
   };
 
@@ -72,11 +78,15 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = zero16();
 
-  if (t0 < t1) load(t0, 0);
+  if (t0 < t1) {
+    plan(t0, 0);
+    load();
+  }
   for (int t = t0; t < t1; ++t) {
     const int stage = (t - t0) & 1, j0 = tiles.tile(t) * BK;
+    plan(t + 1, stage ^ 1);
     load_wait<0>();
-    if (t + 1 < t1) load(t + 1, stage ^ 1);
+    if (t + 1 < t1) load();
     const unsigned kt = lds0 + stage * 2 * TILE + wk * (32 * KT) * R::PITCH;
     const Straight<T, DP> keys(kt, lane);
     const Transposed<T, DP> values(kt + TILE, lane);
