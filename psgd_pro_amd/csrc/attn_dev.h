@@ -206,6 +206,12 @@ __device__ __forceinline__ int part_begin(int n, int part, int parts) { return u
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
+// over both halves, each lane of which gets it
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // a sequence: its tokens and the position of its first query
 struct Seq {
   int len, start;

@@ -14,7 +14,7 @@ template <typename T, int DP, int WQ, int WK, int BK>
 __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP == 128 ? 1 : 2) attn_forward_kernel(const AttnArgs a, int row_tiles) {
   using R = Rows<T, DP>;
   constexpr int W = WQ * WK, LOADS = R::loads(BK, W), TILE = BK * R::PITCH, KT = BK / WK / 32, DC = DP / 16, DT = DP / 32;
-  constexpr int AHEAD = DT < 4 ? 2 : sizeof(T) == 2 ? 4 : 2;  // at most KT DC and 2 KT DT
+  constexpr int AHEAD = DT < 4 || sizeof(T) == 4 ? 2 : 4;  // at most KT DC and 2 KT DT
   static_assert(LOADS * W * 1024 == TILE && KT * WK * 32 == BK, "whole loads, whole blocks of keys");
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
@@ -91,65 +91,94 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
     const Straight<T, DP> keys(kt, lane);
     const Transposed<T, DP> values(kt + TILE, lane);
 
+    // Keys 32 by 32: their scores, their probabilities beside the products that come next (the next 32 keys' scores, the last
+    // ones' values).
     f32x16_t x[KT];
-#pragma unroll
-    for (int i = 0; i < KT; ++i) x[i] = zero16();
-    frag_t<T> f[AHEAD];
-    const auto key_frag = [&](int i) __attribute__((always_inline)) { return keys(i % KT, i / KT); };
-    first_loads<T>(f, key_frag);
-    __builtin_amdgcn_s_setprio(1);
-    ahead<T, KT * DC>(f, key_frag, [&](int i, frag_t<T> y) __attribute__((always_inline)) {
-      x[i % KT] = mma(y, qf[i / KT], x[i % KT]);
-    });
+    frag_t<T> p[2 * KT], f[AHEAD];
+    const bool look = j0 + BK - 1 > lo || hi >= s.len || (hi - j0 >= a.window && j0 + BK > a.sinks);
+    float mu = 0.f;
+    const auto key_frag = [&](int i) __attribute__((always_inline)) { return keys(i / DC, i % DC); };
     const auto value_frag = [&](int i) __attribute__((always_inline)) { return values(i / DT, i % DT); };
-    __builtin_amdgcn_s_setprio(0);
-    first_loads<T>(f, value_frag);
-    // all keys of the tile are visible to all rows, or each is looked at
-    if (j0 + BK - 1 > lo || hi >= s.len || (hi - j0 >= a.window && j0 + BK > a.sinks)) {
-      const int j = j0 + wk * 32 * KT + 4 * h;
-#pragma unroll
-      for (int i = 0; i < KT; ++i)
+    // the mask and the reference of keys i
+    const auto follow = [&](int i) __attribute__((always_inline)) {
+      if (look) {
+        const int j = j0 + wk * 32 * KT + 32 * i + 4 * h;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = j + 32 * i + 8 * (e >> 2) + (e & 3);
+          const int key = j + 8 * (e >> 2) + (e & 3);
           x[i][e] = (key <= pos) & ((pos - key < a.window) | (key < a.sinks)) ? x[i][e] : -INFINITY;
         }
-    }
-    float top = x[0][0];
-#pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
-    top = fmaxf(top, other_half(top)) * a.scale2;
-    // The reference follows the largest score only where that is over it by more than 2^8: the sums have room for that, and
-    // the products are rarely scaled then.
-    if (__any(top > ref + 8.f)) {
-      const float next = fmaxf(ref, top), by = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - next);
-      ref = next;
-      sum *= by;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] *= by;
-    }
-    const float mu = ref == -INFINITY ? 0.f : ref;
-#pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], a.scale2, -mu));
       }
-    // (bf16: the probabilities are rounded for the matrix cores, and their sum is of the rounded ones)
-    frag_t<T> p[2 * KT];
+      float top = x[i][0];
 #pragma unroll
-    for (int i = 0; i < 2 * KT; ++i) {
-      p[i] = crossed<T>(x[i / 2], i % 2);
-      sum = sum_of(p[i], sum);
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, x[i][e]);
+      top = max_halves(top) * a.scale2;
+      // The reference follows the largest score only where that is over it by more than 2^8: the sums have room for that, and
+      // the products are rarely scaled then.
+      if (__any(top > ref + 8.f)) {
+        const float next = fmaxf(ref, top), by = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - next);
+        ref = next;
+        sum *= by;
+#pragma unroll
+        for (int k = 0; k < DT; ++k)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[k][e] *= by;
+        if (i > 0) {  // (whose values are not added yet)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[0][e] *= by;
+          p[0] = crossed<T>(x[0], 0);
+          p[1] = crossed<T>(x[0], 1);
+        }
+      }
+      mu = ref == -INFINITY ? 0.f : ref;
+    };
+    // (bf16: the probabilities are rounded for the matrix cores, and their sum is of the rounded ones)
+    const auto probability = [&](int i, int e) __attribute__((always_inline)) {
+      float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], a.scale2, -mu));
+      arrived(v);  // (here, beside a product)
+      x[i][e] = v;
+      if (e % 8 == 7) {
+        p[2 * i + e / 8] = crossed<T>(x[i], e / 8);
+        sum = sum_of(p[2 * i + e / 8], sum);
+      }
+    };
+    first_loads<T>(f, key_frag);
+    __builtin_amdgcn_s_setprio(1);
+    x[0] = zero16();
+#pragma unroll
+    for (int i = 0; i < DC; ++i) {
+      x[0] = mma(f[i % AHEAD], qf[i], x[0]);
+      if (i + AHEAD < KT * DC) f[i % AHEAD] = key_frag(i + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    follow(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (KT == 2) {
+      x[1] = zero16();
+#pragma unroll
+      for (int i = 0; i < DC; ++i) {
+        x[1] = mma(f[(DC + i) % AHEAD], qf[i], x[1]);
+        if (DC + i + AHEAD < 2 * DC) f[(DC + i) % AHEAD] = key_frag(DC + i + AHEAD);
+#pragma unroll
+        for (int e = i * 16 / DC; e < (i + 1) * 16 / DC; ++e) probability(0, e);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      first_loads<T>(f, value_frag);
+      follow(1);
+    } else {
+      first_loads<T>(f, value_frag);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) probability(0, e);
     }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
     ahead<T, 2 * KT * DT>(f, value_frag, [&](int i, frag_t<T> y) __attribute__((always_inline)) {
       o[i % DT] = mma(y, p[i / DT], o[i % DT]);
+      if (KT == 2 && i < 2 * DT) {
+#pragma unroll
+        for (int e = i * 16 / (2 * DT); e < (i + 1) * 16 / (2 * DT); ++e) probability(KT - 1, e);
+      }
     });
     __builtin_amdgcn_s_setprio(0);
   }
