@@ -9,7 +9,8 @@ namespace psgdk {
 namespace {
 
 // With P the probabilities, dP = dO V^T, delta = sum of o dO over a row:  dS = P (dP - delta),  dQ = scale dS K.
-// Transposed as the forward pass: a lane has one row, dS^T is the last product's operand where it is made.
+// Transposed as the forward pass: a lane has one row, dS^T is the last product's operand where it is made. 4 x 4096 tokens, 32 / 8
+// heads of 128, bf16: 790 us, 6 d flops a visible pair at 1050 TFLOP/s (the matrix cores busy 56% of the cycles).
 template <typename T, int DP, int BK>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_dq_kernel(const AttnArgs a, int row_tiles) {
   using R = Rows<T, DP>;
@@ -159,7 +160,8 @@ __device__ __forceinline__ void store4(T* out, float y0, float y1, float y2, flo
 // the second products' operands where they are made (dV^T = dO^T P, dK^T = Q^T dS), and a tile of rows serves straight and
 // transposed. Key tiles that hold sinks are seen by all rows: their rows are cut in parts, whose sums attn_dkv_sum adds.
 // KV: the tile's keys and values are fragments in registers; else the values are in LDS (bf16 heads of 128 then fit two waves
-// a SIMD: 1750 -> 1400 us of 4 x 4096 tokens with 32 / 8 heads; 1050 with the tiles of the most rows first).
+// a SIMD: 1750 -> 1400 us of 4 x 4096 tokens with 32 / 8 heads; 1060 with the tiles of the most rows first,
+// 8 d flops a pair at 1040 TFLOP/s).
 template <typename T, int DP, int BR, bool KV>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_dkv_kernel(const AttnArgs a, int key_tiles) {
   using R = Rows<T, DP>;
@@ -434,8 +436,8 @@ int attn_dkv_rows(const AttnArgs& a) { return a.dt == 0 || a.d > 96 ? 32 : 64; }
 
 // Key tiles with sinks, which all rows see, are cut in as many parts as leave each about the rows of another tile's. The others
 // are cut where a round of workgroups would otherwise leave CUs idle: 512 (256 where a wave has a SIMD's registers to itself) run
-// at once, and 564 of equal work take as long as 1024 (16384 tokens, window 1024, 16 / 4 heads of 64: 340 us uncut, XX cut). A
-// part costs about 8 tiles of rows for its keys, its sums and their addition.
+// at once, and 564 of equal work take as long as 1024 (16384 tokens, window 1024, 16 / 4 heads of 64: 340 us uncut, 230 in three
+// parts and 18 adding them). A part costs about 8 tiles of rows for its keys, its sums and their addition.
 void attn_backward_parts(AttnArgs& a) {
   const long long br = attn_dkv_rows(a), pairs = (long long)a.batch * a.kv, tiles = (a.m + kAttnKeys - 1) / kAttnKeys;
   const long long all = (a.rows + br - 1) / br;

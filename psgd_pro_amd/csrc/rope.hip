@@ -80,7 +80,10 @@ __device__ __forceinline__ const T* head_of(const RopeSide& x, long long b, long
 
 // A wave has a token (or `waves` waves share its heads), 64 / lanes heads at a time, so that the rotation's angles are made
 // once for all heads. A lane has V pairs of elements S times: pair i of the rotated part is (i, i + rot / 2), or (2 i, 2 i + 1)
-// interleaved, and of the rest, which is only normalised, (2 i, 2 i + 1).
+// interleaved, and of the rest, which is only normalised, (2 i, 2 i + 1). Forward: memory (4 x 4096 tokens, 32 + 8 heads of 128,
+// bf16: 61 us, 5.5 TB/s). Backward the same bytes and half as much again in 119 us, 4.2 TB/s: the vector unit, and two row sums in
+// series; with the next heads' loads on their way it took 167 of then 154, and queries apart from keys saved 13 (no weight and
+// no sum is chosen by the lane).
 template <typename T, int V, int S, bool INTER, bool BACK>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
