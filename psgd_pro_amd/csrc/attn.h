@@ -29,6 +29,7 @@ struct AttnArgs {
   // backward
   void *dq, *dk, *dv;                 // null: not wanted; dq as (batch, n, heads, d), dk and dv as (batch, m, kv, d)
   float* delta;                       // [batch][kv][rows]: sum of o do over d, written by the dq pass
+  int* row_pos;                       // the same: the row's position, -1 where it sees nothing
   int sink_tiles, sink_parts, rest_parts;  // key tiles that hold sinks, and parts of the rows they and the others are cut in
   float* part_kv;                     // [tile parts][2][128][dp] sums of dk and dv where a tile has more than one part
 };

@@ -46,7 +46,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_d
   }
   delta += other_half(delta);
   const long long at = (long long)pair * a.rows + r;
-  if (there && h == 0) a.delta[at] = delta;
+  if (there && h == 0) {
+    a.delta[at] = delta;
+    a.row_pos[at] = pos;
+  }
   if (!a.dq) return;
   float lse = there ? a.lse[at] : 0.f;
   arrived(lse);
@@ -232,6 +235,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_d
   };
   const bool whole = BR % a.group == 0;
   place(0);
+  const float* const of_rows = wave == 0 ? a.lse : wave == 1 ? a.delta : reinterpret_cast<const float*>(a.row_pos);
   i32x4_t rq, rg, rs;
   unsigned ring, sums;
   int lo_tok, hi_tok, next0;
@@ -241,7 +245,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_d
     if (!whole) place(next0);
     rq = rsrc_words(qp + tok0 * a.q.sn, 0x7fffffff);
     rg = rsrc_words(gp + tok0 * a.dout.sn, 0x7fffffff);
-    rs = rsrc_words((wave == 0 ? a.lse : a.delta) + (long long)pair * a.rows + next0, 0x7fffffff);
+    rs = rsrc_words(of_rows + (long long)pair * a.rows + next0, 0x7fffffff);
     ring = uniform(lds0 + VALUES + (t & 1) * STAGE + wave * LOADS * 1024);
     sums = uniform(lds0 + VALUES + (t & 1) * STAGE + 2 * TILE + wave * 256);
     asm volatile("s_nop 4" : "+s"(rq), "+s"(rg), "+s"(rs), "+s"(ring), "+s"(sums));
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_d
       load_lds(rq, in ? oq[i] : kOob, ring + i * 1024);
       load_lds(rg, in ? og[i] : kOob, ring + TILE + i * 1024);
     }
-    if (wave < 2) load_lds4(rs, lane < BR && next0 + lane < a.rows ? lane * 4 : kOob, sums);
+    if (wave < 3) load_lds4(rs, lane < BR && next0 + lane < a.rows ? lane * 4 : kOob, sums);
   };
 
   f32x16_t dk[DT], dv[DT];
@@ -308,11 +312,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_d
         return s / DT % 2 ? query_cols(2 * i + s / (2 * DT), s % DT) : grad_cols(2 * i + s / (2 * DT), s % DT);
       };
       first_loads<T>(f, col_frags);
-      if (look) {
+      if (look) {  // (rows that are not loaded see none of the keys)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int at = row_token(a, r0 + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3)), pos = s.start + at;
-          x[e] = (at < to) & (key <= pos) & ((pos - key < a.window) | (key < a.sinks)) ? x[e] : -INFINITY;
+        for (int e = 0; e < 16; e += 4) {
+          const i32x4_t pos = *(LDS_AS i32x4_t*)(uintptr_t)(ls + 512 + (32 * i + 2 * e + 4 * h) * 4);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            x[e + q] = (key <= pos[q]) & ((pos[q] - key < a.window) | (key < a.sinks)) ? x[e + q] : -INFINITY;
         }
       }
 #pragma unroll

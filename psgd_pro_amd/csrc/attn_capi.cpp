@@ -236,6 +236,7 @@ int psgdk_window_attention_backward(const psgdk_window_attention_t* q, const psg
   a.dv = g->dv;
   Ws m(ws);
   a.delta = m.take<float>((size_t)a.batch * a.kv * a.rows);
+  a.row_pos = m.take<int>((size_t)a.batch * a.kv * a.rows);
   if (a.dk || a.dv) a.part_kv = m.take<float>((size_t)attn_part_tiles(a) * 2 * kAttnKeys * attn_dp(a.d));
   if (!ws) {
     *ws_bytes = m.off;
