@@ -402,7 +402,8 @@ int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const fl
  * is at position p = starts[b] + i (starts NULL: m - n + i, the last of the m tokens) and sees key j where
  *   0 <= p < length,  j <= p  and  (p - j < window or j < sinks),   length = lengths[b] (NULL: m; clamped to 0 .. m);
  * window 0: all of them. o = sum_j softmax_j(scale q . k_j) v_j, 0 where nothing is seen; query head h takes the keys of head
- * h / (heads / kv_heads). Keys and values from `length` on, and queries and their gradients that see nothing, may hold anything.
+ * h / (heads / kv_heads). Keys and values from `length` on, and queries and their gradients that see nothing, may hold anything;
+ * an infinity or NaN within a sequence may reach rows that do not see it.
  * Sums are added in an order that the sizes alone set. With bf16 the probabilities and, backward, the scores' gradients are
  * rounded to bf16 before the matrix cores take them.
  * d: a multiple of 8 up to 128; n and m up to 2^28; with rows = n heads / kv_heads, up to 2^31 - 256, batch kv_heads rows / 32 under
@@ -422,6 +423,8 @@ typedef struct psgdk_window_attention {
   void* o;                  /* (batch, n, heads, d), contiguous: output of the forward call, input of the backward call */
   float* lse;               /* [batch][kv_heads][n][heads / kv_heads]: log2 of the row's sum of e^score, output of the forward
                                call (NULL: not stored), input of the backward call */
+  void* o_rest;             /* optional, as o: what rounding to bf16 took from o, output of the forward call, input of the
+                               backward call, whose gradients it makes a tenth more exact (not used with fp32) */
 } psgdk_window_attention_t;
 int psgdk_window_attention(const psgdk_window_attention_t* a, void* ws, size_t* ws_bytes, psgdk_stream_t stream);
 

@@ -83,7 +83,7 @@ class WindowAttention(C.Structure):
     _fields_ = [("batch", C.c_int64), ("n", C.c_int64), ("m", C.c_int64), ("heads", C.c_int32), ("kv_heads", C.c_int32),
                 ("d", C.c_int32), ("dtype", C.c_int32), ("window", C.c_int64), ("sinks", C.c_int64), ("scale", C.c_float),
                 ("q", Heads), ("k", Heads), ("v", Heads), ("lengths", C.c_void_p), ("starts", C.c_void_p), ("o", C.c_void_p),
-                ("lse", C.c_void_p)]
+                ("lse", C.c_void_p), ("o_rest", C.c_void_p)]
 
 
 class WindowAttentionGrads(C.Structure):

@@ -53,6 +53,7 @@ def _launch(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
     a = L.AdamW(len(params), bits, at, at + n, at + 2 * n, at + 3 * n, at + 4 * n, at + 5 * n, *scales, lr, betas[0], betas[1], eps,
                 weight_decay, max_norm or 0.0, step, seed, None if norm is None else norm.data_ptr())
     _run_ws(params[0], L.lib().psgdk_adamw, C.byref(a))
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])  # (as torch's own in-place operations)
     return norm
 
 

@@ -30,40 +30,41 @@ def _heads(t):
     return L.Heads(t.data_ptr(), sb, sn, sh), t
 
 
-def _attn_block(q, k, v, lengths, starts, o, lse, opt):
+def _attn_block(q, k, v, lengths, starts, o, lse, rest, opt):
     """psgdk_window_attention_t of the inputs, and the (possibly copied) tensors it points to."""
     window, sinks, scale = opt
     a = L.WindowAttention(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], L.dtype_code(q.dtype), window,
                           sinks, scale)
     (a.q, q), (a.k, k), (a.v, v) = _heads(q), _heads(k), _heads(v)
-    a.lengths, a.starts, a.o, a.lse = _ptr(lengths), _ptr(starts), o.data_ptr(), _ptr(lse)
+    a.lengths, a.starts, a.o, a.lse, a.o_rest = _ptr(lengths), _ptr(starts), o.data_ptr(), _ptr(lse), _ptr(rest)
     return a, (q, k, v)
 
 
 def _attn_forward(q, k, v, lengths, starts, opt, stats):
     o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32) if stats else None
+    rest = torch.empty_like(o) if stats and q.dtype == torch.bfloat16 else None
     if not q.numel():
-        return o, lse
+        return o, lse, rest
     if not k.numel():  # no key to see
-        return o.zero_(), None if lse is None else lse.zero_()
-    a, keep = _attn_block(q, k, v, lengths, starts, o, lse, opt)
+        return o.zero_(), lse, rest
+    a, keep = _attn_block(q, k, v, lengths, starts, o, lse, rest, opt)
     _run_ws(q, L.lib().psgdk_window_attention, C.byref(a))
-    return o, lse
+    return o, lse, rest
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, starts, opt):
-        o, lse = _attn_forward(q, k, v, lengths, starts, opt, True)
+        o, lse, rest = _attn_forward(q, k, v, lengths, starts, opt, True)
         ctx.opt = opt
-        ctx.save_for_backward(q, k, v, lengths, starts, o, lse)
+        ctx.save_for_backward(q, k, v, lengths, starts, o, lse, rest)
         return o
 
     @staticmethod
     def backward(ctx, do):
         _once()
-        q, k, v, lengths, starts, o, lse = ctx.saved_tensors
+        q, k, v, lengths, starts, o, lse, rest = ctx.saved_tensors
         outs = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if need else None
                 for t, need in zip((q, k, v), ctx.needs_input_grad)]
         if not q.numel() or not k.numel():
@@ -71,7 +72,7 @@ class _WindowAttention(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
             return (*outs, None, None, None)
-        a, keep = _attn_block(q, k, v, lengths, starts, o, lse, ctx.opt)
+        a, keep = _attn_block(q, k, v, lengths, starts, o, lse, rest, ctx.opt)
         g = L.WindowAttentionGrads()
         g.dout, do = _heads(do)
         g.dq, g.dk, g.dv = (_ptr(t) for t in outs)
@@ -94,7 +95,9 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, lengths=None,
                                                                      last n tokens of each sequence.
 
     A query that sees nothing has output 0 and no gradient; keys and values from lengths[b] on, and queries and gradients of
-    positions outside the sequence, may hold anything. scale: 1 / sqrt(d) if not given. Differentiable in q, k and v."""
+    positions outside the sequence, may hold anything. Within a sequence values are taken to be finite: an infinity or NaN may
+    reach queries that do not see it. bfloat16 probabilities, and backward the scores' gradients, are rounded before the second
+    products. Two runs give the same bits. scale: 1 / sqrt(d) if not given. Differentiable in q, k and v."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         _check(t, name, None if t is q else q)
         if t.dim() != 4 or t.dtype != q.dtype:

@@ -20,6 +20,7 @@ struct AttnArgs {
   float scale, scale2;                // of the scores, and times log2 e
   AttnSide q, k, v;
   AttnSide o, dout;                   // o: written by the forward call, read by the backward call
+  bf16_t* rest;                       // laid out as o, bf16 only: o before its rounding less o (null: not kept)
   const int64_t *lengths, *starts;    // one a sequence in device memory (null: m, m - n)
   float* lse;                         // log2 of a row's sum of e^score: [batch][kv][rows] (forward: null, not stored)
   // forward: the key tiles of a row tile in `parts`; with more than one, each leaves its sums and the largest scores

@@ -43,6 +43,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_d
     const frag_t<T> of = row_frag<T>(op, 16 * i + 8 * h, a.d, pos >= 0);
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta += (float)gf[i][e] * (float)of[e];
+    if constexpr (sizeof(T) == 2) {  // (o's rounding alone would put a third on the gradients' error)
+      if (a.rest) {
+        const frag_t<T> rf = row_frag<T>(a.rest + (op - static_cast<const T*>(a.o.p)), 16 * i + 8 * h, a.d, pos >= 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta += (float)gf[i][e] * (float)rf[e];
+      }
+    }
   }
   delta += other_half(delta);
   const long long at = (long long)pair * a.rows + r;

@@ -81,6 +81,8 @@ int attn_pointers(const psgdk_window_attention_t* q, AttnArgs& a) {
   if (!q->o || (reinterpret_cast<uintptr_t>(q->o) & 15)) return fail(PSGDK_EINVAL, "o: a device pointer of 16-byte alignment");
   const int64_t sn = (int64_t)q->heads * q->d;
   a.o = AttnSide{q->o, q->n * sn, sn, q->d};
+  if (reinterpret_cast<uintptr_t>(q->o_rest) & 15) return fail(PSGDK_EINVAL, "o_rest: 16-byte alignment");
+  a.rest = a.dt == PSGDK_BF16 ? static_cast<bf16_t*>(q->o_rest) : nullptr;
   return PSGDK_OK;
 }
 

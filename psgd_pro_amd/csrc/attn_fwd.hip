@@ -238,8 +238,16 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
       const int col = 32 * i + 2 * e + 4 * h;
       if (col >= a.d) continue;
       const float y0 = o[i][e] * inv, y1 = o[i][e + 1] * inv, y2 = o[i][e + 2] * inv, y3 = o[i][e + 3] * inv;
-      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + col) = make_uint2(pack2_bf16(y0, y1), pack2_bf16(y2, y3));
-      else *reinterpret_cast<f32x4_t*>(out + col) = f32x4_t{y0, y1, y2, y3};
+      if constexpr (sizeof(T) == 2) {
+        const uint2 w = make_uint2(pack2_bf16(y0, y1), pack2_bf16(y2, y3));
+        *reinterpret_cast<uint2*>(out + col) = w;
+        if (a.rest)
+          *reinterpret_cast<uint2*>(a.rest + (out - static_cast<const T*>(a.o.p)) + col) =
+              make_uint2(pack2_bf16(y0 - __uint_as_float(w.x << 16), y1 - __uint_as_float(w.x & 0xffff0000u)),
+                         pack2_bf16(y2 - __uint_as_float(w.y << 16), y3 - __uint_as_float(w.y & 0xffff0000u)));
+      } else {
+        *reinterpret_cast<f32x4_t*>(out + col) = f32x4_t{y0, y1, y2, y3};
+      }
     }
   if (a.lse && h == 0) a.lse[(long long)pair * a.rows + r] = sum == 0.f ? 0.f : ref + __builtin_amdgcn_logf(sum);
 }
@@ -281,7 +289,11 @@ __global__ void __launch_bounds__(32 * G) attn_join_kernel(const AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < G; ++i) x += buf[i][tid];
     T* const out = static_cast<T*>(const_cast<void*>(a.o.p)) + b * a.o.sb + tok * a.o.sn + (head * a.group + g) * a.o.sh;
-    out[tid] = from_f32<T>(total == 0.f ? 0.f : x / total);
+    const float y = total == 0.f ? 0.f : x / total;
+    out[tid] = from_f32<T>(y);
+    if constexpr (sizeof(T) == 2) {
+      if (a.rest) a.rest[(out - static_cast<const T*>(a.o.p)) + tid] = f32_to_bf16(y - to_f32<T>(out[tid]));
+    }
   }
   if (tid == 0 && a.lse) a.lse[row] = total == 0.f ? 0.f : top + __builtin_amdgcn_logf(total);
 }

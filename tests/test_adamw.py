@@ -343,6 +343,17 @@ def test_closure_and_state_dict(bits):
         P.AdamW([rnd((41, 30), 1).requires_grad_()], state_bits=bits).load_state_dict(saved)
 
 
+def test_a_step_between_forward_and_backward_is_noticed():
+    w = rnd((4, 4), 1).requires_grad_()
+    opt = P.AdamW(w)
+    loss = (w ** 2).sum()
+    P.AdamW(w)  # (making one changes nothing)
+    torch.autograd.grad(loss, w, retain_graph=True)
+    opt.step_math([rnd((4, 4), 2)])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, w)
+
+
 def test_captures_are_refused():
     ps, gs, ms, vs = tensors(torch.float32, shapes=[(5,)])
     P.adamw_step(ps, gs, ms, vs, step=1)

@@ -37,7 +37,7 @@ BAD_ATTN = [
 BAD_POINTERS = [
     (dict(q=heads(p=None)), L.EINVAL), (dict(k=heads(p=PTR + 8)), L.EINVAL), (dict(v=heads(sn=60)), L.ESHAPE), (dict(q=heads(sh=36)), L.ESHAPE),
     (dict(q=heads(sb=4100)), L.ESHAPE), (dict(k=heads(sb=-4096)), L.ESHAPE), (dict(k=heads(sn=-64)), L.ESHAPE), (dict(v=heads(sn=1 << 22)), L.ESHAPE),
-    (dict(q=heads(sh=1 << 22)), L.ESHAPE), (dict(o=None), L.EINVAL), (dict(o=PTR + 2), L.EINVAL)]
+    (dict(q=heads(sh=1 << 22)), L.ESHAPE), (dict(o=None), L.EINVAL), (dict(o=PTR + 2), L.EINVAL), (dict(o_rest=PTR + 8), L.EINVAL)]
 
 
 @pytest.mark.parametrize("kw,code", BAD_ATTN + BAD_POINTERS)
