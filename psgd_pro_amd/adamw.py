@@ -44,6 +44,7 @@ def _check_numbers(step, lr, betas, eps, weight_decay, max_norm):
 
 
 def _launch(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm, seed):
+    from . import _tables as T  # (as above)
     buf, bits, keep = _tables(params, grads, ms, vs)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("psgd_pro_amd: an AdamW step is not captured into a graph (its number would stay the same)")
@@ -53,7 +54,7 @@ def _launch(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
     a = L.AdamW(len(params), bits, at, at + n, at + 2 * n, at + 3 * n, at + 4 * n, at + 5 * n, *scales, lr, betas[0], betas[1], eps,
                 weight_decay, max_norm or 0.0, step, seed, None if norm is None else norm.data_ptr())
     _run_ws(params[0], L.lib().psgdk_adamw, C.byref(a))
-    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])  # (as torch's own in-place operations)
+    T.changed(params)  # (as by torch's own in-place operations)
     return norm
 
 

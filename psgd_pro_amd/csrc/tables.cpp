@@ -111,7 +111,19 @@ PyObject* adamw(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {{"adamw", adamw, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+// changed(params): they count as changed in place, as by torch's own operations.
+PyObject* changed(PyObject*, PyObject* params) {
+  HANDLE_TH_ERRORS
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
+    const at::Tensor& p = *tensor(PyList_GET_ITEM(params, i));
+    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {
+    {"adamw", adamw, METH_VARARGS, nullptr}, {"changed", changed, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tables", nullptr, -1, methods};
 
 }  // namespace
