@@ -34,22 +34,28 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_d
   const T* const qp = static_cast<const T*>(a.q.p) + b * a.q.sb + tok * a.q.sn + qh * a.q.sh;
   const T* const gp = static_cast<const T*>(a.dout.p) + b * a.dout.sb + tok * a.dout.sn + qh * a.dout.sh;
   const T* const op = static_cast<const T*>(a.o.p) + b * a.o.sb + tok * a.o.sn + qh * a.o.sh;
+  const T* const some = static_cast<const T*>(a.q.p);
+  const T* const lp = sizeof(T) == 2 && a.rest ? reinterpret_cast<const T*>(a.rest) + (op - static_cast<const T*>(a.o.p)) : nullptr;
   frag_t<T> qf[DC], gf[DC];
   float delta = 0.f;
+  {
+    frag_t<T> of[DC], rf[DC];
 #pragma unroll
-  for (int i = 0; i < DC; ++i) {
-    qf[i] = row_frag<T>(qp, 16 * i + 8 * h, a.d, pos >= 0);
-    gf[i] = row_frag<T>(gp, 16 * i + 8 * h, a.d, pos >= 0);
-    const frag_t<T> of = row_frag<T>(op, 16 * i + 8 * h, a.d, pos >= 0);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) delta += (float)gf[i][e] * (float)of[e];
-    if constexpr (sizeof(T) == 2) {  // (o's rounding alone would put a third on the gradients' error)
-      if (a.rest) {
-        const frag_t<T> rf = row_frag<T>(a.rest + (op - static_cast<const T*>(a.o.p)), 16 * i + 8 * h, a.d, pos >= 0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) delta += (float)gf[i][e] * (float)rf[e];
-      }
+    for (int i = 0; i < DC; ++i) {
+      const int k = 16 * i + 8 * h;
+      gf[i] = row_frag<T>(gp, k, a.d, pos >= 0, some);
+      of[i] = row_frag<T>(op, k, a.d, pos >= 0, some);
+      if constexpr (sizeof(T) == 2) rf[i] = row_frag<T>(lp, k, a.d, pos >= 0 && lp, some);
+      qf[i] = row_frag<T>(qp, k, a.d, pos >= 0, some);
     }
+#pragma unroll
+    for (int i = 0; i < DC; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        delta += (float)gf[i][e] * (float)of[i][e];
+        // (o's rounding would put a tenth on the gradients' error)
+        if constexpr (sizeof(T) == 2) delta += (float)gf[i][e] * (float)rf[i][e];
+      }
   }
   delta += other_half(delta);
   const long long at = (long long)pair * a.rows + r;
@@ -204,8 +210,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_d
   frag_t<T> kf[DC], vf[KV ? DC : 1];
 #pragma unroll
   for (int i = 0; i < DC; ++i) {
-    kf[i] = row_frag<T>(kp + key * a.k.sn, 16 * i + 8 * h, a.d, key < s.len);
-    if constexpr (KV) vf[i] = row_frag<T>(vp + key * a.v.sn, 16 * i + 8 * h, a.d, key < s.len);
+    kf[i] = row_frag<T>(kp + key * a.k.sn, 16 * i + 8 * h, a.d, key < s.len, static_cast<const T*>(a.k.p));
+    if constexpr (KV) vf[i] = row_frag<T>(vp + key * a.v.sn, 16 * i + 8 * h, a.d, key < s.len, static_cast<const T*>(a.v.p));
   }
 #pragma unroll
   for (int i = 0; i < DC; ++i) {

@@ -169,21 +169,24 @@ __device__ __forceinline__ void first_loads(frag_t<T> (&f)[D], Load load) {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// 8 elements at p + k for k = 16 c + 8 h, zeros from d on (d a multiple of 8) or where !ok, times `by`
+// 8 elements at p + k for k = 16 c + 8 h, zeros from d on (d a multiple of 8) or where !ok; `some` is what is read then (no
+// branch: the loads of a row are on their way together)
 template <typename T>
-__device__ __forceinline__ frag_t<T> row_frag(const T* p, int k, int d, bool ok) {
+__device__ __forceinline__ frag_t<T> row_frag(const T* p, int k, int d, bool ok, const T* some) {
+  ok = ok & (k < d);
+  const T* const at = ok ? p + k : some;
   frag_t<T> f;
-  if (ok && k < d) {
-    if constexpr (sizeof(T) == 2) {
-      f = *reinterpret_cast<const frag_t<T>*>(p + k);
-    } else {
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p + k), y = *reinterpret_cast<const f32x4_t*>(p + k + 4);
-      f = frag_t<T>{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-    }
+  if constexpr (sizeof(T) == 2) {
+    f = *reinterpret_cast<const frag_t<T>*>(at);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0;
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(at), y = *reinterpret_cast<const f32x4_t*>(at + 4);
+    f = frag_t<T>{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   }
+  uint32_t w[sizeof f / 4];
+  __builtin_memcpy(w, &f, sizeof f);
+#pragma unroll
+  for (uint32_t& v : w) v = ok ? v : 0;
+  __builtin_memcpy(&f, w, sizeof f);
   return f;
 }
 

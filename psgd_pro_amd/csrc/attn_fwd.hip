@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
   const T* const qp = static_cast<const T*>(a.q.p) + b * a.q.sb + tok * a.q.sn + (head * a.group + g) * a.q.sh;
   frag_t<T> qf[DC];
 #pragma unroll
-  for (int i = 0; i < DC; ++i) qf[i] = row_frag<T>(qp, 16 * i + 8 * h, a.d, pos >= 0);
+  for (int i = 0; i < DC; ++i) qf[i] = row_frag<T>(qp, 16 * i + 8 * h, a.d, pos >= 0, static_cast<const T*>(a.q.p));
 #pragma unroll
   for (int i = 0; i < DC; ++i) arrived(qf[i]);
 
