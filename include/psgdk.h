@@ -409,7 +409,8 @@ int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const fl
  * d: a multiple of 8 up to 128; n and m up to 2^28; with rows = n heads / kv_heads, up to 2^31 - 256, batch kv_heads rows / 32 under
  * 2^24, and backward batch kv_heads m / 128 under 2^23. */
 typedef struct psgdk_heads { /* (batch, tokens, heads, d), d contiguous; strides in elements, whole 16 bytes and up to 2^21 for
-                                tokens and (up to 128 heads; in inverse proportion for more) heads; 16-byte aligned */
+                                tokens and, of q and dout, for heads (in inverse proportion for more than 128; of k and v any
+                                distance apart); 16-byte aligned */
   const void* p;
   int64_t batch_stride, token_stride, head_stride;
 } psgdk_heads_t;

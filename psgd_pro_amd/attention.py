@@ -16,15 +16,16 @@ from .train import _NORMS, _check, _once, _ptr, _run, _run_ws, _wants_grad
 
 __all__ = ["qk_norm_rope", "window_attention"]
 
-_MAX_STRIDE = 1 << 21  # of tokens and heads, in elements
+_MAX_STRIDE = 1 << 21  # of tokens, and of queries' heads, in elements
 
 
-def _heads(t):
-    """(psgdk_heads_t of t, the tensor it points to): t itself where its rows are aligned, else a copy."""
+def _heads(t, keys=False):
+    """(psgdk_heads_t of t, the tensor it points to): t itself where its rows are aligned, else a copy. Heads of keys may lie any
+    distance apart (a cache of each head's tokens), those of queries are rows of one tile."""
     unit = 16 // t.element_size()
     sb, sn, sh, sd = t.stride()
     if (sd != 1 or t.data_ptr() % 16 or sb % unit or sn % unit or sh % unit or sn > _MAX_STRIDE
-            or sh * max(t.shape[2], 128) > _MAX_STRIDE * 128):
+            or (not keys and sh * max(t.shape[2], 128) > _MAX_STRIDE * 128)):
         t = t.clone(memory_format=torch.contiguous_format)
         sb, sn, sh, _ = t.stride()
     return L.Heads(t.data_ptr(), sb, sn, sh), t
@@ -35,7 +36,7 @@ def _attn_block(q, k, v, lengths, starts, o, lse, rest, opt):
     window, sinks, scale = opt
     a = L.WindowAttention(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], L.dtype_code(q.dtype), window,
                           sinks, scale)
-    (a.q, q), (a.k, k), (a.v, v) = _heads(q), _heads(k), _heads(v)
+    (a.q, q), (a.k, k), (a.v, v) = _heads(q), _heads(k, True), _heads(v, True)
     a.lengths, a.starts, a.o, a.lse, a.o_rest = _ptr(lengths), _ptr(starts), o.data_ptr(), _ptr(lse), _ptr(rest)
     return a, (q, k, v)
 

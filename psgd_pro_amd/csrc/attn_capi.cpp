@@ -1,5 +1,5 @@
-// The C ABI of attention and of the norms and rotation in front of it (include/psgdk.h, level 3): argument validation, workspace layout and launches. Host code only; every
-// launch goes to the caller's stream, nothing synchronizes.
+// The C ABI of attention and of the norms and rotation in front of it (include/psgdk.h, level 3): argument validation, workspace
+// layout and launches. Host code only; every launch goes to the caller's stream, nothing synchronizes.
 #include <algorithm>
 #include <cmath>
 
@@ -12,10 +12,11 @@ using namespace psgdk;
 namespace {
 
 // Strides in elements: what a tile of up to 128 rows reaches stays within 32-bit byte offsets.
-constexpr int64_t kMaxStride = (int64_t)1 << 21;
+constexpr int64_t kMaxStride = (int64_t)1 << 21, kFar = (int64_t)1 << 40;
+int64_t query_heads(const psgdk_window_attention_t* q) { return kMaxStride * 128 / std::max(q->heads, 128); }
 
 // rows of 16-byte vectors: a base and strides that keep them aligned
-int check_side(const psgdk_heads_t& t, int dt, int64_t tokens, int64_t heads, const char* name, AttnSide& out) {
+int check_side(const psgdk_heads_t& t, int dt, int64_t tokens, int64_t heads, int64_t max_head_stride, const char* name, AttnSide& out) {
   if (!t.p) return fail(PSGDK_EINVAL, "%s: null device pointer", name);
   const int64_t unit = dt == PSGDK_BF16 ? 8 : 4;
   if (reinterpret_cast<uintptr_t>(t.p) & 15) return fail(PSGDK_EINVAL, "%s: 16-byte alignment", name);
@@ -23,7 +24,7 @@ int check_side(const psgdk_heads_t& t, int dt, int64_t tokens, int64_t heads, co
     return fail(PSGDK_ESHAPE, "%s: strides of whole 16 bytes", name);
   if (t.batch_stride < 0) return fail(PSGDK_ESHAPE, "%s: negative stride", name);
   if (tokens > 1) PSGDK_TRY(check_size(t.token_stride, 0, kMaxStride, name));
-  if (heads > 1) PSGDK_TRY(check_size(t.head_stride, 0, kMaxStride * 128 / std::max<int64_t>(heads, 128), name));
+  if (heads > 1) PSGDK_TRY(check_size(t.head_stride, 0, max_head_stride, name));
   out = AttnSide{t.p, t.batch_stride, tokens > 1 ? t.token_stride : 0, heads > 1 ? t.head_stride : 0};
   return PSGDK_OK;
 }
@@ -75,9 +76,10 @@ int attn_args(const psgdk_window_attention_t* q, AttnArgs& a) {
   return check_launch(q->batch * a.kv, (rows + 31) / 32, (int64_t)1 << 24, "rows");
 }
 int attn_pointers(const psgdk_window_attention_t* q, AttnArgs& a) {
-  PSGDK_TRY(check_side(q->q, a.dt, q->n, q->heads, "q", a.q));
-  PSGDK_TRY(check_side(q->k, a.dt, q->m, q->kv_heads, "k", a.k));
-  PSGDK_TRY(check_side(q->v, a.dt, q->m, q->kv_heads, "v", a.v));
+  // (a tile's rows are of several query heads, its keys of one)
+  PSGDK_TRY(check_side(q->q, a.dt, q->n, q->heads, query_heads(q), "q", a.q));
+  PSGDK_TRY(check_side(q->k, a.dt, q->m, q->kv_heads, kFar, "k", a.k));
+  PSGDK_TRY(check_side(q->v, a.dt, q->m, q->kv_heads, kFar, "v", a.v));
   if (!q->o || (reinterpret_cast<uintptr_t>(q->o) & 15)) return fail(PSGDK_EINVAL, "o: a device pointer of 16-byte alignment");
   const int64_t sn = (int64_t)q->heads * q->d;
   a.o = AttnSide{q->o, q->n * sn, sn, q->d};
@@ -246,7 +248,7 @@ int psgdk_window_attention_backward(const psgdk_window_attention_t* q, const psg
   }
   if (*ws_bytes < m.off) return fail(PSGDK_EWORKSPACE, "workspace %zu < %zu bytes", *ws_bytes, m.off);
   PSGDK_TRY(attn_pointers(q, a));
-  PSGDK_TRY(check_side(g->dout, a.dt, q->n, q->heads, "dout", a.dout));
+  PSGDK_TRY(check_side(g->dout, a.dt, q->n, q->heads, query_heads(q), "dout", a.dout));
   if (!a.lse) return fail(PSGDK_EINVAL, "lse: null device pointer");
   for (const void* p : {(const void*)a.dq, (const void*)a.dk, (const void*)a.dv})
     if (reinterpret_cast<uintptr_t>(p) & 15) return fail(PSGDK_EINVAL, "dq, dk, dv: 16-byte alignment");

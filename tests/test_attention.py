@@ -184,6 +184,26 @@ def test_strides(dtype):
     check(x[:, :, :4], x[:, :, 4:6], x[:, :, 6:], rnd((2, 90, 4, 1), 7, dtype).expand(2, 90, 4, 64))
 
 
+def test_a_long_cache_of_each_heads_tokens_is_read_in_place():
+    b, m, h, kv, d = 1, 40000, 4, 2, 64  # heads 2.56 M elements apart
+    q, do = rnd((b, 2, h, d), 70, torch.bfloat16), rnd((b, 2, h, d), 71, torch.bfloat16)
+    kc, vc = (rnd((b, kv, m, d), s, torch.bfloat16).transpose(1, 2) for s in (72, 73))
+    lengths = torch.tensor([m - 5], device=DEV)
+    starts = lengths - 2
+    ref, bounds = reference(q, kc, vc, None, 1000, 3, lengths, starts)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    o = P.window_attention(q, kc, vc, window=1000, sinks=3, lengths=lengths, starts=starts)
+    assert torch.cuda.max_memory_allocated() - before < kc.numel() * 2  # (no copy of either cache)
+    within(o, ref[0], bounds[0])
+    leaves = [t.detach().requires_grad_() for t in (q, kc, vc)]
+    grads = torch.autograd.grad(P.window_attention(*leaves, window=1000, sinks=3, lengths=lengths, starts=starts), leaves, do)
+    near = [t.detach().contiguous().requires_grad_() for t in (q, kc, vc)]
+    for x, y in zip(grads, torch.autograd.grad(P.window_attention(*near, window=1000, sinks=3, lengths=lengths, starts=starts), near, do)):
+        assert torch.equal(x, y)
+
+
 def test_offsets_beyond_32_bits():
     """A cache of 2^33 bytes: the window at its end, and the first tokens."""
     m, kv, d = 1 << 22, 8, 128
