@@ -402,3 +402,17 @@ def test_refusals_of_tensors():
         P.AdamW([torch.zeros(3, device=DEV)])
     with pytest.raises(ValueError):
         P.AdamW([torch.zeros(3, device=DEV, requires_grad=True)], state_bits=16)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_given_twice_is_refused(bits):
+    ps, gs = [[torch.ones(300, device=DEV) for _ in range(2)] for _ in range(2)]
+    ms, vs = [[P.adamw_state(p, bits) for p in ps] for _ in range(2)]
+    for m, v in ((ms, ms), ([ms[0], ms[0]], vs), (ms, [vs[0], vs[0]])):
+        with pytest.raises(RuntimeError, match="twice"):
+            P.adamw_step(ps, gs, m, v, step=1)
+    assert all(bool((p == 1).all()) for p in ps)
+    if bits == 8:
+        with pytest.raises(RuntimeError, match="twice"):
+            P.adamw_step(ps, gs, [ms[0], (ms[1][0], ms[0][1])], vs, step=1)
+    P.adamw_step(ps, gs, ms, vs, step=1)
