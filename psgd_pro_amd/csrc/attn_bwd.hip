@@ -10,7 +10,7 @@ namespace {
 
 // With P the probabilities, dP = dO V^T, delta = sum of o dO over a row:  dS = P (dP - delta),  dQ = scale dS K.
 // Transposed as the forward pass: a lane has one row, dS^T is the last product's operand where it is made. 4 x 4096 tokens, 32 / 8
-// heads of 128, bf16: 790 us, 6 d flops a visible pair at 1050 TFLOP/s (the matrix cores busy 56% of the cycles).
+// heads of 128, bf16: 794 us, 6 d flops a visible pair at 1040 TFLOP/s (the matrix cores busy 56% of the cycles).
 template <typename T, int DP, int BK>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_dq_kernel(const AttnArgs a, int row_tiles) {
   using R = Rows<T, DP>;
