@@ -202,7 +202,9 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
           x[s][e] = in[s] ? x[s][e] - mean : 0.f;
           sq += x[s][e] * x[s][e];
         }
-      const float rstd = a.norm == NORM_NONE ? 1.f : 1.f / sqrtf(lanes_sum(sq, a.lanes) * inv_d + a.eps);
+      float rstd = a.norm == NORM_NONE ? 1.f : 1.f / sqrtf(lanes_sum(sq, a.lanes) * inv_d + a.eps);
+      // lanes without a head hold zeros, whose rstd is infinite where eps is 0: the weights' sums would get NaN
+      if constexpr (BACK) rstd = there ? rstd : 0.f;
 
       float out[S][2 * V];
       if constexpr (!BACK) {
