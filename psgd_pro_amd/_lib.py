@@ -5,6 +5,7 @@ on torch's streams and allocations. There is no fallback: when the library is mi
 """
 import collections
 import ctypes as C
+import importlib
 import os
 
 import torch
@@ -183,8 +184,9 @@ _SIGS = {
 
 EXPORTED = tuple(_SIGS)
 ABI_VERSION = 7  # PSGDK_VERSION of include/psgdk.h that these signatures and structures follow
+TABLES_VERSION = 2  # kVersion of csrc/tables.cpp
 
-_lib = None
+_lib = _tables = None
 
 
 def lib():
@@ -204,6 +206,21 @@ def lib():
                                f"{ABI_VERSION}; rebuild it with `python -m psgd_pro_amd.build`")
         _lib = L
     return _lib
+
+
+def tables():
+    """The Python module of csrc/tables.cpp, which fills host tables by address; raises when it is missing or of another build."""
+    global _tables
+    if _tables is None:
+        try:
+            t = importlib.import_module(__package__ + "._tables")
+        except ImportError as e:
+            raise RuntimeError(f"psgd_pro_amd: the module _tables is not there ({e}); build it with `python -m psgd_pro_amd.build`") from e
+        if getattr(t, "VERSION", None) != TABLES_VERSION:  # a stale build: it may fill them in another layout
+            raise RuntimeError(f"psgd_pro_amd: {t.__file__} has version {getattr(t, 'VERSION', None)}, the bindings expect "
+                               f"{TABLES_VERSION}; rebuild it with `python -m psgd_pro_amd.build`")
+        _tables = t
+    return _tables
 
 
 def check(rc):

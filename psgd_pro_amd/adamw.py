@@ -25,9 +25,8 @@ _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 def _tables(params, grads, ms, vs):
     """The host arrays of psgdk_adamw_t for lists of tensors, checked (csrc/tables.cpp): (their buffer, the states' bits, copies of
     gradients that had to be made contiguous)."""
-    from . import _tables as T  # (after torch; built beside the library)
     buf = (C.c_int64 * (8 * len(params)))()
-    return (buf, *T.adamw(params, grads, ms, vs, C.addressof(buf)))
+    return (buf, *L.tables().adamw(params, grads, ms, vs, C.addressof(buf), len(buf)))
 
 
 def _check_numbers(step, lr, betas, eps, weight_decay, max_norm):
@@ -44,7 +43,6 @@ def _check_numbers(step, lr, betas, eps, weight_decay, max_norm):
 
 
 def _launch(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm, seed):
-    from . import _tables as T  # (as above)
     buf, bits, keep = _tables(params, grads, ms, vs)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("psgd_pro_amd: an AdamW step is not captured into a graph (its number would stay the same)")
@@ -54,7 +52,7 @@ def _launch(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
     a = L.AdamW(len(params), bits, at, at + n, at + 2 * n, at + 3 * n, at + 4 * n, at + 5 * n, *scales, lr, betas[0], betas[1], eps,
                 weight_decay, max_norm or 0.0, step, seed, None if norm is None else norm.data_ptr())
     _run_ws(params[0], L.lib().psgdk_adamw, C.byref(a))
-    T.changed(params)  # (as by torch's own in-place operations)
+    L.tables().changed(params)  # (as by torch's own in-place operations)
     return norm
 
 

@@ -8,6 +8,7 @@
 
 namespace {
 
+constexpr int kVersion = 2;      // of these functions and of the layout of what they fill: the bindings ask for their own (_lib.py)
 constexpr int64_t kBlock = 256;  // elements that share a scale
 
 struct Fail {
@@ -58,13 +59,15 @@ void* state(PyObject* o, const at::Tensor& p, at::ScalarType type, int64_t size,
   return t->data_ptr();
 }
 
-// adamw(params, grads, exp_avgs, exp_avg_sqs, address): fills 8 int64 a parameter at `address`, array by array: elements, dtype
-// (two 32-bit numbers each, the first half), the addresses of parameters, gradients, first moments, second moments and their
-// scales. Returns (bits of the states, the gradients that were copied to be contiguous).
+// adamw(params, grads, exp_avgs, exp_avg_sqs, address, count): fills the `count` int64 at `address`, 8 a parameter, array by array:
+// elements, dtype (two 32-bit numbers each, the first half), the addresses of parameters, gradients, first moments, second moments
+// and their scales. Returns (bits of the states, the gradients that were copied to be contiguous).
 PyObject* adamw(PyObject*, PyObject* args) {
   PyObject *params, *grads, *ms, *vs;
   unsigned long long address;
-  if (!PyArg_ParseTuple(args, "O!O!O!O!K", &PyList_Type, &params, &PyList_Type, &grads, &PyList_Type, &ms, &PyList_Type, &vs, &address))
+  Py_ssize_t count;
+  if (!PyArg_ParseTuple(args, "O!O!O!O!Kn", &PyList_Type, &params, &PyList_Type, &grads, &PyList_Type, &ms, &PyList_Type, &vs, &address,
+                        &count))
     return nullptr;
   HANDLE_TH_ERRORS
   try {
@@ -73,6 +76,7 @@ PyObject* adamw(PyObject*, PyObject* args) {
     if (PyList_GET_SIZE(grads) != n) refuse(PyExc_RuntimeError, PyList_GET_SIZE(grads), " gradients for ", n, " parameters");
     if (PyList_GET_SIZE(ms) != n) refuse(PyExc_RuntimeError, PyList_GET_SIZE(ms), " exp_avgs for ", n, " parameters");
     if (PyList_GET_SIZE(vs) != n) refuse(PyExc_RuntimeError, PyList_GET_SIZE(vs), " exp_avg_sqs for ", n, " parameters");
+    if (count != 8 * n) refuse(PyExc_RuntimeError, "a buffer of ", 8 * n, " numbers expected, got one of ", count);
     int64_t* const numel = reinterpret_cast<int64_t*>(address);
     int32_t* const dtype = reinterpret_cast<int32_t*>(numel + n);
     void** const at = reinterpret_cast<void**>(numel + 2 * n);
@@ -149,4 +153,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tables", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tables() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__tables() {
+  PyObject* const m = PyModule_Create(&module);
+  if (m && PyModule_AddIntConstant(m, "VERSION", kVersion) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
