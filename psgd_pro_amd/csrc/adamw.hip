@@ -100,7 +100,7 @@ __device__ __forceinline__ float max32(float m) {
   return fmaxf(m, __shfl_xor(m, 16, 64));
 }
 // The scale's exponent field for a largest magnitude of bits `top`: with it that lies in (224, 448], e4m3's top. The largest
-// field is 246, so that 2^(127 - field) is a normal number too. Infinite or NaN: 255.
+// field is 247, so that 2^(127 - field) is a normal number too. Infinite or NaN: 255.
 __device__ __forceinline__ uint32_t scale_field(float top) {
   const uint32_t u = __float_as_uint(top);
   if (u >= 0x7f800000u) return 255;
@@ -128,72 +128,86 @@ __device__ __forceinline__ uint2 pack8(const float (&x)[8], uint32_t field, cons
 }
 
 // m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, each product and sum rounded, so that the same inputs give the same codes
-// wherever they are computed; then p.
+// wherever they are computed; then p. ROOTS: v holds roots before. WIDE: where a square is out of range, its root is made of a
+// 2^-64th of root and gradient (infinite and NaN ones stay so).
+template <bool ROOTS, bool WIDE>
 __device__ __forceinline__ void adam8(const AdamArgs& a, float coef, bool scaled, float (&p)[8], const float (&g0)[8], float (&m)[8],
                                       float (&v)[8], float (&root)[8]) {
 #pragma clang fp contract(off)
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float g = scaled ? g0[i] * coef : g0[i];
+    const float g = scaled ? g0[i] * coef : g0[i], r = v[i];
     m[i] = m[i] * a.b1 + g * a.c1;
-    v[i] = v[i] * a.b2 + g * g * a.c2;
+    v[i] = (ROOTS ? r * r : r) * a.b2 + g * g * a.c2;
     root[i] = sqrtf(v[i]);
+    if constexpr (WIDE) {
+      const float s = r * 0x1p-64f, h = g * 0x1p-64f;
+      if (!(v[i] < INFINITY)) root[i] = sqrtf(s * s * a.b2 + h * h * a.c2) * 0x1p64f;
+    }
     p[i] = p[i] * a.keep - a.rate * m[i] * __builtin_amdgcn_rcpf(root[i] * a.root + a.eps);
   }
 }
 
 // 28 bytes an element with fp32 parameters and states, 10 with bf16 parameters and 8 bits: bound by memory. 386 M elements: fp32
-// 2035 us, 5.3 TB/s; bf16 with 8 bits 707 us, 5.5 TB/s, some 65 vector instructions an element (a third of them Philox, which is
+// 2035 us, 5.3 TB/s; bf16 with 8 bits 700 us, 5.5 TB/s, some 65 vector instructions an element (a third of them Philox, which is
 // why both states share a number). A thread has 8 elements that lie together, twice, 32 lanes a block of 256.
-// WHOLE: the chunk is all there.
-template <typename T, int BITS, bool WHOLE>
-__device__ __forceinline__ void adamw_chunk(const AdamArgs& a, int t, long long n, long long i0) {
+// WHOLE: the chunk is all there. With 8 bits, false where the block has a moment out of range: nothing is stored then, but
+// where WIDE (that path apart, and from memory again, costs the other nothing).
+template <typename T, int BITS, bool WHOLE, bool WIDE>
+__device__ __forceinline__ bool adamw_elements(const AdamArgs& a, int t, long long n, long long i, float coef) {
   T* const p = static_cast<T*>(a.p[t]);
   const T* const g = static_cast<const T*>(a.g[t]);
-  const float coef = a.coef ? *a.coef : 1.f;
+  const int left = WHOLE ? 8 : (int)min(max(n - i, 0ll), 8ll);
+  float x[8], y[8], m[8], v[8], root[8];
+  ld8(p + i, left, x);
+  ld8(g + i, left, y);
+  if constexpr (BITS == 32) {
+    ld8(static_cast<const float*>(a.m[t]) + i, left, m);
+    ld8(static_cast<const float*>(a.v[t]) + i, left, v);
+    adam8<false, false>(a, coef, a.coef != nullptr, x, y, m, v, root);
+    st8(static_cast<float*>(a.m[t]) + i, left, m);
+    st8(static_cast<float*>(a.v[t]) + i, left, v);
+  } else {
+    const long long block = i / kAdamBlock;
+    uint8_t* const mc = static_cast<uint8_t*>(a.m[t]) + i;
+    uint8_t* const vc = static_cast<uint8_t*>(a.v[t]) + i;
+    unpack8(ld_codes(mc, left), left ? scale_of(a.ms[t][block]) : 0.f, m);
+    unpack8(ld_codes(vc, left), left ? scale_of(a.vs[t][block]) : 0.f, v);
+    adam8<true, WIDE>(a, coef, a.coef != nullptr, x, y, m, v, root);
+    float mt = 0.f, vt = 0.f;
+    bool bad = false;  // (a largest of NaN and a number is the number)
 #pragma unroll
-  for (int r = 0; r < kAdamChunk / 2048; ++r) {
-    const long long i = i0 + r * 2048 + threadIdx.x * 8;
-    const int left = WHOLE ? 8 : (int)min(max(n - i, 0ll), 8ll);
-    float x[8], y[8], m[8], v[8], root[8];
-    ld8(p + i, left, x);
-    ld8(g + i, left, y);
-    if constexpr (BITS == 32) {
-      ld8(static_cast<const float*>(a.m[t]) + i, left, m);
-      ld8(static_cast<const float*>(a.v[t]) + i, left, v);
-      adam8(a, coef, a.coef != nullptr, x, y, m, v, root);
-      st8(static_cast<float*>(a.m[t]) + i, left, m);
-      st8(static_cast<float*>(a.v[t]) + i, left, v);
-    } else {
-      const long long block = i / kAdamBlock;
-      uint8_t* const mc = static_cast<uint8_t*>(a.m[t]) + i;
-      uint8_t* const vc = static_cast<uint8_t*>(a.v[t]) + i;
-      unpack8(ld_codes(mc, left), left ? scale_of(a.ms[t][block]) : 0.f, m);
-      unpack8(ld_codes(vc, left), left ? scale_of(a.vs[t][block]) : 0.f, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= v[e];
-      adam8(a, coef, a.coef != nullptr, x, y, m, v, root);
-      float mt = 0.f, vt = 0.f;
-      bool bad = false;  // (a largest of NaN and a number is the number)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float am = e < left ? fabsf(m[e]) : 0.f, av = e < left ? root[e] : 0.f;
-        bad = bad || !(am < INFINITY) || !(av < INFINITY);
-        mt = fmaxf(mt, am);
-        vt = fmaxf(vt, av);
-      }
-      const uint32_t mf = scale_field(max32(bad ? INFINITY : mt)), vf = scale_field(max32(bad ? INFINITY : vt));
-      const long long w = (a.at[t] + i) / 8;
-      uint32_t rnd[4] = {(uint32_t)w, (uint32_t)(w >> 32), a.step, (uint32_t)a.index[t]};
-      philox4x32_10(rnd, a.k0, a.k1);
-      st_codes(mc, left, pack8<false>(m, mf, rnd));
-      st_codes(vc, left, pack8<true>(root, vf, rnd));
-      if (left && threadIdx.x % 32 == 0) {
-        a.ms[t][block] = (uint8_t)mf;
-        a.vs[t][block] = (uint8_t)vf;
-      }
+    for (int e = 0; e < 8; ++e) {
+      const float am = e < left ? fabsf(m[e]) : 0.f, av = e < left ? root[e] : 0.f;
+      bad = bad || !(am < INFINITY) || !(av < INFINITY);
+      mt = fmaxf(mt, am);
+      vt = fmaxf(vt, av);
     }
-    st8(p + i, left, x);
+    const uint32_t mf = scale_field(max32(bad ? INFINITY : mt)), vf = scale_field(max32(bad ? INFINITY : vt));
+    if (!WIDE && mf == 255) return false;
+    const long long w = (a.at[t] + i) / 8;
+    uint32_t rnd[4] = {(uint32_t)w, (uint32_t)(w >> 32), a.step, (uint32_t)a.index[t]};
+    philox4x32_10(rnd, a.k0, a.k1);
+    st_codes(mc, left, pack8<false>(m, mf, rnd));
+    st_codes(vc, left, pack8<true>(root, vf, rnd));
+    if (left && threadIdx.x % 32 == 0) {
+      a.ms[t][block] = (uint8_t)mf;
+      a.vs[t][block] = (uint8_t)vf;
+    }
+  }
+  st8(p + i, left, x);
+  return true;
+}
+template <typename T, int BITS, bool WHOLE>
+__device__ __forceinline__ void adamw_chunk(const AdamArgs& a, int t, long long n, long long i0) {
+  const float coef = a.coef ? *a.coef : 1.f;
+  bool done[kAdamChunk / 2048];
+#pragma unroll
+  for (int r = 0; r < kAdamChunk / 2048; ++r) done[r] = adamw_elements<T, BITS, WHOLE, false>(a, t, n, i0 + r * 2048 + threadIdx.x * 8, coef);
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int r = 0; r < kAdamChunk / 2048; ++r)
+      if (!done[r]) adamw_elements<T, BITS, false, true>(a, t, n, i0 + r * 2048 + threadIdx.x * 8, coef);
   }
 }
 template <typename T, int BITS>
