@@ -442,7 +442,8 @@ int psgdk_window_attention_backward(const psgdk_window_attention_t* a, const psg
  *   u = N(x) * w  (PSGDK_NORM_* over the head's d, no bias; w NULL: 1; NONE: u = x),   y = R(p) u:
  * pair i of the first rotary_dim elements, (i, i + rotary_dim / 2) or interleaved (2 i, 2 i + 1), becomes
  * (a cos t - b sin t, b cos t + a sin t) with t = p theta^(-2 i / rotary_dim) for position p; the others stay. The angle is kept
- * as a 64-bit fraction of a turn, so that far positions lose nothing. positions NULL: a token's index in its sequence. */
+ * as a 64-bit fraction of a turn: right to fp32's rounding up to position 2^24 and to |p| 2^-48 beyond, and additive in p.
+ * positions NULL: a token's index in its sequence. */
 typedef struct psgdk_qk_norm_rope {
   int64_t batch, n;           /* batch * n up to 2^30 */
   int32_t heads, kv_heads;    /* kv_heads 0: no keys */

@@ -203,8 +203,9 @@ def qk_norm_rope(q, k=None, *, norm="rms", q_weight=None, k_weight=None, eps=1e-
     norm: "rms" (v / sqrt(mean v^2 + eps)), "layer" ((v - mean) / sqrt(var + eps)) or None (no weights then); weights may be
     absent and may be float32 beside bfloat16 inputs. Pair i of the first rotary_dim elements (d if not given; even) is
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved; the elements behind are not rotated. positions: int64 (n,) or
-    (batch, n); a token's index in its sequence if not given. Angles are exact to float32's rounding at any position. d is even
-    and up to 512, q and k may have any strides; q' and k' are contiguous. Differentiable in q, k and the weights."""
+    (batch, n); a token's index in its sequence if not given. Angles are right to float32's rounding up to position 2^24 and to
+    |p| 2^-48 beyond, and add up as positions do. d is even and up to 512, q and k may have any strides; q' and k' are
+    contiguous. Differentiable in q, k and the weights."""
     if norm not in _NORMS:
         raise ValueError(f"norm = {norm!r}: 'rms', 'layer' or None")
     _check(q, "q")

@@ -132,8 +132,9 @@ int rope_args(const psgdk_qk_norm_rope_t* q, RopeArgs& a, Aligned& al) {
   a.eps = q->eps;
   a.pos = q->positions;
   a.pos_sb = q->positions_stride;
-  double p = q->rotary_dim ? std::pow(q->theta, -2.0 / q->rotary_dim) : 1.0;
-  for (int k = 0; k < kRopePowers; ++k, p *= p) a.ratio[k] = p;
+  // (squared in 64 bits of mantissa, so that each power is the nearest double: squared as doubles the 2^7th is 2^7 roundings off)
+  long double p = q->rotary_dim ? std::pow((long double)q->theta, -2.0L / q->rotary_dim) : 1.0L;
+  for (int k = 0; k < kRopePowers; ++k, p *= p) a.ratio[k] = (double)p;
   a.interleaved = q->interleaved != 0;
   a.x[0] = rope_side(q->q, q->batch, q->n, q->heads, a.dt, al);
   if (q->kv_heads) a.x[1] = rope_side(q->k, q->batch, q->n, q->kv_heads, a.dt, al);
