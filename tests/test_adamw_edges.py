@@ -2,12 +2,11 @@
 rounding does in the long run."""
 import math
 
-import numpy as np
 import pytest
 import torch
 
 import psgd_pro_amd as P
-from test_adamw import DEV, DTYPES, E, U, formula, host, rnd, unpack, within
+from test_adamw import DEV, DTYPES, E, formula, host, rnd, unpack, within
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +53,47 @@ def test_32_bits_leave_an_element_whose_square_overflows():
         P.adamw_step(p, g, ms, vs, step=step, weight_decay=0.0)
         P.adamw_step(alone[:1], alone[1:], mz, vz, step=step, weight_decay=0.0)
         assert torch.equal(p[0], alone[0]) and float(p[0][70]) == 1.0
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_the_clip_is_over_tensors_of_all_launches(bits):
+    """300 tensors, both dtypes in turn, empty and long ones among them: one norm, and each tensor as by itself with the gradients
+    that it scales."""
+    n, max_norm = 300, 2.5
+    shapes = [(5 + i % 7, 11 + i % 3) if i % 50 else (0,) if i == 50 else (3 * 4096 + 7 * i,) for i in range(n)]
+    ps = [rnd(s, i, DTYPES[i % 2]) for i, s in enumerate(shapes)]
+    gs = [rnd(s, 1000 + i, p.dtype, std=0.3) for i, (s, p) in enumerate(zip(shapes, ps))]
+    ms, vs = ([P.adamw_state(p, bits) for p in ps] for _ in range(2))
+    before = [p.clone() for p in ps]
+    norm = P.adamw_step(ps, gs, ms, vs, step=1, lr=0.01, max_norm=max_norm, seed=4)
+    want = math.sqrt(sum(float(g.double().square().sum()) for g in gs))
+    assert abs(float(norm) - want) <= 2 * E * want and want > 4 * max_norm
+    for i, p in enumerate(before):
+        zero = torch.zeros(p.shape, device=DEV)
+        refs, bounds = formula(p, gs[i], zero, zero, 1, lr=0.01, coef=max_norm / want)
+        within(ps[i], refs[0], bounds[0], i)
+        for state, ref, e in ((ms[i], refs[1], bounds[1]), (vs[i], refs[2] if bits == 32 else refs[2].sqrt(), bounds[2])):
+            if bits == 32:
+                within(state, ref, e, i)
+            elif ref.numel():
+                got = torch.from_numpy(unpack(host(state[0]), host(state[1]))).to(DEV).view(p.shape)
+                least = (state[1].float().double() * 2.0 ** -9).repeat_interleave(256)[:got.numel()].view(p.shape)
+                within(got, ref, torch.maximum(ref.abs() / 8, least) * (1 + 64 * E), i)
+
+
+def test_8_bits_in_the_long_run():
+    """What the documents say of 4000 steps with gradients of one size, to half of the last digit of each figure: second moments
+    .04 too large on average and off by .3, first moments off by .09. (Their mean is over 2^18 elements.)"""
+    n = 1 << 18
+    p, q = [torch.zeros(n, device=DEV)], [torch.zeros(n, device=DEV)]
+    ms, vs, m, v = [P.adamw_state(p[0], 8)], [P.adamw_state(p[0], 8)], [P.adamw_state(q[0])], [P.adamw_state(q[0])]
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    for step in range(1, 4001):
+        g = [torch.randn(n, device=DEV, generator=gen)]
+        P.adamw_step(p, g, ms, vs, step=step, seed=1)
+        P.adamw_step(q, g, m, v, step=step)
+    value = lambda s: s[0].float() * s[1].float().repeat_interleave(256)  # noqa: E731
+    square = value(vs[0]).square()
+    assert abs(float(square.mean() / v[0].mean()) - 1.04) < 0.005
+    assert abs(float(((square - v[0]) / v[0]).square().mean().sqrt()) - 0.3) < 0.05
+    assert abs(float((value(ms[0]) - m[0]).norm() / m[0].norm()) - 0.09) < 0.005
