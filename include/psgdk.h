@@ -404,8 +404,8 @@ int psgdk_scale_by(int nb, const int64_t* n, int dtype, void* const* x, const fl
  * window 0: all of them. o = sum_j softmax_j(scale q . k_j) v_j, 0 where nothing is seen; query head h takes the keys of head
  * h / (heads / kv_heads). Keys and values from `length` on, and queries and their gradients that see nothing, may hold anything;
  * an infinity or NaN within a sequence may reach rows that do not see it.
- * Sums are added in an order that the sizes alone set. With bf16 the probabilities and, backward, the scores' gradients are
- * rounded to bf16 before the matrix cores take them.
+ * Sums are added in an order that the sizes alone set. With bf16 the probabilities (forward with more than 64 rows, below) and,
+ * backward, the scores' gradients are rounded to bf16 before the matrix cores take them.
  * d: a multiple of 8 up to 128; n and m up to 2^28; with rows = n heads / kv_heads, up to 2^31 - 256, batch kv_heads rows / 32 under
  * 2^24, and backward batch kv_heads m / 128 under 2^23. */
 typedef struct psgdk_heads { /* (batch, tokens, heads, d), d contiguous; strides in elements, whole 16 bytes and up to 2^21 for

@@ -97,8 +97,8 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, lengths=None,
 
     A query that sees nothing has output 0 and no gradient; keys and values from lengths[b] on, and queries and gradients of
     positions outside the sequence, may hold anything. Within a sequence values are taken to be finite: an infinity or NaN may
-    reach queries that do not see it. bfloat16 probabilities, and backward the scores' gradients, are rounded before the second
-    products. Two runs give the same bits. scale: 1 / sqrt(d) if not given. Differentiable in q, k and v."""
+    reach queries that do not see it. bfloat16 probabilities (where a key head has more than 64 queries), and backward the
+    scores' gradients, are rounded before the second products. Two runs give the same bits. scale: 1 / sqrt(d) if not given. Differentiable in q, k and v."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         _check(t, name, None if t is q else q)
         if t.dim() != 4 or t.dtype != q.dtype:

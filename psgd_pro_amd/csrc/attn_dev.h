@@ -48,6 +48,14 @@ __device__ __forceinline__ frag_t<T> crossed(const f32x16_t& c, int u) {
   }
 }
 
+// what rounding took from those 8 values, f being crossed's
+__device__ __forceinline__ bf16x8_t crossed_rest(const f32x16_t& c, int u, bf16x8_t f) {
+  f32x16_t r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = c[8 * u + i] - (float)f[i];
+  return crossed<bf16_t>(r, 0);
+}
+
 // sum + the 8 values
 __device__ __forceinline__ float sum_of(bf16x8_t f, float sum) {
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));

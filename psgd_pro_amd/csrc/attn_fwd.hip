@@ -20,7 +20,12 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
   using R = Rows<T, DP>;
   constexpr int W = WQ * WK, LOADS = R::loads(BK, W), TILE = BK * R::PITCH, KT = BK / WK / 32, DC = DP / 16, DT = DP / 32;
   constexpr int AHEAD = DT < 4 || sizeof(T) == 4 ? 2 : 4;  // at most KT DC and 2 KT DT
+  // Few rows wait for the keys and values: the matrix cores then take what rounding takes from a probability too, in a product
+  // of its own (outputs .0017 of their norm off, as exact ones rounded to bf16, not .0021 to .0024; a token over
+  // 131072 keys of 8 heads: 107.3 us without, 107.7 with)
+  constexpr bool REST = sizeof(T) == 2 && WK > 1;
   static_assert(LOADS * W * 1024 == TILE && KT * WK * 32 == BK, "whole loads, whole blocks of keys");
+  static_assert(!REST || KT == 1, "32 keys a wave");  // (a reference that moves between the first and the second 32 would scale a rest)
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -99,7 +104,7 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
     // Keys 32 by 32: their scores, their probabilities beside the products that come next (the next 32 keys' scores, the last
     // ones' values).
     f32x16_t x[KT];
-    frag_t<T> p[2 * KT], f[AHEAD];
+    frag_t<T> p[2 * KT], p_rest[REST ? 2 * KT : 1], f[AHEAD];
     const bool look = j0 + BK - 1 > lo || hi >= s.len || (hi - j0 >= a.window && j0 + BK > a.sinks);
     float mu = 0.f;
     const auto key_frag = [&](int i) __attribute__((always_inline)) { return keys(i / DC, i % DC); };
@@ -137,14 +142,16 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
       }
       mu = ref == -INFINITY ? 0.f : ref;
     };
-    // (bf16: the probabilities are rounded for the matrix cores, and their sum is of the rounded ones)
+    // (bf16: the probabilities are rounded for the matrix cores, and without their rest their sum is of the rounded ones)
     const auto probability = [&](int i, int e) __attribute__((always_inline)) {
       float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], a.scale2, -mu));
       arrived(v);  // (here, beside a product)
       x[i][e] = v;
+      if constexpr (REST) sum += v;
       if (e % 8 == 7) {
         p[2 * i + e / 8] = crossed<T>(x[i], e / 8);
-        sum = sum_of(p[2 * i + e / 8], sum);
+        if constexpr (REST) p_rest[2 * i + e / 8] = crossed_rest(x[i], e / 8, p[2 * i + e / 8]);
+        else sum = sum_of(p[2 * i + e / 8], sum);
       }
     };
     first_loads<T>(f, key_frag);
@@ -180,6 +187,7 @@ __global__ void __launch_bounds__(64 * WQ * WK, sizeof(T) == 4 && WK == 2 && DP 
     __builtin_amdgcn_s_setprio(1);
     ahead<T, 2 * KT * DT>(f, value_frag, [&](int i, frag_t<T> y) __attribute__((always_inline)) {
       o[i % DT] = mma(y, p[i / DT], o[i % DT]);
+      if constexpr (REST) o[i % DT] = mma(y, p_rest[i / DT], o[i % DT]);
       if (KT == 2 && i < 2 * DT) {
 #pragma unroll
         for (int e = i * 16 / (2 * DT); e < (i + 1) * 16 / (2 * DT); ++e) probability(KT - 1, e);
