@@ -154,9 +154,7 @@ __device__ __forceinline__ void adam8(const AdamArgs& a, float coef, bool scaled
 // WHOLE: the chunk is all there. With 8 bits, false where the block has a moment out of range: nothing is stored then, but
 // where WIDE (that path apart, and from memory again, costs the other nothing).
 template <typename T, int BITS, bool WHOLE, bool WIDE>
-__device__ __forceinline__ bool adamw_elements(const AdamArgs& a, int t, long long n, long long i, float coef) {
-  T* const p = static_cast<T*>(a.p[t]);
-  const T* const g = static_cast<const T*>(a.g[t]);
+__device__ __forceinline__ bool adamw_elements(const AdamArgs& a, int t, T* p, const T* g, float coef, long long n, long long i) {
   const int left = WHOLE ? 8 : (int)min(max(n - i, 0ll), 8ll);
   float x[8], y[8], m[8], v[8], root[8];
   ld8(p + i, left, x);
@@ -200,14 +198,17 @@ __device__ __forceinline__ bool adamw_elements(const AdamArgs& a, int t, long lo
 }
 template <typename T, int BITS, bool WHOLE>
 __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, int t, long long n, long long i0) {
+  T* const p = static_cast<T*>(a.p[t]);
+  const T* const g = static_cast<const T*>(a.g[t]);
   const float coef = a.coef ? *a.coef : 1.f;
+  i0 += threadIdx.x * 8;
   bool done[kAdamChunk / 2048];
 #pragma unroll
-  for (int r = 0; r < kAdamChunk / 2048; ++r) done[r] = adamw_elements<T, BITS, WHOLE, false>(a, t, n, i0 + r * 2048 + threadIdx.x * 8, coef);
+  for (int r = 0; r < kAdamChunk / 2048; ++r) done[r] = adamw_elements<T, BITS, WHOLE, false>(a, t, p, g, coef, n, i0 + r * 2048);
   if constexpr (BITS == 8) {
 #pragma unroll
     for (int r = 0; r < kAdamChunk / 2048; ++r)
-      if (!done[r]) adamw_elements<T, BITS, false, true>(a, t, n, i0 + r * 2048 + threadIdx.x * 8, coef);
+      if (!done[r]) adamw_elements<T, BITS, false, true>(a, t, p, g, coef, n, i0 + r * 2048);
   }
 }
 template <typename T, int BITS>
