@@ -425,7 +425,8 @@ typedef struct psgdk_window_attention {
   float* lse;               /* [batch][kv_heads][n][heads / kv_heads]: log2 of the row's sum of e^score, output of the forward
                                call (NULL: not stored), input of the backward call */
   void* o_rest;             /* optional, as o: what rounding to bf16 took from o, output of the forward call, input of the
-                               backward call, whose gradients it makes a tenth more exact (not used with fp32) */
+                               backward call, whose gradients it makes a tenth more exact, and tenfold where values have a mean far
+                               from 0 (not used with fp32) */
 } psgdk_window_attention_t;
 int psgdk_window_attention(const psgdk_window_attention_t* a, void* ws, size_t* ws_bytes, psgdk_stream_t stream);
 

@@ -149,7 +149,7 @@ __device__ __forceinline__ void adam8(const AdamArgs& a, float coef, bool scaled
 }
 
 // 28 bytes an element with fp32 parameters and states, 10 with bf16 parameters and 8 bits: bound by memory. 386 M elements: fp32
-// 2035 us, 5.3 TB/s; bf16 with 8 bits 700 us, 5.5 TB/s, some 65 vector instructions an element (a third of them Philox, which is
+// 2048 us, 5.3 TB/s; bf16 with 8 bits 735 us, 5.3 TB/s, some 65 vector instructions an element (a third of them Philox, which is
 // why both states share a number). A thread has 8 elements that lie together, twice, 32 lanes a block of 256.
 // WHOLE: the chunk is all there. With 8 bits, false where the block has a moment out of range: nothing is stored then, but
 // where WIDE (that path apart, and from memory again, costs the other nothing).

@@ -10,7 +10,8 @@ namespace {
 
 // With P the probabilities, dP = dO V^T, delta = sum of o dO over a row:  dS = P (dP - delta),  dQ = scale dS K.
 // Transposed as the forward pass: a lane has one row, dS^T is the last product's operand where it is made. 4 x 4096 tokens, 32 / 8
-// heads of 128, bf16: 794 us, 6 d flops a visible pair at 1040 TFLOP/s (the matrix cores busy 56% of the cycles).
+// heads of 128, bf16: 770 to 819 us by the box, 6 d flops a visible pair at 1010 to 1070 TFLOP/s (the matrix cores busy 55% of the
+// cycles, the vector unit 42%).
 template <typename T, int DP, int BK>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_dq_kernel(const AttnArgs a, int row_tiles) {
   using R = Rows<T, DP>;
@@ -53,7 +54,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) attn_d
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         delta += (float)gf[i][e] * (float)of[i][e];
-        // (o's rounding would put a tenth on the gradients' error)
+        // (o's rounding would put a tenth on the gradients' error, and .03 of their norm where values lie around 16)
         if constexpr (sizeof(T) == 2) delta += (float)gf[i][e] * (float)rf[i][e];
       }
   }
@@ -177,7 +178,7 @@ __device__ __forceinline__ void store4(T* out, float y0, float y1, float y2, flo
 // transposed. Key tiles that hold sinks are seen by all rows: their rows are cut in parts, whose sums attn_dkv_sum adds.
 // KV: the tile's keys and values are fragments in registers; else the values are in LDS (bf16 heads of 128 then fit two waves
 // a SIMD: 1750 -> 1400 us of 4 x 4096 tokens with 32 / 8 heads; 1060 with the tiles of the most rows first,
-// 8 d flops a pair at 1040 TFLOP/s).
+// 8 d flops a pair at 1040 TFLOP/s; 1017 to 1103 by the box, the matrix cores busy 57% of the cycles, the vector unit 43%).
 template <typename T, int DP, int BR, bool KV>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 ? 1 : 2) attn_dkv_kernel(const AttnArgs a, int key_tiles) {
   using R = Rows<T, DP>;

@@ -10,9 +10,9 @@ namespace {
 // Scores and outputs are computed transposed, S^T = K Q^T and O^T = V^T P^T: a lane then has one row's scores (of half of the
 // keys, the other half is in lane + 32), so that the row's largest score and sum are sums inside a lane, and P^T is the second
 // product's operand in the registers where it was made. WQ waves have 32 rows each, WK waves share a tile's keys.
-// 4 x 4096 tokens, 32 / 8 heads of 128, bf16: 575 us, 960 TFLOP/s of the visible pairs' 4 d flops (609 where o's rest is stored
-// too), the matrix cores and the vector unit each busy half of the cycles: without the exponentials 546, without the reads of LDS
-// 535, without the loads 520, without both 465. Tiles of 32 keys with three waves a SIMD: 590; 64 rows a wave, one wave a SIMD,
+// 4 x 4096 tokens, 32 / 8 heads of 128, bf16: 575 us, 960 TFLOP/s of the visible pairs' 4 d flops (603 to 632 where o's rest
+// is stored too, by the box), the matrix cores busy 46% of the cycles and the vector unit 45%: without the exponentials 546, without
+// the reads of LDS 535, without the loads 520, without both 465. Tiles of 32 keys with three waves a SIMD: 590; 64 rows a wave, one wave a SIMD,
 // products and exponentials in one stream: 910 (two hundred registers moved to and from accumulation registers). A single token
 // over 131072 keys of 8 heads: the keys' and values' bytes at 5.4 TB/s, 100 us.
 template <typename T, int DP, int WQ, int WK, int BK>
