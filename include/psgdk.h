@@ -481,8 +481,8 @@ int psgdk_qk_norm_rope_backward(const psgdk_qk_norm_rope_t* a, const psgdk_qk_no
  * around it by chance, so that its expected value is its own: element i of tensor t takes the 16-bit number i % 8 (low half of a
  * word first) of block i / 8 of Philox4x32-10 (key seed; upper counter words step, t), and the magnitude's bits below the code
  * plus 16 times that number carry or not. A root that is not 0 gets no code 0. Zeroed codes and scales are zero states.
- * Gradients from 2^64 on, whose square is no float: with 32 bits v is infinite and the element stays where it is; with 8 bits they
- * count as any other up to 2^125. An infinity or NaN makes NaN of its 256 elements' states with 8 bits.
+ * Gradients from 2^64 on, whose square is no float: with 32 bits v is infinite and the element only decays from then on; with 8 bits
+ * they count as any other up to 2^125. An infinity or NaN makes NaN of its 256 elements' states with 8 bits.
  * p NULL: nothing but the norm. Tensors may begin anywhere (whole elements). norm: optional, one float in device memory.
  * Two runs with the same inputs give the same bits. */
 typedef struct psgdk_adamw {

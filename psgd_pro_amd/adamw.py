@@ -81,8 +81,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     States are adamw_state's, all of one kind: float32 tensors, or with 8 bits (codes, scales) of the first moment and of the
     second's root. Codes are rounded up or down by chance, by Philox4x32-10 under (seed, step, the tensor's place in the list), so
     that an average does not stop where a step's change is less than half a code; the update takes the values before rounding.
-    Gradients from 2^64 on: with 32 bits v is infinite and the element stays where it is from then on; with 8 bits, which hold the
-    root, they count as any other up to 2^125. An infinity or NaN makes NaN of its 256 elements' states with 8 bits.
+    Gradients from 2^64 on: with 32 bits v is infinite and the element only decays from then on; with 8 bits, which hold the root,
+    they count as any other up to 2^125. An infinity or NaN makes NaN of its 256 elements' states with 8 bits.
     bfloat16 parameters are rounded to nearest. Tensors may begin anywhere in their storage, parameters and states are contiguous.
     Returns the gradients' norm before clipping (a 0-d float32 tensor) where max_norm is given. Capture into a graph is refused."""
     _check_numbers(step, lr, betas, eps, weight_decay, max_norm)
